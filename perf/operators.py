@@ -236,6 +236,8 @@ def _held(s):
 # the largest code, and how far a row may reach: the largest value of a code that the type it comes from can hold
 LARGEST = {'int8': 127.0, 'e4m3': 448.0}
 REACH = {('fp16', 'int8'): 127 * 2.0 ** 9, ('fp16', 'e4m3'): 1.875 * 2.0 ** 15, ('bf16', 'int8'): 127 * 2.0 ** 121, ('bf16', 'e4m3'): 1.875 * 2.0 ** 127}
+# the least exponent: with fp16 the finest codes are then 2^-24 apart, as its own finest values are
+LEAST = {('fp16', 'int8'): -24, ('fp16', 'e4m3'): -15, ('bf16', 'int8'): -100, ('bf16', 'e4m3'): -100}
 
 
 def _power(e):
@@ -244,13 +246,14 @@ def _power(e):
 
 
 def _quantise(x, kind, cache):
-    """Codes and exponents of the rows of x (fp32): the least power of two, from 2^-100 up, under which a row's largest magnitude is no larger than
+    """Codes and exponents of the rows of x (fp32): the least power of two, from 2^LEAST up, under which a row's largest magnitude is no larger than
     the largest code."""
     x = x.clamp(-REACH[kind, cache], REACH[kind, cache])
     m, e = torch.frexp(x.abs().amax(-1))                           # m in [1/2, 1)
     m_top, e_top = (127 / 128, 7) if cache == 'int8' else (7 / 8, 9)
-    e = torch.where(m > 0, e - e_top + (m > m_top), -100).clamp(min=-100)
-    scaled = x * _power(-e.clamp(min=-126, max=126)).unsqueeze(-1)
+    least = LEAST[kind, cache]
+    e = torch.where(m > 0, e - e_top + (m > m_top), least).clamp(min=least)
+    scaled = x * _power(-e).unsqueeze(-1)
     return (scaled.round() if cache == 'int8' else scaled).to(CODES[cache]), e.to(torch.int8)
 
 
@@ -360,7 +363,7 @@ def _rounded(x, kind, cache):
     the even one of two."""
     x = torch.clamp(x, -REACH[kind, cache], REACH[kind, cache])
     big = x.abs().amax(-1)
-    e = torch.full_like(big, -100.0)
+    e = torch.full_like(big, float(LEAST[kind, cache]))
     e = torch.maximum(e, torch.floor(torch.log2(torch.where(big > 0, big, 1e-300) / LARGEST[cache])))
     e = torch.where(big > LARGEST[cache] * torch.pow(2.0, e), e + 1, e)
     y = x / torch.pow(2.0, e).unsqueeze(-1)
