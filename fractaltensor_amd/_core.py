@@ -31,6 +31,7 @@ EXPORTS = (
     'ftk_stacked_lstm_f16_workspace_bytes', 'ftk_stacked_lstm_f16',
     'ftk_b2b_gemm_f16', 'ftk_b2b_gemm_f16_supported', 'ftk_b2b_gemm_rowmajor_f16', 'ftk_gemm_f16', 'ftk_batched_gemm_f16', 'ftk_flash_attn_f16', 'ftk_flash_attn_f16_workspace_bytes', 'ftk_flash_attn_ws_f16', 'ftk_flash_attn_f32_workspace_bytes', 'ftk_flash_attn_f32', 'ftk_online_softmax_f32', 'ftk_embedding_gather_f32',
     'ftk_grid_rnn_workspace_bytes', 'ftk_grid_rnn_f32', 'ftk_windowed_attn_f32',
+    'ftk_kv_cache_write', 'ftk_kv_cache_read', 'ftk_paged_attn_workspace_bytes', 'ftk_paged_attn', 'ftk_verify_drafts_workspace_bytes', 'ftk_verify_drafts',
 )
 
 
@@ -45,6 +46,18 @@ class FtkError(RuntimeError):
 class LstmOptions(ctypes.Structure):
     """ftk_lstm_options of include/ftk.h."""
     _fields_ = [('products', ctypes.c_int), ('spin_limit', ctypes.c_int)]
+
+
+class KvPages(ctypes.Structure):
+    """ftk_kv_pages of include/ftk.h."""
+    _fields_ = [('k', ctypes.c_void_p), ('v', ctypes.c_void_p), ('k_exps', ctypes.c_void_p), ('v_exps', ctypes.c_void_p), ('type', ctypes.c_int),
+                ('pages', ctypes.c_int), ('heads', ctypes.c_int), ('page_size', ctypes.c_int), ('head_size', ctypes.c_int)]
+
+
+class KvBatch(ctypes.Structure):
+    """ftk_kv_batch of include/ftk.h."""
+    _fields_ = [('table', ctypes.c_void_p), ('lens', ctypes.c_void_p), ('starts', ctypes.c_void_p), ('sequences', ctypes.c_int),
+                ('table_width', ctypes.c_int), ('tokens', ctypes.c_int)]
 
 
 class DeviceInfo(ctypes.Structure):
@@ -74,9 +87,14 @@ def _load() -> ctypes.CDLL:
     lib.ftk_flash_attn_f32_workspace_bytes.argtypes = [ctypes.c_int] * 5
     lib.ftk_flash_attn_f16_workspace_bytes.restype = ctypes.c_size_t
     lib.ftk_flash_attn_f16_workspace_bytes.argtypes = [ctypes.c_int] * 5
+    lib.ftk_paged_attn_workspace_bytes.restype = ctypes.c_size_t
+    lib.ftk_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(KvPages), ctypes.POINTER(KvBatch)] + [ctypes.c_int] * 3
+    lib.ftk_verify_drafts_workspace_bytes.restype = ctypes.c_size_t
+    lib.ftk_verify_drafts_workspace_bytes.argtypes = [ctypes.c_int] * 2
     for name in EXPORTS:
         if name not in ('ftk_last_error', 'ftk_stacked_lstm_workspace_bytes', 'ftk_stacked_lstm_f16_workspace_bytes', 'ftk_grid_rnn_workspace_bytes',
-                        'ftk_flash_attn_f32_workspace_bytes', 'ftk_flash_attn_f16_workspace_bytes'):
+                        'ftk_flash_attn_f32_workspace_bytes', 'ftk_flash_attn_f16_workspace_bytes', 'ftk_paged_attn_workspace_bytes',
+                        'ftk_verify_drafts_workspace_bytes'):
             getattr(lib, name).restype = ctypes.c_int
     return lib
 
@@ -133,11 +151,12 @@ def _count(name: str) -> None:
 
 
 try:
-    from . import _fast
+    from . import _fast, _serving
 except ImportError as e:
-    raise ImportError(f'{_HERE}/_fast.so cannot be loaded ({e}): build it with `make -C fractaltensor_amd/csrc` '
+    raise ImportError(f'{_HERE}/_fast.so or _serving.so cannot be loaded ({e}): build them with `make -C fractaltensor_amd/csrc` '
                       '(or __graft_entry__.build()); there is no fallback path') from e
 _fast.init(launch_counts, _check)
+_serving.init(launch_counts, _check)
 
 
 def version() -> int:
@@ -762,3 +781,204 @@ def windowed_attention(Q, K, V, window: int, dilation: int = 1, extra_idx: Optio
                                      ctypes.c_int(D), ctypes.c_int(window), ctypes.c_int(dilation), ctypes.c_int(R),
                                      ctypes.c_float(scale), _stream()))
     return out
+
+
+# ---- serving on a paged cache of keys and values ------------------------------------------
+#
+# The cache: k_pages, v_pages [pages, kv heads, page size, D], fp16, bf16, float8_e4m3fn or int8; the last two with
+# k_exps, v_exps [pages, kv heads, page size] int8, an exponent for each row (element = code * 2^exponent).
+# The batch, int32: starts [B + 1], the packed rows starts[b] .. starts[b + 1] - 1 are the new tokens of sequence b; lens [B], its length
+# with them, so that they are its last positions; table [B, W], position p lies in row p % page size of page table[b, p // page size].
+# What these arrays hold is looked at on the device only (include/ftk.h says what becomes of entries that point nowhere).
+
+KV_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2, torch.int8: 3}
+
+
+def _req_on(t, dtype, shape, device, name: str) -> None:
+    _req(t, dtype, name)
+    if t.device != device:
+        raise RuntimeError(f'{name} lives on {t.device}, the others on {device}')
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f'{name} must be {tuple(shape)}, got {tuple(t.shape)}')
+
+
+def _req_rows(t, dtype, heads, D: int, device, name: str) -> None:
+    """[tokens, heads, D] with the elements of a head next to each other and strides of 8 elements otherwise."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f'{name} must be a torch.Tensor')
+    if not t.is_cuda:
+        raise RuntimeError(f'{name} must live on the GPU (got {t.device}); there is no CPU path')
+    if t.device != device:
+        raise RuntimeError(f'{name} lives on {t.device}, the others on {device}')
+    if t.dtype != dtype:
+        raise TypeError(f'{name} must be {dtype}, got {t.dtype}')
+    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or t.shape[2] != D:
+        raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {D}], got {tuple(t.shape)}")
+    if t.stride(2) != 1 or any(t.shape[i] > 1 and t.stride(i) % 8 for i in (0, 1)):
+        raise ValueError(f'{name}: the elements of a head must be contiguous and the other strides multiples of 8, got strides {t.stride()}')
+
+
+def _req_cache(k_pages, v_pages, table, lens, starts, k_exps, v_exps) -> None:
+    """Says what is wrong with a cache and a batch, if something is."""
+    for t, name in ((k_pages, 'k_pages'), (v_pages, 'v_pages')):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f'{name} must be a torch.Tensor')
+        if t.dtype not in KV_TYPES:
+            raise TypeError(f'{name} must be float16, bfloat16, float8_e4m3fn or int8, got {t.dtype}')
+        if t.dim() != 4:
+            raise ValueError(f'{name} must be [pages, kv heads, page size, D], got {tuple(t.shape)}')
+    device = k_pages.device
+    _req(k_pages, k_pages.dtype, 'k_pages')
+    _req_on(v_pages, k_pages.dtype, k_pages.shape, device, 'v_pages')
+    codes = k_pages.dtype in (torch.float8_e4m3fn, torch.int8)
+    for t, name in ((k_exps, 'k_exps'), (v_exps, 'v_exps')):
+        if codes:
+            if t is None:
+                raise ValueError(f'pages of {k_pages.dtype} need {name}')
+            _req_on(t, torch.int8, k_pages.shape[:3], device, name)
+        elif t is not None:
+            raise ValueError(f'pages of {k_pages.dtype} have no {name}')
+    _req_on(lens, torch.int32, None, device, 'lens')
+    if lens.dim() != 1:
+        raise ValueError(f'lens must be [B], got {tuple(lens.shape)}')
+    _req_on(starts, torch.int32, (lens.shape[0] + 1,), device, 'starts')
+    _req_on(table, torch.int32, None, device, 'table')
+    if table.dim() != 2 or table.shape[0] != lens.shape[0]:
+        raise ValueError(f'table must be [B, W] with B = {lens.shape[0]}, got {tuple(table.shape)}')
+
+
+def _req_pages_of(dtype, k_pages, name: str) -> None:
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f'{name} must be float16 or bfloat16, got {dtype}')
+    if k_pages.dtype in (torch.float16, torch.bfloat16) and k_pages.dtype != dtype:
+        raise TypeError(f'{name} must have the type of the pages, {k_pages.dtype}, got {dtype}')
+
+
+def _not_negative(**values) -> None:
+    for name, v in values.items():
+        if isinstance(v, bool) or not isinstance(v, int) or not 0 <= v < 2 ** 31:
+            raise ValueError(f'{name} must be a whole number from 0 up, got {v!r}')
+
+
+def kv_cache_write(keys, values, k_pages, v_pages, table, lens, starts, k_exps=None, v_exps=None) -> None:
+    """Writes the keys and values of new tokens, [tokens, kv heads, D] fp16 or bf16 (views with strides that are multiples of 8 are fine), into
+    their pages: as they are into pages of their type, else as codes of 8 bits under the least power of two of each row and head that keeps it
+    within the codes, rounded to nearest."""
+    if _serving.kv_cache_write(keys, values, k_pages, v_pages, table, lens, starts, k_exps, v_exps):
+        return
+    _req_cache(k_pages, v_pages, table, lens, starts, k_exps, v_exps)
+    for t, name in ((keys, 'keys'), (values, 'values')):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f'{name} must be a torch.Tensor')
+        _req_pages_of(t.dtype, k_pages, name)
+        _req_rows(t, keys.dtype, k_pages.shape[1], k_pages.shape[3], k_pages.device, name)
+    raise ValueError(f'keys and values must have as many tokens, got {keys.shape[0]} and {values.shape[0]}')
+
+
+def kv_cache_read(k_pages, v_pages, table, lens, starts, tokens: int, dtype=None, k_exps=None, v_exps=None,
+                  out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The last starts[b + 1] - starts[b] positions of every sequence as dense keys and values [tokens, kv heads, D]; tokens is what the
+    arrays hold rows of (rows that are no sequence's are left as they were).  dtype: fp16, bf16 or fp32, for pages of 16 bits their own type (the
+    default) or fp32; for codes of 8 bits there is no default."""
+    if dtype is None:
+        dtype = getattr(k_pages, 'dtype', None)
+    ok, ov = (None, None) if out is None else out
+    if dtype in (torch.float16, torch.bfloat16, torch.float32) and (k_pages.dtype not in (torch.float16, torch.bfloat16) or dtype in (k_pages.dtype, torch.float32)):
+        done = _serving.kv_cache_read(_LIKE[dtype], k_pages, v_pages, table, lens, starts, k_exps, v_exps, tokens, ok, ov)
+        if done is not None:
+            return done
+    _req_cache(k_pages, v_pages, table, lens, starts, k_exps, v_exps)
+    _not_negative(tokens=tokens)
+    if dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError(f'dtype must be float16, bfloat16 or float32, got {dtype}')
+    if k_pages.dtype in (torch.float16, torch.bfloat16) and dtype not in (k_pages.dtype, torch.float32):
+        raise TypeError(f'pages of {k_pages.dtype} are read in that type or in float32, not {dtype}')
+    shape = (tokens, k_pages.shape[1], k_pages.shape[3])
+    for t, name in ((ok, 'out[0]'), (ov, 'out[1]')):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f'{name} must be a torch.Tensor')
+        _req_out(t, dtype, shape, name)
+        _req_on(t, dtype, shape, k_pages.device, name)
+    raise ValueError('kv_cache_read: these arguments are not taken')
+
+
+_LIKE = {t: torch.empty(0, dtype=t) for t in (torch.float16, torch.bfloat16, torch.float32)}
+
+
+def paged_attention_workspace_bytes(q, k_pages, table, max_queries: int = 0, max_keys: int = 0) -> int:
+    """Bytes that paged_attention wants for a batch of this shape on the device of q; 0 where the keys are not cut into parts."""
+    pages = KvPages(None, None, None, None, KV_TYPES[k_pages.dtype], *k_pages.shape)
+    batch = KvBatch(None, None, None, table.shape[0], table.shape[1], q.shape[0])
+    with torch.cuda.device(q.device):
+        return int(lib.ftk_paged_attn_workspace_bytes(ctypes.byref(pages), ctypes.byref(batch), q.shape[1], max_queries, max_keys))
+
+
+def paged_attention(q, k_pages, v_pages, table, lens, starts, k_exps=None, v_exps=None, scale: Optional[float] = None, causal: bool = True,
+                    window: int = 0, max_queries: int = 0, max_keys: int = 0, out: Optional[torch.Tensor] = None, return_lse=False,
+                    workspace: Optional[torch.Tensor] = None):
+    """Attention of new tokens q [tokens, heads, D] (fp16 or bf16; views with strides that are multiples of 8 are fine) over the cache, which holds
+    their own keys and values already: one token a sequence, drafts, chunks of prompts or whole ones, in any mixture.  heads is a multiple
+    of the kv heads; each of these serves heads / kv heads neighbours.  causal: the token at position p sees positions up to p; window > 0: from
+    p - window + 1 on.  scale defaults to D ** -0.5.  A token that sees nothing gets zeros (and -inf).
+    max_queries, max_keys: the most new tokens and the greatest length of a sequence, where the program knows them (0: not known); they decide which
+    kernel runs and how it cuts the keys, and no sequence may have more new tokens than max_queries.
+    Returns o [tokens, heads, D], or (o, lse [tokens, heads] fp32) with return_lse (True, or the tensor to write to): the logs of the sums of
+    exponentials.  The workspace (paged_attention_workspace_bytes) is allocated here unless one is given."""
+    args = (k_pages, v_pages, table, lens, starts, k_exps, v_exps)
+    done = _serving.paged_attention(q, *args, scale, causal, window, max_queries, max_keys, out, return_lse, workspace)
+    if done is None:
+        _req_cache(*args)
+        if not isinstance(q, torch.Tensor):
+            raise TypeError('q must be a torch.Tensor')
+        _req_pages_of(q.dtype, k_pages, 'q')
+        _req_rows(q, q.dtype, None, k_pages.shape[3], k_pages.device, 'q')
+        _not_negative(window=window, max_queries=max_queries, max_keys=max_keys)
+        if out is not None:
+            _req_out(out, q.dtype, q.shape, 'out')
+            _req_on(out, q.dtype, q.shape, q.device, 'out')
+        if isinstance(return_lse, torch.Tensor):
+            _req_out(return_lse, torch.float32, q.shape[:2], 'return_lse')
+            _req_on(return_lse, torch.float32, q.shape[:2], q.device, 'return_lse')
+        if workspace is not None:
+            _req_on(_req_workspace(workspace), workspace.dtype, None, q.device, 'workspace')
+        done = _serving.paged_attention(q, *args, None if scale is None else float(scale), bool(causal), window, max_queries, max_keys, out,
+                                        return_lse if isinstance(return_lse, torch.Tensor) else bool(return_lse), workspace)
+        if done is None:
+            raise ValueError('paged_attention: these arguments are not taken')
+    return done[0] if done[1] is None else done
+
+
+def verify_drafts(target, draft, drafts, accept_uniforms, sample_uniforms, draft_lens=None,
+                  workspace: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Which drafted tokens a target model accepts, and the token that follows them.
+
+    target [B, K + 1, V]: the target's probabilities before each draft and behind the last; draft [B, K, V]: those the drafts were drawn from
+    (the same type: fp32, fp16 or bf16), or None for drafts that were not drawn at random; drafts [B, K] int32 or int64; uniform numbers of
+    [0, 1) accept_uniforms [B, K] and sample_uniforms [B] fp32; draft_lens [B] int32: how many drafts a sequence has (None: K).
+    A draft is accepted, if all before it are, where uniform * draft < target; the next token is drawn from max(target - draft, 0) of the
+    first that is not, or from the target behind the last.  Returns tokens [B, K + 1] of drafts' type (the accepted ones, the next, then -1) and
+    accepted [B] int32.  The numbers decide everything: the same ones give the same tokens."""
+    args = (target, draft, drafts, accept_uniforms, sample_uniforms, draft_lens, workspace)
+    done = _serving.verify_drafts(*args)
+    if done is not None:
+        return done
+    if not isinstance(target, torch.Tensor) or not isinstance(drafts, torch.Tensor):
+        raise TypeError('target and drafts must be torch.Tensors')
+    if target.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f'target must be float32, float16 or bfloat16, got {target.dtype}')
+    if drafts.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f'drafts must be int32 or int64, got {drafts.dtype}')
+    if target.dim() != 3 or drafts.dim() != 2:
+        raise ValueError(f'target must be [B, K + 1, V] and drafts [B, K], got {tuple(target.shape)} and {tuple(drafts.shape)}')
+    (B, K), V, device = drafts.shape, target.shape[2], target.device
+    _req_on(target, target.dtype, (B, K + 1, V), device, 'target')
+    _req_on(drafts, drafts.dtype, None, device, 'drafts')
+    if draft is not None:
+        _req_on(draft, target.dtype, (B, K, V), device, 'draft')
+    _req_on(accept_uniforms, torch.float32, (B, K), device, 'accept_uniforms')
+    _req_on(sample_uniforms, torch.float32, (B,), device, 'sample_uniforms')
+    if draft_lens is not None:
+        _req_on(draft_lens, torch.int32, (B,), device, 'draft_lens')
+    if workspace is not None:
+        _req_on(_req_workspace(workspace), workspace.dtype, None, device, 'workspace')
+    raise ValueError('verify_drafts: these arguments are not taken')

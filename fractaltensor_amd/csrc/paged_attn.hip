@@ -1,0 +1,993 @@
+// Attention of the new tokens of a batch of sequences over a paged cache of keys and values, grouped heads included.
+//
+// The G = query heads / kv heads query heads that share a kv head, times the new tokens of a sequence, are the ROWS of one
+// product with that head's keys: row r is token r / G, head r % G.  Two kernels by the number of rows:
+//
+//   narrow  (at most 64 rows: decoding, drafts): bound by reading the cache once.  A workgroup has 16 NQ rows; its four waves cut the
+//           KEYS, each walking every fourth 32-key tile from copies straight into its own LDS, with no barrier in the loop.
+//   wide    (chunks and prompts): bound by the matrix pipe.  A wave has 32 rows, and the four waves of a workgroup share 64-key tiles.
+//
+// Products are transposed in both, so that a lane has one row: S^T = K Q^T, O^T = V^T P^T with P as it comes out of the
+// first product (the contraction takes the keys in the order a lane holds them).  Long sequences are cut into parts of
+// `part_keys` keys, a workgroup each, which leave (reference, sum, unnormalised O) for a second launch to join.
+//
+// Rounding: scores, softmax state and O are fp32 and Q is not scaled beforehand; the one rounding is that of the weights to 16 bits
+// as operands of P V, half a step (2^-12 fp16, 2^-9 bf16) each.  A cache of 8 bits enters the products as its exact values.
+#include <algorithm>
+
+#include "kv_common.h"
+
+namespace ftk {
+
+constexpr int kWaves = 4;
+constexpr float kNoRef = -3.402823466e38f;   // the reference before any score: finite, so that -inf minus it is -inf
+constexpr float kSlack = 8.0f;               // the reference moves when a score is above it by 2^8 in the weights
+
+struct AttnArgs {
+  const void* q;
+  void* o;
+  float* lse;                                 // may be NULL
+  long long q_token, q_head;                  // strides, elements
+  KvPages pages;
+  KvBatch batch;
+  int heads, group;                           // query heads, query heads of a kv head
+  float scale_log2e;
+  int causal, window;
+  int slots_per_seq;                          // blocks of rows of a sequence; 0: numbered over the packed rows
+  int nparts, part_keys;
+  float *part_o, *part_ml;                    // [tokens * heads][nparts][D], [..][2]
+};
+
+// ---- which rows and which keys a workgroup has ----------------------------------------
+
+struct Job {
+  int b, start, n, first;      // the sequence, its first packed row, its new tokens, the position of the first
+  int row0, rows;              // first row of this workgroup, rows of the sequence
+  int len;                     // keys there are
+  int lo, hi;                  // keys [lo, hi) that the rows of this workgroup and its part see
+  int sure_lo, sure_hi;        // keys that each of its rows sees
+  int part, parts;             // parts of this sequence
+};
+
+// The keys that some row of the sequence sees begin here (a multiple of 64).
+__device__ __forceinline__ int seq_first_key(const AttnArgs& a, int first) {
+  return a.window > 0 ? (int)max(0LL, (long long)first - a.window + 1) & ~63 : 0;
+}
+__device__ __forceinline__ int seq_parts(const AttnArgs& a, int first, int len) {
+  if (a.nparts == 1) return 1;
+  const int keys = max(0, len - seq_first_key(a, first));
+  return min(max((int)(((long long)keys + a.part_keys - 1) / a.part_keys), 1), a.nparts);
+}
+__device__ __forceinline__ int clamp_position(long long x, int len) { return (int)(x < 0 ? 0 : x > len ? len : x); }
+
+// False: there is nothing to do in this slot.
+template <int R>
+__device__ __forceinline__ bool find_job(const AttnArgs& a, int slot, int part, Job& j) {
+  int tile;
+  if (a.slots_per_seq > 0) {
+    j.b = slot / a.slots_per_seq;
+    tile = slot - j.b * a.slots_per_seq;
+  } else {
+    // sequence b has the slots from starts[b] * G / R + b on, at least as many as it needs
+    const auto first_slot = [&](int b) { return (long long)min(max(a.batch.starts[b], 0), a.batch.tokens) * a.group / R + b; };
+    j.b = max(count_at_most(a.batch.sequences, slot, first_slot) - 1, 0);
+    j.b = __builtin_amdgcn_readfirstlane(j.b);
+    const long long t = slot - first_slot(j.b);
+    if (t < 0) return false;
+    tile = (int)t;
+  }
+  const KvChunk c = kv_chunk(a.batch, j.b);
+  j.start = c.start;
+  j.n = c.n;
+  j.first = c.first;
+  j.rows = c.n * a.group;
+  j.row0 = tile * R;
+  if (tile >= (j.rows + R - 1) / R) return false;
+  j.len = min(c.len, kv_capacity(a.batch, a.pages.page_shift));
+  const int t_lo = j.row0 / a.group, t_hi = (min(j.row0 + R, j.rows) - 1) / a.group;
+  const long long p_lo = (long long)c.first + t_lo, p_hi = (long long)c.first + t_hi;
+  j.hi = a.causal ? clamp_position(p_hi + 1, j.len) : j.len;
+  j.sure_hi = a.causal ? clamp_position(p_lo + 1, j.len) : j.len;
+  j.lo = a.window > 0 ? clamp_position(p_lo - a.window + 1, j.len) : 0;
+  j.sure_lo = a.window > 0 ? clamp_position(p_hi - a.window + 1, j.len) : 0;
+  j.part = part;
+  j.parts = seq_parts(a, c.first, j.len);
+  if (part >= j.parts) return false;
+  if (j.parts > 1) {
+    const long long from = (long long)seq_first_key(a, c.first) + (long long)part * a.part_keys;
+    j.lo = max(j.lo, clamp_position(from, j.len));
+    if (part < j.parts - 1) j.hi = min(j.hi, clamp_position(from + a.part_keys, j.len));
+  }
+  return true;
+}
+
+// The keys [lo, hi) that a row sees, and its place among the packed rows times heads.
+struct Row {
+  int lo, hi;
+  long long at;
+};
+__device__ __forceinline__ Row row_of(const AttnArgs& a, const Job& j, int kv_head, int row) {
+  const int t = row / a.group, g = row - t * a.group;
+  const long long p = (long long)j.first + t;
+  Row r;
+  r.hi = a.causal ? clamp_position(p + 1, j.len) : j.len;
+  r.lo = a.window > 0 ? clamp_position(p - a.window + 1, j.len) : 0;
+  r.at = (long long)(j.start + t) * a.heads + kv_head * a.group + g;
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ const typename T::scalar* query_of(const AttnArgs& a, const Job& j, int kv_head, int row) {
+  const int t = row / a.group, g = row - t * a.group;
+  return (const typename T::scalar*)a.q + (j.start + t) * a.q_token + (long long)(kv_head * a.group + g) * a.q_head;
+}
+
+// First cache row (of a kv head) of the block of 16 keys that begins at `key`, a multiple of 16, or 16 times that of the key nearest to it
+// in [lo, hi) where the block lies outside: a block that holds no key of the range is never looked at.
+__device__ __forceinline__ long long block_row(const AttnArgs& a, int b, int kv_head, int key, int lo, int hi) {
+  const int inside = min(max(key, lo & ~15), (hi - 1) & ~15);
+  const int page = kv_page(a.batch, b, inside >> a.pages.page_shift, a.pages.pages);
+  return (((long long)page * a.pages.heads + kv_head) << a.pages.page_shift) + (inside & ((1 << a.pages.page_shift) - 1));
+}
+
+// The 16-byte slot that chunk c of a tile's row takes: c ^ swizzle(row), for the reads of one chunk of 16 rows (K, rows of BYTES bytes).
+template <int BYTES>
+__device__ __forceinline__ int swizzle(int row) {
+  if constexpr (BYTES == 256) return row & 15;
+  else if constexpr (BYTES == 128) return (row >> 1) & 7;
+  else if constexpr (BYTES == 192 || BYTES == 64) return (row >> 2) & 3;
+  else return (row >> 3) & 1;                       // 96 and 32
+}
+
+// Which of eight elements are not finite, a bit each.
+template <typename T>
+__device__ __forceinline__ unsigned not_finite(typename T::v8 x) {
+  const v4u w = __builtin_bit_cast(v4u, x);
+  unsigned bits = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((w[i] & T::kExpMask) == T::kExpMask) bits |= 1u << (2 * i);
+    if ((w[i] & (T::kExpMask << 16)) == (T::kExpMask << 16)) bits |= 2u << (2 * i);
+  }
+  return bits;
+}
+template <typename T>
+__device__ __forceinline__ typename T::v8 ones_at(unsigned bits) {
+  v4u w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = T::pack(bits & (1u << (2 * i)) ? 1.0f : 0.0f, bits & (2u << (2 * i)) ? 1.0f : 0.0f);
+  return __builtin_bit_cast(typename T::v8, w);
+}
+template <typename T>
+__device__ __forceinline__ typename T::v8 zeros_at(typename T::v8 x, unsigned bits) {
+  v4u w = __builtin_bit_cast(v4u, x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] &= (bits & (1u << (2 * i)) ? 0u : 0xffffu) | (bits & (2u << (2 * i)) ? 0u : 0xffff0000u);
+  return __builtin_bit_cast(typename T::v8, w);
+}
+
+// log of the sum of exponentials from the reference (in powers of two) and the sum
+__device__ __forceinline__ float log_sum(float ref, float l) { return (ref + __builtin_log2f(l)) * 0.6931471805599453f; }
+
+// ---- narrow ---------------------------------------------------------------------------
+
+template <KvFormat F, int D>
+struct NarrowShape {
+  static constexpr int BYTES = F == kSame ? 2 * D : D;        // of a row of the cache
+  static constexpr int TILE = 32 * BYTES;                     // of a K or V tile of 32 keys
+  static constexpr int COPIES = TILE / 1024;
+  static constexpr int EXPS = F == kSame ? 0 : 256;           // the exponents of a tile's keys and values, one copy of 4 bytes a lane
+  static constexpr int STAGE = 2 * TILE + EXPS;
+  static constexpr int LOADS = 2 * COPIES + (F == kSame ? 0 : 1);
+  static constexpr int STAGES = TILE >= 6144 ? 2 : TILE >= 3072 ? 3 : 4;
+  static constexpr int RING = kWaves * STAGES * STAGE;
+  static constexpr int JOIN = kWaves * (D / 16) * 64 * 16 + kWaves * 16 * 8;
+  static constexpr int LDS = RING > JOIN ? RING : JOIN;
+};
+
+// 16 (4) bytes a lane from an address of its own, otherwise as lds_dma16
+__device__ __forceinline__ void lds_dma16_from(const unsigned char* from, void* lds_base) {
+  const unsigned lds_addr = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)lds_base);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void lds_dma4_from(const signed char* from, void* lds_base) {
+  const unsigned lds_addr = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)lds_base);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds_addr), "v"(from) : "memory", "m0");
+}
+
+template <typename T, KvFormat F, int D, int NQ>
+__device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j, int kv_head, unsigned char* smem) {
+  using S = NarrowShape<F, D>;
+  using v8 = typename T::v8;
+  using scalar = typename T::scalar;
+  constexpr int KS = D / 32, DT = D / 16, CH = S::BYTES / 16, STAGES = S::STAGES;
+  using lds_v4s = __attribute__((address_space(3))) v4s;
+  using lds_v2i = __attribute__((address_space(3))) v2i;
+  typedef short v8s __attribute__((ext_vector_type(8)));
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m = lane & 15, kg = lane >> 4;
+  const int base = j.lo & ~31;
+  const int ntiles = j.hi > j.lo ? (j.hi - base + 31) / 32 : 0;
+  unsigned char* const ring = smem + wave * (STAGES * S::STAGE);
+  const int mine = ntiles > wave ? (ntiles - wave + kWaves - 1) / kWaves : 0;
+
+  // a tile's two blocks of 16 keys, each in one page
+  struct Blocks {
+    long long r0, r1;
+  };
+  auto blocks_of = [&](int i) __attribute__((always_inline)) {
+    const int key0 = base + 32 * (wave + kWaves * i);
+    return Blocks{block_row(a, j.b, kv_head, key0, j.lo, j.hi), block_row(a, j.b, kv_head, key0 + 16, j.lo, j.hi)};
+  };
+  // Rows outside [lo, hi) repeat the nearest key inside: their weights are zero, and what they hold is finite if the cache is.
+  auto issue = [&](int i, int stage, const Blocks& at) __attribute__((always_inline)) {
+    const int key0 = base + 32 * (wave + kWaves * i);
+    unsigned char* const dst = ring + stage * S::STAGE;
+    const int least = j.lo - key0, most = j.hi - 1 - key0;
+    const bool edge = least > 0 || most < 31;
+#pragma unroll
+    for (int c = 0; c < S::COPIES; ++c) {
+      const int p = 64 * c + lane, row = p / CH, slot = p - row * CH;
+      const int chunk = slot ^ swizzle<S::BYTES>(row);
+      const int key = edge ? min(max(row, least), most) : row;
+      const long long at_row = key >= 16 ? at.r1 + key - 16 : at.r0 + key;
+      const size_t off = (size_t)at_row * S::BYTES + 16 * chunk;
+      lds_dma16_from(a.pages.k + off, dst + 1024 * c);
+      lds_dma16_from(a.pages.v + off, dst + S::TILE + 1024 * c);
+    }
+    if constexpr (F != kSame) {
+      // lanes 0..7: the exponents of K, four keys each, lanes 8..15: of V
+      const int four = 4 * (lane & 7);
+      const int key = edge ? min(max(four, least & ~3), most & ~3) : four;
+      const long long at_row = key >= 16 ? at.r1 + key - 16 : at.r0 + key;
+      lds_dma4_from((lane & 8 ? a.pages.v_exps : a.pages.k_exps) + at_row, dst + 2 * S::TILE);
+    }
+  };
+
+  v8 qf[NQ][KS];
+  int row_lo[NQ], row_hi[NQ];
+#pragma unroll
+  for (int nq = 0; nq < NQ; ++nq) {
+    const int row = min(j.row0 + 16 * nq + m, j.rows - 1);
+    const Row r = row_of(a, j, kv_head, row);
+    row_lo[nq] = r.lo;
+    row_hi[nq] = r.hi;
+    const scalar* const q = query_of<T>(a, j, kv_head, row) + 8 * kg;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[nq][s] = *reinterpret_cast<const v8*>(q + 32 * s);
+  }
+  asm volatile("" ::: "memory");
+
+  v4f o[NQ][DT];
+  float ref[NQ], l[NQ];
+#pragma unroll
+  for (int nq = 0; nq < NQ; ++nq) {
+    ref[nq] = kNoRef;
+    l[nq] = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[nq][dt] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+
+  Blocks next{0, 0};
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i)
+    if (i < mine) issue(i, i, blocks_of(i));
+  if (STAGES - 1 < mine) next = blocks_of(STAGES - 1);
+  // the queries are there before the loop, which would otherwise wait for all that is on its way wherever they are used
+#pragma unroll
+  for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[nq][s]));
+  int stage = 0;
+  for (int i = 0; i < mine; ++i) {
+    const int key0 = base + 32 * (wave + kWaves * i);
+    if (i + STAGES - 1 < mine) {
+      issue(i + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1, next);
+      if (i + STAGES < mine) next = blocks_of(i + STAGES);
+      constexpr int N = S::LOADS * (STAGES - 1);
+      static_assert(N < 64, "vmcnt counts to 63");
+      __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+    } else {
+      __builtin_amdgcn_s_waitcnt(0x0F70);
+    }
+    asm volatile("" ::: "memory");
+    const unsigned char* const kt = ring + stage * S::STAGE;
+    const unsigned char* const vt = kt + S::TILE;
+    const bool masked = key0 < j.sure_lo || key0 + 32 > j.sure_hi;
+
+    // scores times the factor of their key, in powers of two; lane (row m, kg) has keys 16 h + 4 kg + r
+    float kfac[2][4], vfac[2][4];
+    if constexpr (F != kSame) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned ke = *reinterpret_cast<const unsigned*>(kt + 2 * S::TILE + 16 * h + 4 * kg);
+        const unsigned ve = *reinterpret_cast<const unsigned*>(kt + 2 * S::TILE + 32 + 16 * h + 4 * kg);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = key0 + 16 * h + 4 * kg + r;
+          const bool in = key >= j.lo && key < j.hi;              // what lies behind a sequence's keys has no exponent
+          kfac[h][r] = in ? power_of_two((signed char)(ke >> (8 * r))) * a.scale_log2e : 0.0f;
+          vfac[h][r] = in ? power_of_two((signed char)(ve >> (8 * r))) : 0.0f;
+        }
+      }
+    }
+    v4f sc[NQ][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int nq = 0; nq < NQ; ++nq) sc[nq][h] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int row = 16 * h + m;
+        v8 kf;
+        if constexpr (F == kSame) kf = *reinterpret_cast<const v8*>(kt + row * S::BYTES + (((4 * s + kg) ^ swizzle<S::BYTES>(row)) * 16));
+        else kf = decode8<T, F>(*reinterpret_cast<const v2u*>(kt + row * S::BYTES + (((2 * s + (kg >> 1)) ^ swizzle<S::BYTES>(row)) * 16) + 8 * (kg & 1)), 1.0f);
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq) sc[nq][h] = T::mma16(kf, qf[nq][s], sc[nq][h]);
+      }
+    }
+    v8 p[NQ];
+    unsigned seen[NQ];                                            // masked tiles: which of the lane's eight keys its row sees
+#pragma unroll
+    for (int nq = 0; nq < NQ; ++nq) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[nq][h][r] *= F == kSame ? a.scale_log2e : kfac[h][r];
+      seen[nq] = 255;
+      if (masked) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int key = key0 + 16 * h + 4 * kg + r;
+            if (key < max(row_lo[nq], j.lo) || key >= min(row_hi[nq], j.hi)) {
+              sc[nq][h][r] = -INFINITY;
+              seen[nq] &= ~(1u << (4 * h + r));
+            }
+          }
+      }
+      float mx = fmaxf(fmaxf(fmaxf(sc[nq][0][0], sc[nq][0][1]), fmaxf(sc[nq][0][2], sc[nq][0][3])),
+                       fmaxf(fmaxf(sc[nq][1][0], sc[nq][1][1]), fmaxf(sc[nq][1][2], sc[nq][1][3])));
+      if (__builtin_amdgcn_ballot_w64(!(mx <= ref[nq] + kSlack)) != 0) {
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float moved = fmaxf(ref[nq], mx);
+        const float alpha = __builtin_amdgcn_exp2f(ref[nq] - moved);
+        ref[nq] = moved;
+        l[nq] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[nq][dt][r] *= alpha;
+      }
+      // bf16 weights take the power of two of their value's row with them; those of fp16 could leave its range, and V takes it
+      unsigned w[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          float p0 = __builtin_amdgcn_exp2f(sc[nq][h][r] - ref[nq]), p1 = __builtin_amdgcn_exp2f(sc[nq][h][r + 1] - ref[nq]);
+          l[nq] += p0 + p1;
+          if constexpr (F != kSame && std::is_same<T, Brain>::value) {
+            p0 *= vfac[h][r];
+            p1 *= vfac[h][r + 1];
+          }
+          w[2 * h + r / 2] = T::pack(p0, p1);
+        }
+      p[nq] = __builtin_bit_cast(v8, (v4u{w[0], w[1], w[2], w[3]}));
+    }
+    v2h vpair[4];
+    if constexpr (F != kSame && std::is_same<T, Half>::value) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) vpair[2 * h + r / 2] = v2h{(_Float16)vfac[h][r], (_Float16)vfac[h][r + 1]};
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      v8 vf;
+      if constexpr (F == kSame) {
+        // 16 lanes hand in a block of 4 keys x 16 columns
+        const int a4 = (lane & 15) >> 2, b4 = lane & 3;
+        v4s half[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = 16 * h + 4 * kg + a4;
+          half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_v4s*)(vt + row * S::BYTES + (((2 * dt + (b4 >> 1)) ^ swizzle<S::BYTES>(row)) * 16) + 8 * (b4 & 1)));
+        }
+        const v8s both = {half[0][0], half[0][1], half[0][2], half[0][3], half[1][0], half[1][1], half[1][2], half[1][3]};
+        vf = __builtin_bit_cast(v8, both);
+      } else {
+        // 16 lanes hand in 8 keys x 16 columns, a pair of lanes a key
+        const int a8 = (lane & 15) >> 1;
+        const int row = 16 * (a8 >> 2) + 4 * kg + (a8 & 3);
+        const v2i w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i*)(vt + row * S::BYTES + ((dt ^ swizzle<S::BYTES>(row)) * 16) + 8 * (lane & 1)));
+        vf = decode8<T, F>(__builtin_bit_cast(v2u, w), 1.0f);
+        if constexpr (std::is_same<T, Half>::value) {
+          v4u pairs = __builtin_bit_cast(v4u, vf);
+#pragma unroll
+          for (int i2 = 0; i2 < 4; ++i2) {
+            const unsigned pair = pairs[i2];                      // (a bit cast of a vector's element itself takes the first element)
+            pairs[i2] = __builtin_bit_cast(unsigned, __builtin_bit_cast(v2h, pair) * vpair[i2]);
+          }
+          vf = __builtin_bit_cast(v8, pairs);
+        }
+      }
+      if (masked && j.n > 1) {
+        // A value that is not finite must not reach the rows that do not see it (0 x inf): it leaves the product, and makes NaN of
+        // the rows that do see it.
+        const unsigned bad = not_finite<T>(vf);
+        if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {
+          vf = zeros_at<T>(vf, bad);
+          const v8 flags = ones_at<T>(bad);
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq) {
+            const v4f hits = T::mma16(flags, ones_at<T>(seen[nq]), v4f{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (hits[r] > 0.0f) o[nq][dt][r] = __builtin_nanf("");
+          }
+        }
+      }
+#pragma unroll
+      for (int nq = 0; nq < NQ; ++nq) o[nq][dt] = T::mma16(vf, p[nq], o[nq][dt]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
+  }
+
+  // ---- the four waves meet, 16 rows at a time: O as [wave][tile][lane] in LDS, (ref, l) behind it
+  v4f* const so = reinterpret_cast<v4f*>(smem);
+  float* const sml = reinterpret_cast<float*>(smem + kWaves * DT * 64 * sizeof(v4f));   // [wave][row][2]
+#pragma unroll
+  for (int nq = 0; nq < NQ; ++nq) {
+    if (j.row0 + 16 * nq >= j.rows) break;
+    l[nq] += __shfl_xor(l[nq], 16);
+    l[nq] += __shfl_xor(l[nq], 32);
+    __syncthreads();
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) so[(wave * DT + dt) * 64 + lane] = o[nq][dt];
+    if (kg == 0) {
+      sml[(wave * 16 + m) * 2] = ref[nq];
+      sml[(wave * 16 + m) * 2 + 1] = l[nq];
+    }
+    __syncthreads();
+    const int q = tid & 15, row = j.row0 + 16 * nq + q;
+    if (row < j.rows) {
+      float top = kNoRef, sum = 0.0f, w[kWaves];
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) top = fmaxf(top, sml[(i * 16 + q) * 2]);
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) {
+        w[i] = __builtin_amdgcn_exp2f(sml[(i * 16 + q) * 2] - top);
+        sum += w[i] * sml[(i * 16 + q) * 2 + 1];
+      }
+      const Row r = row_of(a, j, kv_head, row);
+      const bool none = r.hi <= r.lo;
+      const float inv = none ? 0.0f : 1.0f / sum;
+      for (int g = tid >> 4; g < D / 4; g += kWaves * 4) {   // columns 4 g .. +3: tile g / 4, lane group g % 4
+        v4f acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+          const v4f v = so[(i * DT + (g >> 2)) * 64 + 16 * (g & 3) + q];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] += w[i] * v[e];
+        }
+        if (j.parts == 1) {
+          *reinterpret_cast<v2u*>((scalar*)a.o + r.at * D + 4 * g) = v2u{T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
+        } else {
+          *reinterpret_cast<v4f*>(a.part_o + (r.at * a.nparts + j.part) * D + 4 * g) = acc;
+        }
+      }
+      if (tid < 16) {
+        if (j.parts > 1) {
+          float* const ml = a.part_ml + 2 * (r.at * a.nparts + j.part);
+          ml[0] = top;
+          ml[1] = sum;
+        } else if (a.lse) {
+          a.lse[r.at] = none ? -INFINITY : log_sum(top, sum);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, KvFormat F, int D, int NQ>
+__global__ __launch_bounds__(kWaves * 64) void paged_narrow_kernel(AttnArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int kv_head = blockIdx.x % a.pages.heads, rest = blockIdx.x / a.pages.heads;
+  const int slot = rest / a.nparts, part = rest - slot * a.nparts;
+  Job j;
+  if (!find_job<16 * NQ>(a, slot, part, j)) return;
+  narrow_attention<T, F, D, NQ>(a, j, kv_head, smem);
+}
+
+// ---- wide -----------------------------------------------------------------------------
+
+constexpr int kWideRows = 32 * kWaves;
+
+template <int D>
+struct WideShape {
+  static constexpr int BYTES = 2 * D, TILE = 64 * BYTES;
+  static constexpr int ORS = BYTES + 16;                       // a padded row of the O tiles that the waves turn round at the end
+  static constexpr int RING = 4 * TILE;                        // two tiles of K, two of V
+  static constexpr int LDS = RING > kWaves * 32 * ORS ? RING : kWaves * 32 * ORS;
+};
+
+// V: the transposing read of a 32-lane pass covers 4 keys x 64 bytes, which these bring into four different groups of 64 bytes
+template <int D>
+__device__ __forceinline__ int v_swizzle(int row) {
+  if constexpr (D == 128) return 4 * (row & 3);
+  else if constexpr (D == 64) return 4 * ((row >> 1) & 1);
+  else return 0;                                               // rows of 192 and 64 bytes lie that way
+}
+
+template <typename T, KvFormat F, int D>
+__device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, int kv_head, unsigned char* smem) {
+  using S = WideShape<D>;
+  using v8 = typename T::v8;
+  using scalar = typename T::scalar;
+  constexpr int DS = D / 16, DT = D / 32, CH = S::BYTES / 16;
+  using lds_v4s = __attribute__((address_space(3))) v4s;
+  typedef short v8s __attribute__((ext_vector_type(8)));
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int jr = lane & 31, hh = lane >> 5;
+  unsigned char* const Kb = smem;
+  unsigned char* const Vb = smem + 2 * S::TILE;
+  const int base = j.lo & ~63;
+  const int ntiles = j.hi > j.lo ? (j.hi - base + 63) / 64 : 0;
+
+  // rows of this wave
+  const int wrow0 = j.row0 + 32 * wave;
+  const bool idle = wrow0 >= j.rows;
+  const int row = min(wrow0 + jr, j.rows - 1);
+  const Row r = row_of(a, j, kv_head, row);
+  int wave_lo, wave_hi, sure_lo, sure_hi;                      // keys that some, and that each, of the wave's rows see
+  {
+    const int t_lo = min(wrow0, j.rows - 1) / a.group, t_hi = (min(wrow0 + 32, j.rows) - 1) / a.group;
+    const long long p_lo = (long long)j.first + t_lo, p_hi = (long long)j.first + t_hi;
+    wave_hi = min(a.causal ? clamp_position(p_hi + 1, j.len) : j.len, j.hi);
+    sure_hi = min(a.causal ? clamp_position(p_lo + 1, j.len) : j.len, j.hi);
+    wave_lo = max(a.window > 0 ? clamp_position(p_lo - a.window + 1, j.len) : 0, j.lo);
+    sure_lo = max(a.window > 0 ? clamp_position(p_hi - a.window + 1, j.len) : 0, j.lo);
+  }
+  const int my_lo = max(r.lo, j.lo), my_hi = min(r.hi, j.hi);
+
+  v8 qf[DS];
+  {
+    const scalar* const q = query_of<T>(a, j, kv_head, row) + 8 * hh;
+#pragma unroll
+    for (int s = 0; s < DS; ++s) qf[s] = *reinterpret_cast<const v8*>(q + 16 * s);
+  }
+  asm volatile("" ::: "memory");
+
+  // ---- tiles into LDS: wave w brings the 16 keys from 16 w on, which lie in one page
+  constexpr int CP = D / 32;                                   // 1 KB copies of 16 rows of 16-bit elements
+  unsigned k_src[CP], v_src[CP];
+  if constexpr (F == kSame) {
+#pragma unroll
+    for (int i = 0; i < CP; ++i) {
+      const int p = 64 * i + lane, rw = p / CH, slot = p - rw * CH, in_tile = 16 * wave + rw;
+      k_src[i] = rw * S::BYTES + 16 * (slot ^ swizzle<S::BYTES>(in_tile));
+      v_src[i] = rw * S::BYTES + 16 * (slot ^ v_swizzle<D>(in_tile));
+    }
+  }
+  auto block_at = [&](int t) __attribute__((always_inline)) { return block_row(a, j.b, kv_head, base + 64 * t + 16 * wave, j.lo, j.hi); };
+  auto copy = [&](int t, int buf, long long at) __attribute__((always_inline)) {
+    const int key0 = base + 64 * t + 16 * wave;
+    const unsigned char* const kb = a.pages.k + (size_t)at * S::BYTES;
+    const unsigned char* const vb = a.pages.v + (size_t)at * S::BYTES;
+    unsigned char* const kd = Kb + buf * S::TILE + wave * (16 * S::BYTES);
+    unsigned char* const vd = Vb + buf * S::TILE + wave * (16 * S::BYTES);
+    if (key0 >= j.lo && key0 + 16 <= j.hi) {
+#pragma unroll
+      for (int i = 0; i < CP; ++i) {
+        lds_dma16(kb, k_src[i], kd + 1024 * i);
+        lds_dma16(vb, v_src[i], vd + 1024 * i);
+      }
+    } else {                                                   // rows outside [lo, hi) repeat the nearest key inside
+      const int inside = min(max(key0, j.lo & ~15), (j.hi - 1) & ~15);   // where `at` begins
+      const int least = max(j.lo - inside, 0), most = min(j.hi - 1 - inside, 15);
+#pragma unroll
+      for (int i = 0; i < CP; ++i) {
+        const int p = 64 * i + lane, rw = p / CH;
+        const int to = min(max(key0 + rw - inside, least), most);
+        const int move = (to - rw) * S::BYTES;
+        lds_dma16(kb, k_src[i] + move, kd + 1024 * i);
+        lds_dma16(vb, v_src[i] + move, vd + 1024 * i);
+      }
+    }
+  };
+  // 8 bits: 16 codes a lane through registers, written as 16-bit elements
+  constexpr int LD = (D + 63) / 64;                            // 16-byte pieces of a block of 16 rows, D of them, by 64 lanes
+  v4u kc[LD], vc[LD];
+  float ks[LD], vs[LD];
+  auto load = [&](int t, long long at) __attribute__((always_inline)) {
+    const int key0 = base + 64 * t + 16 * wave;
+    const int inside = min(max(key0, j.lo & ~15), (j.hi - 1) & ~15);
+    const int least = max(j.lo - inside, 0), most = min(j.hi - 1 - inside, 15);
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+      const int p = min(64 * i + lane, D - 1), rw = p / (D / 16), piece = p - rw * (D / 16);
+      const long long row_at = at + min(max(key0 + rw - inside, least), most);
+      kc[i] = *reinterpret_cast<const v4u*>(a.pages.k + (size_t)row_at * D + 16 * piece);
+      vc[i] = *reinterpret_cast<const v4u*>(a.pages.v + (size_t)row_at * D + 16 * piece);
+      ks[i] = power_of_two(a.pages.k_exps[row_at]);
+      vs[i] = power_of_two(a.pages.v_exps[row_at]);
+    }
+  };
+  auto store = [&](int buf) __attribute__((always_inline)) {
+    if constexpr (F != kSame) {
+#pragma unroll
+      for (int i = 0; i < LD; ++i) {
+        const int p = 64 * i + lane, rw = p / (D / 16), piece = p - rw * (D / 16), in_tile = 16 * wave + rw;
+        if (D % 64 == 0 || p < D) {
+          unsigned char* const kd = Kb + buf * S::TILE + in_tile * S::BYTES;
+          unsigned char* const vd = Vb + buf * S::TILE + in_tile * S::BYTES;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            *reinterpret_cast<v8*>(kd + 16 * ((2 * piece + c) ^ swizzle<S::BYTES>(in_tile))) = decode8<T, F>(v2u{kc[i][2 * c], kc[i][2 * c + 1]}, ks[i]);
+            *reinterpret_cast<v8*>(vd + 16 * ((2 * piece + c) ^ v_swizzle<D>(in_tile))) = decode8<T, F>(v2u{vc[i][2 * c], vc[i][2 * c + 1]}, vs[i]);
+          }
+        }
+      }
+    }
+  };
+
+  // ---- fragments: K row 32 h + jr, bytes [32 s + 16 hh, +16); V the block of 4 keys x 16 columns that 16 lanes hand in
+  unsigned k_off[DS], v_off[DT];
+#pragma unroll
+  for (int s = 0; s < DS; ++s) k_off[s] = jr * S::BYTES + (((2 * s + hh) ^ swizzle<S::BYTES>(jr)) * 16);
+  const int v_row = 4 * hh + ((lane & 15) >> 2);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) v_off[dt] = v_row * S::BYTES + (((4 * dt) ^ v_swizzle<D>(v_row)) * 16) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+  auto read_v = [&](const unsigned char* vt, int key, int dt) __attribute__((always_inline)) {   // keys key + 4 hh + .. and 8 more
+    const unsigned char* const p = vt + key * S::BYTES + v_off[dt];
+    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p));
+    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p + 8 * S::BYTES));
+    const v8s both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_bit_cast(v8, both);
+  };
+
+  v16f o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+  float ref = kNoRef, l = 0.0f;
+
+  auto compute = [&](int t, auto masked_c) __attribute__((always_inline)) {
+    constexpr bool masked = decltype(masked_c)::value;
+    const int key0 = base + 64 * t;
+    const unsigned char* const kt = Kb + (t & 1) * S::TILE;
+    const unsigned char* const vt = Vb + (t & 1) * S::TILE;
+    v16f sc[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[h][e] = 0.0f;
+#pragma unroll
+      for (int s = 0; s < DS; ++s) sc[h] = T::mma32(*reinterpret_cast<const v8*>(kt + 32 * h * S::BYTES + k_off[s]), qf[s], sc[h]);
+    }
+    unsigned seen = 0xffffffffu;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        sc[h][e] *= a.scale_log2e;
+        if constexpr (masked) {
+          const int key = key0 + 32 * h + 8 * (e >> 2) + 4 * hh + (e & 3);
+          if (key < my_lo || key >= my_hi) {
+            sc[h][e] = -INFINITY;
+            seen &= ~(1u << (16 * h + e));
+          }
+        }
+      }
+    float mx = sc[0][0];
+#pragma unroll
+    for (int e = 1; e < 32; ++e) mx = fmaxf(mx, sc[e >> 4][e & 15]);
+    if (__builtin_amdgcn_ballot_w64(!(mx <= ref + kSlack)) != 0) {
+      mx = max_with_other_half(mx);
+      const float moved = fmaxf(ref, mx);
+      const float alpha = __builtin_amdgcn_exp2f(ref - moved);
+      ref = moved;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+    }
+    v8 pf[2][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        v4u w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p0 = __builtin_amdgcn_exp2f(sc[h][8 * s + 2 * i] - ref), p1 = __builtin_amdgcn_exp2f(sc[h][8 * s + 2 * i + 1] - ref);
+          l += p0 + p1;
+          w[i] = T::pack(p0, p1);
+        }
+        pf[h][s] = __builtin_bit_cast(v8, w);
+      }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          v8 vf = read_v(vt, 32 * h + 16 * s, dt);
+          if constexpr (masked) {                              // see the narrow kernel
+            const unsigned bad = not_finite<T>(vf);
+            if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {
+              vf = zeros_at<T>(vf, bad);
+              v16f hits;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) hits[e] = 0.0f;
+              hits = T::mma32(ones_at<T>(bad), ones_at<T>(seen >> (16 * h + 8 * s)), hits);
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (hits[e] > 0.0f) o[dt][e] = __builtin_nanf("");
+            }
+          }
+          o[dt] = T::mma32(vf, pf[h][s], o[dt]);
+        }
+  };
+
+  long long at = 0;
+  if (ntiles > 0) {
+    at = block_at(0);
+    if constexpr (F == kSame) copy(0, 0, at);
+    else load(0, at);
+    if (ntiles > 1) at = block_at(1);
+  }
+  for (int t = 0; t < ntiles; ++t) {
+    if constexpr (F == kSame) {
+      __builtin_amdgcn_s_waitcnt(0x0F70);                      // vmcnt(0): this wave's copies of tile t
+      __syncthreads();
+      if (t + 1 < ntiles) copy(t + 1, (t + 1) & 1, at);
+    } else {
+      store(t & 1);
+      __syncthreads();
+      if (t + 1 < ntiles) load(t + 1, at);
+    }
+    if (t + 2 < ntiles) at = block_at(t + 2);
+    const int key0 = base + 64 * t;
+    if (!idle && key0 < wave_hi && key0 + 64 > wave_lo) {
+      if (key0 < sure_lo || key0 + 64 > sure_hi) compute(t, std::true_type{});
+      else compute(t, std::false_type{});
+    }
+  }
+  __syncthreads();
+  l += __shfl_xor(l, 32);
+  if (j.parts > 1) {
+    if (wrow0 + jr < j.rows) {
+      float* const po = a.part_o + (r.at * a.nparts + j.part) * D;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<v4f*>(po + 32 * dt + 8 * g + 4 * hh) = v4f{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+      if (hh == 0) {
+        float* const ml = a.part_ml + 2 * (r.at * a.nparts + j.part);
+        ml[0] = ref;
+        ml[1] = l;
+      }
+    }
+    return;
+  }
+  if (idle) return;
+  // the wave turns its 32 x D tile round through LDS and stores whole rows
+  const bool none = r.hi <= r.lo;
+  const float inv = none ? 0.0f : 1.0f / l;
+  unsigned char* const ot = smem + wave * (32 * S::ORS);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<v2u*>(ot + jr * S::ORS + 2 * (32 * dt + 8 * g + 4 * hh)) =
+          v2u{T::pack(o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv), T::pack(o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv)};
+  if (a.lse && hh == 0 && wrow0 + jr < j.rows) a.lse[r.at] = none ? -INFINITY : log_sum(ref, l);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  for (int idx = lane; idx < 32 * CH; idx += 64) {
+    const int rw = idx / CH, c = idx - rw * CH;
+    if (wrow0 + rw >= j.rows) break;
+    const Row to = row_of(a, j, kv_head, wrow0 + rw);
+    *reinterpret_cast<v4u*>((unsigned char*)a.o + to.at * S::BYTES + 16 * c) = *reinterpret_cast<const v4u*>(ot + rw * S::ORS + 16 * c);
+  }
+}
+
+template <typename T, KvFormat F, int D>
+__global__ __launch_bounds__(kWaves * 64, 2) void paged_wide_kernel(AttnArgs a, int slots) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  // the head goes fastest, so that the row blocks of a head meet on the XCDs that have its keys; the last rows, with the most keys
+  // under a causal mask, go first
+  const int kv_head = blockIdx.x % a.pages.heads, rest = blockIdx.x / a.pages.heads;
+  const int slot = slots - 1 - rest / a.nparts, part = rest % a.nparts;
+  Job j;
+  if (!find_job<kWideRows>(a, slot, part, j)) return;
+  wide_attention<T, F, D>(a, j, kv_head, smem);
+}
+
+// ---- parts ------------------------------------------------------------------------------
+
+// m = max m_p, l = sum l_p 2^(m_p - m), O = sum O_p 2^(m_p - m) / l over the parts of a row; D / 4 lanes a row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a) {
+  constexpr int L = D / 4;
+  const long long at = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
+  const int c = threadIdx.x % L;
+  const long long rows = (long long)a.batch.tokens * a.heads;
+  const int token = (int)(min(at, rows - 1) / a.heads);
+  const int first_token = __builtin_amdgcn_readfirstlane(token);
+  int b = count_at_most(a.batch.sequences, first_token, [&](int i) { return a.batch.starts[i + 1]; });
+  while (b < a.batch.sequences && a.batch.starts[b + 1] <= token) ++b;
+  if (at >= rows || threadIdx.x / L >= 256 / L || b >= a.batch.sequences) return;
+  const int start = min(max(a.batch.starts[b], 0), a.batch.tokens), end = min(max(a.batch.starts[b + 1], start), a.batch.tokens);
+  if (token < start || token >= end) return;
+  const int len_all = max(a.batch.lens[b], 0), first = len_all - (end - start);
+  const int len = min(len_all, kv_capacity(a.batch, a.pages.page_shift));
+  const int parts = seq_parts(a, first, len);
+  if (parts == 1) return;                                      // written already
+  const float* const ml = a.part_ml + 2 * at * a.nparts;
+  float top = kNoRef;
+  for (int p = 0; p < parts; ++p) top = fmaxf(top, ml[2 * p]);
+  float sum = 0.0f;
+  v4f acc = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < parts; ++p) {
+    const float w = __builtin_amdgcn_exp2f(ml[2 * p] - top), lp = ml[2 * p + 1];
+    const v4f v = *reinterpret_cast<const v4f*>(a.part_o + (at * a.nparts + p) * D + 4 * c);
+    sum += w * lp;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += w * v[e];
+  }
+  const long long position = (long long)first + (token - start);
+  const int hi = a.causal ? clamp_position(position + 1, len) : len, lo = a.window > 0 ? clamp_position(position - a.window + 1, len) : 0;
+  const bool none = hi <= lo;
+  const float inv = none ? 0.0f : 1.0f / sum;
+  *reinterpret_cast<v2u*>((typename T::scalar*)a.o + at * D + 4 * c) = v2u{T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
+  if (a.lse && c == 0) a.lse[at] = none ? -INFINITY : log_sum(top, sum);
+}
+
+// ---- host side ----------------------------------------------------------------------------
+
+// How a call is cut.
+struct Plan {
+  bool narrow;
+  int nq;                  // narrow: blocks of 16 rows
+  int slots, slots_per_seq;
+  int nparts, part_keys;
+};
+
+static size_t workspace_of(long long rows, int D, int nparts) { return nparts > 1 ? (size_t)rows * nparts * (D + 2) * 4 : 0; }
+
+static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, int heads, int max_queries, int max_keys, int cus, size_t room) {
+  const int D = pages.head_size, group = heads / pages.heads;
+  Plan p;
+  const long long most = max_queries > 0 ? std::min(max_queries, b.tokens) : b.tokens;   // new tokens of a sequence
+  const long long most_rows = most * group;
+  p.narrow = most_rows <= 64;
+  p.nq = most_rows <= 16 ? 1 : most_rows <= 32 ? 2 : 4;
+  const int R = p.narrow ? 16 * p.nq : kWideRows;
+  const long long per_seq = (most_rows + R - 1) / R, packed = (long long)b.tokens * group / R + b.sequences;
+  p.slots_per_seq = b.sequences * per_seq <= packed ? (int)per_seq : 0;
+  p.slots = (int)std::min<long long>(p.slots_per_seq ? b.sequences * per_seq : packed, INT_MAX);
+  const long long capacity = (long long)b.width << page_shift;
+  const int keys = (int)std::min<long long>(max_keys > 0 ? std::min<long long>(max_keys, capacity) : capacity, INT_MAX - 1024);
+  const long long units = (long long)p.slots * pages.heads;
+  const long long target = 4LL * cus;
+  const int least = p.narrow ? 256 : 512;                       // keys of a part
+  long long n = std::max<long long>(1, std::min<long long>(target / std::max<long long>(units, 1), keys / least));
+  for (;; --n) {
+    p.part_keys = (int)(((keys + n - 1) / n + 127) / 128 * 128);
+    p.nparts = std::max(1, (keys + p.part_keys - 1) / p.part_keys);
+    if (n == 1 || workspace_of((long long)b.tokens * heads, D, p.nparts) <= room) return p;
+  }
+}
+
+static int check_attention(const char* who, int heads, const ftk_kv_pages* pages) {
+  if (heads <= 0 || heads % pages->heads) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: query heads must be a multiple of the kv heads, got %d and %d", who, heads, pages->heads);
+  return FTK_OK;
+}
+
+template <typename K, typename... Args>
+static int launch_with_lds(const char* name, K kernel, DeviceOnce& once, long long blocks, int lds, hipStream_t s, Args... args) {
+  if (blocks > INT_MAX) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "ftk_paged_attn: grid too large");
+  unsigned bit;
+  if (once.pending(&bit)) {
+    FTK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    once.done(bit);
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kWaves * 64), lds, s, args...);
+  return check_launch(name);
+}
+
+}  // namespace ftk
+
+extern "C" {
+
+size_t ftk_paged_attn_workspace_bytes(const ftk_kv_pages* pages, const ftk_kv_batch* batch, int heads, int max_queries, int max_keys) {
+  using namespace ftk;
+  const DeviceProps* d = nullptr;
+  if (!pages || !batch || pages->heads <= 0 || heads <= 0 || heads % pages->heads || batch->tokens <= 0 || batch->sequences <= 0 || batch->table_width <= 0 ||
+      pages->page_size <= 0 || device_props(&d))
+    return 0;
+  KvBatch b{};
+  b.tokens = batch->tokens;
+  b.sequences = batch->sequences;
+  b.width = batch->table_width;
+  const Plan p = plan(*pages, b, __builtin_ctz((unsigned)pages->page_size), heads, max_queries, max_keys, d->cus, SIZE_MAX);
+  return workspace_of((long long)b.tokens * heads, pages->head_size, p.nparts);
+}
+
+int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long q_head_stride, const ftk_kv_pages* pages, const ftk_kv_batch* batch,
+                   void* o, float* lse, int heads, float scale, int causal, int window, int max_queries, int max_keys, void* workspace,
+                   size_t workspace_bytes, ftk_stream_t stream) {
+  using namespace ftk;
+  const char* who = "ftk_paged_attn";
+  AttnArgs a;
+  int rc = check_kv_pages(who, pages, &a.pages);
+  if (rc || (rc = check_kv_batch(who, batch, &a.batch)) || (rc = check_attention(who, heads, pages))) return rc;
+  if (type != FTK_F16 && type != FTK_BF16) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: queries must be fp16 or bf16", who);
+  if ((pages->type == FTK_F16 || pages->type == FTK_BF16) && pages->type != type) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: pages of 16 bits must have the type of the queries", who);
+  if (!(scale > 0.0f) || scale > 3.0e38f) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: scale must be positive and finite", who);
+  if (window < 0 || max_queries < 0 || max_keys < 0) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: window, max_queries and max_keys must not be negative", who);
+  if (a.batch.tokens == 0) return FTK_OK;
+  if (!q || !o || !aligned16(q) || !aligned16(o)) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: q and o must be non-NULL and 16-byte aligned", who);
+  if ((uintptr_t)lse & 3) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: lse must be 4-byte aligned", who);
+  if (q_token_stride < 0 || q_head_stride < 0 || q_token_stride % 8 || q_head_stride % 8) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: strides must be multiples of 8 elements", who);
+  if ((long long)a.batch.tokens * (heads / pages->heads) > INT_MAX / 2) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: too many rows", who);
+  const DeviceProps* d = nullptr;
+  if ((rc = device_props(&d))) return rc;
+  if (workspace && !aligned16(workspace)) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", who);
+  const Plan p = plan(*pages, a.batch, a.pages.page_shift, heads, max_queries, max_keys, d->cus, workspace ? workspace_bytes : 0);
+  a.q = q;
+  a.o = o;
+  a.lse = lse;
+  a.q_token = q_token_stride;
+  a.q_head = q_head_stride;
+  a.heads = heads;
+  a.group = heads / pages->heads;
+  a.scale_log2e = scale * 1.4426950408889634f;
+  a.causal = causal != 0;
+  a.window = window;
+  a.slots_per_seq = p.slots_per_seq;
+  a.nparts = p.nparts;
+  a.part_keys = p.part_keys;
+  const long long rows = (long long)a.batch.tokens * heads;
+  a.part_o = (float*)workspace;
+  a.part_ml = a.part_o + (size_t)rows * p.nparts * pages->head_size;
+  const long long blocks = (long long)p.slots * pages->heads * p.nparts;
+  const hipStream_t s = (hipStream_t)stream;
+  return with_kv_types(type, pages->type, pages->head_size, [&](auto t, auto f, auto dc) -> int {
+    using T = decltype(t);
+    constexpr KvFormat F = decltype(f)::value;
+    constexpr int D = decltype(dc)::value;
+    int bad;
+    if (p.narrow) {
+      auto launch = [&](auto nq) -> int {
+        constexpr int NQ = decltype(nq)::value;
+        static DeviceOnce once;
+        return launch_with_lds("paged_narrow_kernel", paged_narrow_kernel<T, F, D, NQ>, once, blocks, NarrowShape<F, D>::LDS, s, a);
+      };
+      bad = p.nq == 1 ? launch(std::integral_constant<int, 1>{}) : p.nq == 2 ? launch(std::integral_constant<int, 2>{}) : launch(std::integral_constant<int, 4>{});
+    } else {
+      static DeviceOnce once;
+      bad = launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D>, once, blocks, WideShape<D>::LDS, s, a, p.slots);
+    }
+    if (bad || p.nparts == 1) return bad;
+    constexpr int RPB = 256 / (D / 4);
+    const long long mblocks = (rows + RPB - 1) / RPB;
+    if (mblocks > INT_MAX) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: grid too large", who);
+    hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3((unsigned)mblocks), dim3(256), 0, s, a);
+    return check_launch("paged_merge_kernel");
+  });
+}
+
+}  // extern "C"

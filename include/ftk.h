@@ -579,6 +579,163 @@ int ftk_windowed_attn_f32(const float* Q, const float* K, const float* V,
 int ftk_online_softmax_f32(const float* x, float* y, int rows, int cols,
                            ftk_stream_t stream);
 
+/* ------------------------------------------- serving on a paged cache -- */
+
+/*
+ * The entry points below have no counterpart in the reference, whose attention
+ * reads dense keys and values (examples/flash_attention/flash_attention.py:14-91).
+ *
+ * Element types of the arguments called `type`.
+ */
+#define FTK_F16 0
+#define FTK_BF16 1
+#define FTK_E4M3 2 /* pages only: 8-bit floats of 4 exponent and 3 fraction bits, no infinities */
+#define FTK_INT8 3 /* pages only */
+#define FTK_F32 4
+
+/*
+ * A cache of keys and values in pages: k and v [pages, heads, page_size,
+ * head_size] of `type`, 16-byte aligned.  page_size is a power of two from 16 to
+ * 1024, head_size 32, 64, 96 or 128.  A cache of 8 bits has an exponent for each
+ * row, k_exps and v_exps [pages, heads, page_size], signed bytes: element = code *
+ * 2^exponent.  For 16 bits both are NULL.
+ */
+typedef struct ftk_kv_pages {
+  void* k;
+  void* v;
+  void* k_exps;
+  void* v_exps;
+  int type;
+  int pages;
+  int heads;
+  int page_size;
+  int head_size;
+} ftk_kv_pages;
+
+/*
+ * A batch of sequences with new tokens, int32 arrays on the device.  The new
+ * tokens of sequence b are the packed rows starts[b] .. starts[b + 1] - 1
+ * (starts [sequences + 1], not decreasing); lens[b] is its length with them, so
+ * that they are its last positions.  Position p lies in row p % page_size of page
+ * table[b, p / page_size] (table [sequences, table_width]).  `tokens` is how many
+ * rows the packed arrays have; rows from starts[sequences] on are nobody's: they are
+ * neither read nor written.  A sequence may have no new tokens, or no length;
+ * without sequences or tokens a call does nothing.
+ *
+ * What the arrays hold is looked at on the device, where it cannot be refused:
+ * nothing is read or written outside the pages, the table and the packed rows
+ * whatever they say.  Positions below 0 (more new tokens than the length) and
+ * past the table, and pages outside [0, pages), are not written; they are read as
+ * zeros by ftk_kv_cache_read, and in attention the former hold no keys, while for
+ * the latter the nearest page is read.
+ */
+typedef struct ftk_kv_batch {
+  const int* table;
+  const int* lens;
+  const int* starts;
+  int sequences;
+  int table_width;
+  int tokens;
+} ftk_kv_batch;
+
+/*
+ * Writes the keys and values of the new tokens into their pages.  keys, values:
+ * fp16 or bf16 (`type`), element (token, head, i) at token * token_stride + head *
+ * head_stride + i, strides in elements and multiples of 8, both 16-byte aligned.
+ * Pages of 16 bits have the same type.  Into pages of 8 bits a row goes under the
+ * least power of two 2^e that keeps its largest magnitude within the largest code
+ * (448 e4m3, 127 int8): code = x / 2^e rounded to the nearest code, ties to even.
+ * e is at least -15 (e4m3) or -24 (int8) from fp16, so that no finite value gets
+ * a coarser grid than fp16's own finest, and at least -100 from bf16.  Every code
+ * * 2^e is a value of the input's type: magnitudes above 61440 (e4m3) or 65024
+ * (int8) from fp16, 1.875 * 2^127 or 127 * 2^121 from bf16, infinities included,
+ * become that value.  A NaN is NaN in e4m3 and 0 in int8, and does not count for
+ * its row's e.  The results do not depend on anything but the row.  A page of
+ * positions that are written belongs to one place of the table: with two, which of
+ * two tokens a row ends up with is open.
+ */
+int ftk_kv_cache_write(const void* keys, const void* values, int type,
+                       long long key_token_stride, long long key_head_stride,
+                       long long value_token_stride, long long value_head_stride,
+                       const ftk_kv_pages* pages, const ftk_kv_batch* batch,
+                       ftk_stream_t stream);
+
+/*
+ * Reads the last starts[b + 1] - starts[b] positions of every sequence back into
+ * dense rows: keys, values [tokens, heads, head_size], 16-byte aligned, fp16, bf16
+ * or fp32 (`type`; pages of 16 bits: their type or fp32).  code * 2^e, rounded once
+ * to `type` (exact in fp32 and in the type it was written from).
+ */
+int ftk_kv_cache_read(const ftk_kv_pages* pages, const ftk_kv_batch* batch,
+                      int type, void* keys, void* values, ftk_stream_t stream);
+
+/*
+ * Attention of the new tokens over the cache, which holds their own keys and
+ * values already.  q: fp16 or bf16 (`type`; that of 16-bit pages), element (token,
+ * head, i) at token * q_token_stride + head * q_head_stride + i, strides in elements and
+ * multiples of 8, 16-byte aligned; `heads` is a multiple of pages->heads, and query
+ * head h reads head h / (heads / pages->heads) of the cache.  The token at position
+ * p sees the positions k < lens[b] with k <= p (causal != 0) and k > p - window
+ * (window > 0).  Into o [tokens, heads, head_size], of q's type and 16-byte
+ * aligned:
+ *   o = sum_k w_k v_k / sum_k w_k,  w_k = exp(scale * q . k_k),  scale > 0,
+ * and into lse [tokens, heads] fp32, if not NULL, log sum_k w_k.  A token without
+ * positions to see gets zeros and -inf.  Keys and values that a token does not
+ * see never matter to it, NaN and infinities included; one that is not finite
+ * makes NaN of what sees it (a component of o for a value, all of it for a key).
+ * fp32 accumulation; the one rounding on the way is that of the weights to the 16
+ * bits of `type`.  Head sizes, pages and tokens in any mixture run on two kernels:
+ * sequences of at most 64 rows (new tokens times heads / pages->heads) on one that
+ * reads the cache once, larger ones on one made for the matrix unit.
+ *
+ * max_queries, max_keys: promises that no sequence has more new tokens, or is
+ * longer (0: no promise).  They decide which kernel runs and how the keys are
+ * cut over workgroups; tokens beyond max_queries may be left out, keys beyond
+ * max_keys are not.  The workspace (16-byte aligned) holds the results of parts of
+ * the keys until a second launch joins them; with NULL or less than
+ * ftk_paged_attn_workspace_bytes the keys are cut less, or not at all, which
+ * costs time, and the last bits of the results may differ.  Calls that may run at
+ * the same time need workspaces of their own.
+ */
+size_t ftk_paged_attn_workspace_bytes(const ftk_kv_pages* pages,
+                                      const ftk_kv_batch* batch, int heads,
+                                      int max_queries, int max_keys);
+int ftk_paged_attn(const void* q, int type, long long q_token_stride,
+                   long long q_head_stride, const ftk_kv_pages* pages,
+                   const ftk_kv_batch* batch, void* o, float* lse, int heads,
+                   float scale, int causal, int window, int max_queries,
+                   int max_keys, void* workspace, size_t workspace_bytes,
+                   ftk_stream_t stream);
+
+/*
+ * Verifies drafted tokens against a target model.  target [sequences, drafted + 1,
+ * vocabulary]: its probabilities before each drafted token and behind the last;
+ * draft [sequences, drafted, vocabulary]: those the tokens were drawn from, of the
+ * same type (fp32, fp16, bf16), or NULL for drafts that were not drawn at random
+ * (probability 1); drafts [sequences, drafted] int32 or int64; uniform numbers of
+ * [0, 1) accept_uniforms [sequences, drafted] and sample_uniforms [sequences];
+ * draft_lens [sequences] or NULL: how many of a sequence's drafts there are.  Draft i
+ * is accepted if those before it are and accept_uniforms[i] * draft[i, token] <
+ * target[i, token].  The next token is the least t with sum_{k <= t} w_k > u *
+ * sum_k w_k, u the sequence's sample uniform and w = max(target[i] - draft[i], 0) for
+ * the first rejected i, or target[i] where these are all zero, and behind the last
+ * draft.  Comparisons of single probabilities are exact, sums in 64 bits in a fixed
+ * order.  NaN and negative weights count as zero; where no weight is positive the
+ * token is -1.  A drafted id outside [0, vocabulary) is rejected.
+ * tokens [sequences, drafted + 1], of drafts' type: the accepted drafts, the next token,
+ * then -1; accepted [sequences]: how many were.  drafted is 0 to 63 (0: one token is
+ * drawn from each row).  workspace: 8-byte aligned,
+ * ftk_verify_drafts_workspace_bytes(sequences, vocabulary) bytes.
+ */
+size_t ftk_verify_drafts_workspace_bytes(int sequences, int vocabulary);
+int ftk_verify_drafts(const void* target, const void* draft, int type,
+                      const void* drafts, int drafts_are_64bit,
+                      const float* accept_uniforms, const float* sample_uniforms,
+                      const int* draft_lens, void* tokens, int* accepted,
+                      int sequences, int drafted, int vocabulary,
+                      void* workspace, size_t workspace_bytes,
+                      ftk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

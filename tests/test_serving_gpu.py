@@ -1,0 +1,575 @@
+"""The serving kernels against their definitions in 64 bits: writing to and reading from a paged cache, attention over it, verification of drafts,
+and a run of them together."""
+import math
+
+import pytest
+import torch
+
+import serving_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, F32, E4M3, I8 = torch.float16, torch.bfloat16, torch.float32, torch.float8_e4m3fn, torch.int8
+
+
+@pytest.fixture(scope='module')
+def core():
+    import fractaltensor_amd._core as c
+    return c
+
+
+def _cuda(tensors):
+    return [None if t is None else t.cuda() for t in tensors]
+
+
+def _junk(pages):
+    """Fills pages and exponents with what must never matter."""
+    for t in pages:
+        if t is not None:
+            t.view(torch.uint8).fill_(0x7f)                      # NaN in e4m3 and fp16; 2^127 as an exponent
+    return pages
+
+
+def _same(a, b):
+    return torch.equal(a.cpu().view(torch.uint8), b.cpu().view(torch.uint8))
+
+
+# ---- writing and reading -----------------------------------------------------------------
+
+def _rows(kind, n, heads, D, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((n, heads, D), generator=g)
+    if kind == 'edges':                                          # rows whose largest is at, just above and just below a change of the exponent; ties; ends of the range
+        tops = [127.0, 127.25, 126.75, 448.0, 450.0, 446.0, 1.0, 0.0, 2.0 ** -24, 2.0 ** -16, 1e-5, 65504.0, 61440.0, 65024.0, 30000.0, 3e38, 1e-38, 1e-41]
+        x = torch.round(x * 8) / 2
+        for i in range(n):
+            for h in range(heads):
+                top = tops[(i * heads + h) % len(tops)]
+                if dtype == F16:
+                    top = min(top, 65504.0)
+                x[i, h] = x[i, h] / 32 * top
+                x[i, h, (i + h) % D] = top
+    elif kind == 'odd':                                          # infinities and NaN among others
+        x[0, 0, 0] = math.inf
+        x[n // 2, heads - 1, D - 1] = -math.inf
+        x[n - 1, 0, D // 2] = math.nan
+        x[n // 3, 0] = math.nan
+        x[n // 4, heads - 1] = math.inf
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize('kind', ['normal', 'edges', 'odd'])
+@pytest.mark.parametrize('dtype,cache,D,page,heads', [
+    (F16, E4M3, 128, 16, 2), (F16, I8, 64, 32, 3), (BF16, E4M3, 32, 64, 1), (BF16, I8, 96, 16, 2), (F16, I8, 128, 256, 1), (BF16, E4M3, 96, 1024, 5),
+    (F16, None, 96, 16, 3), (BF16, None, 32, 128, 2),
+])
+def test_written_rows_are_the_nearest_codes(core, kind, dtype, cache, D, page, heads):
+    new, lens = [3, 0, 17, 1, 5], [3, 40, 50, 300, 2]            # the last has three new tokens without a position
+    batch = ref.make_batch(new, lens, page, 1, tail=2)
+    keys, values = _rows(kind, batch['tokens'], heads, D, dtype, 2), _rows(kind, batch['tokens'], heads, D, dtype, 3)
+    pages = ref.make_pages(batch, heads, D, cache, dtype, 4)
+    want = [None if t is None else t.clone() for t in pages]
+    for x, p, e in ((keys, want[0], want[2]), (values, want[1], want[3])):
+        for b in range(len(lens)):
+            for row, at, r in ref.places(batch, b):
+                for h in range(heads):
+                    if cache is None:
+                        p[at, h, r] = x[row, h]
+                    else:
+                        codes, exponent = ref.quantise_row(x[row, h].double(), dtype, cache)
+                        p[at, h, r] = torch.tensor(codes, dtype=torch.float64).to(cache)
+                        e[at, h, r] = exponent
+    pages = _cuda(pages)
+    core.kv_cache_write(keys.cuda(), values.cuda(), *pages[:2], *ref.on_device(batch), *pages[2:])
+    for got, expected in zip(pages, want):
+        if got is None:
+            continue
+        if cache == E4M3 and got.dtype == E4M3 and kind == 'odd':   # a NaN has two codes
+            assert torch.equal(torch.nan_to_num(got.cpu().float(), nan=-1e9), torch.nan_to_num(expected.float(), nan=-1e9))
+        else:
+            assert _same(got, expected)
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16, F32])
+@pytest.mark.parametrize('cache,D,page,heads,came_from', [(E4M3, 128, 16, 2, F16), (I8, 64, 32, 3, F16), (E4M3, 32, 64, 1, F16), (I8, 96, 256, 2, F16), (None, 128, 32, 2, F16),
+                                                        (None, 96, 16, 3, BF16)])
+def test_read_rows_are_what_the_codes_stand_for(core, dtype, cache, D, page, heads, came_from):
+    if cache is None and dtype not in (came_from, F32):
+        pytest.skip('pages of 16 bits are read in their type or in fp32')
+    new, lens = [7, 0, 64, 1, 5], [7, 40, 64, 300, 2]
+    batch = ref.make_batch(new, lens, page, 5, tail=3)
+    pages = ref.make_pages(batch, heads, D, cache, came_from, 6)
+    want = [ref.held(pages[0], pages[2]).to(dtype), ref.held(pages[1], pages[3]).to(dtype)]
+    pages = _cuda(pages)
+    out = [torch.full((batch['tokens'], heads, D), 7.0, dtype=dtype, device='cuda') for _ in range(2)]
+    got = core.kv_cache_read(*pages[:2], *ref.on_device(batch), batch['tokens'], dtype, *pages[2:], out=tuple(out))
+    assert got[0].data_ptr() == out[0].data_ptr()
+    for x, w in zip(got, want):
+        expected = torch.full((batch['tokens'], heads, D), 7.0, dtype=dtype)
+        expected[:batch['starts'][-1]] = 0.0                      # positions below zero are read as zeros
+        for b in range(len(lens)):
+            for row, at, r in ref.places(batch, b):
+                expected[row] = w[at, :, r]
+        assert torch.equal(x.cpu(), expected)
+
+
+def test_rows_of_a_joint_projection_are_written_in_place(core):
+    """Views of one [tokens, query + key + value heads, D] product, and of one with the heads outermost."""
+    heads, D, page = 2, 64, 16
+    batch = ref.make_batch([5, 9], [20, 9], page, 7)
+    joint = torch.randn((batch['tokens'], 4 + 2 * heads, D), generator=torch.Generator().manual_seed(8)).to(BF16).cuda()
+    for k, v in ((joint[:, 4:6], joint[:, 6:8]), (joint.permute(1, 0, 2).contiguous().permute(1, 0, 2)[:, 4:6], joint[:, 6:8])):
+        first, second = (_cuda(ref.make_pages(batch, heads, D, I8, BF16, 9)) for _ in range(2))
+        core.kv_cache_write(k, v, *first[:2], *ref.on_device(batch), *first[2:])
+        core.kv_cache_write(k.contiguous(), v.contiguous(), *second[:2], *ref.on_device(batch), *second[2:])
+        assert all(_same(a, b) for a, b in zip(first, second))
+
+
+def test_a_large_cache_is_written_and_read_past_32_bits(core):
+    """Pages of 5 GB: the last ones."""
+    heads, D, page = 4, 128, 64
+    n = 5 * (1 << 30) // (heads * D * page) + 3
+    pages = [torch.empty((n, heads, page, D), dtype=I8, device='cuda') for _ in range(2)]
+    exps = [torch.empty((n, heads, page), dtype=I8, device='cuda') for _ in range(2)]
+    table = torch.tensor([[n - 1, 0, n - 2]], dtype=torch.int32, device='cuda')
+    lens, starts = torch.tensor([150], dtype=torch.int32, device='cuda'), torch.tensor([0, 150], dtype=torch.int32, device='cuda')
+    g = torch.Generator(device='cuda').manual_seed(10)
+    keys, values, q = (torch.randn((150, h, D), generator=g, device='cuda').to(BF16) for h in (heads, heads, 8))
+    core.kv_cache_write(keys, values, *pages, table, lens, starts, *exps)
+    k, v = core.kv_cache_read(*pages, table, lens, starts, 150, F32, *exps)
+    for got, x in ((k, keys.float()), (v, values.float())):
+        step = 2.0 ** torch.ceil(torch.log2(x.abs().amax(-1, keepdim=True) / 127))
+        assert bool(((got - x).abs() <= step / 2).all())
+    small_table = torch.arange(3, dtype=torch.int32, device='cuda')[None]
+    small = [t[torch.tensor([n - 1, 0, n - 2], device='cuda')].contiguous() for t in (*pages, *exps)]
+    for hint in (0, 150):                                          # and both kernels of attention
+        got = core.paged_attention(q, *pages, table, lens, starts, *exps, max_queries=hint)
+        assert torch.equal(got, core.paged_attention(q, *small[:2], small_table, lens, starts, *small[2:], max_queries=hint))
+    one = torch.tensor([0, 1], dtype=torch.int32, device='cuda')
+    assert torch.equal(core.paged_attention(q[:1].contiguous(), *pages, table, lens, one, *exps, max_queries=1),
+                       core.paged_attention(q[:1].contiguous(), *small[:2], small_table, lens, one, *small[2:], max_queries=1))
+
+
+# ---- attention --------------------------------------------------------------------------
+
+def _attention_case(core, dtype, cache, D, page, heads, G, new, lens, seed, causal=True, window=0, hints=True, scale=None, tail=0, junk=True, workspace=None, pages=None):
+    batch = ref.make_batch(new, lens, page, seed, tail=tail)
+    if pages is None:
+        pages = ref.make_pages(batch, heads, D, cache, dtype, seed + 1)
+    if junk:                                                       # what no position of a sequence holds must not matter
+        used = torch.zeros(pages[0].shape[:3], dtype=torch.bool)
+        for b, n in enumerate(lens):
+            for p in range(min(n, len(batch['table'][b]) * page)):
+                used[batch['table'][b][p // page], :, p % page] = True
+        for t in pages[:2]:
+            t.view(torch.uint8).view(*used.shape, -1)[~used] = 0x7f
+        for t in pages[2:]:
+            if t is not None:
+                t[~used] = 127
+    q = torch.randn((batch['tokens'], heads * G, D), generator=torch.Generator().manual_seed(seed + 2)).to(dtype)
+    scale = D ** -0.5 if scale is None else scale
+    want = ref.attention(q, ref.held(pages[0], pages[2]), ref.held(pages[1], pages[3]), batch, heads, scale, causal, window)
+    dev = _cuda(pages)
+    out = torch.full(q.shape, 7.0, dtype=dtype, device='cuda')
+    lse = torch.full(q.shape[:2], 7.0, device='cuda')
+    core.paged_attention(q.cuda(), *dev[:2], *ref.on_device(batch), *dev[2:], scale=scale, causal=causal, window=window, max_queries=max(new) if hints else 0,
+                         max_keys=max(lens) if hints else 0, out=out, return_lse=lse, workspace=workspace)
+    bo, bl = ref.attention_bounds(want, dtype, D)
+    got, got_lse = out.cpu().double(), lse.cpu().double()
+    n = batch['starts'][-1]
+    assert bool((got[n:] == 7).all()) and bool((got_lse[n:] == 7).all()), 'rows behind the last sequence were written'
+    nans = torch.isnan(want['o'][:n])
+    assert torch.equal(torch.isnan(got[:n]), nans)
+    worst = ((got[:n] - want['o'][:n]).abs() / bo[:n])[~nans]
+    assert worst.numel() == 0 or float(worst.max()) <= 1.0, f'o is {float(worst.max()):.3g} times its bound off'
+    ends = torch.isneginf(want['lse'][:n])
+    assert torch.equal(torch.isneginf(got_lse[:n]), ends)
+    fine = ~ends & ~torch.isnan(want['lse'][:n])
+    off = ((got_lse[:n] - want['lse'][:n]).abs() / bl[:n])[fine]
+    assert off.numel() == 0 or float(off.max()) <= 1.0, f'lse is {float(off.max()):.3g} times its bound off'
+    return batch, q, dev, out
+
+
+SHAPES = [
+    # new tokens and lengths: decoding, drafts, chunks, whole prompts, sequences that pause, no length, fewer positions than tokens
+    ([1, 1, 1], [1, 37, 200]),
+    ([1, 0, 1, 1, 0], [64, 10, 129, 33, 0]),
+    ([5, 3, 4], [5, 100, 333]),
+    ([17, 1, 0, 40], [17, 300, 5, 250]),
+    ([130, 1, 65], [130, 70, 400]),
+    ([3, 9, 2], [1, 4, 0]),
+]
+
+
+@pytest.mark.parametrize('new,lens', SHAPES)
+@pytest.mark.parametrize('dtype', [F16, BF16])
+@pytest.mark.parametrize('cache', [None, E4M3, I8])
+@pytest.mark.parametrize('D,page,heads,G', [(128, 16, 2, 4), (64, 32, 1, 1), (96, 64, 3, 2), (32, 16, 2, 7)])
+def test_attention_over_a_paged_cache(core, dtype, cache, D, page, heads, G, new, lens):
+    _attention_case(core, dtype, cache, D, page, heads, G, new, lens, 11, tail=2)
+
+
+@pytest.mark.parametrize('causal,window', [(False, 0), (True, 1), (True, 16), (True, 50), (False, 33)])
+@pytest.mark.parametrize('cache,D,page,G', [(None, 64, 16, 3), (E4M3, 128, 64, 1), (I8, 96, 32, 8)])
+@pytest.mark.parametrize('new,lens', [([1, 1], [200, 31]), ([6, 2], [150, 40]), ([100, 3], [150, 90])])
+def test_attention_windows_and_without_a_causal_mask(core, causal, window, cache, D, page, G, new, lens):
+    _attention_case(core, BF16 if D == 96 else F16, cache, D, page, 2, G, new, lens, 21, causal=causal, window=window, hints=window != 16)
+
+
+@pytest.mark.parametrize('dtype,cache,D,page,heads,G,new,lens', [
+    (F16, None, 128, 16, 1, 4, [1, 1], [3000, 700]),
+    (BF16, E4M3, 128, 128, 2, 8, [1, 2], [2500, 100]),
+    (F16, I8, 64, 32, 1, 1, [1], [5000]),
+    (F16, E4M3, 32, 16, 1, 2, [3], [4000]),
+    (BF16, None, 96, 64, 1, 5, [8, 1], [2600, 2000]),
+    (BF16, I8, 128, 256, 1, 4, [40, 1], [3100, 2600]),       # the wide kernel, in parts
+    (F16, None, 64, 16, 1, 2, [150], [2777]),
+    (F16, I8, 96, 16, 1, 2, [70], [2100]),
+    (F16, E4M3, 32, 32, 1, 2, [70], [2100]),
+])
+@pytest.mark.parametrize('window', [0, 1111])
+def test_long_sequences_in_parts(core, dtype, cache, D, page, heads, G, new, lens, window):
+    batch = ref.make_batch(new, lens, page, 31)
+    q = torch.empty((batch['tokens'], heads * G, D), dtype=dtype, device='cuda')
+    like = torch.empty((batch['pages'], heads, page, D), dtype=cache or dtype, device='cuda')
+    need = core.paged_attention_workspace_bytes(q, like, ref.on_device(batch)[0], max(new), max(lens))
+    assert need > 0                                              # more than one part
+    for space in (None, torch.empty(need // 2, dtype=torch.uint8, device='cuda'), torch.empty(0, dtype=torch.uint8, device='cuda')):
+        _attention_case(core, dtype, cache, D, page, heads, G, new, lens, 31, window=window, workspace=space)
+
+
+@pytest.mark.parametrize('new,lens', [([6], [70]), ([5, 100], [33, 130]), ([2], [64])])
+@pytest.mark.parametrize('dtype,cache', [(F16, None), (BF16, None), (F16, E4M3), (BF16, E4M3)])
+def test_keys_and_values_that_are_not_finite_reach_only_who_sees_them(core, dtype, cache, new, lens):
+    """The last new key of every sequence and one in the middle of its chunk: earlier tokens do not see them."""
+    D, page, heads, G = 64, 16, 2, 2
+    batch = ref.make_batch(new, lens, page, 41)
+    pages = ref.make_pages(batch, heads, D, cache, dtype, 42)
+    nan = math.nan if cache == E4M3 else math.inf
+    for b, n in enumerate(lens):
+        last, middle = n - 1, n - 1 - new[b] // 2
+        at = lambda p: (batch['table'][b][p // page], p % page)
+        pages[1][at(last)[0], 0, at(last)[1], 5] = math.nan
+        pages[1][at(last)[0], 1, at(last)[1], D - 1] = nan
+        pages[1][at(middle)[0], 1, at(middle)[1], 3] = nan
+        pages[0][at(last)[0], 1, at(last)[1], 0] = math.nan
+    _attention_case(core, dtype, cache, D, page, heads, G, new, lens, 41, junk=True, pages=pages)
+
+
+@pytest.mark.parametrize('D,cache', [(64, None), (128, I8)])
+@pytest.mark.parametrize('new', [1, 40])
+def test_scores_of_any_size(core, D, cache, new):
+    """Scores far from zero on both sides, and keys whose scores are all alike."""
+    for scale in (1e-6, 3.0):
+        _attention_case(core, F16, cache, D, 16, 1, 2, [new], [200], 51, scale=scale)
+
+
+def test_small_and_large_rows_of_codes(core):
+    """Exponents at both ends of what fp16 rows get: values of 2^-24, and of tens of thousands, in one cache."""
+    for cache, least, most in ((I8, -24, 9), (E4M3, -15, 7)):
+        batch = ref.make_batch([1, 30], [100, 90], 16, 61)
+        pages = ref.make_pages(batch, 1, 64, cache, F16, 62)
+        g = torch.Generator().manual_seed(63)
+        pages[3] = torch.where(torch.rand(pages[3].shape, generator=g) < 0.5, least, most).to(torch.int8)
+        for new, lens in (([1, 2], [100, 90]), ([1, 130], [100, 140])):
+            batch = ref.make_batch(new, lens, 16, 61)
+            big = ref.make_pages(batch, 1, 64, cache, F16, 62)
+            big[3] = torch.where(torch.rand(big[3].shape, generator=g) < 0.5, least, most).to(torch.int8)
+            _attention_case(core, F16, cache, 64, 16, 1, 4, new, lens, 61, pages=big)
+
+
+def test_pages_that_point_nowhere_hurt_nobody_else(core):
+    """Table entries outside the pages: the sequence beside them is as without, nothing else is written, and reads give zeros."""
+    D, page, heads = 64, 16, 2
+    batch = ref.make_batch([20, 3], [50, 40], page, 71)
+    good = ref.on_device(batch)
+    bad = good[0].clone()
+    bad[0, 1], bad[0, 2], bad[0, 3] = -7, batch['pages'], 2 ** 31 - 1
+    g = torch.Generator().manual_seed(72)
+    keys, values, q = (torch.randn((23, h, D), generator=g).to(F16).cuda() for h in (heads, heads, 4))
+    a, b = (_cuda(ref.make_pages(batch, heads, D, I8, F16, 73)) for _ in range(2))
+    core.kv_cache_write(keys, values, *a[:2], *good, *a[2:])
+    core.kv_cache_write(keys, values, *b[:2], bad, *good[1:], *b[2:])
+    own = [p for p in batch['table'][1][:3]]
+    assert all(_same(x[own], y[own]) for x, y in zip(a, b))
+    others = [p for p in range(batch['pages']) if p not in batch['table'][0][:4] and p not in own]
+    fresh = _cuda(ref.make_pages(batch, heads, D, I8, F16, 73))
+    assert all(_same(x[others], y[others]) for x, y in zip(b, fresh))
+    k, _ = core.kv_cache_read(*a[:2], bad, *good[1:], 23, F32, *a[2:])
+    assert bool((k[:18] == 0).all())                             # positions 30 to 47 lie in pages 1 and 2 of the table
+    for hint in (20, 0):
+        x, y = (core.paged_attention(q, *a[:2], t, *good[1:], *a[2:], max_queries=hint) for t in (good[0], bad))
+        assert torch.equal(x[20:], y[20:])
+
+
+def test_batches_that_make_no_sense_write_nothing_outside(core):
+    """starts that decrease or point past the rows, lengths past the table: in bounds (a launch that was not would fault), and what lies
+    around the outputs is left alone."""
+    D, page, heads = 64, 16, 2
+    batch = ref.make_batch([4, 4, 4], [30, 40, 50], page, 75)
+    table, lens, starts = ref.on_device(batch)
+    g = torch.Generator().manual_seed(76)
+    keys, values, q = (torch.randn((12, h, D), generator=g).to(F16).cuda() for h in (heads, heads, 4))
+    for s, n in (([0, 8, 4, 12], [30, 40, 50]), ([0, 4, 8, 2 ** 31 - 1], [30, 40, 50]), ([-5, 4, 8, 12], [30, -40, 50]), ([0, 4, 8, 12], [30, 4000, 2 ** 31 - 1]), ([12, 0, 0, 0], [0, 0, 0])):
+        ints = [torch.tensor(v, dtype=torch.int32, device='cuda') for v in (n, s)]
+        pages = _cuda(ref.make_pages(batch, heads, D, E4M3, F16, 77))
+        core.kv_cache_write(keys, values, *pages[:2], table, *ints, *pages[2:])
+        core.kv_cache_read(*pages[:2], table, *ints, 12, F16, *pages[2:])
+        for hint in (0, 4, 1):
+            whole = torch.full((14, 4, D), 7.0, dtype=F16, device='cuda')
+            core.paged_attention(q, *pages[:2], table, *ints, *pages[2:], max_queries=hint, out=whole[1:13])
+            assert bool((whole[0] == 7).all()) and bool((whole[13] == 7).all())
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize('new,lens', [([1, 1], [100, 40]), ([100, 1], [130, 40])])
+def test_queries_as_views_and_results_in_their_place(core, new, lens):
+    D, page, heads, G = 128, 32, 2, 4
+    batch = ref.make_batch(new, lens, page, 81)
+    pages = _cuda(ref.make_pages(batch, heads, D, None, BF16, 82))
+    joint = torch.randn((batch['tokens'], heads * G + 2 * heads, D), generator=torch.Generator().manual_seed(83)).to(BF16).cuda()
+    q = joint[:, :heads * G]
+    args = (*pages[:2], *ref.on_device(batch))
+    want = core.paged_attention(q.contiguous(), *args)
+    assert torch.equal(core.paged_attention(q, *args), want)
+    turned = q.permute(1, 0, 2).contiguous().permute(1, 0, 2)
+    assert torch.equal(core.paged_attention(turned, *args), want)
+    own = q.contiguous()
+    core.paged_attention(own, *args, out=own)
+    assert torch.equal(own, want)
+
+
+def test_empty_calls(core):
+    pages = _cuda(ref.make_pages(dict(pages=2, page=16), 2, 64, None, F16, 1))
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device='cuda')
+    table = torch.zeros((1, 1), dtype=torch.int32, device='cuda')
+    none = torch.empty((0, 2, 64), dtype=F16, device='cuda')
+    core.kv_cache_write(none, none, *pages[:2], table, ints(0), ints(0, 0))
+    assert core.kv_cache_read(*pages[:2], table, ints(0), ints(0, 0), 0)[0].shape == (0, 2, 64)
+    assert core.paged_attention(none, *pages[:2], table, ints(0), ints(0, 0)).shape == (0, 2, 64)
+    some = torch.ones((3, 2, 64), dtype=F16, device='cuda')
+    out = torch.full_like(some, 7.0)
+    core.paged_attention(some, *pages[:2], table[:0], ints(), ints(0), out=out)
+    assert bool((out == 7).all())
+    tokens, accepted = core.verify_drafts(torch.ones((0, 3, 8), device='cuda'), None, torch.zeros((0, 2), dtype=torch.int64, device='cuda'), torch.zeros((0, 2), device='cuda'),
+                                          torch.zeros(0, device='cuda'))
+    assert tokens.shape == (0, 3) and accepted.shape == (0,)
+
+
+def test_refusals_on_the_device(core):
+    pages = _cuda(ref.make_pages(dict(pages=2, page=16), 2, 64, None, F16, 1))
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device='cuda')
+    batch = (torch.zeros((1, 1), dtype=torch.int32, device='cuda'), ints(1), ints(0, 1))
+    q = torch.ones((1, 4, 64), dtype=F16, device='cuda')
+    call = lambda q=q, p=pages, b=batch, **kw: core.paged_attention(q, *p[:2], *b, **kw)
+    with pytest.raises(TypeError, match='type of the pages'):
+        call(q.to(BF16))
+    with pytest.raises(TypeError, match='float16 or bfloat16'):
+        call(q.float())
+    with pytest.raises(ValueError, match=r'\[tokens, heads, 64\]'):
+        call(q[:, :, :32])
+    with pytest.raises(core.FtkError) as info:
+        call(q[:, :3].contiguous())
+    assert info.value.code == -1
+    with pytest.raises(ValueError, match='strides'):
+        call(torch.ones((2, 4, 68), dtype=F16, device='cuda')[:, :, 2:66])
+    with pytest.raises(ValueError, match='out must be'):
+        call(out=torch.empty((2, 4, 64), dtype=F16, device='cuda'))
+    with pytest.raises(ValueError, match='window'):
+        call(window=-1)
+    with pytest.raises(core.FtkError):
+        call(scale=0.0)
+    with pytest.raises(ValueError, match='CUDA tensor'):
+        call(workspace=torch.empty(1 << 20, dtype=torch.uint8))
+    with pytest.raises(TypeError, match='table must be'):
+        call(b=(batch[0].long(), *batch[1:]))
+    with pytest.raises(ValueError, match='starts must be'):
+        call(b=(*batch[:2], ints(0)))
+    with pytest.raises(ValueError, match='have no k_exps'):
+        call(k_exps=torch.zeros((2, 2, 16), dtype=torch.int8, device='cuda'))
+    with pytest.raises(ValueError, match='need k_exps'):
+        call(p=[t.to(torch.int8) for t in pages[:2]])
+    k = torch.ones((1, 2, 64), dtype=F16, device='cuda')
+    with pytest.raises(ValueError, match='as many tokens'):
+        core.kv_cache_write(k, torch.ones((2, 2, 64), dtype=F16, device='cuda'), *pages[:2], *batch)
+    with pytest.raises(TypeError, match='read in that type'):
+        core.kv_cache_read(*pages[:2], *batch, 1, BF16)
+    with pytest.raises(ValueError, match='tokens must be'):
+        core.kv_cache_read(*pages[:2], *batch, -1)
+    with pytest.raises(core.FtkError) as info:                   # page sizes that the kernels do not have
+        core.kv_cache_write(k, k, *[t[:, :, :8].contiguous() for t in pages[:2]], *batch)
+    assert info.value.code == -2
+
+
+# ---- verification -----------------------------------------------------------------------
+
+def _drafts(B, K, V, dtype, wide, seed):
+    g = torch.Generator().manual_seed(seed)
+    logits = 2 * torch.randn((B, K + 1, V), generator=g)
+    target = torch.softmax(logits, -1).to(dtype)
+    draft = torch.softmax(logits[:, :K] + 0.7 * torch.randn((B, K, V), generator=g), -1).to(dtype)
+    drafts = torch.multinomial(draft.float().view(-1, V), 1, generator=g).view(B, K) if B * K else torch.zeros((B, K), dtype=torch.int64)
+    return target, draft, drafts.to(torch.int64 if wide else torch.int32), torch.rand((B, K), generator=g), torch.rand(B, generator=g)
+
+
+def _verified(core, target, draft, drafts, accept, sample, counts=None):
+    want = ref.verify(target, draft, drafts, accept, sample, None if counts is None else counts.tolist())
+    got = core.verify_drafts(target.cuda(), None if draft is None else draft.cuda(), drafts.cuda(), accept.cuda(), sample.cuda(), None if counts is None else counts.cuda())
+    assert torch.equal(got[1].cpu(), want[1])
+    assert torch.equal(got[0].cpu(), want[0])
+    return want
+
+
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+@pytest.mark.parametrize('B,K,V', [(1, 1, 1), (3, 2, 7), (5, 4, 1000), (2, 5, 2048), (4, 3, 2049), (3, 0, 4096), (2, 63, 301), (2, 2, 70001)])
+def test_verified_drafts(core, dtype, B, K, V):
+    t = _drafts(B, K, V, dtype, K % 2, 91)
+    _verified(core, *t)
+    _verified(core, t[0], None, *t[2:])
+    _verified(core, *t, counts=torch.tensor([(2 * b) % (K + 2) - (b == 2) for b in range(B)], dtype=torch.int32))
+
+
+def test_verified_drafts_at_the_ends_of_their_ranges(core):
+    B, K, V = 8, 3, 5000
+    target, draft, drafts, accept, sample = _drafts(B, K, V, F32, True, 92)
+    target[0] = draft[0, :1]                                      # nothing left of the target's row
+    accept[0] = 1.0                                               # (a uniform of 1: rejected even so)
+    drafts[1, 1], drafts[2, 0] = V, -1                            # no such tokens
+    target[3, 0, drafts[3, 0]] = 0.0                              # impossible
+    accept[4], sample[4] = 0.0, 0.0                               # every draft with a chance is accepted; the first token with one
+    target[4, K, :17] = 0.0
+    sample[5] = 1.0 - 2.0 ** -24
+    target[6, 0] = 0.0                                            # no token has a chance
+    accept[6] = 0.5
+    target[7, 0, 5], draft[7, 0, 6] = math.nan, math.nan
+    accept[7] = 1.0
+    want = _verified(core, target, draft, drafts, accept, sample)
+    assert want[1].tolist()[0] == 0 and int(want[1][1]) <= 1 and int(want[1][2]) == 0 and int(want[1][3]) == 0 and int(want[0][6][0]) == -1
+
+
+def test_verified_drafts_at_odd_addresses(core):
+    """Rows that do not begin at 16-byte boundaries, by the size of the vocabulary and by the place of the tensors."""
+    for V in (999, 4096):
+        target, draft, drafts, accept, sample = _drafts(3, 2, V, F16, False, 93)
+        space = [torch.empty(t.numel() + 1, dtype=F16, device='cuda')[1:] for t in (target, draft)]
+        views = [s.copy_(t.flatten()).view(t.shape) for s, t in zip(space, (target, draft))]
+        want = ref.verify(target, draft, drafts, accept, sample)
+        got = core.verify_drafts(*views, drafts.cuda(), accept.cuda(), sample.cuda())
+        assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+
+
+# ---- together -----------------------------------------------------------------------------
+
+def _step_inputs(seed, new, heads, G, D, V, dtype):
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    n = sum(new)
+    rows = [torch.randn((n, h, D), generator=g, device='cuda').to(dtype) for h in (heads, heads, heads * G)]
+    return rows, torch.randn((heads * G * D, V), generator=g, device='cuda') * 0.3, [torch.rand(s, generator=g, device='cuda') for s in ((len(new), new[0] - 1), (len(new),))]
+
+
+@pytest.mark.parametrize('dtype,cache', [(F16, E4M3), (BF16, I8), (BF16, None)])
+def test_a_served_step(core, dtype, cache):
+    """Prompts into the cache, then drafts: written, attended to, turned into probabilities, verified; the rejected ones are overwritten by the next step.
+    Attention of a chunk equals attention of its tokens one by one to rounding, and what it reads is what was written."""
+    heads, G, D, V, page, K = 2, 4, 64, 500, 16, 3
+    prompts = [40, 7, 90]
+    batch = ref.make_batch(prompts, [n + 20 for n in prompts], page, 101)
+    table = ref.on_device(batch)[0]
+    pages = _junk(_cuda(ref.make_pages(batch, heads, D, cache, dtype, 102)))
+    kv, exps = pages[:2], pages[2:]
+    lens = list(prompts)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device='cuda')
+    starts = lambda new: ints([sum(new[:i]) for i in range(len(new) + 1)])
+    (k, v, q), _, _ = _step_inputs(103, prompts, heads, G, D, V, dtype)
+    at = (table, ints(lens), starts(prompts))
+    core.kv_cache_write(k, v, *kv, *at, *exps)
+    whole = core.paged_attention(q, *kv, *at, *exps, max_queries=max(prompts), max_keys=max(lens))
+    last = torch.tensor([sum(prompts[:i + 1]) - 1 for i in range(3)], device='cuda')
+    single = core.paged_attention(q[last].contiguous(), *kv, table, ints(lens), starts([1] * 3), *exps, max_queries=1, max_keys=max(lens))
+    u = torch.finfo(dtype).eps
+    assert bool(((whole[last].float() - single.float()).abs() <= 4 * u * (1 + single.float().abs())).all())
+    generated = [[] for _ in prompts]
+    for step in range(4):
+        new = [K + 1] * 3
+        lens = [n + K + 1 for n in lens]
+        (k, v, q), head, (accept, sample) = _step_inputs(200 + step, new, heads, G, D, V, dtype)
+        at = (table, ints(lens), starts(new))
+        core.kv_cache_write(k, v, *kv, *at, *exps)
+        o = core.paged_attention(q, *kv, *at, *exps, max_queries=K + 1, max_keys=max(lens))
+        target = core.online_softmax((o.float().view(sum(new), -1) @ head).contiguous()).view(3, K + 1, V)
+        draft = core.online_softmax((target[:, :K] + 1e-3).log().mul(0.8).reshape(-1, V)).view(3, K, V)
+        drafts = torch.multinomial(draft.view(-1, V), 1, generator=torch.Generator(device='cuda').manual_seed(step)).view(3, K)
+        tokens, accepted = core.verify_drafts(target, draft, drafts, accept, sample)
+        want = ref.verify(target.cpu(), draft.cpu(), drafts.cpu(), accept.cpu(), sample.cpu())
+        assert torch.equal(tokens.cpu(), want[0]) and torch.equal(accepted.cpu(), want[1])
+        read_k, _ = core.kv_cache_read(*kv, *at, sum(new), F32, *exps)
+        if cache is None:
+            assert torch.equal(read_k, k.float())
+        else:
+            # int8: top > 127 2^(e - 1), so half a step, 2^(e - 1), is less than top / 127 (and may be more than top / 128); e4m3: half a step of three bits
+            top = k.float().abs().amax(-1, keepdim=True)
+            assert bool(((read_k - k.float()).abs() <= top * (2.0 ** -4 if cache == E4M3 else 1 / 127)).all())
+        for b, n in enumerate(accepted.tolist()):
+            generated[b] += tokens[b, :n + 1].tolist()
+            lens[b] -= K - n                                     # the rejected positions are free again
+    assert all(0 <= t < V for s in generated for t in s)
+
+
+def test_other_streams_and_replays(core):
+    """The calls on a stream of their own, recorded and replayed with other contents of the same buffers (lengths, pages, tokens among them), with eager work between the
+    replays; two graphs on workspaces of their own."""
+    heads, G, D, V, page, K = 2, 4, 128, 3000, 16, 3
+    batch = ref.make_batch([4, 4], [2600, 2200], page, 111)
+    need = None
+    variants = []
+    for i, (lens, seed) in enumerate([([2600, 2200], 1), ([100, 2000], 2), ([4, 37], 3)]):
+        g = torch.Generator(device='cuda').manual_seed(seed)
+        rows = [torch.randn((8, h, D), generator=g, device='cuda').to(F16) for h in (heads, heads, heads * G)]
+        probs = [torch.softmax(torch.randn((2, n, V), generator=g, device='cuda') * 2, -1) for n in (K + 1, K)]
+        ids = torch.randint(0, V, (2, K), generator=g, device='cuda')
+        uniforms = [torch.rand(s, generator=g, device='cuda') * 0.2 for s in ((2, K), (2,))]
+        table = torch.tensor(batch['table'], dtype=torch.int32, device='cuda').roll(i, 1)
+        variants.append([*rows, table, torch.tensor(lens, dtype=torch.int32, device='cuda'), *probs, ids, *uniforms])
+    starts = torch.tensor([0, 4, 8], dtype=torch.int32, device='cuda')
+    fresh = lambda: _cuda(ref.make_pages(batch, heads, D, I8, F16, 112))
+
+    def step(x, pages, space, spare):
+        k, v, q, table, lens, target, draft, ids, accept, sample = x
+        core.kv_cache_write(k, v, *pages[:2], table, lens, starts, *pages[2:])
+        read = core.kv_cache_read(*pages[:2], table, lens, starts, 8, F16, *pages[2:])
+        o, lse = core.paged_attention(q, *pages[:2], table, lens, starts, *pages[2:], max_queries=4, max_keys=2600, return_lse=True, workspace=space)
+        return [*read, o, lse, *core.verify_drafts(target, draft, ids, accept, sample, workspace=spare)]
+
+    need = core.paged_attention_workspace_bytes(variants[0][2], fresh()[0], variants[0][3], 4, 2600)
+    assert need > 0
+    spaces = lambda: (torch.empty(need, dtype=torch.uint8, device='cuda'), torch.empty(1 << 16, dtype=torch.uint8, device='cuda'))
+    want = [[t.clone() for t in step(x, fresh(), *spaces())] for x in variants]
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        got = step(variants[1], fresh(), *spaces())
+    stream.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want[1]))
+    graphs = []
+    for _ in range(2):
+        x, pages, space = [t.clone() for t in variants[0]], fresh(), spaces()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = step(x, pages, *space)
+        graphs.append((graph, x, pages, space, out))
+    clean = fresh()
+    for turn in range(6):
+        for i, (graph, x, pages, space, out) in enumerate(graphs):
+            for a, b in zip(pages, clean):
+                a.copy_(b)
+            for a, b in zip(x, variants[(turn + i) % 3]):
+                a.copy_(b)
+        torch.cuda.synchronize()
+        for graph, *_ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for i, (_, _, _, _, out) in enumerate(graphs):
+            assert all(torch.equal(a, b) for a, b in zip(out, want[(turn + i) % 3])), (turn, i)
+        eager = step(variants[turn % 3], fresh(), *spaces())
+        assert all(torch.equal(a, b) for a, b in zip(eager, want[turn % 3]))
