@@ -178,7 +178,7 @@ struct NarrowShape {
   static constexpr int EXPS = F == kSame ? 0 : 256;           // the exponents of a tile's keys and values, one copy of 4 bytes a lane
   static constexpr int STAGE = 2 * TILE + EXPS;
   static constexpr int LOADS = 2 * COPIES + (F == kSame ? 0 : 1);
-  static constexpr int STAGES = TILE >= 6144 ? 2 : TILE >= 3072 ? 3 : 4;
+  static constexpr int STAGES = TILE >= 4096 ? 2 : TILE >= 3072 ? 3 : 4;
   static constexpr int RING = kWaves * STAGES * STAGE;
   static constexpr int JOIN = kWaves * (D / 16) * 64 * 16 + kWaves * 16 * 8;
   static constexpr int LDS = RING > JOIN ? RING : JOIN;
@@ -220,26 +220,49 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
     const int key0 = base + 32 * (wave + kWaves * i);
     return Blocks{block_row(a, j.b, kv_head, key0, j.lo, j.hi), block_row(a, j.b, kv_head, key0 + 16, j.lo, j.hi)};
   };
-  // Rows outside [lo, hi) repeat the nearest key inside: their weights are zero, and what they hold is finite if the cache is.
+  // Where the 16 bytes that a lane copies lie from the first row of their block; a copy's rows repeat every 16, so that both blocks
+  // share these, but for rows of 96 and 32 bytes, of which a copy has rows of both blocks.
+  constexpr bool WHOLE = 16 * S::BYTES % 1024 == 0;
+  constexpr int OFFS = WHOLE ? 16 * S::BYTES / 1024 : S::COPIES;
+  unsigned off[OFFS];
+#pragma unroll
+  for (int c = 0; c < OFFS; ++c) {
+    const int p = 64 * c + lane, row = p / CH, slot = p - row * CH;
+    off[c] = (row & 15) * S::BYTES + 16 * (slot ^ swizzle<S::BYTES>(row));
+  }
   auto issue = [&](int i, int stage, const Blocks& at) __attribute__((always_inline)) {
     const int key0 = base + 32 * (wave + kWaves * i);
     unsigned char* const dst = ring + stage * S::STAGE;
     const int least = j.lo - key0, most = j.hi - 1 - key0;
-    const bool edge = least > 0 || most < 31;
+    if (least <= 0 && most >= 31) {
+      const unsigned char *const k0 = a.pages.k + at.r0 * S::BYTES, *const k1 = a.pages.k + at.r1 * S::BYTES;
+      const unsigned char *const v0 = a.pages.v + at.r0 * S::BYTES, *const v1 = a.pages.v + at.r1 * S::BYTES;
 #pragma unroll
-    for (int c = 0; c < S::COPIES; ++c) {
-      const int p = 64 * c + lane, row = p / CH, slot = p - row * CH;
-      const int chunk = slot ^ swizzle<S::BYTES>(row);
-      const int key = edge ? min(max(row, least), most) : row;
-      const long long at_row = key >= 16 ? at.r1 + key - 16 : at.r0 + key;
-      const size_t off = (size_t)at_row * S::BYTES + 16 * chunk;
-      lds_dma16_from(a.pages.k + off, dst + 1024 * c);
-      lds_dma16_from(a.pages.v + off, dst + S::TILE + 1024 * c);
+      for (int c = 0; c < S::COPIES; ++c) {
+        if constexpr (WHOLE) {
+          lds_dma16(c < OFFS ? k0 : k1, off[c % OFFS], dst + 1024 * c);
+          lds_dma16(c < OFFS ? v0 : v1, off[c % OFFS], dst + S::TILE + 1024 * c);
+        } else {
+          const bool second = (64 * c + lane) / CH >= 16;
+          lds_dma16_from((second ? k1 : k0) + off[c], dst + 1024 * c);
+          lds_dma16_from((second ? v1 : v0) + off[c], dst + S::TILE + 1024 * c);
+        }
+      }
+    } else {
+      // rows outside [lo, hi) repeat the nearest key inside: their weights are zero, and what they hold is finite if the cache is
+#pragma unroll
+      for (int c = 0; c < S::COPIES; ++c) {
+        const int p = 64 * c + lane, row = p / CH, slot = p - row * CH;
+        const int key = min(max(row, least), most);
+        const long long at_row = key >= 16 ? at.r1 + key - 16 : at.r0 + key;
+        const size_t from = (size_t)at_row * S::BYTES + 16 * (slot ^ swizzle<S::BYTES>(row));
+        lds_dma16_from(a.pages.k + from, dst + 1024 * c);
+        lds_dma16_from(a.pages.v + from, dst + S::TILE + 1024 * c);
+      }
     }
     if constexpr (F != kSame) {
       // lanes 0..7: the exponents of K, four keys each, lanes 8..15: of V
-      const int four = 4 * (lane & 7);
-      const int key = edge ? min(max(four, least & ~3), most & ~3) : four;
+      const int four = 4 * (lane & 7), key = min(max(four, least & ~3), most & ~3);
       const long long at_row = key >= 16 ? at.r1 + key - 16 : at.r0 + key;
       lds_dma4_from((lane & 8 ? a.pages.v_exps : a.pages.k_exps) + at_row, dst + 2 * S::TILE);
     }
@@ -279,25 +302,13 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
   for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
     for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[nq][s]));
-  int stage = 0;
-  for (int i = 0; i < mine; ++i) {
-    const int key0 = base + 32 * (wave + kWaves * i);
-    if (i + STAGES - 1 < mine) {
-      issue(i + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1, next);
-      if (i + STAGES < mine) next = blocks_of(i + STAGES);
-      constexpr int N = S::LOADS * (STAGES - 1);
-      static_assert(N < 64, "vmcnt counts to 63");
-      __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
-    } else {
-      __builtin_amdgcn_s_waitcnt(0x0F70);
-    }
-    asm volatile("" ::: "memory");
-    const unsigned char* const kt = ring + stage * S::STAGE;
+  // One tile.  MASKED: some row does not see all of it.
+  auto step = [&](int key0, const unsigned char* kt, auto masked_c) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(masked_c)::value;
     const unsigned char* const vt = kt + S::TILE;
-    const bool masked = key0 < j.sure_lo || key0 + 32 > j.sure_hi;
-
-    // scores times the factor of their key, in powers of two; lane (row m, kg) has keys 16 h + 4 kg + r
-    float kfac[2][4], vfac[2][4];
+    // lane (row m, kg) has keys 16 h + 4 kg + r: the factors of their scores (scale, and the power of two of K's row), and those of V's rows
+    float kfac[2][4];
+    int vexp[2][4];
     if constexpr (F != kSame) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -305,10 +316,15 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
         const unsigned ve = *reinterpret_cast<const unsigned*>(kt + 2 * S::TILE + 32 + 16 * h + 4 * kg);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int key = key0 + 16 * h + 4 * kg + r;
-          const bool in = key >= j.lo && key < j.hi;              // what lies behind a sequence's keys has no exponent
-          kfac[h][r] = in ? power_of_two((signed char)(ke >> (8 * r))) * a.scale_log2e : 0.0f;
-          vfac[h][r] = in ? power_of_two((signed char)(ve >> (8 * r))) : 0.0f;
+          kfac[h][r] = ldexpf(a.scale_log2e, (signed char)(ke >> (8 * r)));
+          vexp[h][r] = (signed char)(ve >> (8 * r));
+          if constexpr (MASKED) {                                  // what lies behind a sequence's keys has no exponent
+            const int key = key0 + 16 * h + 4 * kg + r;
+            if (key < j.lo || key >= j.hi) {
+              kfac[h][r] = 0.0f;
+              vexp[h][r] = 0;
+            }
+          }
         }
       }
     }
@@ -328,15 +344,15 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
       }
     }
     v8 p[NQ];
-    unsigned seen[NQ];                                            // masked tiles: which of the lane's eight keys its row sees
+    unsigned seen[NQ];                                            // MASKED: which of the lane's eight keys its row sees
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int r = 0; r < 4; ++r) sc[nq][h][r] *= F == kSame ? a.scale_log2e : kfac[h][r];
-      seen[nq] = 255;
-      if (masked) {
+      if constexpr (MASKED) {
+        seen[nq] = 255;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -371,8 +387,8 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
           float p0 = __builtin_amdgcn_exp2f(sc[nq][h][r] - ref[nq]), p1 = __builtin_amdgcn_exp2f(sc[nq][h][r + 1] - ref[nq]);
           l[nq] += p0 + p1;
           if constexpr (F != kSame && std::is_same<T, Brain>::value) {
-            p0 *= vfac[h][r];
-            p1 *= vfac[h][r + 1];
+            p0 = ldexpf(p0, vexp[h][r]);
+            p1 = ldexpf(p1, vexp[h][r + 1]);
           }
           w[2 * h + r / 2] = T::pack(p0, p1);
         }
@@ -383,7 +399,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int r = 0; r < 4; r += 2) vpair[2 * h + r / 2] = v2h{(_Float16)vfac[h][r], (_Float16)vfac[h][r + 1]};
+        for (int r = 0; r < 4; r += 2) vpair[2 * h + r / 2] = v2h{(_Float16)ldexpf(1.0f, vexp[h][r]), (_Float16)ldexpf(1.0f, vexp[h][r + 1])};
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
@@ -416,7 +432,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
           vf = __builtin_bit_cast(v8, pairs);
         }
       }
-      if (masked && j.n > 1) {
+      if constexpr (MASKED) {
         // A value that is not finite must not reach the rows that do not see it (0 x inf): it leaves the product, and makes NaN of
         // the rows that do see it.
         const unsigned bad = not_finite<T>(vf);
@@ -436,6 +452,23 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
       for (int nq = 0; nq < NQ; ++nq) o[nq][dt] = T::mma16(vf, p[nq], o[nq][dt]);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
+
+  int stage = 0;
+  for (int i = 0; i < mine; ++i) {
+    const int key0 = base + 32 * (wave + kWaves * i);
+    if (i + STAGES - 1 < mine) {
+      issue(i + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1, next);
+      if (i + STAGES < mine) next = blocks_of(i + STAGES);
+      constexpr int N = S::LOADS * (STAGES - 1);
+      static_assert(N < 64, "vmcnt counts to 63");
+      __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+    } else {
+      __builtin_amdgcn_s_waitcnt(0x0F70);
+    }
+    asm volatile("" ::: "memory");
+    if (key0 < j.sure_lo || key0 + 32 > j.sure_hi || key0 < j.lo || key0 + 32 > j.hi) step(key0, ring + stage * S::STAGE, std::true_type{});
+    else step(key0, ring + stage * S::STAGE, std::false_type{});
     stage = stage == STAGES - 1 ? 0 : stage + 1;
   }
 
@@ -496,7 +529,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
 }
 
 template <typename T, KvFormat F, int D, int NQ>
-__global__ __launch_bounds__(kWaves * 64) void paged_narrow_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kWaves * 64, NQ == 4 ? 1 : 2) void paged_narrow_kernel(AttnArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int kv_head = blockIdx.x % a.pages.heads, rest = blockIdx.x / a.pages.heads;
   const int slot = rest / a.nparts, part = rest - slot * a.nparts;
@@ -817,36 +850,64 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_wide_kernel(AttnArgs a, 
 
 // ---- parts ------------------------------------------------------------------------------
 
-// m = max m_p, l = sum l_p 2^(m_p - m), O = sum O_p 2^(m_p - m) / l over the parts of a row; D / 4 lanes a row.
+// m = max m_p, l = sum l_p 2^(m_p - m), O = sum O_p 2^(m_p - m) / l over the parts of a row; D / 4 lanes a row, and `slices` such
+// groups for the parts of a row where these are many and the rows few.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a) {
-  constexpr int L = D / 4;
-  const long long at = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
-  const int c = threadIdx.x % L;
+__global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int slices) {
+  constexpr int L = D / 4, UNITS = 256 / L;
+  __shared__ v4f so[256];
+  __shared__ float sm[UNITS], sl[UNITS];
+  const int unit = threadIdx.x / L, c = threadIdx.x % L;
+  const int per_block = UNITS / slices, slice = unit % slices;
   const long long rows = (long long)a.batch.tokens * a.heads;
+  const long long at = (long long)blockIdx.x * per_block + unit / slices;
   const int token = (int)(min(at, rows - 1) / a.heads);
   const int first_token = __builtin_amdgcn_readfirstlane(token);
   int b = count_at_most(a.batch.sequences, first_token, [&](int i) { return a.batch.starts[i + 1]; });
   while (b < a.batch.sequences && a.batch.starts[b + 1] <= token) ++b;
-  if (at >= rows || threadIdx.x / L >= 256 / L || b >= a.batch.sequences) return;
-  const int start = min(max(a.batch.starts[b], 0), a.batch.tokens), end = min(max(a.batch.starts[b + 1], start), a.batch.tokens);
-  if (token < start || token >= end) return;
-  const int len_all = max(a.batch.lens[b], 0), first = len_all - (end - start);
-  const int len = min(len_all, kv_capacity(a.batch, a.pages.page_shift));
-  const int parts = seq_parts(a, first, len);
-  if (parts == 1) return;                                      // written already
-  const float* const ml = a.part_ml + 2 * at * a.nparts;
-  float top = kNoRef;
-  for (int p = 0; p < parts; ++p) top = fmaxf(top, ml[2 * p]);
-  float sum = 0.0f;
-  v4f acc = {0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < parts; ++p) {
-    const float w = __builtin_amdgcn_exp2f(ml[2 * p] - top), lp = ml[2 * p + 1];
-    const v4f v = *reinterpret_cast<const v4f*>(a.part_o + (at * a.nparts + p) * D + 4 * c);
-    sum += w * lp;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] += w * v[e];
+  int parts = 1, first = 0, len = 0, start = 0;
+  if (at < rows && unit < per_block * slices && b < a.batch.sequences) {
+    start = min(max(a.batch.starts[b], 0), a.batch.tokens);
+    const int end = min(max(a.batch.starts[b + 1], start), a.batch.tokens);
+    if (token >= start && token < end) {
+      const int len_all = max(a.batch.lens[b], 0);
+      first = len_all - (end - start);
+      len = min(len_all, kv_capacity(a.batch, a.pages.page_shift));
+      parts = seq_parts(a, first, len);                          // 1: written already
+    }
   }
+  float top = kNoRef, sum = 0.0f;
+  v4f acc = {0.f, 0.f, 0.f, 0.f};
+  if (parts > 1) {
+    const float* const ml = a.part_ml + 2 * at * a.nparts;
+    for (int p = slice; p < parts; p += slices) top = fmaxf(top, ml[2 * p]);
+#pragma unroll 4
+    for (int p = slice; p < parts; p += slices) {
+      const float w = __builtin_amdgcn_exp2f(ml[2 * p] - top), lp = ml[2 * p + 1];
+      const v4f v = *reinterpret_cast<const v4f*>(a.part_o + (at * a.nparts + p) * D + 4 * c);
+      sum += w * lp;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += w * v[e];
+    }
+  }
+  if (slices > 1) {
+    so[threadIdx.x] = acc;
+    if (c == 0 && unit < UNITS) {
+      sm[unit] = top;
+      sl[unit] = sum;
+    }
+    __syncthreads();
+    if (slice != 0 || parts == 1) return;
+    for (int i = 1; i < slices; ++i) {
+      const float t = fmaxf(top, sm[unit + i]), w0 = __builtin_amdgcn_exp2f(top - t), w1 = __builtin_amdgcn_exp2f(sm[unit + i] - t);
+      const v4f v = so[threadIdx.x + i * L];
+      sum = sum * w0 + sl[unit + i] * w1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = acc[e] * w0 + v[e] * w1;
+      top = t;
+    }
+  }
+  if (parts == 1) return;
   const long long position = (long long)first + (token - start);
   const int hi = a.causal ? clamp_position(position + 1, len) : len, lo = a.window > 0 ? clamp_position(position - a.window + 1, len) : 0;
   const bool none = hi <= lo;
@@ -982,10 +1043,12 @@ int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long 
       bad = launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D>, once, blocks, WideShape<D>::LDS, s, a, p.slots);
     }
     if (bad || p.nparts == 1) return bad;
-    constexpr int RPB = 256 / (D / 4);
-    const long long mblocks = (rows + RPB - 1) / RPB;
+    constexpr int UNITS = 256 / (D / 4);
+    const int slices = p.nparts >= 2 * UNITS ? UNITS : p.nparts >= 8 ? UNITS / 2 : 1;
+    const int per_block = UNITS / slices;
+    const long long mblocks = (rows + per_block - 1) / per_block;
     if (mblocks > INT_MAX) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: grid too large", who);
-    hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3((unsigned)mblocks), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3((unsigned)mblocks), dim3(256), 0, s, a, slices);
     return check_launch("paged_merge_kernel");
   });
 }
