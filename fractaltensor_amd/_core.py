@@ -88,7 +88,7 @@ def _load() -> ctypes.CDLL:
     lib.ftk_flash_attn_f16_workspace_bytes.restype = ctypes.c_size_t
     lib.ftk_flash_attn_f16_workspace_bytes.argtypes = [ctypes.c_int] * 5
     lib.ftk_paged_attn_workspace_bytes.restype = ctypes.c_size_t
-    lib.ftk_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(KvPages), ctypes.POINTER(KvBatch)] + [ctypes.c_int] * 3
+    lib.ftk_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(KvPages), ctypes.POINTER(KvBatch)] + [ctypes.c_int] * 4
     lib.ftk_verify_drafts_workspace_bytes.restype = ctypes.c_size_t
     lib.ftk_verify_drafts_workspace_bytes.argtypes = [ctypes.c_int] * 2
     for name in EXPORTS:
@@ -905,12 +905,12 @@ def kv_cache_read(k_pages, v_pages, table, lens, starts, tokens: int, dtype=None
 _LIKE = {t: torch.empty(0, dtype=t) for t in (torch.float16, torch.bfloat16, torch.float32)}
 
 
-def paged_attention_workspace_bytes(q, k_pages, table, max_queries: int = 0, max_keys: int = 0) -> int:
+def paged_attention_workspace_bytes(q, k_pages, table, max_queries: int = 0, max_keys: int = 0, window: int = 0) -> int:
     """Bytes that paged_attention wants for a batch of this shape on the device of q; 0 where the keys are not cut into parts."""
     pages = KvPages(None, None, None, None, KV_TYPES[k_pages.dtype], *k_pages.shape)
     batch = KvBatch(None, None, None, table.shape[0], table.shape[1], q.shape[0])
     with torch.cuda.device(q.device):
-        return int(lib.ftk_paged_attn_workspace_bytes(ctypes.byref(pages), ctypes.byref(batch), q.shape[1], max_queries, max_keys))
+        return int(lib.ftk_paged_attn_workspace_bytes(ctypes.byref(pages), ctypes.byref(batch), q.shape[1], window, max_queries, max_keys))
 
 
 def paged_attention(q, k_pages, v_pages, table, lens, starts, k_exps=None, v_exps=None, scale: Optional[float] = None, causal: bool = True,

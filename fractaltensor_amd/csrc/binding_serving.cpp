@@ -177,7 +177,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (a[15] != Py_None) {
       if (!on(a[15], q) || !tensor_of(a[15]).is_contiguous()) Py_RETURN_NONE;
       ws = tensor_of(a[15]);
-    } else if (const size_t need = ftk_paged_attn_workspace_bytes(&c.pages, &c.batch, heads, max_queries, max_keys)) {
+    } else if (const size_t need = ftk_paged_attn_workspace_bytes(&c.pages, &c.batch, heads, window, max_queries, max_keys)) {
       ws = empty({(int64_t)need}, at::kByte, q);
     }
     if (!count("paged_attention")) return nullptr;

@@ -171,6 +171,21 @@ __device__ __forceinline__ typename T::v8 decode8(v2u w, float scale) {
         r[2 * i + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w[i], scale, true));
       }
     }
+  } else if constexpr (std::is_same<T, Half>::value) {
+    // 0x6400 | u is 1024 + u for a byte u = code + 128: two codes in a byte permutation, a subtraction and, unless it is 1, the scale,
+    // where a conversion each takes nine instructions for four
+    const v2h middle = {(_Float16)1152.0f, (_Float16)1152.0f}, times = {(_Float16)scale, (_Float16)scale};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const unsigned u = w[i] ^ 0x80808080u;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const unsigned pair = __builtin_amdgcn_perm(0x64646464u, u, p ? 0x04030402u : 0x04010400u);
+        v2h h = __builtin_bit_cast(v2h, pair) - middle;
+        if (!(__builtin_constant_p(scale) && scale == 1.0f)) h = h * times;
+        r[2 * i + p] = __builtin_bit_cast(unsigned, h);
+      }
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 2; ++i)

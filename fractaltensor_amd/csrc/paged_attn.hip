@@ -14,6 +14,7 @@
 // Rounding: scores, softmax state and O are fp32 and Q is not scaled beforehand; the one rounding is that of the weights to 16 bits
 // as operands of P V, half a step (2^-12 fp16, 2^-9 bf16) each.  A cache of 8 bits enters the products as its exact values.
 #include <algorithm>
+#include <cmath>
 
 #include "kv_common.h"
 
@@ -177,17 +178,18 @@ struct NarrowShape {
   static constexpr int COPIES = TILE / 1024;
   static constexpr int EXPS = F == kSame ? 0 : 256;           // the exponents of a tile's keys and values, one copy of 4 bytes a lane
   static constexpr int STAGE = 2 * TILE + EXPS;
-  static constexpr int LOADS = 2 * COPIES + (F == kSame ? 0 : 1);
-  static constexpr int STAGES = TILE >= 4096 ? 2 : TILE >= 3072 ? 3 : 4;
+  static constexpr int K_LOADS = COPIES + (F == kSame ? 0 : 1);   // (the exponents of both come with K)
+  static constexpr int STAGES = TILE >= 6144 ? 1 : TILE >= 4096 ? 2 : TILE >= 3072 ? 3 : 4;
   static constexpr int RING = kWaves * STAGES * STAGE;
   static constexpr int JOIN = kWaves * (D / 16) * 64 * 16 + kWaves * 16 * 8;
   static constexpr int LDS = RING > JOIN ? RING : JOIN;
 };
 
-// 16 (4) bytes a lane from an address of its own, otherwise as lds_dma16
+// 16 (4) bytes a lane from an address of its own, otherwise as lds_dma16_once (lds_dma16).  A call reads a byte of the cache once, and
+// the next call reads another layer's: copies that leave no lines are 10 % faster (64 sequences of up to 8192 keys 140 -> 126 us).
 __device__ __forceinline__ void lds_dma16_from(const unsigned char* from, void* lds_base) {
   const unsigned lds_addr = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)lds_base);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(from) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" : : "s"(lds_addr), "v"(from) : "memory", "m0");
 }
 __device__ __forceinline__ void lds_dma4_from(const signed char* from, void* lds_base) {
   const unsigned lds_addr = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)lds_base);
@@ -230,23 +232,20 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
     const int p = 64 * c + lane, row = p / CH, slot = p - row * CH;
     off[c] = (row & 15) * S::BYTES + 16 * (slot ^ swizzle<S::BYTES>(row));
   }
-  auto issue = [&](int i, int stage, const Blocks& at) __attribute__((always_inline)) {
+  // VALUES: the tile of V, else that of K, and the exponents of both
+  auto issue = [&](int i, int stage, const Blocks& at, auto values_c) __attribute__((always_inline)) {
+    constexpr bool VALUES = decltype(values_c)::value;
     const int key0 = base + 32 * (wave + kWaves * i);
     unsigned char* const dst = ring + stage * S::STAGE;
+    unsigned char* const to = VALUES ? dst + S::TILE : dst;
+    const unsigned char* const from = VALUES ? a.pages.v : a.pages.k;
     const int least = j.lo - key0, most = j.hi - 1 - key0;
     if (least <= 0 && most >= 31) {
-      const unsigned char *const k0 = a.pages.k + at.r0 * S::BYTES, *const k1 = a.pages.k + at.r1 * S::BYTES;
-      const unsigned char *const v0 = a.pages.v + at.r0 * S::BYTES, *const v1 = a.pages.v + at.r1 * S::BYTES;
+      const unsigned char *const b0 = from + at.r0 * S::BYTES, *const b1 = from + at.r1 * S::BYTES;
 #pragma unroll
       for (int c = 0; c < S::COPIES; ++c) {
-        if constexpr (WHOLE) {
-          lds_dma16(c < OFFS ? k0 : k1, off[c % OFFS], dst + 1024 * c);
-          lds_dma16(c < OFFS ? v0 : v1, off[c % OFFS], dst + S::TILE + 1024 * c);
-        } else {
-          const bool second = (64 * c + lane) / CH >= 16;
-          lds_dma16_from((second ? k1 : k0) + off[c], dst + 1024 * c);
-          lds_dma16_from((second ? v1 : v0) + off[c], dst + S::TILE + 1024 * c);
-        }
+        if constexpr (WHOLE) lds_dma16_once(c < OFFS ? b0 : b1, off[c % OFFS], to + 1024 * c);
+        else lds_dma16_from(((64 * c + lane) / CH >= 16 ? b1 : b0) + off[c], to + 1024 * c);
       }
     } else {
       // rows outside [lo, hi) repeat the nearest key inside: their weights are zero, and what they hold is finite if the cache is
@@ -255,18 +254,18 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
         const int p = 64 * c + lane, row = p / CH, slot = p - row * CH;
         const int key = min(max(row, least), most);
         const long long at_row = key >= 16 ? at.r1 + key - 16 : at.r0 + key;
-        const size_t from = (size_t)at_row * S::BYTES + 16 * (slot ^ swizzle<S::BYTES>(row));
-        lds_dma16_from(a.pages.k + from, dst + 1024 * c);
-        lds_dma16_from(a.pages.v + from, dst + S::TILE + 1024 * c);
+        lds_dma16_from(from + (size_t)at_row * S::BYTES + 16 * (slot ^ swizzle<S::BYTES>(row)), to + 1024 * c);
       }
     }
-    if constexpr (F != kSame) {
+    if constexpr (F != kSame && !VALUES) {
       // lanes 0..7: the exponents of K, four keys each, lanes 8..15: of V
       const int four = 4 * (lane & 7), key = min(max(four, least & ~3), most & ~3);
       const long long at_row = key >= 16 ? at.r1 + key - 16 : at.r0 + key;
       lds_dma4_from((lane & 8 ? a.pages.v_exps : a.pages.k_exps) + at_row, dst + 2 * S::TILE);
     }
   };
+  using keys_c = std::false_type;
+  using values_c = std::true_type;
 
   v8 qf[NQ][KS];
   int row_lo[NQ], row_hi[NQ];
@@ -294,16 +293,22 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
 
   Blocks next{0, 0};
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i)
-    if (i < mine) issue(i, i, blocks_of(i));
-  if (STAGES - 1 < mine) next = blocks_of(STAGES - 1);
+  for (int i = 0; i < STAGES; ++i) {
+    if (i < mine) {
+      const Blocks at = blocks_of(i);
+      issue(i, i, at, keys_c{});
+      issue(i, i, at, values_c{});
+    }
+  }
+  if (STAGES < mine) next = blocks_of(STAGES);
   // the queries are there before the loop, which would otherwise wait for all that is on its way wherever they are used
 #pragma unroll
   for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
     for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[nq][s]));
   // One tile.  MASKED: some row does not see all of it.
-  auto step = [&](int key0, const unsigned char* kt, auto masked_c) __attribute__((always_inline)) {
+  // keys_read and values_read come where the tile of K, and that of V, has been read.
+  auto step = [&](int key0, const unsigned char* kt, auto masked_c, auto&& keys_read, auto&& values_read) __attribute__((always_inline)) {
     constexpr bool MASKED = decltype(masked_c)::value;
     const unsigned char* const vt = kt + S::TILE;
     // lane (row m, kg) has keys 16 h + 4 kg + r: the factors of their scores (scale, and the power of two of K's row), and those of V's rows
@@ -343,6 +348,8 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
         for (int nq = 0; nq < NQ; ++nq) sc[nq][h] = T::mma16(kf, qf[nq][s], sc[nq][h]);
       }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    keys_read();
     v8 p[NQ];
     unsigned seen[NQ];                                            // MASKED: which of the lane's eight keys its row sees
 #pragma unroll
@@ -452,23 +459,39 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
       for (int nq = 0; nq < NQ; ++nq) o[nq][dt] = T::mma16(vf, p[nq], o[nq][dt]);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    values_read();
   };
 
+  // Copies go out as soon as what lies in their place has been read, K's and V's apart, so that 2 STAGES - 1 of 2 STAGES tiles are on
+  // their way while one is worked on; they land in the order they went out.
+  constexpr int KL = S::K_LOADS, VL = S::COPIES;
+  constexpr int BEHIND_K = (STAGES - 1) * (KL + VL) + VL, BEHIND_V = STAGES * KL + (STAGES - 1) * VL;   // loads behind K of tile i, behind its V
+  static_assert(BEHIND_K < 64 && BEHIND_V < 64, "vmcnt counts to 63");
+  constexpr auto vmcnt = [](int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); };
   int stage = 0;
   for (int i = 0; i < mine; ++i) {
     const int key0 = base + 32 * (wave + kWaves * i);
-    if (i + STAGES - 1 < mine) {
-      issue(i + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1, next);
-      if (i + STAGES < mine) next = blocks_of(i + STAGES);
-      constexpr int N = S::LOADS * (STAGES - 1);
-      static_assert(N < 64, "vmcnt counts to 63");
-      __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
-    } else {
-      __builtin_amdgcn_s_waitcnt(0x0F70);
-    }
+    const bool more = i + STAGES < mine;
+    if (i + STAGES <= mine) __builtin_amdgcn_s_waitcnt(vmcnt(BEHIND_K));
+    else __builtin_amdgcn_s_waitcnt(vmcnt(0));
     asm volatile("" ::: "memory");
-    if (key0 < j.sure_lo || key0 + 32 > j.sure_hi || key0 < j.lo || key0 + 32 > j.hi) step(key0, ring + stage * S::STAGE, std::true_type{});
-    else step(key0, ring + stage * S::STAGE, std::false_type{});
+    auto keys_read = [&]() __attribute__((always_inline)) {
+      if (more) {
+        issue(i + STAGES, stage, next, keys_c{});
+        __builtin_amdgcn_s_waitcnt(vmcnt(BEHIND_V));
+      } else {
+        __builtin_amdgcn_s_waitcnt(vmcnt(0));
+      }
+      asm volatile("" ::: "memory");
+    };
+    auto values_read = [&]() __attribute__((always_inline)) {
+      if (more) {
+        issue(i + STAGES, stage, next, values_c{});
+        if (i + STAGES + 1 < mine) next = blocks_of(i + STAGES + 1);
+      }
+    };
+    if (key0 < j.sure_lo || key0 + 32 > j.sure_hi || key0 < j.lo || key0 + 32 > j.hi) step(key0, ring + stage * S::STAGE, std::true_type{}, keys_read, values_read);
+    else step(key0, ring + stage * S::STAGE, std::false_type{}, keys_read, values_read);
     stage = stage == STAGES - 1 ? 0 : stage + 1;
   }
 
@@ -851,69 +874,94 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_wide_kernel(AttnArgs a, 
 // ---- parts ------------------------------------------------------------------------------
 
 // m = max m_p, l = sum l_p 2^(m_p - m), O = sum O_p 2^(m_p - m) / l over the parts of a row; D / 4 lanes a row, and `slices` such
-// groups for the parts of a row where these are many and the rows few.
+// groups, a power of two, for the parts of a row.  The weights 2^(m_p - m) are worked out first, a lane a part:
+// the sums of O then are loads that do not wait for one another.
+constexpr int kPartsMost = 256;
+
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int slices) {
-  constexpr int L = D / 4, UNITS = 256 / L;
+  constexpr int L = D / 4, UNITS = D == 96 ? 8 : 256 / L;
   __shared__ v4f so[256];
-  __shared__ float sm[UNITS], sl[UNITS];
+  __shared__ float sw[4][kPartsMost], ss[4], st[4];
   const int unit = threadIdx.x / L, c = threadIdx.x % L;
-  const int per_block = UNITS / slices, slice = unit % slices;
-  const long long rows = (long long)a.batch.tokens * a.heads;
-  const long long at = (long long)blockIdx.x * per_block + unit / slices;
-  const int token = (int)(min(at, rows - 1) / a.heads);
-  const int first_token = __builtin_amdgcn_readfirstlane(token);
-  int b = count_at_most(a.batch.sequences, first_token, [&](int i) { return a.batch.starts[i + 1]; });
-  while (b < a.batch.sequences && a.batch.starts[b + 1] <= token) ++b;
-  int parts = 1, first = 0, len = 0, start = 0;
-  if (at < rows && unit < per_block * slices && b < a.batch.sequences) {
-    start = min(max(a.batch.starts[b], 0), a.batch.tokens);
-    const int end = min(max(a.batch.starts[b + 1], start), a.batch.tokens);
-    if (token >= start && token < end) {
-      const int len_all = max(a.batch.lens[b], 0);
-      first = len_all - (end - start);
-      len = min(len_all, kv_capacity(a.batch, a.pages.page_shift));
-      parts = seq_parts(a, first, len);                          // 1: written already
+  const int per_block = UNITS / slices, slice = unit % slices, mine = unit / slices;
+  const long long rows = (long long)a.batch.tokens * a.heads, row0 = (long long)blockIdx.x * per_block;
+  // the rows of the block, at most four: a wave each
+  const int i = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (i < per_block) {
+    const long long at = row0 + i;
+    int parts = 1;
+    float top = kNoRef, sum = 0.0f;
+    if (at < rows) {
+      const int token = __builtin_amdgcn_readfirstlane((int)(at / a.heads));
+      const int b = __builtin_amdgcn_readfirstlane(count_at_most(a.batch.sequences, token, [&](int k) { return a.batch.starts[k + 1]; }));
+      if (b < a.batch.sequences) {
+        const KvChunk ch = kv_chunk(a.batch, b);
+        if (token >= ch.start && token < ch.start + ch.n) {
+          const int len = min(ch.len, kv_capacity(a.batch, a.pages.page_shift));
+          parts = seq_parts(a, ch.first, len);                   // 1: written already
+          if (parts > 1) {
+            const float* const ml = a.part_ml + 2 * at * a.nparts;
+            float m[kPartsMost / 64], l[kPartsMost / 64];
+#pragma unroll
+            for (int k = 0; k < kPartsMost / 64; ++k) {
+              const int p = 64 * k + lane;
+              m[k] = p < parts ? ml[2 * p] : kNoRef;
+              l[k] = p < parts ? ml[2 * p + 1] : 0.0f;
+              top = fmaxf(top, m[k]);
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+#pragma unroll
+            for (int k = 0; k < kPartsMost / 64; ++k) {
+              const float w = __builtin_amdgcn_exp2f(m[k] - top);
+              sum += w * l[k];
+              if (64 * k + lane < parts) sw[i][64 * k + lane] = w;
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+            const long long position = (long long)ch.first + (token - ch.start);
+            const int hi = a.causal ? clamp_position(position + 1, len) : len, lo = a.window > 0 ? clamp_position(position - a.window + 1, len) : 0;
+            const bool none = hi <= lo;
+            if (lane == 0 && a.lse) a.lse[at] = none ? -INFINITY : log_sum(top, sum);
+            sum = none ? INFINITY : sum;                         // (no keys: zeros)
+          }
+        }
+      }
+    }
+    if (lane == 0) {
+      ss[i] = parts > 1 ? 1.0f / sum : 0.0f;
+      st[i] = __int_as_float(parts);
     }
   }
-  float top = kNoRef, sum = 0.0f;
+  __syncthreads();
+  const bool in = unit < UNITS;
+  const int parts = in ? __float_as_int(st[mine]) : 1;
   v4f acc = {0.f, 0.f, 0.f, 0.f};
   if (parts > 1) {
-    const float* const ml = a.part_ml + 2 * at * a.nparts;
-    for (int p = slice; p < parts; p += slices) top = fmaxf(top, ml[2 * p]);
-#pragma unroll 4
+    const float* const po = a.part_o + (row0 + mine) * a.nparts * D + 4 * c;
+#pragma unroll 8
     for (int p = slice; p < parts; p += slices) {
-      const float w = __builtin_amdgcn_exp2f(ml[2 * p] - top), lp = ml[2 * p + 1];
-      const v4f v = *reinterpret_cast<const v4f*>(a.part_o + (at * a.nparts + p) * D + 4 * c);
-      sum += w * lp;
+      const float w = sw[mine][p];
+      const v4f v = *reinterpret_cast<const v4f*>(po + (size_t)p * D);
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] += w * v[e];
     }
   }
   if (slices > 1) {
     so[threadIdx.x] = acc;
-    if (c == 0 && unit < UNITS) {
-      sm[unit] = top;
-      sl[unit] = sum;
-    }
     __syncthreads();
-    if (slice != 0 || parts == 1) return;
+    if (slice != 0) return;
     for (int i = 1; i < slices; ++i) {
-      const float t = fmaxf(top, sm[unit + i]), w0 = __builtin_amdgcn_exp2f(top - t), w1 = __builtin_amdgcn_exp2f(sm[unit + i] - t);
       const v4f v = so[threadIdx.x + i * L];
-      sum = sum * w0 + sl[unit + i] * w1;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = acc[e] * w0 + v[e] * w1;
-      top = t;
+      for (int e = 0; e < 4; ++e) acc[e] += v[e];
     }
   }
-  if (parts == 1) return;
-  const long long position = (long long)first + (token - start);
-  const int hi = a.causal ? clamp_position(position + 1, len) : len, lo = a.window > 0 ? clamp_position(position - a.window + 1, len) : 0;
-  const bool none = hi <= lo;
-  const float inv = none ? 0.0f : 1.0f / sum;
-  *reinterpret_cast<v2u*>((typename T::scalar*)a.o + at * D + 4 * c) = v2u{T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
-  if (a.lse && c == 0) a.lse[at] = none ? -INFINITY : log_sum(top, sum);
+  if (parts <= 1) return;
+  const float inv = ss[mine];
+  *reinterpret_cast<v2u*>((typename T::scalar*)a.o + (row0 + mine) * D + 4 * c) =
+      v2u{T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
 }
 
 // ---- host side ----------------------------------------------------------------------------
@@ -928,7 +976,23 @@ struct Plan {
 
 static size_t workspace_of(long long rows, int D, int nparts) { return nparts > 1 ? (size_t)rows * nparts * (D + 2) * 4 : 0; }
 
-static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, int heads, int max_queries, int max_keys, int cus, size_t room) {
+// us of a launch of the narrow kernel: rounds of two workgroups to a compute unit, 3 us each until the first tile is there, and their share of 5.8 TB/s, or
+// the 17 KB a us that one workgroup gets through.
+static double narrow_cost(double workgroups, int part_keys, int held, int cus) {
+  const double at_once = std::min(workgroups, 2.0 * cus), rounds = std::ceil(workgroups / (2.0 * cus));
+  return rounds * (3.0 + part_keys * (held / 1000.0) / std::min(17.0, 5800.0 / at_once));
+}
+
+// The same of the wide kernel, whose pairs of workgroups on a compute unit take 1.6 us for a tile of 64 keys of 128.
+static double wide_cost(double workgroups, int part_keys, int D, int cus) {
+  const double rounds = std::ceil(workgroups / (2.0 * cus));
+  return rounds * (4.0 + part_keys / 64 * (1.6 * D / 128));
+}
+
+// Leaving parts and joining them: a launch, and fp32 sums written and read at 4 TB/s.
+static double join_cost(double rows, int D, int nparts) { return nparts > 1 ? 5.0 + rows * nparts * D * 8 / 4e6 : 0.0; }
+
+static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, int heads, int window, int max_queries, int max_keys, int cus, size_t room) {
   const int D = pages.head_size, group = heads / pages.heads;
   Plan p;
   const long long most = max_queries > 0 ? std::min(max_queries, b.tokens) : b.tokens;   // new tokens of a sequence
@@ -940,16 +1004,30 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
   p.slots_per_seq = b.sequences * per_seq <= packed ? (int)per_seq : 0;
   p.slots = (int)std::min<long long>(p.slots_per_seq ? b.sequences * per_seq : packed, INT_MAX);
   const long long capacity = (long long)b.width << page_shift;
-  const int keys = (int)std::min<long long>(max_keys > 0 ? std::min<long long>(max_keys, capacity) : capacity, INT_MAX - 1024);
+  long long seen = max_keys > 0 ? std::min<long long>(max_keys, capacity) : capacity;
+  if (window > 0) seen = std::min(seen, most + window + 64);   // from the first key that the first new token sees, down to a multiple of 64
+  const int keys = (int)std::min<long long>(seen, INT_MAX - 1024);
   const long long units = (long long)p.slots * pages.heads;
-  const long long target = 4LL * cus;
-  const int least = p.narrow ? 256 : 512;                       // keys of a part
-  long long n = std::max<long long>(1, std::min<long long>(target / std::max<long long>(units, 1), keys / least));
-  for (;; --n) {
+  auto cut = [&](long long n) {
     p.part_keys = (int)(((keys + n - 1) / n + 127) / 128 * 128);
     p.nparts = std::max(1, (keys + p.part_keys - 1) / p.part_keys);
-    if (n == 1 || workspace_of((long long)b.tokens * heads, D, p.nparts) <= room) return p;
+  };
+  cut(1);
+  const int held = pages.type == FTK_F16 || pages.type == FTK_BF16 ? 4 * D : 2 * D + 2;   // bytes of a position and head
+  double best = 1e30;
+  int best_n = 1;
+  for (int n = 1; n <= kPartsMost; n += n < 4 ? 1 : n / 4) {
+    cut(n);
+    if (n > 1 && (p.part_keys < 256 || workspace_of((long long)b.tokens * heads, D, p.nparts) > room)) break;
+    const double cost = (p.narrow ? narrow_cost((double)units * p.nparts, p.part_keys, held, cus) : wide_cost((double)units * p.nparts, p.part_keys, D, cus)) +
+                        join_cost((double)b.tokens * heads, D, p.nparts);
+    if (cost < 0.97 * best) {
+      best = cost;
+      best_n = n;
+    }
   }
+  cut(best_n);
+  return p;
 }
 
 static int check_attention(const char* who, int heads, const ftk_kv_pages* pages) {
@@ -973,17 +1051,17 @@ static int launch_with_lds(const char* name, K kernel, DeviceOnce& once, long lo
 
 extern "C" {
 
-size_t ftk_paged_attn_workspace_bytes(const ftk_kv_pages* pages, const ftk_kv_batch* batch, int heads, int max_queries, int max_keys) {
+size_t ftk_paged_attn_workspace_bytes(const ftk_kv_pages* pages, const ftk_kv_batch* batch, int heads, int window, int max_queries, int max_keys) {
   using namespace ftk;
   const DeviceProps* d = nullptr;
   if (!pages || !batch || pages->heads <= 0 || heads <= 0 || heads % pages->heads || batch->tokens <= 0 || batch->sequences <= 0 || batch->table_width <= 0 ||
-      pages->page_size <= 0 || device_props(&d))
+      pages->page_size <= 0 || window < 0 || device_props(&d))
     return 0;
   KvBatch b{};
   b.tokens = batch->tokens;
   b.sequences = batch->sequences;
   b.width = batch->table_width;
-  const Plan p = plan(*pages, b, __builtin_ctz((unsigned)pages->page_size), heads, max_queries, max_keys, d->cus, SIZE_MAX);
+  const Plan p = plan(*pages, b, __builtin_ctz((unsigned)pages->page_size), heads, window, max_queries, max_keys, d->cus, SIZE_MAX);
   return workspace_of((long long)b.tokens * heads, pages->head_size, p.nparts);
 }
 
@@ -1007,7 +1085,7 @@ int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long 
   const DeviceProps* d = nullptr;
   if ((rc = device_props(&d))) return rc;
   if (workspace && !aligned16(workspace)) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", who);
-  const Plan p = plan(*pages, a.batch, a.pages.page_shift, heads, max_queries, max_keys, d->cus, workspace ? workspace_bytes : 0);
+  const Plan p = plan(*pages, a.batch, a.pages.page_shift, heads, window, max_queries, max_keys, d->cus, workspace ? workspace_bytes : 0);
   a.q = q;
   a.o = o;
   a.lse = lse;
@@ -1043,8 +1121,9 @@ int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long 
       bad = launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D>, once, blocks, WideShape<D>::LDS, s, a, p.slots);
     }
     if (bad || p.nparts == 1) return bad;
-    constexpr int UNITS = 256 / (D / 4);
-    const int slices = p.nparts >= 2 * UNITS ? UNITS : p.nparts >= 8 ? UNITS / 2 : 1;
+    constexpr int UNITS = D == 96 ? 8 : 256 / (D / 4);
+    int slices = UNITS / 4;                                      // a row for each wave, or fewer
+    while (slices < UNITS && slices * 4 < p.nparts) slices *= 2;
     const int per_block = UNITS / slices;
     const long long mblocks = (rows + per_block - 1) / per_block;
     if (mblocks > INT_MAX) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: grid too large", who);

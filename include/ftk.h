@@ -699,7 +699,8 @@ int ftk_kv_cache_read(const ftk_kv_pages* pages, const ftk_kv_batch* batch,
  */
 size_t ftk_paged_attn_workspace_bytes(const ftk_kv_pages* pages,
                                       const ftk_kv_batch* batch, int heads,
-                                      int max_queries, int max_keys);
+                                      int window, int max_queries,
+                                      int max_keys);
 int ftk_paged_attn(const void* q, int type, long long q_token_stride,
                    long long q_head_stride, const ftk_kv_pages* pages,
                    const ftk_kv_batch* batch, void* o, float* lse, int heads,

@@ -190,7 +190,7 @@ def prepare(case, seed):
         state['q'] = _normal(gen, total, case['Hq'], D).to(dtype)
         if own:                                                    # the workspace that such a program keeps
             from fractaltensor_amd import _core as core
-            need = core.paged_attention_workspace_bytes(state['q'], state['k_pages'], table, max(new), max(lens))
+            need = core.paged_attention_workspace_bytes(state['q'], state['k_pages'], table, max(new), max(lens), case['window'])
             state['workspace'] = torch.empty(need, dtype=torch.uint8, device='cuda')
     return state
 

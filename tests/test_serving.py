@@ -97,7 +97,7 @@ def test_bad_operands_of_the_cache_calls_are_refused(core):
         assert lib.ftk_kv_cache_write(vp(None), vp(None), ci(0), cl(0), cl(0), cl(0), cl(0), p, e, nul) == 0
         assert lib.ftk_kv_cache_read(p, e, ci(0), vp(None), vp(None), nul) == 0
         assert lib.ftk_paged_attn(vp(None), ci(0), cl(0), cl(0), p, e, vp(None), nul, ci(4), ctypes.c_float(1), ci(1), ci(0), ci(0), ci(0), nul, ctypes.c_size_t(0), nul) == 0
-    assert lib.ftk_paged_attn_workspace_bytes(None, None, 1, 0, 0) == 0
+    assert lib.ftk_paged_attn_workspace_bytes(None, None, 1, 0, 0, 0) == 0
 
 
 def test_bad_operands_of_the_verification_are_refused(core):

@@ -225,16 +225,16 @@ def test_attention_windows_and_without_a_causal_mask(core, causal, window, cache
     (BF16, I8, 128, 256, 1, 4, [40, 1], [3100, 2600]),       # the wide kernel, in parts
     (F16, None, 64, 16, 1, 2, [150], [2777]),
     (F16, I8, 96, 16, 1, 2, [70], [2100]),
-    (F16, E4M3, 32, 32, 1, 2, [70], [2100]),
+    (F16, E4M3, 32, 32, 1, 2, [70], [9000]),
 ])
 @pytest.mark.parametrize('window', [0, 1111])
 def test_long_sequences_in_parts(core, dtype, cache, D, page, heads, G, new, lens, window):
     batch = ref.make_batch(new, lens, page, 31)
     q = torch.empty((batch['tokens'], heads * G, D), dtype=dtype, device='cuda')
     like = torch.empty((batch['pages'], heads, page, D), dtype=cache or dtype, device='cuda')
-    need = core.paged_attention_workspace_bytes(q, like, ref.on_device(batch)[0], max(new), max(lens))
-    assert need > 0                                              # more than one part
-    for space in (None, torch.empty(need // 2, dtype=torch.uint8, device='cuda'), torch.empty(0, dtype=torch.uint8, device='cuda')):
+    need = core.paged_attention_workspace_bytes(q, like, ref.on_device(batch)[0], max(new), max(lens), window)
+    assert need > 0 or window                                    # more than one part
+    for space in (None, torch.empty(max(need // 2, 16), dtype=torch.uint8, device='cuda'), torch.empty(0, dtype=torch.uint8, device='cuda')):
         _attention_case(core, dtype, cache, D, page, heads, G, new, lens, 31, window=window, workspace=space)
 
 
