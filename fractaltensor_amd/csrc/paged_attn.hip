@@ -5,7 +5,7 @@
 //
 //   narrow  (at most 64 rows: decoding, drafts): bound by reading the cache once.  A workgroup has 16 NQ rows; its four waves cut the
 //           KEYS, each walking every fourth 32-key tile from copies straight into its own LDS, with no barrier in the loop.
-//   wide    (chunks and prompts): bound by the matrix pipe.  A wave has 32 rows, and the four waves of a workgroup share 64-key tiles.
+//   wide    (chunks and prompts): bound by the matrix pipe.  A wave has 32 rows, and the eight waves of a workgroup share 64-key tiles.
 //
 // Products are transposed in both, so that a lane has one row: S^T = K Q^T, O^T = V^T P^T with P as it comes out of the
 // first product (the contraction takes the keys in the order a lane holds them).  Long sequences are cut into parts of
@@ -66,8 +66,8 @@ template <int R>
 __device__ __forceinline__ bool find_job(const AttnArgs& a, int slot, int part, Job& j) {
   int tile;
   if (a.slots_per_seq > 0) {
-    j.b = slot / a.slots_per_seq;
-    tile = slot - j.b * a.slots_per_seq;
+    tile = slot / a.batch.sequences;
+    j.b = slot - tile * a.batch.sequences;
   } else {
     // sequence b has the slots from starts[b] * G / R + b on, at least as many as it needs
     const auto first_slot = [&](int b) { return (long long)min(max(a.batch.starts[b], 0), a.batch.tokens) * a.group / R + b; };
@@ -120,6 +120,13 @@ template <typename T>
 __device__ __forceinline__ const typename T::scalar* query_of(const AttnArgs& a, const Job& j, int kv_head, int row) {
   const int t = row / a.group, g = row - t * a.group;
   return (const typename T::scalar*)a.q + (j.start + t) * a.q_token + (long long)(kv_head * a.group + g) * a.q_head;
+}
+
+// The same pointer, known to be that of every lane.
+__device__ __forceinline__ const unsigned char* uniform(const unsigned char* p) {
+  const unsigned long long x = (unsigned long long)p;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)x), hi = __builtin_amdgcn_readfirstlane((unsigned)(x >> 32));
+  return (const unsigned char*)(((unsigned long long)hi << 32) | lo);
 }
 
 // First cache row (of a kv head) of the block of 16 keys that begins at `key`, a multiple of 16, or 16 times that of the key nearest to it
@@ -563,14 +570,20 @@ __global__ __launch_bounds__(kWaves * 64, NQ == 4 ? 1 : 2) void paged_narrow_ker
 
 // ---- wide -----------------------------------------------------------------------------
 
-constexpr int kWideRows = 32 * kWaves;
+// Eight waves of 32 rows.  A wave alternates between a phase of matrix instructions, M(t): O^T += V(t)^T P(t)^T and then the scores of
+// tile t + 1, and a phase of vector instructions, S(t): the weights of tile t; waves 4 to 7 run one phase behind waves 0 to 3, so that of the two
+// waves of a SIMD one feeds the matrix unit while the other works out weights.  A barrier ends every phase.  Waves 0 to 3 bring V(t + 1),
+// which is read from their M(t + 1) on, into one of three places, waves 4 to 7 K(t + 2) into that of K(t).  16-bit elements are copied straight into
+// LDS; codes of 8 bits go through registers, a tile earlier, and are written as 16-bit elements.
+constexpr int kWideWaves = 8, kWideRows = 32 * kWideWaves;
+constexpr float kMostSum = 32768.0f;          // a lane's sum of weights above this moves the reference
 
 template <int D>
 struct WideShape {
   static constexpr int BYTES = 2 * D, TILE = 64 * BYTES;
   static constexpr int ORS = BYTES + 16;                       // a padded row of the O tiles that the waves turn round at the end
-  static constexpr int RING = 4 * TILE;                        // two tiles of K, two of V
-  static constexpr int LDS = RING > kWaves * 32 * ORS ? RING : kWaves * 32 * ORS;
+  static constexpr int RING = 5 * TILE;                        // two tiles of K, three of V
+  static constexpr int LDS = RING > kWideWaves * 32 * ORS ? RING : kWideWaves * 32 * ORS;
 };
 
 // V: the transposing read of a 32-lane pass covers 4 keys x 64 bytes, which these bring into four different groups of 64 bytes
@@ -590,8 +603,12 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   using lds_v4s = __attribute__((address_space(3))) v4s;
   typedef short v8s __attribute__((ext_vector_type(8)));
 
+  using yes = std::true_type;
+  using no = std::false_type;
+
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = wave >> 2, cw = wave & 3;                   // which of the two run behind; whose 16 keys of a tile this wave brings
   const int jr = lane & 31, hh = lane >> 5;
   unsigned char* const Kb = smem;
   unsigned char* const Vb = smem + 2 * S::TILE;
@@ -607,12 +624,14 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   {
     const int t_lo = min(wrow0, j.rows - 1) / a.group, t_hi = (min(wrow0 + 32, j.rows) - 1) / a.group;
     const long long p_lo = (long long)j.first + t_lo, p_hi = (long long)j.first + t_hi;
-    wave_hi = min(a.causal ? clamp_position(p_hi + 1, j.len) : j.len, j.hi);
+    wave_hi = idle ? 0 : min(a.causal ? clamp_position(p_hi + 1, j.len) : j.len, j.hi);
     sure_hi = min(a.causal ? clamp_position(p_lo + 1, j.len) : j.len, j.hi);
     wave_lo = max(a.window > 0 ? clamp_position(p_lo - a.window + 1, j.len) : 0, j.lo);
     sure_lo = max(a.window > 0 ? clamp_position(p_hi - a.window + 1, j.len) : 0, j.lo);
   }
   const int my_lo = max(r.lo, j.lo), my_hi = min(r.hi, j.hi);
+  auto sees = [&](int t) __attribute__((always_inline)) { return base + 64 * t < wave_hi && base + 64 * t + 64 > wave_lo; };
+  auto masked = [&](int t) __attribute__((always_inline)) { return base + 64 * t < sure_lo || base + 64 * t + 64 > sure_hi; };
 
   v8 qf[DS];
   {
@@ -622,143 +641,113 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   }
   asm volatile("" ::: "memory");
 
-  // ---- tiles into LDS: wave w brings the 16 keys from 16 w on, which lie in one page
+  // ---- tiles into LDS: a wave brings the 16 keys from 16 cw on, which lie in one page; waves 0 to 3 those of V, the others those of K
   constexpr int CP = D / 32;                                   // 1 KB copies of 16 rows of 16-bit elements
-  unsigned k_src[CP], v_src[CP];
-  if constexpr (F == kSame) {
+  const int shift = a.pages.page_shift;
+  const long long page_rows = (long long)a.pages.heads << shift;
+  const long long head_row = (long long)kv_head << shift;
+  const int* const table = a.batch.table + (long long)j.b * a.batch.width;
+  const unsigned char* const from = (half ? a.pages.k : a.pages.v) + head_row * (F == kSame ? S::BYTES : D);
+  const signed char* const from_exps = F == kSame ? nullptr : (half ? a.pages.k_exps : a.pages.v_exps) + head_row;
+  // Cache row (from this head's first) of the 16 keys of this wave in tile t; of the nearest 16 in [lo, hi) where those lie outside (INSIDE: they
+  // do not).
+  auto block_at = [&](int t, auto inside_c) __attribute__((always_inline)) {
+    int key = base + 64 * t + 16 * cw;
+    if constexpr (!decltype(inside_c)::value) key = min(max(key, j.lo & ~15), (j.hi - 1) & ~15);
+    const int page = min(max(load_uniform(table, key >> shift), 0), a.pages.pages - 1);
+    return page * page_rows + (key & ((1 << shift) - 1));
+  };
+  // Where a lane's 16 bytes of a copy lie: with 64 and 128 elements the swizzle makes copy i's places those of the first with some bits turned over.
+  unsigned src[D == 96 ? CP : 1];
 #pragma unroll
-    for (int i = 0; i < CP; ++i) {
-      const int p = 64 * i + lane, rw = p / CH, slot = p - rw * CH, in_tile = 16 * wave + rw;
-      k_src[i] = rw * S::BYTES + 16 * (slot ^ swizzle<S::BYTES>(in_tile));
-      v_src[i] = rw * S::BYTES + 16 * (slot ^ v_swizzle<D>(in_tile));
-    }
+  for (int i = 0; i < (D == 96 ? CP : 1); ++i) {
+    const int p = 64 * i + lane, rw = p / CH, slot = p - rw * CH, in_tile = 16 * cw + rw;
+    src[i] = rw * S::BYTES + 16 * (slot ^ (half ? swizzle<S::BYTES>(in_tile) : v_swizzle<D>(in_tile)));
   }
-  auto block_at = [&](int t) __attribute__((always_inline)) { return block_row(a, j.b, kv_head, base + 64 * t + 16 * wave, j.lo, j.hi); };
-  auto copy = [&](int t, int buf, long long at) __attribute__((always_inline)) {
-    const int key0 = base + 64 * t + 16 * wave;
-    const unsigned char* const kb = a.pages.k + (size_t)at * S::BYTES;
-    const unsigned char* const vb = a.pages.v + (size_t)at * S::BYTES;
-    unsigned char* const kd = Kb + buf * S::TILE + wave * (16 * S::BYTES);
-    unsigned char* const vd = Vb + buf * S::TILE + wave * (16 * S::BYTES);
-    if (key0 >= j.lo && key0 + 16 <= j.hi) {
+  const unsigned turned = half && D != 96 ? 64 : 0;
+  auto source = [&](int i) __attribute__((always_inline)) { return D == 96 ? src[D == 96 ? i : 0] : (src[0] ^ (i * turned)) + 1024 * i; };
+  // 16 rows of tile t, `at` what block_at gave, into the tile at `to`
+  auto copy = [&](unsigned char* to, int t, long long at, auto inside_c) __attribute__((always_inline)) {
+    const int key0 = base + 64 * t + 16 * cw;
+    const unsigned char* const block = uniform(from + at * S::BYTES);
+    unsigned char* const dst = to + cw * (16 * S::BYTES);
+    if (decltype(inside_c)::value || (key0 >= j.lo && key0 + 16 <= j.hi)) {
 #pragma unroll
-      for (int i = 0; i < CP; ++i) {
-        lds_dma16(kb, k_src[i], kd + 1024 * i);
-        lds_dma16(vb, v_src[i], vd + 1024 * i);
-      }
+      for (int i = 0; i < CP; ++i) lds_dma16(block, source(i), dst + 1024 * i);
     } else {                                                   // rows outside [lo, hi) repeat the nearest key inside
       const int inside = min(max(key0, j.lo & ~15), (j.hi - 1) & ~15);   // where `at` begins
       const int least = max(j.lo - inside, 0), most = min(j.hi - 1 - inside, 15);
 #pragma unroll
       for (int i = 0; i < CP; ++i) {
-        const int p = 64 * i + lane, rw = p / CH;
-        const int to = min(max(key0 + rw - inside, least), most);
-        const int move = (to - rw) * S::BYTES;
-        lds_dma16(kb, k_src[i] + move, kd + 1024 * i);
-        lds_dma16(vb, v_src[i] + move, vd + 1024 * i);
+        const int rw = (64 * i + lane) / CH;
+        lds_dma16(block, source(i) + (min(max(key0 + rw - inside, least), most) - rw) * S::BYTES, dst + 1024 * i);
       }
     }
   };
-  // 8 bits: 16 codes a lane through registers, written as 16-bit elements
+  // 8 bits: 16 codes a lane
   constexpr int LD = (D + 63) / 64;                            // 16-byte pieces of a block of 16 rows, D of them, by 64 lanes
-  v4u kc[LD], vc[LD];
-  float ks[LD], vs[LD];
-  auto load = [&](int t, long long at) __attribute__((always_inline)) {
-    const int key0 = base + 64 * t + 16 * wave;
+  v4u codes[LD];
+  float scale[LD];
+  auto load = [&](int t, long long at, auto inside_c) __attribute__((always_inline)) {
+    const int key0 = base + 64 * t + 16 * cw;
     const int inside = min(max(key0, j.lo & ~15), (j.hi - 1) & ~15);
     const int least = max(j.lo - inside, 0), most = min(j.hi - 1 - inside, 15);
 #pragma unroll
     for (int i = 0; i < LD; ++i) {
       const int p = min(64 * i + lane, D - 1), rw = p / (D / 16), piece = p - rw * (D / 16);
-      const long long row_at = at + min(max(key0 + rw - inside, least), most);
-      kc[i] = *reinterpret_cast<const v4u*>(a.pages.k + (size_t)row_at * D + 16 * piece);
-      vc[i] = *reinterpret_cast<const v4u*>(a.pages.v + (size_t)row_at * D + 16 * piece);
-      ks[i] = power_of_two(a.pages.k_exps[row_at]);
-      vs[i] = power_of_two(a.pages.v_exps[row_at]);
+      const long long row_at = at + (decltype(inside_c)::value ? rw : min(max(key0 + rw - inside, least), most));
+      codes[i] = *reinterpret_cast<const v4u*>(from + row_at * D + 16 * piece);
+      scale[i] = power_of_two(from_exps[row_at]);
     }
   };
-  auto store = [&](int buf) __attribute__((always_inline)) {
+  auto store = [&](unsigned char* to) __attribute__((always_inline)) {
     if constexpr (F != kSame) {
 #pragma unroll
       for (int i = 0; i < LD; ++i) {
-        const int p = 64 * i + lane, rw = p / (D / 16), piece = p - rw * (D / 16), in_tile = 16 * wave + rw;
+        const int p = 64 * i + lane, rw = p / (D / 16), piece = p - rw * (D / 16), in_tile = 16 * cw + rw;
         if (D % 64 == 0 || p < D) {
-          unsigned char* const kd = Kb + buf * S::TILE + in_tile * S::BYTES;
-          unsigned char* const vd = Vb + buf * S::TILE + in_tile * S::BYTES;
+          const int swz = half ? swizzle<S::BYTES>(in_tile) : v_swizzle<D>(in_tile);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            *reinterpret_cast<v8*>(kd + 16 * ((2 * piece + c) ^ swizzle<S::BYTES>(in_tile))) = decode8<T, F>(v2u{kc[i][2 * c], kc[i][2 * c + 1]}, ks[i]);
-            *reinterpret_cast<v8*>(vd + 16 * ((2 * piece + c) ^ v_swizzle<D>(in_tile))) = decode8<T, F>(v2u{vc[i][2 * c], vc[i][2 * c + 1]}, vs[i]);
-          }
+          for (int c = 0; c < 2; ++c)
+            *reinterpret_cast<v8*>(to + in_tile * S::BYTES + 16 * ((2 * piece + c) ^ swz)) = decode8<T, F>(v2u{codes[i][2 * c], codes[i][2 * c + 1]}, scale[i]);
         }
       }
     }
   };
 
   // ---- fragments: K row 32 h + jr, bytes [32 s + 16 hh, +16); V the block of 4 keys x 16 columns that 16 lanes hand in
-  unsigned k_off[DS], v_off[DT];
-#pragma unroll
-  for (int s = 0; s < DS; ++s) k_off[s] = jr * S::BYTES + (((2 * s + hh) ^ swizzle<S::BYTES>(jr)) * 16);
+  // (The swizzles touch bits of the chunk's index that are zero in a row's address, so that a step's offset is the first one's with some bits turned
+  // over, and what they leave alone is added.)
+  constexpr int KX = D == 128 ? 15 : D == 64 ? 7 : 3, VX = D == 128 ? 12 : D == 64 ? 4 : 0;   // those bits
+  const unsigned k_off = jr * S::BYTES + ((hh ^ swizzle<S::BYTES>(jr)) * 16);
   const int v_row = 4 * hh + ((lane & 15) >> 2);
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) v_off[dt] = v_row * S::BYTES + (((4 * dt) ^ v_swizzle<D>(v_row)) * 16) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+  const unsigned v_off = v_row * S::BYTES + v_swizzle<D>(v_row) * 16 + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+  auto read_k = [&](const unsigned char* kt, int h, int s) __attribute__((always_inline)) {
+    return *reinterpret_cast<const v8*>(kt + 32 * h * S::BYTES + (k_off ^ (16 * (2 * s & KX))) + 16 * (2 * s & ~KX));
+  };
   auto read_v = [&](const unsigned char* vt, int key, int dt) __attribute__((always_inline)) {   // keys key + 4 hh + .. and 8 more
-    const unsigned char* const p = vt + key * S::BYTES + v_off[dt];
+    const unsigned char* const p = vt + key * S::BYTES + (v_off ^ (16 * (4 * dt & VX))) + 16 * (4 * dt & ~VX);
     const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p));
     const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p + 8 * S::BYTES));
     const v8s both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return __builtin_bit_cast(v8, both);
   };
 
-  v16f o[DT];
+  v16f o[DT], sc[2];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sc[h][e] = 0.0f;
   float ref = kNoRef, l = 0.0f;
+  v8 pf[2][2];
 
-  auto compute = [&](int t, auto masked_c) __attribute__((always_inline)) {
-    constexpr bool masked = decltype(masked_c)::value;
-    const int key0 = base + 64 * t;
-    const unsigned char* const kt = Kb + (t & 1) * S::TILE;
-    const unsigned char* const vt = Vb + (t & 1) * S::TILE;
-    v16f sc[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sc[h][e] = 0.0f;
-#pragma unroll
-      for (int s = 0; s < DS; ++s) sc[h] = T::mma32(*reinterpret_cast<const v8*>(kt + 32 * h * S::BYTES + k_off[s]), qf[s], sc[h]);
-    }
-    unsigned seen = 0xffffffffu;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        sc[h][e] *= a.scale_log2e;
-        if constexpr (masked) {
-          const int key = key0 + 32 * h + 8 * (e >> 2) + 4 * hh + (e & 3);
-          if (key < my_lo || key >= my_hi) {
-            sc[h][e] = -INFINITY;
-            seen &= ~(1u << (16 * h + e));
-          }
-        }
-      }
-    float mx = sc[0][0];
-#pragma unroll
-    for (int e = 1; e < 32; ++e) mx = fmaxf(mx, sc[e >> 4][e & 15]);
-    if (__builtin_amdgcn_ballot_w64(!(mx <= ref + kSlack)) != 0) {
-      mx = max_with_other_half(mx);
-      const float moved = fmaxf(ref, mx);
-      const float alpha = __builtin_amdgcn_exp2f(ref - moved);
-      ref = moved;
-      l *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
-    }
-    v8 pf[2][2];
+  // the weights of the tile's scores as operands of P V; returns this lane's share of their sum
+  auto weights = [&]() __attribute__((always_inline)) {
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -766,61 +755,189 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
         v4u w;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p0 = __builtin_amdgcn_exp2f(sc[h][8 * s + 2 * i] - ref), p1 = __builtin_amdgcn_exp2f(sc[h][8 * s + 2 * i + 1] - ref);
-          l += p0 + p1;
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[h][8 * s + 2 * i], a.scale_log2e, -ref));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[h][8 * s + 2 * i + 1], a.scale_log2e, -ref));
+          sum[i] += p0;
+          sum[i] += p1;
           w[i] = T::pack(p0, p1);
         }
         pf[h][s] = __builtin_bit_cast(v8, w);
       }
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  };
+  // The reference is not compared with every tile's maximum: weights are worked out against it as it is, and only when a lane's sum says that
+  // one of them may not fit 16 bits (or came out infinite, as all do before there is a reference) are the maxima taken, the reference moved, O and the sums
+  // rescaled and the tile's weights worked out again.  Any reference gives the same O / l.
+  auto phase_s = [&](int t, auto clean_c) __attribute__((always_inline)) {
+    if (!decltype(clean_c)::value && masked(t)) {
+      const int key0 = base + 64 * t + 4 * hh;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          v8 vf = read_v(vt, 32 * h + 16 * s, dt);
-          if constexpr (masked) {                              // see the narrow kernel
-            const unsigned bad = not_finite<T>(vf);
-            if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {
-              vf = zeros_at<T>(vf, bad);
-              v16f hits;
-#pragma unroll
-              for (int e = 0; e < 16; ++e) hits[e] = 0.0f;
-              hits = T::mma32(ones_at<T>(bad), ones_at<T>(seen >> (16 * h + 8 * s)), hits);
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (hits[e] > 0.0f) o[dt][e] = __builtin_nanf("");
-            }
-          }
-          o[dt] = T::mma32(vf, pf[h][s], o[dt]);
+        for (int e = 0; e < 16; ++e) {
+          const int key = key0 + 32 * h + 8 * (e >> 2) + (e & 3);
+          if (key < my_lo || key >= my_hi) sc[h][e] = -INFINITY;
         }
+    }
+    float psum = weights();
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(psum <= kMostSum)) != 0, 0)) {
+      float mx = sc[0][0];
+#pragma unroll
+      for (int e = 1; e < 32; ++e) mx = fmaxf(mx, sc[e >> 4][e & 15]);
+      const float moved = fmaxf(ref, max_with_other_half(mx) * a.scale_log2e);
+      const float alpha = __builtin_amdgcn_exp2f(ref - moved);
+      ref = moved;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+      psum = weights();
+    }
+    l += psum;
   };
 
-  long long at = 0;
+  constexpr int LA = 4;                                        // fragments read ahead of the matrix instruction that uses them
+  constexpr int NPV = 4 * DT, NQK = 2 * DS;
+  // PV: P V of a tile; QK: the scores of the next
+  auto phase_m = [&](const unsigned char* vt, const unsigned char* kt, auto pv_c, auto qk_c) __attribute__((always_inline)) {
+    constexpr bool PV = decltype(pv_c)::value, QK = decltype(qk_c)::value;
+    constexpr int N0 = PV ? NPV : 0, N = N0 + (QK ? NQK : 0);
+    auto read = [&](auto n_c) __attribute__((always_inline)) {
+      constexpr int n = decltype(n_c)::value;
+      if constexpr (n < N0) return read_v(vt, 32 * (n / (2 * DT)) + 16 * ((n % (2 * DT)) / DT), n % DT);
+      else return read_k(kt, (n - N0) % 2, (n - N0) / 2);
+    };
+    v8 fr[N];
+    static_for<(LA < N ? LA : N)>([&](auto i_c) __attribute__((always_inline)) { fr[decltype(i_c)::value] = read(i_c); });
+    __builtin_amdgcn_s_setprio(3);
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<N>([&](auto i_c) __attribute__((always_inline)) {
+      constexpr int i = decltype(i_c)::value;
+      if constexpr (i < N0) {
+        constexpr int h = i / (2 * DT), s = (i % (2 * DT)) / DT, dt = i % DT;
+        o[dt] = T::mma32(fr[i], pf[h][s], o[dt]);
+      } else {
+        constexpr int s = (i - N0) / 2, h = (i - N0) % 2;
+        v16f zero;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) zero[e] = 0.0f;
+        sc[h] = T::mma32(fr[i], qf[s], s == 0 ? zero : sc[h]);
+      }
+      if constexpr (i + LA < N) fr[i + LA] = read(std::integral_constant<int, i + LA>{});
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    __builtin_amdgcn_s_setprio(0);
+  };
+  // Whether a tile of V holds anything that is not finite.
+  auto all_finite = [&](const unsigned char* vt) __attribute__((always_inline)) {
+    unsigned bad = 0;
+#pragma unroll 1
+    for (int key = 0; key < 64; key += 16)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) bad |= not_finite<T>(read_v(vt, key, dt));
+    return __builtin_amdgcn_ballot_w64(bad != 0) == 0;
+  };
+  // P V of a tile whose keys not every row sees and whose values are not all finite: those leave the product (0 x inf), and make NaN
+  // of the rows that do see them.
+  auto careful_pv = [&](const unsigned char* vt, int t) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int step = 0; step < 4; ++step) {
+      const v8 p = step == 0 ? pf[0][0] : step == 1 ? pf[0][1] : step == 2 ? pf[1][0] : pf[1][1];
+      const int key0 = base + 64 * t + 16 * step + 4 * hh;
+      unsigned seen = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int key = key0 + 8 * (e >> 2) + (e & 3);
+        if (key >= my_lo && key < my_hi) seen |= 1u << e;
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const v8 vf = read_v(vt, 16 * step, dt);
+        const unsigned bad = not_finite<T>(vf);
+        v16f hits;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) hits[e] = 0.0f;
+        hits = T::mma32(ones_at<T>(bad), ones_at<T>(seen), hits);
+        o[dt] = T::mma32(zeros_at<T>(vf, bad), p, o[dt]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (hits[e] > 0.0f) o[dt][e] = __builtin_nanf("");
+      }
+    }
+  };
+  // a barrier that waits for nothing of the wave's own: whoever wrote what the barrier publishes has waited before it
+  auto phase_barrier = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
   if (ntiles > 0) {
-    at = block_at(0);
-    if constexpr (F == kSame) copy(0, 0, at);
-    else load(0, at);
-    if (ntiles > 1) at = block_at(1);
-  }
-  for (int t = 0; t < ntiles; ++t) {
+    // V(0) by waves 0 to 3, K(0) by the others, and K(1) behind it
+    constexpr int AHEAD = F == kSame ? 0 : 1;                  // codes go through registers a tile earlier
     if constexpr (F == kSame) {
-      __builtin_amdgcn_s_waitcnt(0x0F70);                      // vmcnt(0): this wave's copies of tile t
-      __syncthreads();
-      if (t + 1 < ntiles) copy(t + 1, (t + 1) & 1, at);
+      copy(half ? Kb : Vb, 0, block_at(0, no{}), no{});
+      if (half && ntiles > 1) copy(Kb + S::TILE, 1, block_at(1, no{}), no{});
     } else {
-      store(t & 1);
-      __syncthreads();
-      if (t + 1 < ntiles) load(t + 1, at);
+      load(0, block_at(0, no{}), no{});
+      store(half ? Kb : Vb);
+      if (ntiles > 1) load(1, block_at(1, no{}), no{});
+      if (half) {
+        if (ntiles > 1) store(Kb + S::TILE);
+        if (ntiles > 2) load(2, block_at(2, no{}), no{});
+      }
     }
-    if (t + 2 < ntiles) at = block_at(t + 2);
-    const int key0 = base + 64 * t;
-    if (!idle && key0 < wave_hi && key0 + 64 > wave_lo) {
-      if (key0 < sure_lo || key0 + 64 > sure_hi) compute(t, std::true_type{});
-      else compute(t, std::false_type{});
+    const int ahead = (half ? 2 : 1) + AHEAD;                  // S(t) asks for tile t + ahead
+    long long next = ahead < ntiles ? block_at(ahead, no{}) : 0;
+    __builtin_amdgcn_s_waitcnt(0x0F70);                        // vmcnt(0)
+    __syncthreads();
+    phase_m(Vb, Kb, no{}, yes{});
+    int vcur = 2 * S::TILE, vnext = 3 * S::TILE, vfree = 4 * S::TILE;             // V(t), V(t + 1), the place of V(t + 2)
+    int kcur = 0, knext = S::TILE;                                                // K(t), K(t + 1)
+    // Tiles [clean, dirty): every row sees all of them, and the tiles that they ask for lie inside [lo, hi)
+    const int whole = (j.hi - base) / 64;
+    const int clean = (max(j.sure_lo, j.lo) - base + 63) / 64, dirty = min((min(j.sure_hi, j.hi) - base) / 64, whole - 2 - AHEAD - 1);
+    auto turn = [&](int t, auto clean_c) __attribute__((always_inline)) {
+      constexpr bool CLEAN = decltype(clean_c)::value;
+      // K(t) was last read in the phase before this one, V(t - 2) two before
+      const int bring = t + ahead;
+      if constexpr (F == kSame) {
+        if (CLEAN || bring < ntiles) copy(smem + (half ? kcur : vnext), bring, next, clean_c);
+      } else {
+        if (CLEAN || bring - 1 < ntiles) store(smem + (half ? kcur : vnext));
+        if (CLEAN || bring < ntiles) load(bring, next, clean_c);
+      }
+      if (CLEAN || bring + 1 < ntiles) next = block_at(bring + 1, clean_c);
+      if (CLEAN || sees(t)) phase_s(t, clean_c);
+      if constexpr (F != kSame) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // what was stored
+      phase_barrier();
+      const unsigned char *const vt = smem + vcur, *const kt = smem + knext;
+      if constexpr (CLEAN) {
+        phase_m(vt, kt, yes{}, yes{});
+      } else {
+        if (sees(t)) {
+          if (masked(t) && __builtin_expect(!all_finite(vt), 0)) careful_pv(vt, t);
+          else phase_m(vt, kt, yes{}, no{});
+        }
+        if (t + 1 < ntiles) phase_m(vt, kt, no{}, yes{});
+      }
+      if constexpr (F == kSame) __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the copies that this wave asked for in S(t)
+      phase_barrier();
+      const int v = vcur, k = kcur;
+      vcur = vnext;
+      vnext = vfree;
+      vfree = v;
+      kcur = knext;
+      knext = k;
+    };
+    if (half) phase_barrier();
+    for (int t = 0; t < ntiles; ++t) {
+      if (t == clean)
+        for (; t < dirty; ++t) turn(t, yes{});
+      turn(t, no{});
     }
+    if (!half) phase_barrier();
   }
-  __syncthreads();
   l += __shfl_xor(l, 32);
   if (j.parts > 1) {
     if (wrow0 + jr < j.rows) {
@@ -839,7 +956,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
     return;
   }
   if (idle) return;
-  // the wave turns its 32 x D tile round through LDS and stores whole rows
+  // the wave turns its 32 x D tile round through LDS (nobody reads tiles any more) and stores whole rows
   const bool none = r.hi <= r.lo;
   const float inv = none ? 0.0f : 1.0f / l;
   unsigned char* const ot = smem + wave * (32 * S::ORS);
@@ -860,7 +977,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
 }
 
 template <typename T, KvFormat F, int D>
-__global__ __launch_bounds__(kWaves * 64, 2) void paged_wide_kernel(AttnArgs a, int slots) {
+__global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs a, int slots) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   // the head goes fastest, so that the row blocks of a head meet on the XCDs that have its keys; the last rows, with the most keys
   // under a causal mask, go first
@@ -1001,7 +1118,8 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
   p.nq = most_rows <= 16 ? 1 : most_rows <= 32 ? 2 : 4;
   const int R = p.narrow ? 16 * p.nq : kWideRows;
   const long long per_seq = (most_rows + R - 1) / R, packed = (long long)b.tokens * group / R + b.sequences;
-  p.slots_per_seq = b.sequences * per_seq <= packed ? (int)per_seq : 0;
+  // numbered by row blocks, the last of all sequences first, unless most of such slots would be empty
+  p.slots_per_seq = b.sequences * per_seq <= 2 * packed ? (int)per_seq : 0;
   p.slots = (int)std::min<long long>(p.slots_per_seq ? b.sequences * per_seq : packed, INT_MAX);
   const long long capacity = (long long)b.width << page_shift;
   long long seen = max_keys > 0 ? std::min<long long>(max_keys, capacity) : capacity;
@@ -1036,14 +1154,14 @@ static int check_attention(const char* who, int heads, const ftk_kv_pages* pages
 }
 
 template <typename K, typename... Args>
-static int launch_with_lds(const char* name, K kernel, DeviceOnce& once, long long blocks, int lds, hipStream_t s, Args... args) {
+static int launch_with_lds(const char* name, K kernel, DeviceOnce& once, long long blocks, int waves, int lds, hipStream_t s, Args... args) {
   if (blocks > INT_MAX) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "ftk_paged_attn: grid too large");
   unsigned bit;
   if (once.pending(&bit)) {
     FTK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     once.done(bit);
   }
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kWaves * 64), lds, s, args...);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(waves * 64), lds, s, args...);
   return check_launch(name);
 }
 
@@ -1113,12 +1231,12 @@ int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long 
       auto launch = [&](auto nq) -> int {
         constexpr int NQ = decltype(nq)::value;
         static DeviceOnce once;
-        return launch_with_lds("paged_narrow_kernel", paged_narrow_kernel<T, F, D, NQ>, once, blocks, NarrowShape<F, D>::LDS, s, a);
+        return launch_with_lds("paged_narrow_kernel", paged_narrow_kernel<T, F, D, NQ>, once, blocks, kWaves, NarrowShape<F, D>::LDS, s, a);
       };
       bad = p.nq == 1 ? launch(std::integral_constant<int, 1>{}) : p.nq == 2 ? launch(std::integral_constant<int, 2>{}) : launch(std::integral_constant<int, 4>{});
     } else {
       static DeviceOnce once;
-      bad = launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D>, once, blocks, WideShape<D>::LDS, s, a, p.slots);
+      bad = launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D>, once, blocks, kWideWaves, WideShape<D>::LDS, s, a, p.slots);
     }
     if (bad || p.nparts == 1) return bad;
     constexpr int UNITS = D == 96 ? 8 : 256 / (D / 4);
