@@ -24,6 +24,11 @@ constexpr int kWaves = 4;
 constexpr float kNoRef = -3.402823466e38f;   // the reference before any score: finite, so that -inf minus it is -inf
 constexpr float kSlack = 8.0f;               // the reference moves when a score is above it by 2^8 in the weights
 
+// How the keys of a sequence are cut: at most nparts parts of part_keys keys, the last of which takes what is left.
+struct Cut {
+  int nparts, part_keys;
+};
+
 struct AttnArgs {
   const void* q;
   void* o;
@@ -34,9 +39,11 @@ struct AttnArgs {
   int heads, group;                           // query heads, query heads of a kv head
   float scale_log2e;
   int causal, window;
-  int slots_per_seq;                          // blocks of rows of a sequence; 0: numbered over the packed rows
-  int nparts, part_keys;
-  float *part_o, *part_ml;                    // [tokens * heads][nparts][D], [..][2]
+  int slots, slots_per_seq;                   // blocks of rows, and those of a sequence (0: they are numbered over the packed rows)
+  Cut cut, small;                             // `small` for sequences of at most small_rows rows
+  int small_rows;
+  int stride;                                 // parts that there is room for
+  float *part_o, *part_ml;                    // [tokens * heads][stride][D], [..][2]
 };
 
 // ---- which rows and which keys a workgroup has ----------------------------------------
@@ -54,17 +61,17 @@ struct Job {
 __device__ __forceinline__ int seq_first_key(const AttnArgs& a, int first) {
   return a.window > 0 ? (int)max(0LL, (long long)first - a.window + 1) & ~63 : 0;
 }
-__device__ __forceinline__ int seq_parts(const AttnArgs& a, int first, int len) {
-  if (a.nparts == 1) return 1;
+__device__ __forceinline__ Cut seq_cut(const AttnArgs& a, int n) { return n * a.group <= a.small_rows ? a.small : a.cut; }
+__device__ __forceinline__ int seq_parts(const AttnArgs& a, const Cut& cut, int first, int len) {
+  if (cut.nparts == 1) return 1;
   const int keys = max(0, len - seq_first_key(a, first));
-  return min(max((int)(((long long)keys + a.part_keys - 1) / a.part_keys), 1), a.nparts);
+  return min(max((int)(((long long)keys + cut.part_keys - 1) / cut.part_keys), 1), cut.nparts);
 }
 __device__ __forceinline__ int clamp_position(long long x, int len) { return (int)(x < 0 ? 0 : x > len ? len : x); }
 
-// False: there is nothing to do in this slot.
+// The sequence and the block of R of its rows that a slot stands for; false: none.
 template <int R>
-__device__ __forceinline__ bool find_job(const AttnArgs& a, int slot, int part, Job& j) {
-  int tile;
+__device__ __forceinline__ bool find_rows(const AttnArgs& a, int slot, int* b, int* tile) {
   if (a.slots_per_seq > 0) {
     // Row blocks go out in three passes over the sequences, the last third of every sequence's first: the blocks of a sequence share
     // its keys in the caches, and a launch ends with blocks that see few keys under a causal mask.  (Four prompts of up to 4096 tokens: 177 us, 183 in
@@ -73,30 +80,34 @@ __device__ __forceinline__ bool find_job(const AttnArgs& a, int slot, int part, 
     for (int pass = 3;; --pass) {
       const int take = (left + pass - 1) / pass;
       if (pass == 1 || r < take * a.batch.sequences) {
-        j.b = min(r / max(take, 1), a.batch.sequences - 1);
-        tile = left - 1 - (r - j.b * take);
-        break;
+        *b = min(r / max(take, 1), a.batch.sequences - 1);
+        *tile = left - 1 - (r - *b * take);
+        return *tile >= 0;
       }
       r -= take * a.batch.sequences;
       left -= take;
     }
-    if (tile < 0) return false;
-  } else {
-    // sequence b has the slots from starts[b] * G / R + b on, at least as many as it needs
-    const auto first_slot = [&](int b) { return (long long)min(max(a.batch.starts[b], 0), a.batch.tokens) * a.group / R + b; };
-    j.b = max(count_at_most(a.batch.sequences, slot, first_slot) - 1, 0);
-    j.b = __builtin_amdgcn_readfirstlane(j.b);
-    const long long t = slot - first_slot(j.b);
-    if (t < 0) return false;
-    tile = (int)t;
   }
-  const KvChunk c = kv_chunk(a.batch, j.b);
+  // sequence b has the slots from starts[b] * G / R + b on, at least as many as it needs; the last go out first
+  const int from_end = a.slots - 1 - slot;
+  const auto first_slot = [&](int i) { return (long long)min(max(a.batch.starts[i], 0), a.batch.tokens) * a.group / R + i; };
+  *b = __builtin_amdgcn_readfirstlane(max(count_at_most(a.batch.sequences, from_end, first_slot) - 1, 0));
+  const long long t = from_end - first_slot(*b);
+  *tile = __builtin_amdgcn_readfirstlane((int)t);
+  return t >= 0;
+}
+
+// False: there is nothing to do.  small: the sequence is one of at most small_rows rows, or is not meant.
+template <int R>
+__device__ __forceinline__ bool find_job(const AttnArgs& a, int b, int tile, int part, bool small, Job& j) {
+  j.b = b;
+  const KvChunk c = kv_chunk(a.batch, b);
   j.start = c.start;
   j.n = c.n;
   j.first = c.first;
   j.rows = c.n * a.group;
   j.row0 = tile * R;
-  if (tile >= (j.rows + R - 1) / R) return false;
+  if (tile >= (j.rows + R - 1) / R || (j.rows <= a.small_rows) != small) return false;
   j.len = min(c.len, kv_capacity(a.batch, a.pages.page_shift));
   const int t_lo = j.row0 / a.group, t_hi = (min(j.row0 + R, j.rows) - 1) / a.group;
   const long long p_lo = (long long)c.first + t_lo, p_hi = (long long)c.first + t_hi;
@@ -105,12 +116,13 @@ __device__ __forceinline__ bool find_job(const AttnArgs& a, int slot, int part, 
   j.lo = a.window > 0 ? clamp_position(p_lo - a.window + 1, j.len) : 0;
   j.sure_lo = a.window > 0 ? clamp_position(p_hi - a.window + 1, j.len) : 0;
   j.part = part;
-  j.parts = seq_parts(a, c.first, j.len);
+  const Cut cut = small ? a.small : a.cut;
+  j.parts = seq_parts(a, cut, c.first, j.len);
   if (part >= j.parts) return false;
   if (j.parts > 1) {
-    const long long from = (long long)seq_first_key(a, c.first) + (long long)part * a.part_keys;
+    const long long from = (long long)seq_first_key(a, c.first) + (long long)part * cut.part_keys;
     j.lo = max(j.lo, clamp_position(from, j.len));
-    if (part < j.parts - 1) j.hi = min(j.hi, clamp_position(from + a.part_keys, j.len));
+    if (part < j.parts - 1) j.hi = min(j.hi, clamp_position(from + cut.part_keys, j.len));
   }
   return true;
 }
@@ -216,8 +228,9 @@ __device__ __forceinline__ void lds_dma4_from(const signed char* from, void* lds
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds_addr), "v"(from) : "memory", "m0");
 }
 
+// tid: of the 256 threads that work together
 template <typename T, KvFormat F, int D, int NQ>
-__device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j, int kv_head, unsigned char* smem) {
+__device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j, int kv_head, unsigned char* smem, int tid) {
   using S = NarrowShape<F, D>;
   using v8 = typename T::v8;
   using scalar = typename T::scalar;
@@ -226,7 +239,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
   using lds_v2i = __attribute__((address_space(3))) v2i;
   typedef short v8s __attribute__((ext_vector_type(8)));
 
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, kg = lane >> 4;
   const int base = j.lo & ~31;
@@ -555,12 +568,12 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
         if (j.parts == 1) {
           *reinterpret_cast<v2u*>((scalar*)a.o + r.at * D + 4 * g) = v2u{T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
         } else {
-          *reinterpret_cast<v4f*>(a.part_o + (r.at * a.nparts + j.part) * D + 4 * g) = acc;
+          *reinterpret_cast<v4f*>(a.part_o + (r.at * a.stride + j.part) * D + 4 * g) = acc;
         }
       }
       if (tid < 16) {
         if (j.parts > 1) {
-          float* const ml = a.part_ml + 2 * (r.at * a.nparts + j.part);
+          float* const ml = a.part_ml + 2 * (r.at * a.stride + j.part);
           ml[0] = top;
           ml[1] = sum;
         } else if (a.lse) {
@@ -575,10 +588,11 @@ template <typename T, KvFormat F, int D, int NQ>
 __global__ __launch_bounds__(kWaves * 64, NQ == 4 ? 1 : 2) void paged_narrow_kernel(AttnArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int kv_head = blockIdx.x % a.pages.heads, rest = blockIdx.x / a.pages.heads;
-  const int slot = rest / a.nparts, part = rest - slot * a.nparts;
+  const int slot = rest / a.cut.nparts, part = rest - slot * a.cut.nparts;
   Job j;
-  if (!find_job<16 * NQ>(a, slot, part, j)) return;
-  narrow_attention<T, F, D, NQ>(a, j, kv_head, smem);
+  int b, tile;
+  if (!find_rows<16 * NQ>(a, slot, &b, &tile) || !find_job<16 * NQ>(a, b, tile, part, false, j)) return;
+  narrow_attention<T, F, D, NQ>(a, j, kv_head, smem, threadIdx.x);
 }
 
 // ---- wide -----------------------------------------------------------------------------
@@ -961,14 +975,14 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   l += __shfl_xor(l, 32);
   if (j.parts > 1) {
     if (wrow0 + jr < j.rows) {
-      float* const po = a.part_o + (r.at * a.nparts + j.part) * D;
+      float* const po = a.part_o + (r.at * a.stride + j.part) * D;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
           *reinterpret_cast<v4f*>(po + 32 * dt + 8 * g + 4 * hh) = v4f{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
       if (hh == 0) {
-        float* const ml = a.part_ml + 2 * (r.at * a.nparts + j.part);
+        float* const ml = a.part_ml + 2 * (r.at * a.stride + j.part);
         ml[0] = ref;
         ml[1] = l;
       }
@@ -996,118 +1010,141 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   }
 }
 
+// The first `pairs` workgroups take sequences of at most small_rows = 16 rows, which would leave seven of the eight waves without any: two
+// (sequence, head, part) each, by four waves that cut the keys as in the narrow kernel.  They read while the others multiply.  (A chunk of 512 tokens
+// beside five sequences that decode, 16 heads, 4 of keys, up to 16384 of them: 165 us with all on the wide form, CHUNK_US so.)
 template <typename T, KvFormat F, int D>
-__global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs a, int slots) {
+__global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs a, int pairs) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  // the head goes fastest, so that the row blocks of a head meet on the XCDs that have its keys
-  const int kv_head = blockIdx.x % a.pages.heads, rest = blockIdx.x / a.pages.heads;
-  const int slot = rest / a.nparts, part = rest - slot * a.nparts;
   Job j;
-  if (!find_job<kWideRows>(a, a.slots_per_seq ? slot : slots - 1 - slot, part, j)) return;
+  if ((int)blockIdx.x < pairs) {
+    const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int item = 2 * blockIdx.x + half, kv_head = item % a.pages.heads, rest = item / a.pages.heads;
+    const int b = rest / a.small.nparts, part = rest - b * a.small.nparts;
+    if (b < a.batch.sequences && find_job<16>(a, b, 0, part, true, j)) {
+      narrow_attention<T, F, D, 1>(a, j, kv_head, smem + half * NarrowShape<F, D>::LDS, threadIdx.x & 255);
+    } else {                                                     // the other half's two barriers
+      __syncthreads();
+      __syncthreads();
+    }
+    return;
+  }
+  // the head goes fastest, so that the row blocks of a head meet on the XCDs that have its keys
+  const int id = blockIdx.x - pairs, kv_head = id % a.pages.heads, rest = id / a.pages.heads;
+  const int slot = rest / a.cut.nparts, part = rest - slot * a.cut.nparts;
+  int b, tile;
+  if (!find_rows<kWideRows>(a, slot, &b, &tile) || !find_job<kWideRows>(a, b, tile, part, false, j)) return;
   wide_attention<T, F, D>(a, j, kv_head, smem);
 }
 
 // ---- parts ------------------------------------------------------------------------------
 
-// m = max m_p, l = sum l_p 2^(m_p - m), O = sum O_p 2^(m_p - m) / l over the parts of a row; D / 4 lanes a row, and `slices` such
-// groups, a power of two, for the parts of a row.  The weights 2^(m_p - m) are worked out first, a lane a part:
-// the sums of O then are loads that do not wait for one another.
 constexpr int kPartsMost = 256;
 
-template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int slices) {
-  constexpr int L = D / 4, UNITS = D == 96 ? 8 : 256 / L;
-  __shared__ v4f so[256];
-  __shared__ float sw[4][kPartsMost], ss[4], st[4];
-  const int unit = threadIdx.x / L, c = threadIdx.x % L;
-  const int per_block = UNITS / slices, slice = unit % slices, mine = unit / slices;
-  const long long rows = (long long)a.batch.tokens * a.heads, row0 = (long long)blockIdx.x * per_block;
-  // the rows of the block, at most four: a wave each
-  const int i = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  if (i < per_block) {
-    const long long at = row0 + i;
-    int parts = 1;
-    float top = kNoRef, sum = 0.0f;
-    if (at < rows) {
-      const int token = __builtin_amdgcn_readfirstlane((int)(at / a.heads));
-      const int b = __builtin_amdgcn_readfirstlane(count_at_most(a.batch.sequences, token, [&](int k) { return a.batch.starts[k + 1]; }));
-      if (b < a.batch.sequences) {
-        const KvChunk ch = kv_chunk(a.batch, b);
-        if (token >= ch.start && token < ch.start + ch.n) {
-          const int len = min(ch.len, kv_capacity(a.batch, a.pages.page_shift));
-          parts = seq_parts(a, ch.first, len);                   // 1: written already
-          if (parts > 1) {
-            const float* const ml = a.part_ml + 2 * at * a.nparts;
-            float m[kPartsMost / 64], l[kPartsMost / 64];
+// The parts of the sequence that a packed row belongs to (1: nothing to join), and the keys [*lo, *hi) that it sees.  first_token: that of the wave's first lane.
+__device__ __forceinline__ int row_parts(const AttnArgs& a, int token, int first_token, int* lo, int* hi) {
+  int b = count_at_most(a.batch.sequences, first_token, [&](int k) { return a.batch.starts[k + 1]; });
+  while (b < a.batch.sequences && a.batch.starts[b + 1] <= token) ++b;
+  if (b >= a.batch.sequences) return 1;
+  const int start = min(max(a.batch.starts[b], 0), a.batch.tokens), end = min(max(a.batch.starts[b + 1], start), a.batch.tokens);
+  if (token < start || token >= end) return 1;
+  const int all = max(a.batch.lens[b], 0), first = all - (end - start), len = min(all, kv_capacity(a.batch, a.pages.page_shift));
+  const long long position = (long long)first + (token - start);
+  *hi = a.causal ? clamp_position(position + 1, len) : len;
+  *lo = a.window > 0 ? clamp_position(position - a.window + 1, len) : 0;
+  return seq_parts(a, seq_cut(a, end - start), first, len);
+}
+
+// m = max m_p, l = sum l_p 2^(m_p - m), O = sum O_p 2^(m_p - m) / l over the parts of a row.  A wave (WAVES = 4: the four of a block) to a row: the
+// weights 2^(m_p - m) first, a lane a part, then the sums of O, D / 4 lanes a part, by loads that do not wait for one another.  A wave is given `rows` rows: one, or
+// many where only small sequences are cut and most waves find nothing to do.
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) {
+  constexpr int L = D / 4, SL = 64 / L, K = kPartsMost / 64;    // lanes of a part, parts at once
+  __shared__ v4f so[WAVES == 4 ? 4 * L : 1];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, slice = lane / L, c = lane - slice * L;
+  const long long all_rows = (long long)a.batch.tokens * a.heads;
+  const long long row0 = ((long long)blockIdx.x * (WAVES == 4 ? 1 : 4) + (WAVES == 4 ? 0 : wave)) * rows;
+  if (row0 >= all_rows) return;
+  int lo = 0, hi = 0, parts = 1;
+  {
+    const long long at = min(row0 + min(lane, rows - 1), all_rows - 1);
+    const int token = (int)(at / a.heads);
+    parts = row_parts(a, token, __builtin_amdgcn_readfirstlane(token), &lo, &hi);
+  }
+  unsigned long long todo = __builtin_amdgcn_ballot_w64(lane < rows && row0 + lane < all_rows && parts > 1);
+  while (todo) {
+    const int r = (int)__builtin_ctzll(todo);
+    todo &= todo - 1;
+    const long long at = row0 + r;
+    const int n = __builtin_amdgcn_readlane(parts, r);
+    const bool none = __builtin_amdgcn_readlane(hi, r) <= __builtin_amdgcn_readlane(lo, r);
+    const float* const ml = a.part_ml + 2 * at * a.stride;
+    float m[K], w[K], top = kNoRef, sum = 0.0f;
 #pragma unroll
-            for (int k = 0; k < kPartsMost / 64; ++k) {
-              const int p = 64 * k + lane;
-              m[k] = p < parts ? ml[2 * p] : kNoRef;
-              l[k] = p < parts ? ml[2 * p + 1] : 0.0f;
-              top = fmaxf(top, m[k]);
-            }
+    for (int k = 0; k < K; ++k) {
+      const int p = 64 * k + lane;
+      m[k] = p < n ? ml[2 * p] : kNoRef;
+      w[k] = p < n ? ml[2 * p + 1] : 0.0f;
+      top = fmaxf(top, m[k]);
+    }
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
 #pragma unroll
-            for (int k = 0; k < kPartsMost / 64; ++k) {
-              const float w = __builtin_amdgcn_exp2f(m[k] - top);
-              sum += w * l[k];
-              if (64 * k + lane < parts) sw[i][64 * k + lane] = w;
-            }
+    for (int k = 0; k < K; ++k) {
+      const float e = __builtin_amdgcn_exp2f(m[k] - top);
+      sum += e * w[k];
+      w[k] = e;
+    }
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-            const long long position = (long long)ch.first + (token - ch.start);
-            const int hi = a.causal ? clamp_position(position + 1, len) : len, lo = a.window > 0 ? clamp_position(position - a.window + 1, len) : 0;
-            const bool none = hi <= lo;
-            if (lane == 0 && a.lse) a.lse[at] = none ? -INFINITY : log_sum(top, sum);
-            sum = none ? INFINITY : sum;                         // (no keys: zeros)
-          }
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    const float* const po = a.part_o + at * a.stride * D + 4 * c;
+    v4f acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int last = min(n - 64 * k, 64);
+#pragma unroll 4
+      for (int p0 = (WAVES == 4 ? wave : 0) * SL; p0 < last; p0 += (WAVES == 4 ? 4 : 1) * SL) {
+        const int p = p0 + slice;
+        const float weight = __shfl(w[k], p & 63);
+        if (p < last && slice < SL) {
+          const v4f v = *reinterpret_cast<const v4f*>(po + (size_t)(64 * k + p) * D);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] += weight * v[e];
         }
       }
     }
-    if (lane == 0) {
-      ss[i] = parts > 1 ? 1.0f / sum : 0.0f;
-      st[i] = __int_as_float(parts);
-    }
-  }
-  __syncthreads();
-  const bool in = unit < UNITS;
-  const int parts = in ? __float_as_int(st[mine]) : 1;
-  v4f acc = {0.f, 0.f, 0.f, 0.f};
-  if (parts > 1) {
-    const float* const po = a.part_o + (row0 + mine) * a.nparts * D + 4 * c;
-#pragma unroll 8
-    for (int p = slice; p < parts; p += slices) {
-      const float w = sw[mine][p];
-      const v4f v = *reinterpret_cast<const v4f*>(po + (size_t)p * D);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += w * v[e];
-    }
-  }
-  if (slices > 1) {
-    so[threadIdx.x] = acc;
-    __syncthreads();
-    if (slice != 0) return;
-    for (int i = 1; i < slices; ++i) {
-      const v4f v = so[threadIdx.x + i * L];
+    for (int o = SL / 2; o > 0; o >>= 1)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += v[e];
+      for (int e = 0; e < 4; ++e) acc[e] += __shfl(acc[e], lane + o * L);
+    if constexpr (WAVES == 4) {
+      if (lane < L) so[wave * L + lane] = acc;
+      __syncthreads();
+      if (wave == 0 && lane < L) {
+#pragma unroll
+        for (int i = 1; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] += so[i * L + lane][e];
+      }
+    }
+    if ((WAVES == 1 || wave == 0) && lane < L) {
+      const float inv = none ? 0.0f : 1.0f / sum;
+      *reinterpret_cast<v2u*>((typename T::scalar*)a.o + at * D + 4 * c) = v2u{T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
+      if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : log_sum(top, sum);
     }
   }
-  if (parts <= 1) return;
-  const float inv = ss[mine];
-  *reinterpret_cast<v2u*>((typename T::scalar*)a.o + (row0 + mine) * D + 4 * c) =
-      v2u{T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
 }
 
 // ---- host side ----------------------------------------------------------------------------
 
-// How a call is cut.
+// How a call is run.
 struct Plan {
   bool narrow;
   int nq;                  // narrow: blocks of 16 rows
   int slots, slots_per_seq;
-  int nparts, part_keys;
+  Cut cut, small;
+  int small_rows, stride;
 };
 
 static size_t workspace_of(long long rows, int D, int nparts) { return nparts > 1 ? (size_t)rows * nparts * (D + 2) * 4 : 0; }
@@ -1119,51 +1156,71 @@ static double narrow_cost(double workgroups, int part_keys, int held, int cus) {
   return rounds * (3.0 + part_keys * (held / 1000.0) / std::min(17.0, 5800.0 / at_once));
 }
 
-// The same of the wide kernel, whose pairs of workgroups on a compute unit take 1.6 us for a tile of 64 keys of 128.
-static double wide_cost(double workgroups, int part_keys, int D, int cus) {
-  const double rounds = std::ceil(workgroups / (2.0 * cus));
-  return rounds * (4.0 + part_keys / 64 * (1.6 * D / 128));
-}
+// The same of the wide kernel: rounds of one workgroup to a compute unit, which takes 2 us for a tile of 64 keys of 128.
+static double wide_cost(double workgroups, double part_keys, int D, int cus) { return std::ceil(workgroups / cus) * (6.0 + part_keys / 64 * (2.0 * D / 128)); }
 
 // Leaving parts and joining them: a launch, and fp32 sums written and read at 4 TB/s.
 static double join_cost(double rows, int D, int nparts) { return nparts > 1 ? 5.0 + rows * nparts * D * 8 / 4e6 : 0.0; }
+
+static Cut cut_into(int keys, long long n) {
+  Cut c;
+  c.part_keys = (int)(((keys + n - 1) / n + 127) / 128 * 128);
+  c.nparts = std::max(1, (keys + c.part_keys - 1) / c.part_keys);
+  return c;
+}
+
+// The number of parts that cost() finds cheapest by 3 %, among those whose results have room.
+template <typename C>
+static Cut best_cut(int keys, int least_keys, long long rows, int D, size_t room, C&& cost) {
+  Cut best = cut_into(keys, 1);
+  double least = cost(best);
+  for (int n = 2; n <= kPartsMost; n += n < 4 ? 1 : n / 4) {
+    const Cut c = cut_into(keys, n);
+    if (c.part_keys < least_keys || workspace_of(rows, D, c.nparts) > room) break;
+    const double t = cost(c);
+    if (t < 0.97 * least) {
+      least = t;
+      best = c;
+    }
+  }
+  return best;
+}
 
 static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, int heads, int window, int max_queries, int max_keys, int cus, size_t room) {
   const int D = pages.head_size, group = heads / pages.heads;
   Plan p;
   const long long most = max_queries > 0 ? std::min(max_queries, b.tokens) : b.tokens;   // new tokens of a sequence
-  const long long most_rows = most * group;
+  const long long most_rows = most * group, rows = (long long)b.tokens * heads;
   p.narrow = most_rows <= 64;
   p.nq = most_rows <= 16 ? 1 : most_rows <= 32 ? 2 : 4;
   const int R = p.narrow ? 16 * p.nq : kWideRows;
   const long long per_seq = (most_rows + R - 1) / R, packed = (long long)b.tokens * group / R + b.sequences;
-  // numbered by row blocks, the last of all sequences first, unless most of such slots would be empty
+  // numbered by row blocks, unless most of such slots would be empty
   p.slots_per_seq = b.sequences * per_seq <= 2 * packed ? (int)per_seq : 0;
   p.slots = (int)std::min<long long>(p.slots_per_seq ? b.sequences * per_seq : packed, INT_MAX);
+  p.small_rows = p.narrow || b.sequences == 1 ? 0 : 16;
   const long long capacity = (long long)b.width << page_shift;
   long long seen = max_keys > 0 ? std::min<long long>(max_keys, capacity) : capacity;
   if (window > 0) seen = std::min(seen, most + window + 64);   // from the first key that the first new token sees, down to a multiple of 64
   const int keys = (int)std::min<long long>(seen, INT_MAX - 1024);
-  const long long units = (long long)p.slots * pages.heads;
-  auto cut = [&](long long n) {
-    p.part_keys = (int)(((keys + n - 1) / n + 127) / 128 * 128);
-    p.nparts = std::max(1, (keys + p.part_keys - 1) / p.part_keys);
-  };
-  cut(1);
   const int held = pages.type == FTK_F16 || pages.type == FTK_BF16 ? 4 * D : 2 * D + 2;   // bytes of a position and head
-  double best = 1e30;
-  int best_n = 1;
-  for (int n = 1; n <= kPartsMost; n += n < 4 ? 1 : n / 4) {
-    cut(n);
-    if (n > 1 && (p.part_keys < 256 || workspace_of((long long)b.tokens * heads, D, p.nparts) > room)) break;
-    const double cost = (p.narrow ? narrow_cost((double)units * p.nparts, p.part_keys, held, cus) : wide_cost((double)units * p.nparts, p.part_keys, D, cus)) +
-                        join_cost((double)b.tokens * heads, D, p.nparts);
-    if (cost < 0.97 * best) {
-      best = cost;
-      best_n = n;
+  p.small = Cut{1, keys};
+  if (p.narrow) {
+    const double units = (double)p.slots * pages.heads;
+    p.cut = best_cut(keys, 256, rows, D, room, [&](const Cut& c) { return narrow_cost(units * c.nparts, c.part_keys, held, cus) + join_cost(rows, D, c.nparts); });
+  } else {
+    // whole row blocks; a chunk that sees itself under a causal mask works on half of its own keys
+    const double units = (double)std::max<long long>(1, b.tokens * (long long)group / R) * pages.heads, own = std::min<double>(most, keys) / 2;
+    p.cut = best_cut(keys, 512, rows, D, room,
+                     [&](const Cut& c) { return wide_cost(units * c.nparts, c.part_keys * (1 - own / keys), D, cus) + join_cost(rows, D, c.nparts); });
+    // the small sequences beside them: parts that take no longer than those, as far as there is room for as many
+    if (p.small_rows > 0) {
+      const int want = std::max(1, (int)((long long)keys * held / (20 * 17000)));   // some 20 us each
+      p.small = cut_into(keys, std::min({want, keys / 256 + 1, kPartsMost}));
+      while (p.small.nparts > p.cut.nparts && workspace_of(rows, D, p.small.nparts) > room) p.small = cut_into(keys, p.small.nparts - 1);
     }
   }
-  cut(best_n);
+  p.stride = std::max(p.cut.nparts, p.small.nparts);
   return p;
 }
 
@@ -1199,7 +1256,7 @@ size_t ftk_paged_attn_workspace_bytes(const ftk_kv_pages* pages, const ftk_kv_ba
   b.sequences = batch->sequences;
   b.width = batch->table_width;
   const Plan p = plan(*pages, b, __builtin_ctz((unsigned)pages->page_size), heads, window, max_queries, max_keys, d->cus, SIZE_MAX);
-  return workspace_of((long long)b.tokens * heads, pages->head_size, p.nparts);
+  return workspace_of((long long)b.tokens * heads, pages->head_size, p.stride);
 }
 
 int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long q_head_stride, const ftk_kv_pages* pages, const ftk_kv_batch* batch,
@@ -1233,13 +1290,17 @@ int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long 
   a.scale_log2e = scale * 1.4426950408889634f;
   a.causal = causal != 0;
   a.window = window;
+  a.slots = p.slots;
   a.slots_per_seq = p.slots_per_seq;
-  a.nparts = p.nparts;
-  a.part_keys = p.part_keys;
+  a.cut = p.cut;
+  a.small = p.small;
+  a.small_rows = p.small_rows;
+  a.stride = p.stride;
   const long long rows = (long long)a.batch.tokens * heads;
   a.part_o = (float*)workspace;
-  a.part_ml = a.part_o + (size_t)rows * p.nparts * pages->head_size;
-  const long long blocks = (long long)p.slots * pages->heads * p.nparts;
+  a.part_ml = a.part_o + (size_t)rows * p.stride * pages->head_size;
+  const long long blocks = (long long)p.slots * pages->heads * p.cut.nparts;
+  const long long pairs = p.small_rows ? ((long long)a.batch.sequences * pages->heads * p.small.nparts + 1) / 2 : 0;
   const hipStream_t s = (hipStream_t)stream;
   return with_kv_types(type, pages->type, pages->head_size, [&](auto t, auto f, auto dc) -> int {
     using T = decltype(t);
@@ -1255,16 +1316,19 @@ int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long 
       bad = p.nq == 1 ? launch(std::integral_constant<int, 1>{}) : p.nq == 2 ? launch(std::integral_constant<int, 2>{}) : launch(std::integral_constant<int, 4>{});
     } else {
       static DeviceOnce once;
-      bad = launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D>, once, blocks, kWideWaves, WideShape<D>::LDS, s, a, p.slots);
+      constexpr int lds = std::max(WideShape<D>::LDS, 2 * NarrowShape<F, D>::LDS);
+      bad = launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D>, once, blocks + pairs, kWideWaves, lds, s, a, (int)pairs);
     }
-    if (bad || p.nparts == 1) return bad;
-    constexpr int UNITS = D == 96 ? 8 : 256 / (D / 4);
-    int slices = UNITS / 4;                                      // a row for each wave, or fewer
-    while (slices < UNITS && slices * 4 < p.nparts) slices *= 2;
-    const int per_block = UNITS / slices;
-    const long long mblocks = (rows + per_block - 1) / per_block;
-    if (mblocks > INT_MAX) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: grid too large", who);
-    hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3((unsigned)mblocks), dim3(256), 0, s, a, slices);
+    if (bad || p.stride == 1) return bad;
+    // few rows of many parts: a block to each; only small sequences cut: 16 rows to a wave, most of which have nothing to join
+    if (rows <= 4096 && p.stride >= 16) {
+      hipLaunchKernelGGL((paged_merge_kernel<T, D, 4>), dim3((unsigned)rows), dim3(256), 0, s, a, 1);
+    } else {
+      const int per_wave = p.cut.nparts > 1 ? 1 : 16;
+      const long long mblocks = (rows + 4 * per_wave - 1) / (4 * per_wave);
+      if (mblocks > INT_MAX) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: grid too large", who);
+      hipLaunchKernelGGL((paged_merge_kernel<T, D, 1>), dim3((unsigned)mblocks), dim3(256), 0, s, a, per_wave);
+    }
     return check_launch("paged_merge_kernel");
   });
 }
