@@ -1,7 +1,7 @@
 // Keys and values on their way into a paged cache and out of it again.
 //
 // Both directions move each byte once, 16 bytes of 16-bit elements a lane: the D / 8 lanes of a row are neighbours, a row's
-// maximum is taken over them by exchanges, and a thread has the key's and the value's piece in flight together.  Which
+// maximum is taken over them by exchanges, and a thread has ITEMS pieces of keys and as many of values in flight together.  Which
 // sequence a row belongs to is looked up once per wave, 64 sequences at a time.
 #include "kv_common.h"
 
@@ -23,11 +23,11 @@ struct KvPlace {
   long long row;       // of the cache: (page * heads + head) * page size + row of the page
 };
 
-// Where packed row `token` of head h lives.  first: the token of the wave's first lane.
-__device__ __forceinline__ KvPlace kv_place(const KvBatch& batch, int pages, int heads, int page_shift, int token, int h) {
-  const int first = __builtin_amdgcn_readfirstlane(token);
-  int b = count_at_most(batch.sequences, first, [&](int i) { return batch.starts[i + 1]; });
+// Where packed row `token` of head h lives; *b: a sequence at or before the row's, which becomes that.
+__device__ __forceinline__ KvPlace kv_place(const KvBatch& batch, int pages, int heads, int page_shift, int token, int h, int* seq) {
+  int b = *seq;
   while (b < batch.sequences && batch.starts[b + 1] <= token) ++b;
+  *seq = b;
   KvPlace p{false, false, 0};
   if (b >= batch.sequences) return p;
   const int start = batch.starts[b], end = batch.starts[b + 1];
@@ -42,16 +42,6 @@ __device__ __forceinline__ KvPlace kv_place(const KvBatch& batch, int pages, int
   return p;
 }
 
-// x within the reach of the codes; a NaN stays one and does not count in the maximum.
-template <typename C>
-__device__ __forceinline__ float within(float x, float& most) {
-  const float a = fabsf(x);
-  const bool over = a > C::kReach;
-  if (a <= C::kReach) most = fmaxf(most, a);
-  if (over) most = C::kReach;
-  return over ? copysignf(C::kReach, x) : x;
-}
-
 template <typename T, KvFormat F, int D>
 __device__ __forceinline__ void write_row(const v4u piece, unsigned char* codes, signed char* exps, long long row, int lane, bool valid) {
   if constexpr (F == kSame) {
@@ -61,11 +51,19 @@ __device__ __forceinline__ void write_row(const v4u piece, unsigned char* codes,
     float x[8], most = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      x[2 * i] = within<C>(T::low(piece[i]), most);
-      x[2 * i + 1] = within<C>(T::high(piece[i]), most);
+      x[2 * i] = T::low(piece[i]);
+      x[2 * i + 1] = T::high(piece[i]);
     }
 #pragma unroll
+    for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));   // (a NaN does not count)
+#pragma unroll
     for (int o = kRowLanes<D> / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+    if (most > C::kReach) {
+      most = C::kReach;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (fabsf(x[i]) > C::kReach) x[i] = copysignf(C::kReach, x[i]);
+    }
     const int e = row_exponent<F, T>(most);
     const float down = power_of_two(-e);
     const v2u w = {encode4<F>(x[0] * down, x[1] * down, x[2] * down, x[3] * down), encode4<F>(x[4] * down, x[5] * down, x[6] * down, x[7] * down)};
@@ -76,82 +74,120 @@ __device__ __forceinline__ void write_row(const v4u piece, unsigned char* codes,
   }
 }
 
-template <typename T, KvFormat F, int D>
+// The items (token, head) of a thread: ITEMS of them, a block's apart.
+template <int D, int ITEMS>
+struct Items {
+  long long first;        // of this thread
+  int lane;               // in the row
+  static constexpr int kStep = kKvThreads / kRowLanes<D>;
+  __device__ __forceinline__ Items() : first((long long)blockIdx.x * (ITEMS * kStep) + threadIdx.x / kRowLanes<D>), lane(threadIdx.x % kRowLanes<D>) {}
+  __device__ __forceinline__ long long operator[](int i) const { return first + i * kStep; }
+};
+
+template <typename T, KvFormat F, int D, int ITEMS>
 __global__ __launch_bounds__(kKvThreads) void kv_write_kernel(const typename T::scalar* __restrict__ keys, const typename T::scalar* __restrict__ values,
                                                               KvStrides st, KvPages pages, KvBatch batch, long long items) {
-  constexpr int L = kRowLanes<D>;
-  const long long item = ((long long)blockIdx.x * kKvThreads + threadIdx.x) / L;
-  const int lane = threadIdx.x % L;
-  const bool in = item < items && lane < D / 8;
-  const long long it = min(item, items - 1);
-  const int token = (int)(it / pages.heads), h = (int)(it - (long long)token * pages.heads);
-  v4u k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
-  if (in) {
-    k = *reinterpret_cast<const v4u*>(keys + token * st.k_token + h * st.k_head + 8 * lane);
-    v = *reinterpret_cast<const v4u*>(values + token * st.v_token + h * st.v_head + 8 * lane);
+  const Items<D, ITEMS> mine;
+  v4u k[ITEMS], v[ITEMS];
+  int token[ITEMS], head[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const long long it = min(mine[i], items - 1);
+    token[i] = (int)(it / pages.heads);
+    head[i] = (int)(it - (long long)token[i] * pages.heads);
+    const int piece = min(mine.lane, D / 8 - 1);
+    k[i] = *reinterpret_cast<const v4u*>(keys + token[i] * st.k_token + head[i] * st.k_head + 8 * piece);
+    v[i] = *reinterpret_cast<const v4u*>(values + token[i] * st.v_token + head[i] * st.v_head + 8 * piece);
   }
-  const KvPlace p = kv_place(batch, pages.pages, pages.heads, pages.page_shift, token, h);
-  write_row<T, F, D>(k, pages.k, pages.k_exps, p.row, lane, in && p.valid);
-  write_row<T, F, D>(v, pages.v, pages.v_exps, p.row, lane, in && p.valid);
+  int b = count_at_most(batch.sequences, __builtin_amdgcn_readfirstlane(token[0]), [&](int i) { return batch.starts[i + 1]; });
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const KvPlace p = kv_place(batch, pages.pages, pages.heads, pages.page_shift, token[i], head[i], &b);
+    const bool in = mine[i] < items && mine.lane < D / 8 && p.valid;
+    write_row<T, F, D>(k[i], pages.k, pages.k_exps, p.row, mine.lane, in);
+    write_row<T, F, D>(v[i], pages.v, pages.v_exps, p.row, mine.lane, in);
+  }
 }
 
-// T: the type that the cache came from (F == kSame: that it holds), Out: what is written.
-template <typename T, KvFormat F, typename Out, int D>
-__device__ __forceinline__ void read_row(const unsigned char* codes, const signed char* exps, long long row, int lane, bool valid, Out* out) {
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if constexpr (F == kSame) {
-    v4u piece = {0, 0, 0, 0};
-    if (valid) piece = *reinterpret_cast<const v4u*>(codes + (size_t)row * (2 * D) + 16 * lane);
-    if constexpr (std::is_same<Out, typename T::scalar>::value) {
-      *reinterpret_cast<v4u*>(out) = piece;
-      return;
+// What a lane has of a row in a cache that came from T (kSame: that holds T).
+template <typename T, KvFormat F, int D>
+struct RowPiece {
+  v4u same;
+  v2u codes;
+  int e;
+  __device__ __forceinline__ void load(const unsigned char* from, const signed char* exps, long long row, int lane, bool valid) {
+    same = v4u{0, 0, 0, 0};
+    codes = v2u{0, 0};
+    e = 0;
+    if (!valid) return;
+    if constexpr (F == kSame) {
+      same = *reinterpret_cast<const v4u*>(from + (size_t)row * (2 * D) + 16 * lane);
+    } else {
+      codes = *reinterpret_cast<const v2u*>(from + (size_t)row * D + 8 * lane);
+      e = exps[row];
     }
+  }
+  template <typename Out>
+  __device__ __forceinline__ void store(Out* out) const {
+    float x[8];
+    if constexpr (F == kSame) {
+      if constexpr (std::is_same<Out, typename T::scalar>::value) {
+        *reinterpret_cast<v4u*>(out) = same;
+        return;
+      }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = T::low(piece[i]);
-      x[2 * i + 1] = T::high(piece[i]);
-    }
-  } else {
-    v2u w = {0, 0};
-    float up = 0.0f;
-    if (valid) {
-      w = *reinterpret_cast<const v2u*>(codes + (size_t)row * D + 8 * lane);
-      up = power_of_two(exps[row]);
-    }
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = T::low(same[i]);
+        x[2 * i + 1] = T::high(same[i]);
+      }
+    } else {
+      const float up = power_of_two(e);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if constexpr (F == kInt8) {
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (F == kInt8) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[4 * i + j] = int8_code(w[i], j) * up;
-      } else {
-        x[4 * i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 0) * up;
-        x[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 1) * up;
-        x[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 2) * up;
-        x[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 3) * up;
+          for (int j = 0; j < 4; ++j) x[4 * i + j] = int8_code(codes[i], j) * up;
+        } else {
+          x[4 * i] = __builtin_amdgcn_cvt_f32_fp8((int)codes[i], 0) * up;
+          x[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8((int)codes[i], 1) * up;
+          x[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8((int)codes[i], 2) * up;
+          x[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8((int)codes[i], 3) * up;
+        }
       }
     }
+    if constexpr (std::is_same<Out, float>::value) {
+      *reinterpret_cast<v4f*>(out) = v4f{x[0], x[1], x[2], x[3]};
+      *reinterpret_cast<v4f*>(out + 4) = v4f{x[4], x[5], x[6], x[7]};
+    } else {
+      using O = typename std::conditional<std::is_same<Out, _Float16>::value, Half, Brain>::type;
+      *reinterpret_cast<v4u*>(out) = v4u{O::pack(x[0], x[1]), O::pack(x[2], x[3]), O::pack(x[4], x[5]), O::pack(x[6], x[7])};
+    }
   }
-  if constexpr (std::is_same<Out, float>::value) {
-    *reinterpret_cast<v4f*>(out) = v4f{x[0], x[1], x[2], x[3]};
-    *reinterpret_cast<v4f*>(out + 4) = v4f{x[4], x[5], x[6], x[7]};
-  } else {
-    using O = typename std::conditional<std::is_same<Out, _Float16>::value, Half, Brain>::type;
-    *reinterpret_cast<v4u*>(out) = v4u{O::pack(x[0], x[1]), O::pack(x[2], x[3]), O::pack(x[4], x[5]), O::pack(x[6], x[7])};
-  }
-}
+};
 
-template <typename T, KvFormat F, typename Out, int D>
+template <typename T, KvFormat F, typename Out, int D, int ITEMS>
 __global__ __launch_bounds__(kKvThreads) void kv_read_kernel(KvPages pages, KvBatch batch, Out* __restrict__ keys, Out* __restrict__ values,
                                                              long long items) {
-  constexpr int L = kRowLanes<D>;
-  const long long item = ((long long)blockIdx.x * kKvThreads + threadIdx.x) / L;
-  const int lane = threadIdx.x % L;
-  const long long it = min(item, items - 1);
-  const int token = (int)(it / pages.heads), h = (int)(it - (long long)token * pages.heads);
-  const KvPlace p = kv_place(batch, pages.pages, pages.heads, pages.page_shift, token, h);
-  if (item >= items || lane >= D / 8 || !p.owned) return;
-  read_row<T, F, Out, D>(pages.k, pages.k_exps, p.row, lane, p.valid, keys + it * D + 8 * lane);
-  read_row<T, F, Out, D>(pages.v, pages.v_exps, p.row, lane, p.valid, values + it * D + 8 * lane);
+  const Items<D, ITEMS> mine;
+  RowPiece<T, F, D> k[ITEMS], v[ITEMS];
+  bool in[ITEMS];
+  const int first = __builtin_amdgcn_readfirstlane((int)(min(mine[0], items - 1) / pages.heads));
+  int b = count_at_most(batch.sequences, first, [&](int i) { return batch.starts[i + 1]; });
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const long long it = min(mine[i], items - 1);
+    const int token = (int)(it / pages.heads), h = (int)(it - (long long)token * pages.heads);
+    const KvPlace p = kv_place(batch, pages.pages, pages.heads, pages.page_shift, token, h, &b);
+    in[i] = mine[i] < items && mine.lane < D / 8 && p.owned;
+    k[i].load(pages.k, pages.k_exps, p.row, mine.lane, in[i] && p.valid);
+    v[i].load(pages.v, pages.v_exps, p.row, mine.lane, in[i] && p.valid);
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    if (!in[i]) continue;
+    k[i].store(keys + mine[i] * D + 8 * mine.lane);
+    v[i].store(values + mine[i] * D + 8 * mine.lane);
+  }
 }
 
 // ---- host side ---------------------------------------------------------------------
@@ -191,12 +227,17 @@ static int check_same_type(const char* who, int type, int cache) {
   return FTK_OK;
 }
 
-template <int D>
-static int kv_grid(const char* who, long long items, unsigned* blocks) {
-  const long long n = (items * kRowLanes<D> + kKvThreads - 1) / kKvThreads;
+// Calls f(items of a thread, blocks): four items where that leaves two blocks of 256 threads or more to a compute unit (the look-ups of a wave then serve four rows), one
+// for less, whose time is the chain of look-ups.
+template <int D, typename F>
+static int with_items(const char* who, long long items, F&& f) {
+  const DeviceProps* d = nullptr;
+  if (const int rc = device_props(&d)) return rc;
+  constexpr long long step = kKvThreads / kRowLanes<D>;
+  const bool many = items >= 4 * step * 2 * d->cus;
+  const long long per = many ? 4 * step : step, n = (items + per - 1) / per;
   if (n > INT_MAX) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: too many rows for one launch", who);
-  *blocks = (unsigned)n;
-  return FTK_OK;
+  return many ? f(std::integral_constant<int, 4>{}, (unsigned)n) : f(std::integral_constant<int, 1>{}, (unsigned)n);
 }
 
 }  // namespace ftk
@@ -223,11 +264,12 @@ int ftk_kv_cache_write(const void* keys, const void* values, int type, long long
     using T = decltype(t);
     constexpr KvFormat F = decltype(f)::value;
     constexpr int D = decltype(d)::value;
-    unsigned blocks;
-    if (int bad = kv_grid<D>(who, items, &blocks)) return bad;
-    hipLaunchKernelGGL((kv_write_kernel<T, F, D>), dim3(blocks), dim3(kKvThreads), 0, (hipStream_t)stream, (const typename T::scalar*)keys,
-                       (const typename T::scalar*)values, st, p, b, items);
-    return check_launch("kv_write_kernel");
+    return with_items<D>(who, items, [&](auto n, unsigned blocks) -> int {
+      constexpr int ITEMS = decltype(n)::value;
+      hipLaunchKernelGGL((kv_write_kernel<T, F, D, ITEMS>), dim3(blocks), dim3(kKvThreads), 0, (hipStream_t)stream, (const typename T::scalar*)keys,
+                         (const typename T::scalar*)values, st, p, b, items);
+      return check_launch("kv_write_kernel");
+    });
   });
 }
 
@@ -249,12 +291,13 @@ int ftk_kv_cache_read(const ftk_kv_pages* pages, const ftk_kv_batch* batch, int 
     using T = decltype(t);
     constexpr KvFormat F = decltype(f)::value;
     constexpr int D = decltype(d)::value;
-    unsigned blocks;
-    if (int bad = kv_grid<D>(who, items, &blocks)) return bad;
     auto launch = [&](auto out) -> int {
       using Out = decltype(out);
-      hipLaunchKernelGGL((kv_read_kernel<T, F, Out, D>), dim3(blocks), dim3(kKvThreads), 0, (hipStream_t)stream, p, b, (Out*)keys, (Out*)values, items);
-      return check_launch("kv_read_kernel");
+      return with_items<D>(who, items, [&](auto n, unsigned blocks) -> int {
+        constexpr int ITEMS = decltype(n)::value;
+        hipLaunchKernelGGL((kv_read_kernel<T, F, Out, D, ITEMS>), dim3(blocks), dim3(kKvThreads), 0, (hipStream_t)stream, p, b, (Out*)keys, (Out*)values, items);
+        return check_launch("kv_read_kernel");
+      });
     };
     if (type == FTK_F32) return launch(0.0f);
     if constexpr (F == kSame) return launch(typename T::scalar{});

@@ -148,8 +148,10 @@ __device__ __forceinline__ unsigned encode4(float a, float b, float c, float d) 
     int p = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
     return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, p, true);
   } else {
-    const auto code = [](float x) { return (unsigned)(int)__builtin_rintf(x) & 255u; };   // (NaN: 0)
-    return code(a) | code(b) << 8 | code(c) << 16 | code(d) << 24;
+    // x + 1.5 * 2^23 rounds x to the nearest whole number, the even one of two, which the low bits then hold (a NaN's are zeros)
+    const auto bits = [](float x) { return __float_as_uint(x + 12582912.0f); };
+    const unsigned low = __builtin_amdgcn_perm(bits(b), bits(a), 0x0c0c0400u), high = __builtin_amdgcn_perm(bits(d), bits(c), 0x04000c0cu);
+    return low | high;
   }
 }
 
