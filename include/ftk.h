@@ -725,7 +725,7 @@ int ftk_paged_attn(const void* q, int type, long long q_token_stride,
  * token is -1.  A drafted id outside [0, vocabulary) is rejected.
  * tokens [sequences, drafted + 1], of drafts' type: the accepted drafts, the next token,
  * then -1; accepted [sequences]: how many were.  drafted is 0 to 63 (0: one token is
- * drawn from each row).  workspace: 8-byte aligned,
+ * drawn from each row).  workspace: 16-byte aligned,
  * ftk_verify_drafts_workspace_bytes(sequences, vocabulary) bytes.
  */
 size_t ftk_verify_drafts_workspace_bytes(int sequences, int vocabulary);

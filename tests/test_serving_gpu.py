@@ -421,7 +421,7 @@ def _verified(core, target, draft, drafts, accept, sample, counts=None):
 
 
 @pytest.mark.parametrize('dtype', [F32, F16, BF16])
-@pytest.mark.parametrize('B,K,V', [(1, 1, 1), (3, 2, 7), (5, 4, 1000), (2, 5, 2048), (4, 3, 2049), (3, 0, 4096), (2, 63, 301), (2, 2, 70001)])
+@pytest.mark.parametrize('B,K,V', [(1, 1, 1), (3, 2, 7), (5, 4, 1000), (2, 5, 2048), (4, 3, 2049), (3, 0, 4096), (2, 63, 301), (2, 2, 65536), (2, 2, 70001), (3, 1, 131072), (2, 1, 150003), (2, 1, 262145)])
 def test_verified_drafts(core, dtype, B, K, V):
     t = _drafts(B, K, V, dtype, K % 2, 91)
     _verified(core, *t)
