@@ -8,6 +8,8 @@ kernel calls on FractalTensors that live on the GPU.
   b2b_gemm       (a @ b) @ c, the computation of benchmarks/fused_two_hgemms
   grid_rnn       the nested-scan program of examples/grid_rnn/grid_rnn.py:40-137 over a batch of samples
   windowed_attention  shifted_slide + the map of sparse_attn of examples/sparse_attention/sparse_attention.py:25-71
+  kv_cache_write, kv_cache_read, paged_attention, verify_drafts   serving: the new tokens of a batch of sequences and a paged cache
+                 of keys and values; one sequence is one item of a FractalTensor, of any length
 
 A regular (non-ragged) FractalTensor already is a dense row-major tensor in
 its flat buffer, so inputs are handed to the kernels as views and outputs are
@@ -26,7 +28,8 @@ from ..tensor import Tensor
 from ..types import FractalTensorStorage, TensorStorage, torch_type_to_internal_type
 
 __all__ = ['pack_lstm_weights', 'pad_time_major', 'unpad_time_major', 'stacked_lstm', 'dilated_lstm', 'lstm_cell', 'flash_attention', 'b2b_gemm', 'mm',
-           'online_softmax', 'embedding_lookup', 'grid_rnn', 'windowed_attention']
+           'online_softmax', 'embedding_lookup', 'grid_rnn', 'windowed_attention', 'kv_cache_write', 'kv_cache_read', 'paged_attention',
+           'verify_drafts']
 
 
 def _core():
@@ -331,3 +334,93 @@ def windowed_attention(query: FractalTensor, key: FractalTensor, value: FractalT
     out = _core().windowed_attention(q.reshape(-1, S, D).float().contiguous(), k.reshape(-1, S, D).float().contiguous(),
                                      v.reshape(-1, S, D).float().contiguous(), window_size, dilation, extra, 1.0)
     return FractalTensor.from_dense(out.reshape(q.shape), depth)
+
+
+def _new_tokens(tss: FractalTensor, name: str, pages: torch.Tensor):
+    """[sequence][token] of [heads, D], ragged or not -> (the packed rows [tokens, heads, D] in the type that goes with the pages, tokens
+    of each sequence)."""
+    if not isinstance(tss, FractalTensor):
+        raise TypeError(f'{name} should be a FractalTensor.')
+    if tss.depth != 2 or len(tss.element_shape) != 2:
+        raise ValueError(f'{name} should have depth 2 and [heads, D] items, got depth {tss.depth} of {list(tss.element_shape)}.')
+    if tss._T is None or not tss.has_indices:
+        raise RuntimeError('FractalTensor is not initialized.')
+    rows = tss.data.reshape(-1, *tss.element_shape)
+    if not rows.is_cuda:
+        raise RuntimeError(f'{name} lives on {rows.device}; the fused kernels run on the GPU only.')
+    return rows.to(torch.bfloat16 if pages.dtype == torch.bfloat16 else torch.float16), tss.width_by_depth(1)
+
+
+def _starts(counts, device) -> torch.Tensor:
+    starts = [0]
+    for n in counts:
+        starts.append(starts[-1] + n)
+    return torch.tensor(starts, dtype=torch.int32, device=device)
+
+
+def _by_sequence(rows: torch.Tensor, counts) -> FractalTensor:
+    """Packed rows -> [sequence][token] of what a row is."""
+    if counts and counts[0] > 0 and all(n == counts[0] for n in counts):
+        return FractalTensor.from_dense(rows.reshape(len(counts), counts[0], *rows.shape[1:]), 2)
+    ft = FractalTensor(FractalTensorStorage(TensorStorage(tuple(rows.shape[1:]), torch_type_to_internal_type(rows.dtype), device=rows.device.type)))
+    indices, at = [], 0
+    for n in counts:
+        indices.append(list(range(at, at + n)))
+        at += n
+    ft.indices = indices
+    ft._T = rows.reshape(-1)
+    return ft
+
+
+def kv_cache_write(keyss: FractalTensor, valuess: FractalTensor, k_pages, v_pages, table, lens, k_exps=None, v_exps=None) -> None:
+    """Writes the keys and values of new tokens, [sequence][token] of [kv heads, D] (any number of tokens in each sequence, none too), into their
+    pages: the last positions of the lens[b] that sequence b has with them.  Pages [pages, kv heads, page size, D] are fp16, bf16, or 8-bit codes
+    (float8_e4m3fn or int8) with an exponent for each row in k_exps, v_exps [pages, kv heads, page size] int8; table [B, columns] and lens [B] are int32.
+    fp32 tokens are rounded to fp16 (to bf16 for bf16 pages) first."""
+    keys, counts = _new_tokens(keyss, 'keyss', k_pages)
+    values, same = _new_tokens(valuess, 'valuess', k_pages)
+    if counts != same:
+        raise ValueError('keyss and valuess should have one structure.')
+    _core().kv_cache_write(keys, values, k_pages, v_pages, table, lens, _starts(counts, keys.device), k_exps, v_exps)
+
+
+def kv_cache_read(k_pages, v_pages, table, lens, counts: Sequence[int], dtype=torch.float32, k_exps=None, v_exps=None):
+    """The last counts[b] positions of every sequence, as kv_cache_write would have been given them: (keyss, valuess), [sequence][token] of [kv
+    heads, D] of fp32 (fp16 if asked for and the pages are not bf16)."""
+    counts = [int(n) for n in counts]
+    if any(n < 0 for n in counts):
+        raise ValueError('counts should not be negative.')
+    keys, values = _core().kv_cache_read(k_pages, v_pages, table, lens, _starts(counts, k_pages.device), sum(counts), dtype, k_exps, v_exps)
+    return _by_sequence(keys, counts), _by_sequence(values, counts)
+
+
+def paged_attention(qss: FractalTensor, k_pages, v_pages, table, lens, k_exps=None, v_exps=None, scale: Optional[float] = None, causal: bool = True,
+                    window: int = 0, max_keys: int = 0) -> FractalTensor:
+    """Attention of new tokens, [sequence][token] of [heads, D], over a paged cache that holds their keys and values already (kv_cache_write): one
+    token a sequence, drafted ones, chunks of prompts and whole prompts, in any mixture.  heads is a multiple of the cache's.  `scale` multiplies the
+    scores and defaults to 1.0, as in flash_attention.  causal: a token sees the positions up to its own; window > 0: no more than that many of them.
+    max_keys: the greatest of lens where the program knows it.  The result has the structure and the type of qss; a token that sees nothing gets zeros."""
+    q, counts = _new_tokens(qss, 'qss', k_pages)
+    o = _core().paged_attention(q, k_pages, v_pages, table, lens, _starts(counts, q.device), k_exps, v_exps, 1.0 if scale is None else float(scale), causal, window,
+                                max(counts, default=0), max_keys)
+    return _by_sequence(o.to(qss.data.dtype), counts)
+
+
+def verify_drafts(targets: FractalTensor, drafts: FractalTensor, accept_uniforms: torch.Tensor, sample_uniforms: torch.Tensor,
+                  draft_probabilities: Optional[FractalTensor] = None) -> FractalTensor:
+    """Which drafted tokens a target model accepts, and the token that follows them: [sequence][token] of [1] integers, from one to K + 1 tokens a sequence.
+
+    targets: [B][K + 1] of [1, V], the target's probabilities before each draft and behind the last; drafts: [B][K] of [1] int32 or int64; draft_probabilities:
+    [B][K] of [1, V] that the drafts were drawn from, or None for drafts that were not drawn at random; accept_uniforms [B, K] and sample_uniforms [B]:
+    uniform numbers of [0, 1), fp32.  The tokens left are distributed as the target's own."""
+    p = _dense_gpu(targets, 'targets', 2)
+    d = _dense_gpu(drafts, 'drafts', 2)
+    q = None if draft_probabilities is None else _dense_gpu(draft_probabilities, 'draft_probabilities', 2)
+    if p.dim() != 4 or p.shape[2] != 1 or (q is not None and (q.dim() != 4 or q.shape[2] != 1)):
+        raise ValueError('targets and draft_probabilities should have [1, V] items.')
+    if drafts.element_size != 1:
+        raise ValueError('drafts should hold single integers.')
+    tokens, accepted = _core().verify_drafts(p.squeeze(2).contiguous(), None if q is None else q.squeeze(2).contiguous(), d.reshape(d.shape[0], d.shape[1]).contiguous(),
+                                             accept_uniforms, sample_uniforms)
+    kept = torch.arange(tokens.shape[1], device=tokens.device) <= accepted[:, None]
+    return _by_sequence(tokens[kept].reshape(-1, 1), [n + 1 for n in accepted.tolist()])

@@ -170,3 +170,21 @@ def test_reference_codes_stand_for_values_of_their_type(dtype, cache):
         if scale == info.max / 4:
             codes, e = ref.quantise_row(torch.tensor([info.max]), dtype, cache)
             assert math.isfinite(float(torch.tensor(codes[0] * 2.0 ** e, dtype=torch.float64).to(dtype)))
+
+
+def test_fractal_tensors_on_the_cpu_are_refused():
+    from fractaltensor_amd.kaleido import FractalTensor, operations as ops
+    x = FractalTensor.from_dense(torch.zeros(2, 3, 2, 64), 2)
+    pages = [torch.zeros(4, 2, 16, 64, dtype=torch.float16) for _ in range(2)]
+    table, lens = torch.zeros((2, 2), dtype=torch.int32), torch.full((2,), 3, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match='GPU only'):
+        ops.fused.kv_cache_write(x, x, *pages, table, lens)
+    with pytest.raises(RuntimeError, match='GPU only'):
+        ops.fused.paged_attention(x, *pages, table, lens)
+    with pytest.raises(ValueError, match='not be negative'):
+        ops.fused.kv_cache_read(*pages, table, lens, [1, -1])
+    with pytest.raises(TypeError, match='should be a FractalTensor'):
+        ops.fused.paged_attention(x.data, *pages, table, lens)
+    probs, ids = FractalTensor.from_dense(torch.zeros(2, 3, 1, 8), 2), FractalTensor.from_dense(torch.zeros(2, 2, 1, dtype=torch.int64), 2)
+    with pytest.raises(RuntimeError, match='GPU only'):
+        ops.fused.verify_drafts(probs, ids, torch.zeros(2, 2), torch.zeros(2))

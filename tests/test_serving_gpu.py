@@ -573,3 +573,52 @@ def test_other_streams_and_replays(core):
             assert all(torch.equal(a, b) for a, b in zip(out, want[(turn + i) % 3])), (turn, i)
         eager = step(variants[turn % 3], fresh(), *spaces())
         assert all(torch.equal(a, b) for a, b in zip(eager, want[turn % 3]))
+
+
+# ---- on FractalTensors --------------------------------------------------------------------
+
+@pytest.mark.parametrize('new,dtype,cache', [([3, 1, 17], F16, E4M3), ([2, 2], F32, I8), ([4, 0, 1], F32, 'bf16')])
+def test_serving_on_fractal_tensors(core, new, dtype, cache):
+    """Sequences of any number of tokens as FractalTensors: the same as the packed rows, to the bit."""
+    from fractaltensor_amd.kaleido import FractalTensor, operations as ops
+    heads, G, D, page = 2, 3, 64, 16
+    held = BF16 if cache == 'bf16' else F16                      # what the tokens are rounded to
+    batch = ref.make_batch(new, [n + 21 for n in new], page, 121)
+    table, lens, starts = ref.on_device(batch)
+    pages = _cuda(ref.make_pages(batch, heads, D, None if cache == 'bf16' else cache, held, 122))
+    other = [None if t is None else t.clone() for t in pages]
+    g = torch.Generator(device='cuda').manual_seed(123)
+    k, v, q = [torch.randn((sum(new), h, D), generator=g, device='cuda').to(dtype) for h in (heads, heads, heads * G)]
+    as_ft = lambda t: ops.fused._by_sequence(t, new)
+    assert as_ft(q).width_by_depth(1) == new and isinstance(as_ft(q), FractalTensor)
+    core.kv_cache_write(k.to(held), v.to(held), *pages[:2], table, lens, starts, *pages[2:])
+    want = core.paged_attention(q.to(held), *pages[:2], table, lens, starts, *pages[2:], scale=0.2, window=30, max_queries=max(new), max_keys=40).to(dtype)
+    ops.fused.kv_cache_write(as_ft(k), as_ft(v), *other[:2], table, lens, *other[2:])
+    assert all(a is None or _same(a, b) for a, b in zip(pages, other))
+    got = ops.fused.paged_attention(as_ft(q), *other[:2], table, lens, *other[2:], scale=0.2, window=30, max_keys=40)
+    assert got.depth == 2 and got.width_by_depth(1) == new and got.element_shape == (heads * G, D) and got.data.dtype == dtype
+    assert torch.equal(got.data.view_as(want), want)
+    back = ops.fused.kv_cache_read(*other[:2], table, lens, new, F32, *other[2:])
+    for a, b in zip(back, core.kv_cache_read(*pages[:2], table, lens, starts, sum(new), F32, *pages[2:])):
+        assert a.width_by_depth(1) == new and torch.equal(a.data.view_as(b), b)
+    one = got[0][0].data                                         # the first token alone, through an ordinary index
+    assert torch.equal(one, want[0])
+    with pytest.raises(ValueError, match='one structure'):
+        ops.fused.kv_cache_write(as_ft(k), ops.fused._by_sequence(v, [sum(new)]), *other[:2], table, lens, *other[2:])
+    with pytest.raises(ValueError, match='depth 2'):
+        ops.fused.paged_attention(FractalTensor.from_dense(q, 1), *other[:2], table, lens, *other[2:])
+
+
+def test_verification_on_fractal_tensors(core):
+    from fractaltensor_amd.kaleido import FractalTensor, operations as ops
+    B, K, V = 5, 4, 300
+    target, draft, drafts, accept, sample = _drafts(B, K, V, F32, True, 131)
+    want = ref.verify(target, draft, drafts, accept, sample)
+    target, draft, drafts, accept, sample = (t.cuda() for t in (target, draft, drafts, accept, sample))
+    ft = lambda t: FractalTensor.from_dense(t.reshape(*t.shape[:2], 1, V), 2)
+    got = ops.fused.verify_drafts(ft(target), FractalTensor.from_dense(drafts.reshape(B, K, 1), 2), accept, sample, ft(draft))
+    counts = [n + 1 for n in want[1].tolist()]
+    assert got.depth == 2 and got.width_by_depth(1) == counts and got.data.dtype == torch.int64
+    assert got.data.tolist() == [t for b, n in enumerate(counts) for t in want[0][b, :n].tolist()]
+    with pytest.raises(ValueError, match=r'\[1, V\] items'):
+        ops.fused.verify_drafts(FractalTensor.from_dense(target, 2), FractalTensor.from_dense(drafts.reshape(B, K, 1), 2), accept, sample)
