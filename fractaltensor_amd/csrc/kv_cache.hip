@@ -1,8 +1,8 @@
 // Keys and values on their way into a paged cache and out of it again.
 //
 // Both directions move each byte once, 16 bytes of 16-bit elements a lane: the D / 8 lanes of a row are neighbours, a row's
-// maximum is taken over them by exchanges, and a thread has ITEMS pieces of keys and as many of values in flight together.  Which
-// sequence a row belongs to is looked up once per wave, 64 sequences at a time.
+// maximum is taken over them by exchanges, and a lane has ITEMS pieces of keys and as many of values in flight together.  Where the tokens
+// of a wave live is looked up once, a lane to a token, and handed to the lanes that need it.
 #include "kv_common.h"
 
 namespace ftk {
@@ -17,29 +17,64 @@ struct KvStrides {
   long long k_token, k_head, v_token, v_head;   // elements
 };
 
-struct KvPlace {
-  bool valid;          // the row is a sequence's, at a position that the cache has room for, in a page that there is
-  bool owned;          // the row is a sequence's
-  long long row;       // of the cache: (page * heads + head) * page size + row of the page
+// The rows of a wave: `tokens` tokens from token0 on with heads head0 .. of each; row r of them is token r / heads, head r % heads.
+struct WaveRows {
+  int token0, tokens, head0, heads, rows;
+  unsigned inverse;                              // ceil(2^16 / heads): r / heads for the rows of a wave, 64 at most
 };
+struct KvSplit {
+  int tokens, heads;                             // of a wave
+};
+template <int D, int ITEMS>
+constexpr int kWaveRows = ITEMS * (64 / kRowLanes<D>);
 
-// Where packed row `token` of head h lives; *b: a sequence at or before the row's, which becomes that.
-__device__ __forceinline__ KvPlace kv_place(const KvBatch& batch, int pages, int heads, int page_shift, int token, int h, int* seq) {
-  int b = *seq;
-  while (b < batch.sequences && batch.starts[b + 1] <= token) ++b;
-  *seq = b;
-  KvPlace p{false, false, 0};
+__device__ __forceinline__ WaveRows wave_rows(const KvSplit& split, const KvBatch& batch, int heads) {
+  WaveRows w;
+  const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * (kKvThreads / 64) + (threadIdx.x >> 6));
+  w.token0 = wave * split.tokens;
+  w.tokens = min(split.tokens, batch.tokens - w.token0);
+  w.head0 = blockIdx.y * split.heads;
+  w.heads = min(split.heads, heads - w.head0);
+  w.rows = w.tokens * w.heads;
+  w.inverse = (65536u + w.heads - 1) / (unsigned)w.heads;
+  return w;
+}
+
+constexpr int kNoPlace = -1, kNoSequence = -2;
+
+// Where the tokens of a wave live: lane i has the page of the i-th (kNoPlace: the cache has no room for its position or no such page;
+// kNoSequence: it is no sequence's) and its row in that page.
+struct WavePlaces {
+  int page, row;
+};
+__device__ __forceinline__ WavePlaces wave_places(const KvBatch& batch, const KvPages& pages, const WaveRows& w, int lane) {
+  const int first = count_at_most(batch.sequences, w.token0, [&](int i) { return batch.starts[i + 1]; });
+  const int token = w.token0 + lane;
+  // the ends of the 64 sequences from `first` on; how many of them are at or before a lane's token
+  const int end = first + lane < batch.sequences ? batch.starts[first + 1 + lane] : INT_MAX;
+  int n = 0;
+#pragma unroll
+  for (int step = 32; step > 0; step >>= 1)
+    if (__shfl(end, n + step - 1) <= token) n += step;
+  int b = first + n;
+  WavePlaces p{kNoSequence, 0};
+  if (lane >= w.tokens) return p;
+  if (n == 63)
+    while (b < batch.sequences && batch.starts[b + 1] <= token) ++b;
   if (b >= batch.sequences) return p;
-  const int start = batch.starts[b], end = batch.starts[b + 1];
+  const int start = batch.starts[b], stop = batch.starts[b + 1];
   if (token < start) return p;
-  p.owned = true;
-  const long long position = (long long)batch.lens[b] - end + token;
-  if (position < 0 || position >= kv_capacity(batch, page_shift)) return p;
-  const int page = batch.table[(long long)b * batch.width + (position >> page_shift)];
-  if (page < 0 || page >= pages) return p;
-  p.valid = true;
-  p.row = (((long long)page * heads + h) << page_shift) + (position & ((1 << page_shift) - 1));
+  p.page = kNoPlace;
+  const long long position = (long long)batch.lens[b] - stop + token;
+  if (position < 0 || position >= kv_capacity(batch, pages.page_shift)) return p;
+  const int page = batch.table[(long long)b * batch.width + (position >> pages.page_shift)];
+  if (page < 0 || page >= pages.pages) return p;
+  p.page = page;
+  p.row = (int)(position & ((1 << pages.page_shift) - 1));
   return p;
+}
+__device__ __forceinline__ long long cache_row(const KvPages& pages, int page, int head, int row) {
+  return (((long long)page * pages.heads + head) << pages.page_shift) + row;
 }
 
 template <typename T, KvFormat F, int D>
@@ -74,38 +109,31 @@ __device__ __forceinline__ void write_row(const v4u piece, unsigned char* codes,
   }
 }
 
-// The items (token, head) of a thread: ITEMS of them, a block's apart.
-template <int D, int ITEMS>
-struct Items {
-  long long first;        // of this thread
-  int lane;               // in the row
-  static constexpr int kStep = kKvThreads / kRowLanes<D>;
-  __device__ __forceinline__ Items() : first((long long)blockIdx.x * (ITEMS * kStep) + threadIdx.x / kRowLanes<D>), lane(threadIdx.x % kRowLanes<D>) {}
-  __device__ __forceinline__ long long operator[](int i) const { return first + i * kStep; }
-};
-
 template <typename T, KvFormat F, int D, int ITEMS>
 __global__ __launch_bounds__(kKvThreads) void kv_write_kernel(const typename T::scalar* __restrict__ keys, const typename T::scalar* __restrict__ values,
-                                                              KvStrides st, KvPages pages, KvBatch batch, long long items) {
-  const Items<D, ITEMS> mine;
+                                                              KvStrides st, KvPages pages, KvBatch batch, KvSplit split) {
+  const WaveRows w = wave_rows(split, batch, pages.heads);
+  if (w.tokens <= 0) return;
+  const int lane = threadIdx.x & 63, piece = lane % kRowLanes<D>;
   v4u k[ITEMS], v[ITEMS];
   int token[ITEMS], head[ITEMS];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    const long long it = min(mine[i], items - 1);
-    token[i] = (int)(it / pages.heads);
-    head[i] = (int)(it - (long long)token[i] * pages.heads);
-    const int piece = min(mine.lane, D / 8 - 1);
-    k[i] = *reinterpret_cast<const v4u*>(keys + token[i] * st.k_token + head[i] * st.k_head + 8 * piece);
-    v[i] = *reinterpret_cast<const v4u*>(values + token[i] * st.v_token + head[i] * st.v_head + 8 * piece);
+    const int r = min(i * (64 / kRowLanes<D>) + lane / kRowLanes<D>, w.rows - 1);
+    token[i] = r * w.inverse >> 16;
+    head[i] = w.head0 + r - token[i] * w.heads;
+    const int at = min(piece, D / 8 - 1) * 8;
+    k[i] = *reinterpret_cast<const v4u*>(keys + (long long)(w.token0 + token[i]) * st.k_token + head[i] * st.k_head + at);
+    v[i] = *reinterpret_cast<const v4u*>(values + (long long)(w.token0 + token[i]) * st.v_token + head[i] * st.v_head + at);
   }
-  int b = count_at_most(batch.sequences, __builtin_amdgcn_readfirstlane(token[0]), [&](int i) { return batch.starts[i + 1]; });
+  const WavePlaces places = wave_places(batch, pages, w, lane);
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    const KvPlace p = kv_place(batch, pages.pages, pages.heads, pages.page_shift, token[i], head[i], &b);
-    const bool in = mine[i] < items && mine.lane < D / 8 && p.valid;
-    write_row<T, F, D>(k[i], pages.k, pages.k_exps, p.row, mine.lane, in);
-    write_row<T, F, D>(v[i], pages.v, pages.v_exps, p.row, mine.lane, in);
+    const int page = __shfl(places.page, token[i]), row = __shfl(places.row, token[i]);
+    const bool in = i * (64 / kRowLanes<D>) + lane / kRowLanes<D> < w.rows && piece < D / 8 && page >= 0;
+    const long long at = cache_row(pages, page, head[i], row);
+    write_row<T, F, D>(k[i], pages.k, pages.k_exps, at, piece, in);
+    write_row<T, F, D>(v[i], pages.v, pages.v_exps, at, piece, in);
   }
 }
 
@@ -166,27 +194,29 @@ struct RowPiece {
 };
 
 template <typename T, KvFormat F, typename Out, int D, int ITEMS>
-__global__ __launch_bounds__(kKvThreads) void kv_read_kernel(KvPages pages, KvBatch batch, Out* __restrict__ keys, Out* __restrict__ values,
-                                                             long long items) {
-  const Items<D, ITEMS> mine;
+__global__ __launch_bounds__(kKvThreads) void kv_read_kernel(KvPages pages, KvBatch batch, Out* __restrict__ keys, Out* __restrict__ values, KvSplit split) {
+  const WaveRows w = wave_rows(split, batch, pages.heads);
+  if (w.tokens <= 0) return;
+  const int lane = threadIdx.x & 63, piece = lane % kRowLanes<D>;
   RowPiece<T, F, D> k[ITEMS], v[ITEMS];
-  bool in[ITEMS];
-  const int first = __builtin_amdgcn_readfirstlane((int)(min(mine[0], items - 1) / pages.heads));
-  int b = count_at_most(batch.sequences, first, [&](int i) { return batch.starts[i + 1]; });
+  int out[ITEMS];                                              // row of the result behind token0's first; -1: none
+  const WavePlaces places = wave_places(batch, pages, w, lane);
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    const long long it = min(mine[i], items - 1);
-    const int token = (int)(it / pages.heads), h = (int)(it - (long long)token * pages.heads);
-    const KvPlace p = kv_place(batch, pages.pages, pages.heads, pages.page_shift, token, h, &b);
-    in[i] = mine[i] < items && mine.lane < D / 8 && p.owned;
-    k[i].load(pages.k, pages.k_exps, p.row, mine.lane, in[i] && p.valid);
-    v[i].load(pages.v, pages.v_exps, p.row, mine.lane, in[i] && p.valid);
+    const int r = i * (64 / kRowLanes<D>) + lane / kRowLanes<D>, token = min(r, w.rows - 1) * w.inverse >> 16, head = w.head0 + r - token * w.heads;
+    const int page = __shfl(places.page, token), row = __shfl(places.row, token);
+    const bool in = r < w.rows && piece < D / 8;
+    out[i] = in && page != kNoSequence ? token * pages.heads + head : -1;
+    const long long at = cache_row(pages, page, head, row);
+    k[i].load(pages.k, pages.k_exps, at, piece, in && page >= 0);
+    v[i].load(pages.v, pages.v_exps, at, piece, in && page >= 0);
   }
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    if (!in[i]) continue;
-    k[i].store(keys + mine[i] * D + 8 * mine.lane);
-    v[i].store(values + mine[i] * D + 8 * mine.lane);
+    if (out[i] < 0) continue;
+    const long long at = ((long long)w.token0 * pages.heads + out[i]) * D + 8 * piece;
+    k[i].store(keys + at);
+    v[i].store(values + at);
   }
 }
 
@@ -227,17 +257,24 @@ static int check_same_type(const char* who, int type, int cache) {
   return FTK_OK;
 }
 
-// Calls f(items of a thread, blocks): four items where that leaves two blocks of 256 threads or more to a compute unit (the look-ups of a wave then serve four rows), one
-// for less, whose time is the chain of look-ups.
+// Calls f(rows that a lane has a piece of, grid, tokens and heads of a wave): two rows where that leaves two blocks or more to a compute unit,
+// one for less, whose time is the chain of look-ups.  (Prompts of 4750 tokens, 8 heads of 128 in bf16, into int8: 9.1 us with two, 10.5 with one, 9.6 with
+// four; 42800 such tokens out of int8: 50 us with two or four, 55 with eight, 62 with a look-up for each row.)
 template <int D, typename F>
-static int with_items(const char* who, long long items, F&& f) {
+static int with_items(const char* who, int tokens, int heads, F&& f) {
   const DeviceProps* d = nullptr;
   if (const int rc = device_props(&d)) return rc;
-  constexpr long long step = kKvThreads / kRowLanes<D>;
-  const bool many = items >= 4 * step * 2 * d->cus;
-  const long long per = many ? 4 * step : step, n = (items + per - 1) / per;
-  if (n > INT_MAX) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: too many rows for one launch", who);
-  return many ? f(std::integral_constant<int, 4>{}, (unsigned)n) : f(std::integral_constant<int, 1>{}, (unsigned)n);
+  auto with = [&](auto items) -> int {
+    constexpr int R = kWaveRows<D, decltype(items)::value>;
+    const KvSplit split{std::max(1, R / heads), std::min(R, heads)};
+    const long long blocks = ((long long)tokens + 4LL * split.tokens - 1) / (4LL * split.tokens);
+    const int parts = (heads + split.heads - 1) / split.heads;
+    if (parts > 65535 || blocks > UINT_MAX / kKvThreads) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: too many heads or tokens for one launch", who);
+    return f(items, dim3((unsigned)blocks, (unsigned)parts), split);
+  };
+  static_assert(kKvThreads == 4 * 64, "four waves");
+  const bool many = (long long)tokens * heads >= 4LL * kWaveRows<D, 2> * 2 * d->cus;
+  return many ? with(std::integral_constant<int, 2>{}) : with(std::integral_constant<int, 1>{});
 }
 
 }  // namespace ftk
@@ -259,15 +296,14 @@ int ftk_kv_cache_write(const void* keys, const void* values, int type, long long
   for (long long s : {st.k_token, st.k_head, st.v_token, st.v_head})
     if (s < 0 || s % 8) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: strides must be multiples of 8 elements", who);
   if (!aligned16(keys) || !aligned16(values)) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: keys and values must be 16-byte aligned", who);
-  const long long items = (long long)b.tokens * p.heads;
   return with_kv_types(type, pages->type, pages->head_size, [&](auto t, auto f, auto d) -> int {
     using T = decltype(t);
     constexpr KvFormat F = decltype(f)::value;
     constexpr int D = decltype(d)::value;
-    return with_items<D>(who, items, [&](auto n, unsigned blocks) -> int {
+    return with_items<D>(who, b.tokens, p.heads, [&](auto n, dim3 grid, KvSplit split) -> int {
       constexpr int ITEMS = decltype(n)::value;
-      hipLaunchKernelGGL((kv_write_kernel<T, F, D, ITEMS>), dim3(blocks), dim3(kKvThreads), 0, (hipStream_t)stream, (const typename T::scalar*)keys,
-                         (const typename T::scalar*)values, st, p, b, items);
+      hipLaunchKernelGGL((kv_write_kernel<T, F, D, ITEMS>), grid, dim3(kKvThreads), 0, (hipStream_t)stream, (const typename T::scalar*)keys,
+                         (const typename T::scalar*)values, st, p, b, split);
       return check_launch("kv_write_kernel");
     });
   });
@@ -285,7 +321,6 @@ int ftk_kv_cache_read(const ftk_kv_pages* pages, const ftk_kv_batch* batch, int 
   if (!codes && type != FTK_F32 && type != pages->type) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: pages of 16 bits are read in their type or in fp32", who);
   if (b.tokens == 0) return FTK_OK;
   if (!keys || !values || !aligned16(keys) || !aligned16(values)) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: keys and values must be non-NULL and 16-byte aligned", who);
-  const long long items = (long long)b.tokens * p.heads;
   // what codes stand for does not depend on the type they came from
   return with_kv_types(pages->type == FTK_BF16 ? FTK_BF16 : FTK_F16, pages->type, pages->head_size, [&](auto t, auto f, auto d) -> int {
     using T = decltype(t);
@@ -293,9 +328,9 @@ int ftk_kv_cache_read(const ftk_kv_pages* pages, const ftk_kv_batch* batch, int 
     constexpr int D = decltype(d)::value;
     auto launch = [&](auto out) -> int {
       using Out = decltype(out);
-      return with_items<D>(who, items, [&](auto n, unsigned blocks) -> int {
+      return with_items<D>(who, b.tokens, p.heads, [&](auto n, dim3 grid, KvSplit split) -> int {
         constexpr int ITEMS = decltype(n)::value;
-        hipLaunchKernelGGL((kv_read_kernel<T, F, Out, D, ITEMS>), dim3(blocks), dim3(kKvThreads), 0, (hipStream_t)stream, p, b, (Out*)keys, (Out*)values, items);
+        hipLaunchKernelGGL((kv_read_kernel<T, F, Out, D, ITEMS>), grid, dim3(kKvThreads), 0, (hipStream_t)stream, p, b, (Out*)keys, (Out*)values, split);
         return check_launch("kv_read_kernel");
       });
     };
