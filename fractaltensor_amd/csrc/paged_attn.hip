@@ -1060,9 +1060,11 @@ __device__ __forceinline__ int row_parts(const AttnArgs& a, int token, int first
 // many where only small sequences are cut and most waves find nothing to do.
 template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) {
-  constexpr int L = D / 4, SL = 64 / L, K = kPartsMost / 64;    // lanes of a part, parts at once
+  constexpr int L = D / 4, SL = 64 / L, K = kPartsMost / 64;    // lanes of a part, parts of a wave at once
+  constexpr int TURN = SL * WAVES, PRE = WAVES == 4 ? kPartsMost / TURN : std::min(8, 64 / TURN);    // parts at once; turns whose loads go out first
   __shared__ v4f so[WAVES == 4 ? 4 * L : 1];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, slice = lane / L, c = lane - slice * L;
+  const int mine = (WAVES == 4 ? wave * SL : 0) + slice;
   const long long all_rows = (long long)a.batch.tokens * a.heads;
   const long long row0 = ((long long)blockIdx.x * (WAVES == 4 ? 1 : 4) + (WAVES == 4 ? 0 : wave)) * rows;
   if (row0 >= all_rows) return;
@@ -1080,6 +1082,14 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
     const int n = __builtin_amdgcn_readlane(parts, r);
     const bool none = __builtin_amdgcn_readlane(hi, r) <= __builtin_amdgcn_readlane(lo, r);
     const float* const ml = a.part_ml + 2 * at * a.stride;
+    // the first PRE turns' sums are asked for beside (m, l): all of them where four waves share a row
+    const float* const po = a.part_o + at * a.stride * D + 4 * c;
+    v4f early[PRE];
+#pragma unroll
+    for (int i = 0; i < PRE; ++i) {
+      const int p = i * TURN + mine;
+      early[i] = p < n && slice < SL ? *reinterpret_cast<const v4f*>(po + (size_t)p * D) : v4f{0.f, 0.f, 0.f, 0.f};
+    }
     float m[K], w[K], top = kNoRef, sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -1098,19 +1108,26 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-    const float* const po = a.part_o + at * a.stride * D + 4 * c;
     v4f acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int last = min(n - 64 * k, 64);
-#pragma unroll 4
-      for (int p0 = (WAVES == 4 ? wave : 0) * SL; p0 < last; p0 += (WAVES == 4 ? 4 : 1) * SL) {
-        const int p = p0 + slice;
-        const float weight = __shfl(w[k], p & 63);
-        if (p < last && slice < SL) {
-          const v4f v = *reinterpret_cast<const v4f*>(po + (size_t)(64 * k + p) * D);
+    for (int i = 0; i < PRE; ++i) {
+      const float weight = __shfl(w[i * TURN / 64], (i * TURN + mine) & 63);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] += weight * v[e];
+      for (int e = 0; e < 4; ++e) acc[e] += weight * early[i][e];
+    }
+    if constexpr (WAVES == 1) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int last = min(n - 64 * k, 64);
+#pragma unroll 4
+        for (int p0 = k == 0 ? PRE * TURN : 0; p0 < last; p0 += TURN) {
+          const int p = p0 + slice;
+          const float weight = __shfl(w[k], p & 63);
+          if (p < last && slice < SL) {
+            const v4f v = *reinterpret_cast<const v4f*>(po + (size_t)(64 * k + p) * D);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += weight * v[e];
+          }
         }
       }
     }
