@@ -1010,16 +1010,17 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   }
 }
 
-// The first `pairs` workgroups take sequences of at most small_rows = 16 rows, which would leave seven of the eight waves without any: two
-// (sequence, head, part) each, by four waves that cut the keys as in the narrow kernel.  They read while the others multiply.  (A chunk of 512 tokens
-// beside five sequences that decode, 16 heads, 4 of keys, up to 16384 of them: 165 us with all on the wide form, CHUNK_US so.)
+// The workgroups behind the first `wide` take sequences of at most small_rows = 16 rows, which would leave seven of the eight waves without
+// any: two (sequence, head, part) each, by four waves that cut the keys as in the narrow kernel.  They read on the compute units that the others
+// leave free, or have left, while those multiply.  (A chunk of 512 tokens beside five sequences that decode, 16 heads, 4 of keys, up to
+// 16384 of them, in int8: 165 us with all on the wide form, CHUNK_US so.)
 template <typename T, KvFormat F, int D>
-__global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs a, int pairs) {
+__global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs a, int wide) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   Job j;
-  if ((int)blockIdx.x < pairs) {
+  if ((int)blockIdx.x >= wide) {
     const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
-    const int item = 2 * blockIdx.x + half, kv_head = item % a.pages.heads, rest = item / a.pages.heads;
+    const int item = 2 * (blockIdx.x - wide) + half, kv_head = item % a.pages.heads, rest = item / a.pages.heads;
     const int b = rest / a.small.nparts, part = rest - b * a.small.nparts;
     if (b < a.batch.sequences && find_job<16>(a, b, 0, part, true, j)) {
       narrow_attention<T, F, D, 1>(a, j, kv_head, smem + half * NarrowShape<F, D>::LDS, threadIdx.x & 255);
@@ -1030,7 +1031,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs
     return;
   }
   // the head goes fastest, so that the row blocks of a head meet on the XCDs that have its keys
-  const int id = blockIdx.x - pairs, kv_head = id % a.pages.heads, rest = id / a.pages.heads;
+  const int id = blockIdx.x, kv_head = id % a.pages.heads, rest = id / a.pages.heads;
   const int slot = rest / a.cut.nparts, part = rest - slot * a.cut.nparts;
   int b, tile;
   if (!find_rows<kWideRows>(a, slot, &b, &tile) || !find_job<kWideRows>(a, b, tile, part, false, j)) return;
@@ -1173,8 +1174,12 @@ static double narrow_cost(double workgroups, int part_keys, int held, int cus) {
   return rounds * (3.0 + part_keys * (held / 1000.0) / std::min(17.0, 5800.0 / at_once));
 }
 
-// The same of the wide kernel: rounds of one workgroup to a compute unit, which takes 2 us for a tile of 64 keys of 128.
-static double wide_cost(double workgroups, double part_keys, int D, int cus) { return std::ceil(workgroups / cus) * (6.0 + part_keys / 64 * (2.0 * D / 128)); }
+// The same of the wide kernel: rounds of one workgroup to a compute unit, which takes 2 us for a tile of 64 keys of 128; then what is left of `small` us of
+// other workgroups when these have filled the last round.
+static double wide_cost(double workgroups, double part_keys, int D, int cus, double small) {
+  const double each = 6.0 + part_keys / 64 * (2.0 * D / 128), rounds = std::ceil(workgroups / cus);
+  return rounds * each + std::max(0.0, small - (rounds * cus - workgroups) * each) / cus;
+}
 
 // Leaving parts and joining them: a launch, and fp32 sums written and read at 4 TB/s.
 static double join_cost(double rows, int D, int nparts) { return nparts > 1 ? 5.0 + rows * nparts * D * 8 / 4e6 : 0.0; }
@@ -1226,16 +1231,18 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
     const double units = (double)p.slots * pages.heads;
     p.cut = best_cut(keys, 256, rows, D, room, [&](const Cut& c) { return narrow_cost(units * c.nparts, c.part_keys, held, cus) + join_cost(rows, D, c.nparts); });
   } else {
+    // the small sequences: as many as there can be beside ones of `most` tokens, in parts of some 20 us
+    double small = 0.0;
+    if (p.small_rows > 0) {
+      p.small = cut_into(keys, std::min({std::max(1, (int)((long long)keys * held / (20 * 17000))), keys / 256 + 1, kPartsMost}));
+      while (p.small.nparts > 1 && workspace_of(rows, D, p.small.nparts) > room) p.small = cut_into(keys, p.small.nparts - 1);
+      const double sequences = std::max(0.0, b.sequences - std::ceil((double)(b.tokens - b.sequences) / std::max(1LL, most - 1)));
+      small = sequences * pages.heads * p.small.nparts / 2 * (3.0 + p.small.part_keys * (held / 17000.0));
+    }
     // whole row blocks; a chunk that sees itself under a causal mask works on half of its own keys
     const double units = (double)std::max<long long>(1, b.tokens * (long long)group / R) * pages.heads, own = std::min<double>(most, keys) / 2;
     p.cut = best_cut(keys, 512, rows, D, room,
-                     [&](const Cut& c) { return wide_cost(units * c.nparts, c.part_keys * (1 - own / keys), D, cus) + join_cost(rows, D, c.nparts); });
-    // the small sequences beside them: parts that take no longer than those, as far as there is room for as many
-    if (p.small_rows > 0) {
-      const int want = std::max(1, (int)((long long)keys * held / (20 * 17000)));   // some 20 us each
-      p.small = cut_into(keys, std::min({want, keys / 256 + 1, kPartsMost}));
-      while (p.small.nparts > p.cut.nparts && workspace_of(rows, D, p.small.nparts) > room) p.small = cut_into(keys, p.small.nparts - 1);
-    }
+                     [&](const Cut& c) { return wide_cost(units * c.nparts, c.part_keys * (1 - own / keys), D, cus, small) + join_cost(rows, D, c.nparts); });
   }
   p.stride = std::max(p.cut.nparts, p.small.nparts);
   return p;
@@ -1334,7 +1341,7 @@ int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long 
     } else {
       static DeviceOnce once;
       constexpr int lds = std::max(WideShape<D>::LDS, 2 * NarrowShape<F, D>::LDS);
-      bad = launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D>, once, blocks + pairs, kWideWaves, lds, s, a, (int)pairs);
+      bad = launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D>, once, blocks + pairs, kWideWaves, lds, s, a, (int)blocks);
     }
     if (bad || p.stride == 1) return bad;
     // few rows of many parts: a block to each; only small sequences cut: 16 rows to a wave, most of which have nothing to join
