@@ -1013,7 +1013,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
 // The workgroups behind the first `wide` take sequences of at most small_rows = 16 rows, which would leave seven of the eight waves without
 // any: two (sequence, head, part) each, by four waves that cut the keys as in the narrow kernel.  They read on the compute units that the others
 // leave free, or have left, while those multiply.  (A chunk of 512 tokens beside five sequences that decode, 16 heads, 4 of keys, up to
-// 16384 of them, in int8: 165 us with all on the wide form, CHUNK_US so.)
+// 16384 of them, in int8: 165 us with all on the wide form, 110 so, and 11 for joining.)
 template <typename T, KvFormat F, int D>
 __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs a, int wide) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -1168,10 +1168,13 @@ struct Plan {
 static size_t workspace_of(long long rows, int D, int nparts) { return nparts > 1 ? (size_t)rows * nparts * (D + 2) * 4 : 0; }
 
 // us of a launch of the narrow kernel: rounds of two workgroups to a compute unit, 3 us each until the first tile is there, and their share of 5.8 TB/s, or
-// the 17 KB a us that one workgroup gets through.
-static double narrow_cost(double workgroups, int part_keys, int held, int cus) {
-  const double at_once = std::min(workgroups, 2.0 * cus), rounds = std::ceil(workgroups / (2.0 * cus));
-  return rounds * (3.0 + part_keys * (held / 1000.0) / std::min(17.0, 5800.0 / at_once));
+// the 17 KB a us that one workgroup gets through.  The lengths of several sequences are not known here, only the greatest: the mean of that with all of them alike
+// and that with two thirds of the work, where workgroups follow one another as they end and no round is waited for.  (Five tokens each of 16 sequences
+// of up to 4096 keys: 31 us with three parts, as all alike would have it, 26 with four.)
+static double narrow_cost(double workgroups, int part_keys, int held, int cus, bool alike) {
+  const double at_once = std::min(workgroups, 2.0 * cus), rounds = std::ceil(workgroups / (2.0 * cus)), kb = part_keys * (held / 1000.0);
+  const double same = rounds * (3.0 + kb / std::min(17.0, 5800.0 / at_once));
+  return alike ? same : 0.5 * (same + 3.0 + std::max(workgroups * kb * (2.0 / 3) / 5800.0, kb / 17.0));
 }
 
 // The same of the wide kernel: rounds of one workgroup to a compute unit, which takes 2 us for a tile of 64 keys of 128; then what is left of `small` us of
@@ -1229,7 +1232,7 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
   p.small = Cut{1, keys};
   if (p.narrow) {
     const double units = (double)p.slots * pages.heads;
-    p.cut = best_cut(keys, 256, rows, D, room, [&](const Cut& c) { return narrow_cost(units * c.nparts, c.part_keys, held, cus) + join_cost(rows, D, c.nparts); });
+    p.cut = best_cut(keys, 256, rows, D, room, [&](const Cut& c) { return narrow_cost(units * c.nparts, c.part_keys, held, cus, b.sequences == 1) + join_cost(rows, D, c.nparts); });
   } else {
     // the small sequences: as many as there can be beside ones of `most` tokens, in parts of some 20 us
     double small = 0.0;
