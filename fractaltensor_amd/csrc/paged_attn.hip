@@ -11,8 +11,10 @@
 // first product (the contraction takes the keys in the order a lane holds them).  Long sequences are cut into parts of
 // `part_keys` keys, a workgroup each, which leave (reference, sum, unnormalised O) for a second launch to join.
 //
-// Rounding: scores, softmax state and O are fp32 and Q is not scaled beforehand; the one rounding is that of the weights to 16 bits
-// as operands of P V, half a step (2^-12 fp16, 2^-9 bf16) each.  A cache of 8 bits enters the products as its exact values.
+// Rounding: scores, softmax state and O are fp32 and Q is not scaled beforehand.  Weights enter P V in 16 bits: in the wide kernel rounded, half a
+// step (2^-12 fp16, 2^-9 bf16) each, which with the result's own rounding is sqrt(2) of the error of that alone; in the narrow kernel, whose matrix unit has
+// time for a second product, as the rounded weight and what it leaves, also in 16 bits (2 to 4 % of the time; without it results of few elements were now and
+// then 1.5 times as far off as their own rounding).  A cache of 8 bits enters the products as its exact values.
 #include <algorithm>
 #include <cmath>
 
@@ -383,7 +385,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     keys_read();
-    v8 p[NQ];
+    v8 p[NQ], rest[NQ];
     unsigned seen[NQ];                                            // MASKED: which of the lane's eight keys its row sees
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
@@ -419,7 +421,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
           for (int r = 0; r < 4; ++r) o[nq][dt][r] *= alpha;
       }
       // bf16 weights take the power of two of their value's row with them; those of fp16 could leave its range, and V takes it
-      unsigned w[4];
+      unsigned w[4], u[4];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -430,9 +432,12 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
             p0 = ldexpf(p0, vexp[h][r]);
             p1 = ldexpf(p1, vexp[h][r + 1]);
           }
-          w[2 * h + r / 2] = T::pack(p0, p1);
+          const unsigned pair = T::pack(p0, p1);
+          w[2 * h + r / 2] = pair;
+          u[2 * h + r / 2] = T::pack(p0 - T::low(pair), p1 - T::high(pair));
         }
       p[nq] = __builtin_bit_cast(v8, (v4u{w[0], w[1], w[2], w[3]}));
+      rest[nq] = __builtin_bit_cast(v8, (v4u{u[0], u[1], u[2], u[3]}));
     }
     v2h vpair[4];
     if constexpr (F != kSame && std::is_same<T, Half>::value) {
@@ -489,7 +494,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
         }
       }
 #pragma unroll
-      for (int nq = 0; nq < NQ; ++nq) o[nq][dt] = T::mma16(vf, p[nq], o[nq][dt]);
+      for (int nq = 0; nq < NQ; ++nq) o[nq][dt] = T::mma16(vf, rest[nq], T::mma16(vf, p[nq], o[nq][dt]));
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     values_read();
