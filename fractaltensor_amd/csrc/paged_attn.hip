@@ -3,18 +3,19 @@
 // The G = query heads / kv heads query heads that share a kv head, times the new tokens of a sequence, are the ROWS of one
 // product with that head's keys: row r is token r / G, head r % G.  Two kernels by the number of rows:
 //
-//   narrow  (at most 64 rows: decoding, drafts): bound by reading the cache once.  A workgroup has 16 NQ rows; its four waves cut the
-//           KEYS, each walking every fourth 32-key tile from copies straight into its own LDS, with no barrier in the loop.
+//   narrow  (at most 64 rows: decoding, drafts): bound by reading the cache once.  A workgroup has 16 NQ rows, 16 or 32; its four waves cut the
+//           KEYS, each walking every fourth 32-key tile from copies straight into its own LDS, with no barrier in the loop.  The two
+//           to four workgroups of more rows run next to one another, and all but one find what they read in the caches.
 //   wide    (chunks and prompts): bound by the matrix pipe.  A wave has 32 rows, and the eight waves of a workgroup share 64-key tiles.
 //
 // Products are transposed in both, so that a lane has one row: S^T = K Q^T, O^T = V^T P^T with P as it comes out of the
 // first product (the contraction takes the keys in the order a lane holds them).  Long sequences are cut into parts of
 // `part_keys` keys, a workgroup each, which leave (reference, sum, unnormalised O) for a second launch to join.
 //
-// Rounding: scores, softmax state and O are fp32 and Q is not scaled beforehand.  Weights enter P V in 16 bits: in the wide kernel rounded, half a
-// step (2^-12 fp16, 2^-9 bf16) each, which with the result's own rounding is sqrt(2) of the error of that alone; in the narrow kernel, whose matrix unit has
-// time for a second product, as the rounded weight and what it leaves, also in 16 bits (2 to 4 % of the time; without it results of few elements were now and
-// then 1.5 times as far off as their own rounding).  A cache of 8 bits enters the products as its exact values.
+// Rounding: scores, softmax state and O are fp32 and Q is not scaled beforehand.  Weights enter P V in 16 bits: rounded, half a step (2^-12 fp16,
+// 2^-9 bf16) each, which with the result's own rounding makes sqrt(2) of the error of that alone; but at most 16 rows, whose results may be so few that this
+// comes to 1.5 now and then, leave the matrix unit time for a second product, and there a weight is the rounded one and what that leaves, also in
+// 16 bits (2 to 4 % of the time).  A cache of 8 bits enters the products as its exact values.
 #include <algorithm>
 #include <cmath>
 
@@ -220,10 +221,13 @@ struct NarrowShape {
 };
 
 // 16 (4) bytes a lane from an address of its own, otherwise as lds_dma16_once (lds_dma16).  A call reads a byte of the cache once, and
-// the next call reads another layer's: copies that leave no lines are 10 % faster (64 sequences of up to 8192 keys 140 -> 126 us).
+// the next call reads another layer's: copies that leave no lines are 10 % faster (64 sequences of up to 8192 keys 140 -> 126 us).  KEPT: another workgroup
+// is about to read the same.
+template <bool KEPT>
 __device__ __forceinline__ void lds_dma16_from(const unsigned char* from, void* lds_base) {
   const unsigned lds_addr = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)lds_base);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" : : "s"(lds_addr), "v"(from) : "memory", "m0");
+  if constexpr (KEPT) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(from) : "memory", "m0");
+  else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" : : "s"(lds_addr), "v"(from) : "memory", "m0");
 }
 __device__ __forceinline__ void lds_dma4_from(const signed char* from, void* lds_base) {
   const unsigned lds_addr = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)lds_base);
@@ -231,7 +235,7 @@ __device__ __forceinline__ void lds_dma4_from(const signed char* from, void* lds
 }
 
 // tid: of the 256 threads that work together
-template <typename T, KvFormat F, int D, int NQ>
+template <typename T, KvFormat F, int D, int NQ, bool KEPT>
 __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j, int kv_head, unsigned char* smem, int tid) {
   using S = NarrowShape<F, D>;
   using v8 = typename T::v8;
@@ -279,8 +283,9 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
       const unsigned char *const b0 = from + at.r0 * S::BYTES, *const b1 = from + at.r1 * S::BYTES;
 #pragma unroll
       for (int c = 0; c < S::COPIES; ++c) {
-        if constexpr (WHOLE) lds_dma16_once(c < OFFS ? b0 : b1, off[c % OFFS], to + 1024 * c);
-        else lds_dma16_from(((64 * c + lane) / CH >= 16 ? b1 : b0) + off[c], to + 1024 * c);
+        if constexpr (WHOLE && KEPT) lds_dma16(c < OFFS ? b0 : b1, off[c % OFFS], to + 1024 * c);
+        else if constexpr (WHOLE) lds_dma16_once(c < OFFS ? b0 : b1, off[c % OFFS], to + 1024 * c);
+        else lds_dma16_from<KEPT>(((64 * c + lane) / CH >= 16 ? b1 : b0) + off[c], to + 1024 * c);
       }
     } else {
       // rows outside [lo, hi) repeat the nearest key inside: their weights are zero, and what they hold is finite if the cache is
@@ -289,7 +294,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
         const int p = 64 * c + lane, row = p / CH, slot = p - row * CH;
         const int key = min(max(row, least), most);
         const long long at_row = key >= 16 ? at.r1 + key - 16 : at.r0 + key;
-        lds_dma16_from(from + (size_t)at_row * S::BYTES + 16 * (slot ^ swizzle<S::BYTES>(row)), to + 1024 * c);
+        lds_dma16_from<KEPT>(from + (size_t)at_row * S::BYTES + 16 * (slot ^ swizzle<S::BYTES>(row)), to + 1024 * c);
       }
     }
     if constexpr (F != kSame && !VALUES) {
@@ -385,6 +390,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     keys_read();
+    constexpr bool REST = NQ == 1;                                // weights as two operands: rounded, and what that leaves
     v8 p[NQ], rest[NQ];
     unsigned seen[NQ];                                            // MASKED: which of the lane's eight keys its row sees
 #pragma unroll
@@ -434,7 +440,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
           }
           const unsigned pair = T::pack(p0, p1);
           w[2 * h + r / 2] = pair;
-          u[2 * h + r / 2] = T::pack(p0 - T::low(pair), p1 - T::high(pair));
+          u[2 * h + r / 2] = REST ? T::pack(p0 - T::low(pair), p1 - T::high(pair)) : 0;
         }
       p[nq] = __builtin_bit_cast(v8, (v4u{w[0], w[1], w[2], w[3]}));
       rest[nq] = __builtin_bit_cast(v8, (v4u{u[0], u[1], u[2], u[3]}));
@@ -494,7 +500,10 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
         }
       }
 #pragma unroll
-      for (int nq = 0; nq < NQ; ++nq) o[nq][dt] = T::mma16(vf, rest[nq], T::mma16(vf, p[nq], o[nq][dt]));
+      for (int nq = 0; nq < NQ; ++nq) {
+        o[nq][dt] = T::mma16(vf, p[nq], o[nq][dt]);
+        if constexpr (REST) o[nq][dt] = T::mma16(vf, rest[nq], o[nq][dt]);
+      }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     values_read();
@@ -589,15 +598,22 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
   }
 }
 
-template <typename T, KvFormat F, int D, int NQ>
-__global__ __launch_bounds__(kWaves * 64, NQ == 4 ? 1 : 2) void paged_narrow_kernel(AttnArgs a) {
+// The slots are `tiles` row blocks of each of `sequences`.  Workgroups that are 8 apart run on one XCD, at about the same time: the row blocks of a (sequence, head, part)
+// are, and the head goes fastest.
+template <typename T, KvFormat F, int D, int NQ, bool KEPT>
+__global__ __launch_bounds__(kWaves * 64, 2) void paged_narrow_kernel(AttnArgs a, int tiles) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  const int kv_head = blockIdx.x % a.pages.heads, rest = blockIdx.x / a.pages.heads;
-  const int slot = rest / a.cut.nparts, part = rest - slot * a.cut.nparts;
+  int id = blockIdx.x, tile = 0;
+  if (KEPT) {
+    const int units = gridDim.x / tiles, group = id / (8 * tiles) * 8, width = min(8, units - group), in = id - group * tiles;   // the last group may be narrower
+    tile = in / width;
+    id = group + in - tile * width;
+  }
+  const int kv_head = id % a.pages.heads, rest = id / a.pages.heads;
+  const int b = a.batch.sequences - 1 - rest / a.cut.nparts, part = rest % a.cut.nparts;
   Job j;
-  int b, tile;
-  if (!find_rows<16 * NQ>(a, slot, &b, &tile) || !find_job<16 * NQ>(a, b, tile, part, false, j)) return;
-  narrow_attention<T, F, D, NQ>(a, j, kv_head, smem, threadIdx.x);
+  if (!find_job<16 * NQ>(a, b, tile, part, false, j)) return;
+  narrow_attention<T, F, D, NQ, KEPT>(a, j, kv_head, smem, threadIdx.x);
 }
 
 // ---- wide -----------------------------------------------------------------------------
@@ -1028,7 +1044,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs
     const int item = 2 * (blockIdx.x - wide) + half, kv_head = item % a.pages.heads, rest = item / a.pages.heads;
     const int b = rest / a.small.nparts, part = rest - b * a.small.nparts;
     if (b < a.batch.sequences && find_job<16>(a, b, 0, part, true, j)) {
-      narrow_attention<T, F, D, 1>(a, j, kv_head, smem + half * NarrowShape<F, D>::LDS, threadIdx.x & 255);
+      narrow_attention<T, F, D, 1, false>(a, j, kv_head, smem + half * NarrowShape<F, D>::LDS, threadIdx.x & 255);
     } else {                                                     // the other half's two barriers
       __syncthreads();
       __syncthreads();
@@ -1164,7 +1180,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
 // How a call is run.
 struct Plan {
   bool narrow;
-  int nq;                  // narrow: blocks of 16 rows
+  int nq;                  // narrow: blocks of 16 rows of a workgroup, 1 or 2
   int slots, slots_per_seq;
   Cut cut, small;
   int small_rows, stride;
@@ -1222,17 +1238,19 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
   const long long most = max_queries > 0 ? std::min(max_queries, b.tokens) : b.tokens;   // new tokens of a sequence
   const long long most_rows = most * group, rows = (long long)b.tokens * heads;
   p.narrow = most_rows <= 64;
-  p.nq = most_rows <= 16 ? 1 : most_rows <= 32 ? 2 : 4;
-  const int R = p.narrow ? 16 * p.nq : kWideRows;
-  const long long per_seq = (most_rows + R - 1) / R, packed = (long long)b.tokens * group / R + b.sequences;
-  // numbered by row blocks, unless most of such slots would be empty
-  p.slots_per_seq = b.sequences * per_seq <= 2 * packed ? (int)per_seq : 0;
-  p.slots = (int)std::min<long long>(p.slots_per_seq ? b.sequences * per_seq : packed, INT_MAX);
-  p.small_rows = p.narrow || b.sequences == 1 ? 0 : 16;
   const long long capacity = (long long)b.width << page_shift;
   long long seen = max_keys > 0 ? std::min<long long>(max_keys, capacity) : capacity;
   if (window > 0) seen = std::min(seen, most + window + 64);   // from the first key that the first new token sees, down to a multiple of 64
   const int keys = (int)std::min<long long>(seen, INT_MAX - 1024);
+  // 32 rows to a narrow workgroup read the keys half as often as 16; those are the faster ones where even parts of 256 keys are fewer than the compute
+  // units.  (Six tokens, 64 heads, 8 of keys of 128: 16 sequences of up to 4096 keys 64 us by 32 rows, 63 to 73 by 16; two of up to 1000 keys 15 and 12.)
+  p.nq = most_rows <= 16 || ((most_rows + 31) / 32) * b.sequences * pages.heads * ((keys + 255) / 256) < cus ? 1 : 2;
+  const int R = p.narrow ? 16 * p.nq : kWideRows;
+  const long long per_seq = (most_rows + R - 1) / R, packed = (long long)b.tokens * group / R + b.sequences;
+  // numbered by row blocks, unless most of such slots would be empty (as those of narrow workgroups, four to a sequence at most, cannot be)
+  p.slots_per_seq = p.narrow || b.sequences * per_seq <= 2 * packed ? (int)per_seq : 0;
+  p.slots = (int)std::min<long long>(p.slots_per_seq ? b.sequences * per_seq : packed, INT_MAX);
+  p.small_rows = p.narrow || b.sequences == 1 ? 0 : 16;
   const int held = pages.type == FTK_F16 || pages.type == FTK_BF16 ? 4 * D : 2 * D + 2;   // bytes of a position and head
   p.small = Cut{1, keys};
   if (p.narrow) {
@@ -1340,12 +1358,13 @@ int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long 
     constexpr int D = decltype(dc)::value;
     int bad;
     if (p.narrow) {
-      auto launch = [&](auto nq) -> int {
+      auto launch = [&](auto nq, auto kept) -> int {
         constexpr int NQ = decltype(nq)::value;
         static DeviceOnce once;
-        return launch_with_lds("paged_narrow_kernel", paged_narrow_kernel<T, F, D, NQ>, once, blocks, kWaves, NarrowShape<F, D>::LDS, s, a);
+        return launch_with_lds("paged_narrow_kernel", paged_narrow_kernel<T, F, D, NQ, decltype(kept)::value>, once, blocks, kWaves, NarrowShape<F, D>::LDS, s, a, p.slots_per_seq);
       };
-      bad = p.nq == 1 ? launch(std::integral_constant<int, 1>{}) : p.nq == 2 ? launch(std::integral_constant<int, 2>{}) : launch(std::integral_constant<int, 4>{});
+      auto with_kept = [&](auto nq) { return p.slots_per_seq == 1 ? launch(nq, std::false_type{}) : launch(nq, std::true_type{}); };
+      bad = p.nq == 1 ? with_kept(std::integral_constant<int, 1>{}) : with_kept(std::integral_constant<int, 2>{});
     } else {
       static DeviceOnce once;
       constexpr int lds = std::max(WideShape<D>::LDS, 2 * NarrowShape<F, D>::LDS);
