@@ -13,9 +13,9 @@
 // `part_keys` keys, a workgroup each, which leave (reference, sum, unnormalised O) for a second launch to join.
 //
 // Rounding: scores, softmax state and O are fp32 and Q is not scaled beforehand.  Weights enter P V in 16 bits: rounded, half a step (2^-12 fp16,
-// 2^-9 bf16) each, which with the result's own rounding makes sqrt(2) of the error of that alone; but at most 16 rows, whose results may be so few that this
-// comes to 1.5 now and then, leave the matrix unit time for a second product, and there a weight is the rounded one and what that leaves, also in
-// 16 bits (2 to 4 % of the time).  A cache of 8 bits enters the products as its exact values.
+// 2^-9 bf16) each, which with the result's own rounding makes sqrt(2) of the error of that alone in the mean, and more now and then where results are few.
+// Calls of few results, by blocks of 16 rows, leave the matrix unit time for a second product: there a weight is the rounded one and what that leaves, also in
+// 16 bits.  (4 % of the time of 64 decoding sequences of up to 8192 keys, which therefore go without.)  A cache of 8 bits enters the products as its exact values.
 #include <algorithm>
 #include <cmath>
 
@@ -25,6 +25,7 @@ namespace ftk {
 
 constexpr int kWaves = 4;
 constexpr float kNoRef = -3.402823466e38f;   // the reference before any score: finite, so that -inf minus it is -inf
+constexpr long long kFewResults = 1 << 15;   // elements of o whose weights enter P V with what their rounding leaves
 constexpr float kSlack = 8.0f;               // the reference moves when a score is above it by 2^8 in the weights
 
 // How the keys of a sequence are cut: at most nparts parts of part_keys keys, the last of which takes what is left.
@@ -235,7 +236,7 @@ __device__ __forceinline__ void lds_dma4_from(const signed char* from, void* lds
 }
 
 // tid: of the 256 threads that work together
-template <typename T, KvFormat F, int D, int NQ, bool KEPT>
+template <typename T, KvFormat F, int D, int NQ, bool KEPT, bool REST>
 __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j, int kv_head, unsigned char* smem, int tid) {
   using S = NarrowShape<F, D>;
   using v8 = typename T::v8;
@@ -390,8 +391,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     keys_read();
-    constexpr bool REST = NQ == 1;                                // weights as two operands: rounded, and what that leaves
-    v8 p[NQ], rest[NQ];
+    v8 p[NQ], rest[NQ];                                           // REST: weights as two operands, rounded and what that leaves
     unsigned seen[NQ];                                            // MASKED: which of the lane's eight keys its row sees
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
@@ -600,7 +600,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
 
 // The slots are `tiles` row blocks of each of `sequences`.  Workgroups that are 8 apart run on one XCD, at about the same time: the row blocks of a (sequence, head, part)
 // are, and the head goes fastest.
-template <typename T, KvFormat F, int D, int NQ, bool KEPT>
+template <typename T, KvFormat F, int D, int NQ, bool KEPT, bool REST>
 __global__ __launch_bounds__(kWaves * 64, 2) void paged_narrow_kernel(AttnArgs a, int tiles) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   int id = blockIdx.x, tile = 0;
@@ -610,10 +610,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_narrow_kernel(AttnArgs a
     id = group + in - tile * width;
   }
   const int kv_head = id % a.pages.heads, rest = id / a.pages.heads;
-  const int b = a.batch.sequences - 1 - rest / a.cut.nparts, part = rest % a.cut.nparts;
+  const int b = rest / a.cut.nparts, part = rest % a.cut.nparts;
   Job j;
   if (!find_job<16 * NQ>(a, b, tile, part, false, j)) return;
-  narrow_attention<T, F, D, NQ, KEPT>(a, j, kv_head, smem, threadIdx.x);
+  narrow_attention<T, F, D, NQ, KEPT, REST>(a, j, kv_head, smem, threadIdx.x);
 }
 
 // ---- wide -----------------------------------------------------------------------------
@@ -1044,7 +1044,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs
     const int item = 2 * (blockIdx.x - wide) + half, kv_head = item % a.pages.heads, rest = item / a.pages.heads;
     const int b = rest / a.small.nparts, part = rest - b * a.small.nparts;
     if (b < a.batch.sequences && find_job<16>(a, b, 0, part, true, j)) {
-      narrow_attention<T, F, D, 1, false>(a, j, kv_head, smem + half * NarrowShape<F, D>::LDS, threadIdx.x & 255);
+      narrow_attention<T, F, D, 1, false, false>(a, j, kv_head, smem + half * NarrowShape<F, D>::LDS, threadIdx.x & 255);
     } else {                                                     // the other half's two barriers
       __syncthreads();
       __syncthreads();
@@ -1358,13 +1358,18 @@ int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long 
     constexpr int D = decltype(dc)::value;
     int bad;
     if (p.narrow) {
-      auto launch = [&](auto nq, auto kept) -> int {
-        constexpr int NQ = decltype(nq)::value;
+      using yes = std::true_type;
+      using no = std::false_type;
+      auto launch = [&](auto nq, auto kept, auto rest) -> int {
         static DeviceOnce once;
-        return launch_with_lds("paged_narrow_kernel", paged_narrow_kernel<T, F, D, NQ, decltype(kept)::value>, once, blocks, kWaves, NarrowShape<F, D>::LDS, s, a, p.slots_per_seq);
+        return launch_with_lds("paged_narrow_kernel", paged_narrow_kernel<T, F, D, decltype(nq)::value, decltype(kept)::value, decltype(rest)::value>, once, blocks, kWaves,
+                               NarrowShape<F, D>::LDS, s, a, p.slots_per_seq);
       };
-      auto with_kept = [&](auto nq) { return p.slots_per_seq == 1 ? launch(nq, std::false_type{}) : launch(nq, std::true_type{}); };
-      bad = p.nq == 1 ? with_kept(std::integral_constant<int, 1>{}) : with_kept(std::integral_constant<int, 2>{});
+      auto with_kept = [&](auto nq, auto rest) { return p.slots_per_seq == 1 ? launch(nq, no{}, rest) : launch(nq, yes{}, rest); };
+      using one = std::integral_constant<int, 1>;
+      if (p.nq == 2) bad = with_kept(std::integral_constant<int, 2>{}, no{});
+      else if (rows * D <= kFewResults) bad = with_kept(one{}, yes{});
+      else bad = with_kept(one{}, no{});
     } else {
       static DeviceOnce once;
       constexpr int lds = std::max(WideShape<D>::LDS, 2 * NarrowShape<F, D>::LDS);

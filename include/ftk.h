@@ -619,7 +619,7 @@ typedef struct ftk_kv_pages {
  * that they are its last positions.  Position p lies in row p % page_size of page
  * table[b, p / page_size] (table [sequences, table_width]).  `tokens` is how many
  * rows the packed arrays have; rows from starts[sequences] on are nobody's: they are
- * neither read nor written.  A sequence may have no new tokens, or no length;
+ * never written, and what they hold does not matter.  A sequence may have no new tokens, or no length;
  * without sequences or tokens a call does nothing.
  *
  * What the arrays hold is looked at on the device, where it cannot be refused:
@@ -684,9 +684,10 @@ int ftk_kv_cache_read(const ftk_kv_pages* pages, const ftk_kv_batch* batch,
  * see never matter to it, NaN and infinities included; one that is not finite
  * makes NaN of what sees it (a component of o for a value, all of it for a key).
  * fp32 accumulation; the one rounding on the way is that of the weights to the 16
- * bits of `type`.  Head sizes, pages and tokens in any mixture run on two kernels:
- * sequences of at most 64 rows (new tokens times heads / pages->heads) on one that
- * reads the cache once, larger ones on one made for the matrix unit.
+ * bits of `type`.  Sequences of any mixture of sizes go in one call: where max_queries
+ * leaves none with more than 64 rows (new tokens times heads / pages->heads), all run
+ * on a kernel made for reading the cache once; otherwise those of more than 16 rows run
+ * on one made for the matrix unit, the others beside them.
  *
  * max_queries, max_keys: promises that no sequence has more new tokens, or is
  * longer (0: no promise).  They decide which kernel runs and how the keys are
