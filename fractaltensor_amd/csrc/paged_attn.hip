@@ -25,6 +25,7 @@ namespace ftk {
 
 constexpr int kWaves = 4;
 constexpr float kNoRef = -3.402823466e38f;   // the reference before any score: finite, so that -inf minus it is -inf
+constexpr int kSmallRows = 16;                // sequences of at most so many rows, beside larger ones, are small
 constexpr long long kFewResults = 1 << 15;   // elements of o whose weights enter P V with what their rounding leaves
 constexpr float kSlack = 8.0f;               // the reference moves when a score is above it by 2^8 in the weights
 
@@ -46,8 +47,8 @@ struct AttnArgs {
   int slots, slots_per_seq;                   // blocks of rows, and those of a sequence (0: they are numbered over the packed rows)
   Cut cut, small;                             // `small` for sequences of at most small_rows rows
   int small_rows;
-  int stride;                                 // parts that there is room for
-  float *part_o, *part_ml;                    // [tokens * heads][stride][D], [..][2]
+  long long small_first;                      // parts of small sequences stand behind these many
+  float *part_o, *part_ml;                    // [tokens * heads][cut.nparts] parts, then [sequences][kv heads][kSmallRows][small.nparts]: D floats; two
 };
 
 // ---- which rows and which keys a workgroup has ----------------------------------------
@@ -59,13 +60,13 @@ struct Job {
   int lo, hi;                  // keys [lo, hi) that the rows of this workgroup and its part see
   int sure_lo, sure_hi;        // keys that each of its rows sees
   int part, parts;             // parts of this sequence
+  bool small;
 };
 
 // The keys that some row of the sequence sees begin here (a multiple of 64).
 __device__ __forceinline__ int seq_first_key(const AttnArgs& a, int first) {
   return a.window > 0 ? (int)max(0LL, (long long)first - a.window + 1) & ~63 : 0;
 }
-__device__ __forceinline__ Cut seq_cut(const AttnArgs& a, int n) { return n * a.group <= a.small_rows ? a.small : a.cut; }
 __device__ __forceinline__ int seq_parts(const AttnArgs& a, const Cut& cut, int first, int len) {
   if (cut.nparts == 1) return 1;
   const int keys = max(0, len - seq_first_key(a, first));
@@ -120,6 +121,7 @@ __device__ __forceinline__ bool find_job(const AttnArgs& a, int b, int tile, int
   j.lo = a.window > 0 ? clamp_position(p_lo - a.window + 1, j.len) : 0;
   j.sure_lo = a.window > 0 ? clamp_position(p_hi - a.window + 1, j.len) : 0;
   j.part = part;
+  j.small = small;
   const Cut cut = small ? a.small : a.cut;
   j.parts = seq_parts(a, cut, c.first, j.len);
   if (part >= j.parts) return false;
@@ -129,6 +131,11 @@ __device__ __forceinline__ bool find_job(const AttnArgs& a, int b, int tile, int
     if (part < j.parts - 1) j.hi = min(j.hi, clamp_position(from + cut.part_keys, j.len));
   }
   return true;
+}
+
+// The first part of a row among all parts; at: its place among the packed rows times heads.
+__device__ __forceinline__ long long first_part(const AttnArgs& a, bool small, int b, int kv_head, int row, long long at) {
+  return small ? a.small_first + (((long long)b * a.pages.heads + kv_head) * kSmallRows + row) * a.small.nparts : at * a.cut.nparts;
 }
 
 // The keys [lo, hi) that a row sees, and its place among the packed rows times heads.
@@ -582,12 +589,12 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
         if (j.parts == 1) {
           *reinterpret_cast<v2u*>((scalar*)a.o + r.at * D + 4 * g) = v2u{T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
         } else {
-          *reinterpret_cast<v4f*>(a.part_o + (r.at * a.stride + j.part) * D + 4 * g) = acc;
+          *reinterpret_cast<v4f*>(a.part_o + (first_part(a, j.small, j.b, kv_head, row, r.at) + j.part) * D + 4 * g) = acc;
         }
       }
       if (tid < 16) {
         if (j.parts > 1) {
-          float* const ml = a.part_ml + 2 * (r.at * a.stride + j.part);
+          float* const ml = a.part_ml + 2 * (first_part(a, j.small, j.b, kv_head, row, r.at) + j.part);
           ml[0] = top;
           ml[1] = sum;
         } else if (a.lse) {
@@ -996,14 +1003,14 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   l += __shfl_xor(l, 32);
   if (j.parts > 1) {
     if (wrow0 + jr < j.rows) {
-      float* const po = a.part_o + (r.at * a.stride + j.part) * D;
+      float* const po = a.part_o + (r.at * a.cut.nparts + j.part) * D;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
           *reinterpret_cast<v4f*>(po + 32 * dt + 8 * g + 4 * hh) = v4f{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
       if (hh == 0) {
-        float* const ml = a.part_ml + 2 * (r.at * a.stride + j.part);
+        float* const ml = a.part_ml + 2 * (r.at * a.cut.nparts + j.part);
         ml[0] = ref;
         ml[1] = l;
       }
@@ -1063,8 +1070,10 @@ __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs
 
 constexpr int kPartsMost = 256;
 
-// The parts of the sequence that a packed row belongs to (1: nothing to join), and the keys [*lo, *hi) that it sees.  first_token: that of the wave's first lane.
-__device__ __forceinline__ int row_parts(const AttnArgs& a, int token, int first_token, int* lo, int* hi) {
+// The parts of the sequence that row `at` of the packed rows times heads belongs to (1: nothing to join), the first of them, and the keys [*lo, *hi) that the row
+// sees.  first_token: that of the wave's first lane.
+__device__ __forceinline__ int row_parts(const AttnArgs& a, long long at, int first_token, int* lo, int* hi, long long* first_of) {
+  const int token = (int)(at / a.heads), head = (int)(at - (long long)token * a.heads);
   int b = count_at_most(a.batch.sequences, first_token, [&](int k) { return a.batch.starts[k + 1]; });
   while (b < a.batch.sequences && a.batch.starts[b + 1] <= token) ++b;
   if (b >= a.batch.sequences) return 1;
@@ -1074,7 +1083,10 @@ __device__ __forceinline__ int row_parts(const AttnArgs& a, int token, int first
   const long long position = (long long)first + (token - start);
   *hi = a.causal ? clamp_position(position + 1, len) : len;
   *lo = a.window > 0 ? clamp_position(position - a.window + 1, len) : 0;
-  return seq_parts(a, seq_cut(a, end - start), first, len);
+  const int kv_head = head / a.group;
+  const bool small = (end - start) * a.group <= a.small_rows;
+  *first_of = first_part(a, small, b, kv_head, (token - start) * a.group + head - kv_head * a.group, at);
+  return seq_parts(a, small ? a.small : a.cut, first, len);
 }
 
 // m = max m_p, l = sum l_p 2^(m_p - m), O = sum O_p 2^(m_p - m) / l over the parts of a row.  A wave (WAVES = 4: the four of a block) to a row: the
@@ -1090,12 +1102,9 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
   const long long all_rows = (long long)a.batch.tokens * a.heads;
   const long long row0 = ((long long)blockIdx.x * (WAVES == 4 ? 1 : 4) + (WAVES == 4 ? 0 : wave)) * rows;
   if (row0 >= all_rows) return;
-  int lo = 0, hi = 0, parts = 1;
-  {
-    const long long at = min(row0 + min(lane, rows - 1), all_rows - 1);
-    const int token = (int)(at / a.heads);
-    parts = row_parts(a, token, __builtin_amdgcn_readfirstlane(token), &lo, &hi);
-  }
+  int lo = 0, hi = 0;
+  long long first = 0;
+  const int parts = row_parts(a, min(row0 + min(lane, rows - 1), all_rows - 1), __builtin_amdgcn_readfirstlane((int)(row0 / a.heads)), &lo, &hi, &first);
   unsigned long long todo = __builtin_amdgcn_ballot_w64(lane < rows && row0 + lane < all_rows && parts > 1);
   while (todo) {
     const int r = (int)__builtin_ctzll(todo);
@@ -1103,9 +1112,11 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
     const long long at = row0 + r;
     const int n = __builtin_amdgcn_readlane(parts, r);
     const bool none = __builtin_amdgcn_readlane(hi, r) <= __builtin_amdgcn_readlane(lo, r);
-    const float* const ml = a.part_ml + 2 * at * a.stride;
+    const long long part0 = (long long)(((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(first >> 32), r) << 32) |
+                                        (unsigned)__builtin_amdgcn_readlane((int)first, r));
+    const float* const ml = a.part_ml + 2 * part0;
     // the first PRE turns' sums are asked for beside (m, l): all of them where four waves share a row
-    const float* const po = a.part_o + at * a.stride * D + 4 * c;
+    const float* const po = a.part_o + part0 * D + 4 * c;
     v4f early[PRE];
 #pragma unroll
     for (int i = 0; i < PRE; ++i) {
@@ -1183,10 +1194,12 @@ struct Plan {
   int nq;                  // narrow: blocks of 16 rows of a workgroup, 1 or 2
   int slots, slots_per_seq;
   Cut cut, small;
-  int small_rows, stride;
+  int small_rows;
+  size_t large, all;       // parts that there is room for: of sequences that are not small, and with those that are
 };
 
-static size_t workspace_of(long long rows, int D, int nparts) { return nparts > 1 ? (size_t)rows * nparts * (D + 2) * 4 : 0; }
+static size_t parts_of(long long rows, int nparts) { return nparts > 1 ? (size_t)rows * nparts : 0; }
+static size_t workspace_of(size_t parts, int D) { return parts * (D + 2) * 4; }
 
 // us of a launch of the narrow kernel: rounds of two workgroups to a compute unit, 3 us each until the first tile is there, and their share of 5.8 TB/s, or
 // the 17 KB a us that one workgroup gets through.  The lengths of several sequences are not known here, only the greatest: the mean of that with all of them alike
@@ -1222,7 +1235,7 @@ static Cut best_cut(int keys, int least_keys, long long rows, int D, size_t room
   double least = cost(best);
   for (int n = 2; n <= kPartsMost; n += n < 4 ? 1 : n / 4) {
     const Cut c = cut_into(keys, n);
-    if (c.part_keys < least_keys || workspace_of(rows, D, c.nparts) > room) break;
+    if (c.part_keys < least_keys || workspace_of(parts_of(rows, c.nparts), D) > room) break;
     const double t = cost(c);
     if (t < 0.97 * least) {
       least = t;
@@ -1244,14 +1257,15 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
   const int keys = (int)std::min<long long>(seen, INT_MAX - 1024);
   // 32 rows to a narrow workgroup read the keys half as often as 16; those are the faster ones where even parts of 256 keys are fewer than the compute
   // units.  (Six tokens, 64 heads, 8 of keys of 128: 16 sequences of up to 4096 keys 64 us by 32 rows, 63 to 73 by 16; two of up to 1000 keys 15 and 12.)
-  p.nq = most_rows <= 16 || ((most_rows + 31) / 32) * b.sequences * pages.heads * ((keys + 255) / 256) < cus ? 1 : 2;
+  p.nq = most_rows <= 16 || (p.narrow && ((most_rows + 31) / 32) * b.sequences * pages.heads * ((keys + 255) / 256) < cus) ? 1 : 2;
   const int R = p.narrow ? 16 * p.nq : kWideRows;
   const long long per_seq = (most_rows + R - 1) / R, packed = (long long)b.tokens * group / R + b.sequences;
   // numbered by row blocks, unless most of such slots would be empty (as those of narrow workgroups, four to a sequence at most, cannot be)
   p.slots_per_seq = p.narrow || b.sequences * per_seq <= 2 * packed ? (int)per_seq : 0;
   p.slots = (int)std::min<long long>(p.slots_per_seq ? b.sequences * per_seq : packed, INT_MAX);
-  p.small_rows = p.narrow || b.sequences == 1 ? 0 : 16;
+  p.small_rows = p.narrow || b.sequences == 1 ? 0 : kSmallRows;
   const int held = pages.type == FTK_F16 || pages.type == FTK_BF16 ? 4 * D : 2 * D + 2;   // bytes of a position and head
+  const long long small_rows = (long long)b.sequences * pages.heads * kSmallRows;
   p.small = Cut{1, keys};
   if (p.narrow) {
     const double units = (double)p.slots * pages.heads;
@@ -1261,7 +1275,8 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
     double small = 0.0;
     if (p.small_rows > 0) {
       p.small = cut_into(keys, std::min({std::max(1, (int)((long long)keys * held / (20 * 17000))), keys / 256 + 1, kPartsMost}));
-      while (p.small.nparts > 1 && workspace_of(rows, D, p.small.nparts) > room) p.small = cut_into(keys, p.small.nparts - 1);
+      while (p.small.nparts > 1 && workspace_of(parts_of(small_rows, p.small.nparts), D) > room) p.small = cut_into(keys, p.small.nparts - 1);
+      room -= workspace_of(parts_of(small_rows, p.small.nparts), D);
       const double sequences = std::max(0.0, b.sequences - std::ceil((double)(b.tokens - b.sequences) / std::max(1LL, most - 1)));
       small = sequences * pages.heads * p.small.nparts / 2 * (3.0 + p.small.part_keys * (held / 17000.0));
     }
@@ -1270,7 +1285,8 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
     p.cut = best_cut(keys, 512, rows, D, room,
                      [&](const Cut& c) { return wide_cost(units * c.nparts, c.part_keys * (1 - own / keys), D, cus, small) + join_cost(rows, D, c.nparts); });
   }
-  p.stride = std::max(p.cut.nparts, p.small.nparts);
+  p.large = parts_of(rows, p.cut.nparts);
+  p.all = p.large + parts_of(small_rows, p.small.nparts);
   return p;
 }
 
@@ -1306,7 +1322,7 @@ size_t ftk_paged_attn_workspace_bytes(const ftk_kv_pages* pages, const ftk_kv_ba
   b.sequences = batch->sequences;
   b.width = batch->table_width;
   const Plan p = plan(*pages, b, __builtin_ctz((unsigned)pages->page_size), heads, window, max_queries, max_keys, d->cus, SIZE_MAX);
-  return workspace_of((long long)b.tokens * heads, pages->head_size, p.stride);
+  return workspace_of(p.all, pages->head_size);
 }
 
 int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long q_head_stride, const ftk_kv_pages* pages, const ftk_kv_batch* batch,
@@ -1345,10 +1361,10 @@ int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long 
   a.cut = p.cut;
   a.small = p.small;
   a.small_rows = p.small_rows;
-  a.stride = p.stride;
+  a.small_first = (long long)p.large;
   const long long rows = (long long)a.batch.tokens * heads;
   a.part_o = (float*)workspace;
-  a.part_ml = a.part_o + (size_t)rows * p.stride * pages->head_size;
+  a.part_ml = a.part_o + p.all * pages->head_size;
   const long long blocks = (long long)p.slots * pages->heads * p.cut.nparts;
   const long long pairs = p.small_rows ? ((long long)a.batch.sequences * pages->heads * p.small.nparts + 1) / 2 : 0;
   const hipStream_t s = (hipStream_t)stream;
@@ -1375,9 +1391,9 @@ int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long 
       constexpr int lds = std::max(WideShape<D>::LDS, 2 * NarrowShape<F, D>::LDS);
       bad = launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D>, once, blocks + pairs, kWideWaves, lds, s, a, (int)blocks);
     }
-    if (bad || p.stride == 1) return bad;
+    if (bad || p.all == 0) return bad;
     // few rows of many parts: a block to each; only small sequences cut: 16 rows to a wave, most of which have nothing to join
-    if (rows <= 4096 && p.stride >= 16) {
+    if (rows <= 4096 && std::max(p.cut.nparts, p.small.nparts) >= 16) {
       hipLaunchKernelGGL((paged_merge_kernel<T, D, 4>), dim3((unsigned)rows), dim3(256), 0, s, a, 1);
     } else {
       const int per_wave = p.cut.nparts > 1 ? 1 : 16;

@@ -150,6 +150,31 @@ def test_a_large_cache_is_written_and_read_past_32_bits(core):
                        core.paged_attention(q[:1].contiguous(), *small[:2], small_table, lens, one, *small[2:], max_queries=1))
 
 
+@pytest.mark.parametrize('dtype,cache,D,page,heads', [(F16, None, 128, 32, 12), (BF16, I8, 128, 16, 3), (F16, E4M3, 96, 64, 40), (BF16, E4M3, 64, 128, 7), (F16, I8, 32, 16, 5), (BF16, None, 64, 16, 1)])
+def test_many_rows_at_once_are_those_of_few(core, dtype, cache, D, page, heads):
+    """Long prompts among short ones, pauses and sequences of no length, in one call: the bytes that a call for each piece of ten tokens leaves and reads."""
+    new = [700, 0, 1, 3000, 0, 0, 17, 1, 1, 1, 900, 0] * (6 if heads < 6 else 2) + [2000] * (12 if heads == 1 else 0)
+    batch = ref.make_batch(new, [n + (5 * b) % 40 for b, n in enumerate(new)], page, 181, tail=3)
+    table, lens, starts = ref.on_device(batch)
+    a, b = (_junk(_cuda(ref.make_pages(batch, heads, D, cache, dtype, 182))) for _ in range(2))
+    g = torch.Generator(device='cuda').manual_seed(183)
+    keys, values = ((torch.randn((batch['tokens'], heads, D), generator=g, device='cuda') * torch.rand((batch['tokens'], heads, 1), generator=g, device='cuda') * 8).to(dtype) for _ in range(2))
+    core.kv_cache_write(keys, values, *a[:2], table, lens, starts, *a[2:])
+    k, v = (torch.full((batch['tokens'], heads, D), 7.0, device='cuda') for _ in range(2))
+    core.kv_cache_read(*a[:2], table, lens, starts, batch['tokens'], F32, *a[2:], out=(k, v))
+    ends = batch['starts'][-1]
+    assert bool((k[ends:] == 7).all()) and bool((v[ends:] == 7).all())
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device='cuda')
+    for s, n in enumerate(new):
+        for t in range(0, n, max(10, n // 20)):
+            m, at = min(max(10, n // 20), n - t), batch['starts'][s] + t
+            one = (table[s:s + 1], ints([batch['lens'][s] - n + t + m]), ints([0, m]))
+            core.kv_cache_write(keys[at:at + m].contiguous(), values[at:at + m].contiguous(), *b[:2], *one, *b[2:])
+            few = core.kv_cache_read(*a[:2], *one, m, F32, *a[2:])
+            assert torch.equal(few[0], k[at:at + m]) and torch.equal(few[1], v[at:at + m]), (s, t)
+    assert all(x is None or _same(x, y) for x, y in zip(a, b))
+
+
 # ---- attention --------------------------------------------------------------------------
 
 def _attention_case(core, dtype, cache, D, page, heads, G, new, lens, seed, causal=True, window=0, hints=True, scale=None, tail=0, junk=True, workspace=None, pages=None):
@@ -236,6 +261,22 @@ def test_long_sequences_in_parts(core, dtype, cache, D, page, heads, G, new, len
     assert need > 0 or window                                    # more than one part
     for space in (None, torch.empty(max(need // 2, 16), dtype=torch.uint8, device='cuda'), torch.empty(0, dtype=torch.uint8, device='cuda')):
         _attention_case(core, dtype, cache, D, page, heads, G, new, lens, 31, window=window, workspace=space)
+
+
+@pytest.mark.parametrize('dtype,cache,D,page,heads,G,n,B,L', [
+    (F16, None, 128, 16, 4, 8, 3, 16, 1100),                     # 24 rows: one block of 32
+    (BF16, I8, 128, 64, 4, 8, 6, 16, 1100),                      # 48 rows: two, the second of which is not full
+    (F16, E4M3, 96, 32, 5, 7, 9, 12, 1100),                      # 63
+    (BF16, E4M3, 64, 16, 9, 2, 32, 10, 700),                     # 64
+    (F16, I8, 32, 128, 12, 5, 8, 12, 600),                       # 40
+    (BF16, None, 128, 16, 3, 4, 11, 11, 300),                    # 44 rows of few keys: blocks of 16
+    (F16, None, 64, 16, 8, 1, 9, 40, 200),                       # 9 rows: many results
+    (F16, I8, 128, 16, 8, 4, 4, 9, 300),                         # 16 rows
+])
+def test_drafts_of_many_sequences(core, dtype, cache, D, page, heads, G, n, B, L):
+    new = [max(0, n - (b % 5 if b % 3 == 1 else 0)) for b in range(B)]
+    lens = [max(1, L - 41 * b) if b % 4 else L for b in range(B)]
+    _attention_case(core, dtype, cache, D, page, heads, G, new, lens, 191, tail=1)
 
 
 @pytest.mark.parametrize('new,lens', [([6], [70]), ([5, 100], [33, 130]), ([2], [64])])
