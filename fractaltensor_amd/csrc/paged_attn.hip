@@ -1041,7 +1041,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
 // The workgroups behind the first `wide` take sequences of at most small_rows = 16 rows, which would leave seven of the eight waves without
 // any: two (sequence, head, part) each, by four waves that cut the keys as in the narrow kernel.  They read on the compute units that the others
 // leave free, or have left, while those multiply.  (A chunk of 512 tokens beside five sequences that decode, 16 heads, 4 of keys, up to
-// 16384 of them, in int8: 165 us with all on the wide form, 110 so, and 11 for joining.)
+// 16384 of them, in int8: 165 us with all on the wide form, 100 so, and 11 for joining.)
 template <typename T, KvFormat F, int D>
 __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs a, int wide) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
