@@ -27,7 +27,16 @@ constexpr int kWaves = 4;
 constexpr float kNoRef = -3.402823466e38f;   // the reference before any score: finite, so that -inf minus it is -inf
 constexpr int kSmallRows = 16;                // sequences of at most so many rows, beside larger ones, are small
 constexpr long long kFewResults = 1 << 15;   // elements of o whose weights enter P V with what their rounding leaves
-constexpr float kSlack = 8.0f;               // the reference moves when a score is above it by 2^8 in the weights
+
+// Weights are 2^(score - reference), and the reference is moved to the largest score less kLift, so that the largest weight is 2^kLift then.  fp16 has 15
+// binades above 1 and no more below it than down to 2^-24: with weights of at most 1, those of many keys beside one that outweighs them (a sink,
+// whose value may be zero) were subnormal, or zero, while their sum counted them.  (4096 keys in fp16, one of a score 20 above the others' with a value
+// of zero: all of the result was lost.)  With nine binades a weight is off by at most 2^-34 of the largest besides its own rounding, which the result's own
+// finest step hides.  bf16 has the range of fp32.
+template <typename T>
+constexpr float kLift = std::is_same<T, Half>::value ? 9.0f : 0.0f;
+template <typename T>
+constexpr float kSlack = std::is_same<T, Half>::value ? 6.0f : 8.0f;   // narrow: the reference moves when a weight would be above 2^(kLift + kSlack)
 
 // How the keys of a sequence are cut: at most nparts parts of part_keys keys, the last of which takes what is left.
 struct Cut {
@@ -421,10 +430,10 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
       }
       float mx = fmaxf(fmaxf(fmaxf(sc[nq][0][0], sc[nq][0][1]), fmaxf(sc[nq][0][2], sc[nq][0][3])),
                        fmaxf(fmaxf(sc[nq][1][0], sc[nq][1][1]), fmaxf(sc[nq][1][2], sc[nq][1][3])));
-      if (__builtin_amdgcn_ballot_w64(!(mx <= ref[nq] + kSlack)) != 0) {
+      if (__builtin_amdgcn_ballot_w64(!(mx <= ref[nq] + (kLift<T> + kSlack<T>))) != 0) {
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float moved = fmaxf(ref[nq], mx);
+        const float moved = fmaxf(ref[nq], mx - kLift<T>);
         const float alpha = __builtin_amdgcn_exp2f(ref[nq] - moved);
         ref[nq] = moved;
         l[nq] *= alpha;
@@ -631,7 +640,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_narrow_kernel(AttnArgs a
 // which is read from their M(t + 1) on, into one of three places, waves 4 to 7 K(t + 2) into that of K(t).  16-bit elements are copied straight into
 // LDS; codes of 8 bits go through registers, a tile earlier, and are written as 16-bit elements.
 constexpr int kWideWaves = 8, kWideRows = 32 * kWideWaves;
-constexpr float kMostSum = 32768.0f;          // a lane's sum of weights above this moves the reference
+constexpr float kMostSum = 32768.0f;          // a lane's sum of 32 weights above this moves the reference, to where it is at most 32 * 2^kLift
 
 template <int D>
 struct WideShape {
@@ -839,7 +848,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
       float mx = sc[0][0];
 #pragma unroll
       for (int e = 1; e < 32; ++e) mx = fmaxf(mx, sc[e >> 4][e & 15]);
-      const float moved = fmaxf(ref, max_with_other_half(mx) * a.scale_log2e);
+      const float moved = fmaxf(ref, max_with_other_half(mx) * a.scale_log2e - kLift<T>);
       const float alpha = __builtin_amdgcn_exp2f(ref - moved);
       ref = moved;
       l *= alpha;

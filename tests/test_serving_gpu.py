@@ -442,6 +442,40 @@ def test_refusals_on_the_device(core):
     assert info.value.code == -2
 
 
+@pytest.mark.parametrize('above', [12.0, 16.0, 20.0])
+@pytest.mark.parametrize('at', [0, 1500])
+@pytest.mark.parametrize('dtype,cache,D,page,G,new', [(F16, None, 64, 16, 4, 1), (F16, I8, 128, 64, 4, 5), (F16, E4M3, 96, 32, 2, 9), (F16, None, 128, 16, 2, 70), (F16, I8, 64, 16, 2, 90),
+                                                      (F16, E4M3, 32, 128, 1, 150), (BF16, None, 64, 16, 4, 1), (BF16, I8, 64, 16, 2, 90)])
+def test_keys_beside_one_that_outweighs_them(core, dtype, cache, D, page, G, new, at, above):
+    """A key whose score is far above the others' and whose value is zero, at the first position or later: the result is what the others leave, by weights
+    of e^-12 to e^-20 of the largest."""
+    length, heads = 4096, 2
+    batch = ref.make_batch([new], [length], page, 201)
+    pages = ref.make_pages(batch, heads, D, None, dtype, 202)
+    pages[1] = pages[1].abs()
+    keys, row = batch['table'][0][at // page], at % page
+    pages[0][..., 0] = 0.0
+    pages[0][keys, :, row] = 0.0
+    pages[0][keys, :, row, 0] = above * 2                          # q 4, scale 1 / 8; a value of both codes
+    pages[1][keys, :, row] = 0.0
+    exps = [None, None]
+    if cache is not None:
+        for i in range(2):
+            x = pages[i].float()
+            e = torch.ceil(torch.log2(x.abs().amax(-1).clamp(min=0.1) / ref.LARGEST[cache])).to(torch.int8)
+            scaled = x / torch.pow(2.0, e.float()).unsqueeze(-1)
+            pages[i], exps[i] = (scaled.round() if cache == I8 else scaled).to(cache), e
+    q = torch.randn((new, heads * G, D), generator=torch.Generator().manual_seed(203)).to(dtype)
+    q[..., 0] = 4.0
+    held = [ref.held(pages[i], exps[i]) for i in range(2)]
+    want = ref.attention(q, *held, batch, heads, 0.125)
+    bound = ref.attention_bounds_by_largest(want, dtype, D)
+    dev = _cuda([*pages[:2], *exps])
+    got = core.paged_attention(q.cuda(), *dev[:2], *ref.on_device(batch), *dev[2:], scale=0.125, max_queries=new, max_keys=length).cpu().double()
+    worst = float(((got - want['o']).abs() / bound).max())
+    assert worst <= 1.0, f'o is {worst:.3g} times its bound off'
+
+
 # ---- verification -----------------------------------------------------------------------
 
 def _drafts(B, K, V, dtype, wide, seed):
