@@ -12,10 +12,11 @@
 // first product (the contraction takes the keys in the order a lane holds them).  Long sequences are cut into parts of
 // `part_keys` keys, a workgroup each, which leave (reference, sum, unnormalised O) for a second launch to join.
 //
-// Rounding: scores, softmax state and O are fp32 and Q is not scaled beforehand.  Weights enter P V in 16 bits: rounded, half a step (2^-12 fp16,
-// 2^-9 bf16) each, which with the result's own rounding makes sqrt(2) of the error of that alone in the mean, and more now and then where results are few.
-// Calls of few results, by blocks of 16 rows, leave the matrix unit time for a second product: there a weight is the rounded one and what that leaves, also in
-// 16 bits.  (4 % of the time of 64 decoding sequences of up to 8192 keys, which therefore go without.)  A cache of 8 bits enters the products as its exact values.
+// Rounding: scores, softmax state and O are fp32 and Q is not scaled beforehand.  Weights enter P V in 16 bits.  In the narrow form, which leaves the matrix unit
+// time for a second product, a weight is the rounded one and what that leaves, also in 16 bits (2^-22 of it fp16, 2^-16 bf16), so that a result is off by its own rounding
+// alone, whatever else the call holds.  In the wide form, bound by the matrix pipe, of which a second product would take half as much again, it is the rounded one
+// alone, half a step (2^-11 of it fp16, 2^-8 bf16), which with the result's own rounding makes sqrt(2) of the error of that alone in the mean.  A cache of 8
+// bits enters the products as its exact values.
 #include <algorithm>
 #include <cmath>
 
@@ -26,7 +27,6 @@ namespace ftk {
 constexpr int kWaves = 4;
 constexpr float kNoRef = -3.402823466e38f;   // the reference before any score: finite, so that -inf minus it is -inf
 constexpr int kSmallRows = 16;                // sequences of at most so many rows, beside larger ones, are small
-constexpr long long kFewResults = 1 << 15;   // elements of o whose weights enter P V with what their rounding leaves
 
 // Weights are 2^(score - reference), and the reference is moved to the largest score less kLift, so that the largest weight is 2^kLift then.  fp16 has 15
 // binades above 1 and no more below it than down to 2^-24: with weights of at most 1, those of many keys beside one that outweighs them (a sink,
@@ -252,7 +252,7 @@ __device__ __forceinline__ void lds_dma4_from(const signed char* from, void* lds
 }
 
 // tid: of the 256 threads that work together
-template <typename T, KvFormat F, int D, int NQ, bool KEPT, bool REST>
+template <typename T, KvFormat F, int D, int NQ, bool KEPT>
 __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j, int kv_head, unsigned char* smem, int tid) {
   using S = NarrowShape<F, D>;
   using v8 = typename T::v8;
@@ -407,7 +407,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     keys_read();
-    v8 p[NQ], rest[NQ];                                           // REST: weights as two operands, rounded and what that leaves
+    v8 p[NQ], rest[NQ];                                           // weights as two operands: rounded, and what that leaves
     unsigned seen[NQ];                                            // MASKED: which of the lane's eight keys its row sees
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
@@ -456,7 +456,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
           }
           const unsigned pair = T::pack(p0, p1);
           w[2 * h + r / 2] = pair;
-          u[2 * h + r / 2] = REST ? T::pack(p0 - T::low(pair), p1 - T::high(pair)) : 0;
+          u[2 * h + r / 2] = T::pack(p0 - T::low(pair), p1 - T::high(pair));
         }
       p[nq] = __builtin_bit_cast(v8, (v4u{w[0], w[1], w[2], w[3]}));
       rest[nq] = __builtin_bit_cast(v8, (v4u{u[0], u[1], u[2], u[3]}));
@@ -518,7 +518,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
 #pragma unroll
       for (int nq = 0; nq < NQ; ++nq) {
         o[nq][dt] = T::mma16(vf, p[nq], o[nq][dt]);
-        if constexpr (REST) o[nq][dt] = T::mma16(vf, rest[nq], o[nq][dt]);
+        o[nq][dt] = T::mma16(vf, rest[nq], o[nq][dt]);
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -616,7 +616,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
 
 // The slots are `tiles` row blocks of each of `sequences`.  Workgroups that are 8 apart run on one XCD, at about the same time: the row blocks of a (sequence, head, part)
 // are, and the head goes fastest.
-template <typename T, KvFormat F, int D, int NQ, bool KEPT, bool REST>
+template <typename T, KvFormat F, int D, int NQ, bool KEPT>
 __global__ __launch_bounds__(kWaves * 64, 2) void paged_narrow_kernel(AttnArgs a, int tiles) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   int id = blockIdx.x, tile = 0;
@@ -629,7 +629,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_narrow_kernel(AttnArgs a
   const int b = rest / a.cut.nparts, part = rest % a.cut.nparts;
   Job j;
   if (!find_job<16 * NQ>(a, b, tile, part, false, j)) return;
-  narrow_attention<T, F, D, NQ, KEPT, REST>(a, j, kv_head, smem, threadIdx.x);
+  narrow_attention<T, F, D, NQ, KEPT>(a, j, kv_head, smem, threadIdx.x);
 }
 
 // ---- wide -----------------------------------------------------------------------------
@@ -1060,7 +1060,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs
     const int item = 2 * (blockIdx.x - wide) + half, kv_head = item % a.pages.heads, rest = item / a.pages.heads;
     const int b = rest / a.small.nparts, part = rest - b * a.small.nparts;
     if (b < a.batch.sequences && find_job<16>(a, b, 0, part, true, j)) {
-      narrow_attention<T, F, D, 1, false, false>(a, j, kv_head, smem + half * NarrowShape<F, D>::LDS, threadIdx.x & 255);
+      narrow_attention<T, F, D, 1, false>(a, j, kv_head, smem + half * NarrowShape<F, D>::LDS, threadIdx.x & 255);
     } else {                                                     // the other half's two barriers
       __syncthreads();
       __syncthreads();
@@ -1385,16 +1385,13 @@ int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long 
     if (p.narrow) {
       using yes = std::true_type;
       using no = std::false_type;
-      auto launch = [&](auto nq, auto kept, auto rest) -> int {
+      auto launch = [&](auto nq, auto kept) -> int {
         static DeviceOnce once;
-        return launch_with_lds("paged_narrow_kernel", paged_narrow_kernel<T, F, D, decltype(nq)::value, decltype(kept)::value, decltype(rest)::value>, once, blocks, kWaves,
-                               NarrowShape<F, D>::LDS, s, a, p.slots_per_seq);
+        return launch_with_lds("paged_narrow_kernel", paged_narrow_kernel<T, F, D, decltype(nq)::value, decltype(kept)::value>, once, blocks, kWaves, NarrowShape<F, D>::LDS, s,
+                               a, p.slots_per_seq);
       };
-      auto with_kept = [&](auto nq, auto rest) { return p.slots_per_seq == 1 ? launch(nq, no{}, rest) : launch(nq, yes{}, rest); };
-      using one = std::integral_constant<int, 1>;
-      if (p.nq == 2) bad = with_kept(std::integral_constant<int, 2>{}, no{});
-      else if (rows * D <= kFewResults) bad = with_kept(one{}, yes{});
-      else bad = with_kept(one{}, no{});
+      auto with_kept = [&](auto nq) { return p.slots_per_seq == 1 ? launch(nq, no{}) : launch(nq, yes{}); };
+      bad = p.nq == 2 ? with_kept(std::integral_constant<int, 2>{}) : with_kept(std::integral_constant<int, 1>{});
     } else {
       static DeviceOnce once;
       constexpr int lds = std::max(WideShape<D>::LDS, 2 * NarrowShape<F, D>::LDS);

@@ -683,11 +683,13 @@ int ftk_kv_cache_read(const ftk_kv_pages* pages, const ftk_kv_batch* batch,
  * positions to see gets zeros and -inf.  Keys and values that a token does not
  * see never matter to it, NaN and infinities included; one that is not finite
  * makes NaN of what sees it (a component of o for a value, all of it for a key).
- * fp32 accumulation; the one rounding on the way is that of the weights to the 16
- * bits of `type`.  Sequences of any mixture of sizes go in one call: where max_queries
+ * fp32 accumulation.  Sequences of any mixture of sizes go in one call: where max_queries
  * leaves none with more than 64 rows (new tokens times heads / pages->heads), all run
  * on a kernel made for reading the cache once; otherwise those of more than 16 rows run
- * on one made for the matrix unit, the others beside them.
+ * on one made for the matrix unit, the others, in the first one's manner, beside them.
+ * On the first weights enter the products with values as two numbers of the 16 bits of
+ * `type`, so that the result's own rounding is the one that counts; on the second they
+ * are rounded to those 16 bits.
  *
  * max_queries, max_keys: promises that no sequence has more new tokens, or is
  * longer (0: no promise).  They decide which kernel runs and how the keys are

@@ -154,14 +154,14 @@ def attention_bounds(ref, dtype, D):
     return o, rest + 2.0 ** -22 * (1 + ref['lse'].abs().nan_to_num(posinf=0.0, neginf=0.0))
 
 
-def attention_bounds_by_largest(ref, dtype, D):
+def attention_bounds_by_largest(ref, dtype, D, split=False):
     """As attention_bounds, but for weights that are held as multiples of 2^9 of the row's largest or more: in fp16, whose steps end at 2^-24, what a
     weight loses besides its own half step is at most 2^-25 / 2^9 = 2^-34 of the largest weight, which is no more than the sum of all; and the result itself ends at steps of
-    2^-24."""
+    2^-24.  split: weights in two parts of 16 bits, the second of which is off by a half step of what the first leaves, so that the result's own half step is what counts."""
     u = torch.finfo(dtype).eps / 2
     scores = ((D + 4) * ref['most'] + ref['lse'].abs().nan_to_num(posinf=0.0, neginf=0.0)) * 2.0 ** -24
     rest = 2 * scores + (ref['count'] + 16) * 2.0 ** -24
-    o = 1.01 * u * (ref['o'].abs() + ref['mean']) + rest.unsqueeze(-1) * ref['mean'] + 2.0 ** -126
+    o = 1.01 * u * (ref['o'].abs() + (u if split else 1.0) * ref['mean']) + rest.unsqueeze(-1) * ref['mean'] + 2.0 ** -126
     if dtype == torch.float16:
         o = o + 2.0 ** -25 + 2.0 ** -34 * ref['count'].unsqueeze(-1) * ref['top']
     return o

@@ -476,6 +476,47 @@ def test_keys_beside_one_that_outweighs_them(core, dtype, cache, D, page, G, new
     assert worst <= 1.0, f'o is {worst:.3g} times its bound off'
 
 
+@pytest.mark.parametrize('dtype,cache,D,G', [(F16, None, 128, 4), (BF16, E4M3, 128, 4), (BF16, None, 64, 1), (F16, I8, 96, 8), (F16, E4M3, 32, 16)])
+def test_a_result_does_not_depend_on_what_else_the_call_holds(core, dtype, cache, D, G):
+    """One token of a sequence alone, among sixty-four that decode, and beside a prompt: the same bits where the keys are not cut, and the error of the result's own rounding
+    alone each time."""
+    heads, page, length = 2, 16, 333
+    lens = [length] + [17 * b % 500 + 1 for b in range(1, 64)]
+    batch = ref.make_batch([1] * 64, lens, page, 211)
+    pages = ref.make_pages(batch, heads, D, cache, dtype, 212)
+    q = 3 * torch.randn((64, heads * G, D), generator=torch.Generator().manual_seed(213))      # a few keys have most of a row's weight
+    q = q.to(dtype)
+    want = ref.attention(q, ref.held(pages[0], pages[2]), ref.held(pages[1], pages[3]), batch, heads, D ** -0.5)
+    bound = ref.attention_bounds_by_largest(want, dtype, D, split=True)
+    dev, (table, at, starts) = _cuda(pages), ref.on_device(batch)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device='cuda')
+    uncut = torch.empty(0, dtype=torch.uint8, device='cuda')
+    call = lambda rows, t, n, s, most: core.paged_attention(rows, *dev[:2], t, n, s, *dev[2:], max_queries=most, max_keys=500, workspace=uncut, return_lse=True)
+    many = call(q.cuda(), table, at, starts, 1)
+    alone = call(q[:1].cuda(), table[:1], at[:1], ints([0, 1]), 1)
+    prompt = torch.cat([q[:1], q[:1].expand(100, -1, -1)]).cuda()
+    beside = call(prompt, table[:1].expand(2, -1).contiguous(), ints([length, 100]), ints([0, 1, 101]), 100)
+    for x in (alone, beside):
+        assert torch.equal(x[0][:1], many[0][:1]) and torch.equal(x[1][:1], many[1][:1])
+    worst = ((many[0].cpu().double() - want['o']).abs() / bound).max()
+    assert float(worst) <= 1.0, f'o is {float(worst):.3g} times its bound off'
+
+
+@pytest.mark.parametrize('dtype,cache,D,G,n', [(F16, None, 128, 4, 5), (BF16, E4M3, 64, 8, 8), (BF16, I8, 128, 8, 6), (F16, I8, 96, 4, 16), (BF16, None, 96, 2, 9)])
+def test_drafts_are_off_by_the_rounding_of_results_alone(core, dtype, cache, D, G, n):
+    """Sequences of 17 to 64 rows, in blocks of 16 and of 32."""
+    for B, L in ((2, 100), (24, 300)):
+        batch = ref.make_batch([n] * B, [L - 3 * b for b in range(B)], 16, 221)
+        pages = ref.make_pages(batch, 6, D, cache, dtype, 222)
+        q = (3 * torch.randn((batch['tokens'], 6 * G, D), generator=torch.Generator().manual_seed(223))).to(dtype)
+        want = ref.attention(q, ref.held(pages[0], pages[2]), ref.held(pages[1], pages[3]), batch, 6, D ** -0.5)
+        bound = ref.attention_bounds_by_largest(want, dtype, D, split=True)
+        dev = _cuda(pages)
+        got = core.paged_attention(q.cuda(), *dev[:2], *ref.on_device(batch), *dev[2:], max_queries=n, max_keys=L).cpu().double()
+        worst = ((got - want['o']).abs() / bound).max()
+        assert float(worst) <= 1.0, f'o is {float(worst):.3g} times its bound off'
+
+
 # ---- verification -----------------------------------------------------------------------
 
 def _drafts(B, K, V, dtype, wide, seed):
