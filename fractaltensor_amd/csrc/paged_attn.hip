@@ -221,6 +221,9 @@ __device__ __forceinline__ typename T::v8 zeros_at(typename T::v8 x, unsigned bi
 // log of the sum of exponentials from the reference (in powers of two) and the sum
 __device__ __forceinline__ float log_sum(float ref, float l) { return (ref + __builtin_log2f(l)) * 0.6931471805599453f; }
 
+// A sum over values as it leaves: one that is infinite, because a value is, as NaN, which it is already where a weight of zero met that value, or a mask cut its tile.
+__device__ __forceinline__ float finite_or_nan(float x) { return __builtin_fmaf(x, 0.0f, x); }
+
 // ---- narrow ---------------------------------------------------------------------------
 
 template <KvFormat F, int D>
@@ -596,6 +599,8 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
           for (int e = 0; e < 4; ++e) acc[e] += w[i] * v[e];
         }
         if (j.parts == 1) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] = finite_or_nan(acc[e]);
           *reinterpret_cast<v2u*>((scalar*)a.o + r.at * D + 4 * g) = v2u{T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
         } else {
           *reinterpret_cast<v4f*>(a.part_o + (first_part(a, j.small, j.b, kv_head, row, r.at) + j.part) * D + 4 * g) = acc;
@@ -1030,6 +1035,10 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   // the wave turns its 32 x D tile round through LDS (nobody reads tiles any more) and stores whole rows
   const bool none = r.hi <= r.lo;
   const float inv = none ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[dt][e] = finite_or_nan(o[dt][e]);
   unsigned char* const ot = smem + wave * (32 * S::ORS);
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -1189,6 +1198,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
     }
     if ((WAVES == 1 || wave == 0) && lane < L) {
       const float inv = none ? 0.0f : 1.0f / sum;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = finite_or_nan(acc[e]);
       *reinterpret_cast<v2u*>((typename T::scalar*)a.o + at * D + 4 * c) = v2u{T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
       if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : log_sum(top, sum);
     }

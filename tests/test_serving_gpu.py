@@ -517,6 +517,20 @@ def test_drafts_are_off_by_the_rounding_of_results_alone(core, dtype, cache, D, 
         assert float(worst) <= 1.0, f'o is {float(worst):.3g} times its bound off'
 
 
+@pytest.mark.parametrize('dtype,cache,new,lens', [(F16, None, [1, 3], [400, 200]), (BF16, None, [1], [3000]), (F16, None, [100, 1], [400, 300]), (BF16, None, [90], [3000])])
+def test_infinite_values_make_nan_wherever_they_lie(core, dtype, cache, new, lens):
+    """In tiles that all rows see, in those that a mask cuts, and beside one another: the same component is NaN, all others are what they were."""
+    D, page, heads, G = 64, 16, 2, 2
+    batch = ref.make_batch(new, lens, page, 231)
+    pages = ref.make_pages(batch, heads, D, cache, dtype, 232)
+    for b, n in enumerate(lens):
+        for i, p in enumerate([0, 5, 70, 71, 100, n - new[b] - 1, n - 1]):
+            at, row = batch['table'][b][p // page], p % page
+            pages[1][at, i % heads, row, 7 * i + 1] = (math.inf, -math.inf)[i % 3 == 1]
+            pages[1][at, 1 - i % heads, row, 60] = (math.inf, -math.inf)[i % 2]
+    _attention_case(core, dtype, cache, D, page, heads, G, new, lens, 231, pages=pages)
+
+
 # ---- verification -----------------------------------------------------------------------
 
 def _drafts(B, K, V, dtype, wide, seed):
