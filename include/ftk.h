@@ -682,8 +682,9 @@ int ftk_kv_cache_read(const ftk_kv_pages* pages, const ftk_kv_batch* batch,
  * and into lse [tokens, heads] fp32, if not NULL, log sum_k w_k.  A token without
  * positions to see gets zeros and -inf.  Keys and values that a token does not
  * see never matter to it, NaN and infinities included.  A value that is not finite
- * makes NaN of that component of o of what sees it, a key that is not finite all of
- * o.  Weights of up to 2^15 times values are summed in fp32: values of
+ * makes NaN of that component of o of what sees it, a key that is NaN all of o; an infinite
+ * key gives the score that it gives, of which -inf has weight zero and any other
+ * makes NaN.  Weights of up to 2^15 times values are summed in fp32: values of
  * bf16 beyond 2^100 may leave its range there, which makes NaN too.
  * fp32 accumulation.  Sequences of any mixture of sizes go in one call: where max_queries
  * leaves none with more than 64 rows (new tokens times heads / pages->heads), all run

@@ -531,6 +531,33 @@ def test_infinite_values_make_nan_wherever_they_lie(core, dtype, cache, new, len
     _attention_case(core, dtype, cache, D, page, heads, G, new, lens, 231, pages=pages)
 
 
+@pytest.mark.parametrize('dtype,new,length', [(F16, 2, 300), (BF16, 1, 3000), (F16, 80, 300), (BF16, 90, 3000)])
+def test_infinite_keys_give_the_scores_that_they_give(core, dtype, new, length):
+    """-inf: a weight of zero, as that of a score far below all others; inf: NaN."""
+    D, page, G = 64, 16, 2
+    batch = ref.make_batch([new], [length], page, 241)
+    pages = ref.make_pages(batch, 1, D, None, dtype, 242)
+    q = torch.randn((new, G, D), generator=torch.Generator().manual_seed(243)).to(dtype)
+    q[:, 0, 0], q[:, 1, 0] = -1.0, 1.0                              # the first head's scores are -inf, the second's inf
+
+    def with_keys(x):
+        for p in (0, 77, length - new):
+            pages[0][batch['table'][0][p // page], 0, p % page, 0] = x
+        return ref.attention(q, ref.held(pages[0], None), ref.held(pages[1], None), batch, 1, 0.125)
+
+    # the weight of a score of -7500 is zero as well; what the other keys' scores are off by is what the bound is made of (rows of a wave move their reference
+    # together, so that one head's scores can change another's last bits)
+    most, want = with_keys(0.0)['most'], with_keys(60000.0)
+    want['most'] = most
+    bound, exact = ref.attention_bounds_by_largest(want, dtype, D), want['o']
+    with_keys(math.inf)
+    dev = _cuda(pages)
+    o, lse = core.paged_attention(q.cuda(), *dev[:2], *ref.on_device(batch), scale=0.125, max_queries=new, max_keys=length, return_lse=True)
+    assert bool(((o[:, 0].cpu().double() - exact[:, 0]).abs() <= bound[:, 0]).all())
+    assert bool(((lse[:, 0].cpu().double() - want['lse'][:, 0]).abs() <= ref.attention_bounds(want, dtype, D)[1][:, 0]).all())
+    assert bool(torch.isnan(o[:, 1]).all()) and bool(torch.isnan(lse[:, 1]).all())
+
+
 # ---- verification -----------------------------------------------------------------------
 
 def _drafts(B, K, V, dtype, wide, seed):
