@@ -158,7 +158,7 @@ __device__ __forceinline__ unsigned encode4(float a, float b, float c, float d) 
 // Two of four codes (the lower or the upper pair) as fp32 pairs of codes.
 __device__ __forceinline__ float int8_code(unsigned w, int i) { return (float)(signed char)(w >> (8 * i)); }
 
-// Eight codes as eight elements of T times `scale` (a power of two).
+// Eight codes as eight elements of T times `scale`, a power of two; of int8 in fp16 one that fits_half.
 template <typename T, KvFormat F>
 __device__ __forceinline__ typename T::v8 decode8(v2u w, float scale) {
   unsigned r[4];
@@ -193,6 +193,33 @@ __device__ __forceinline__ typename T::v8 decode8(v2u w, float scale) {
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int p = 0; p < 2; ++p) r[2 * i + p] = T::pack(int8_code(w[i], 2 * p) * scale, int8_code(w[i], 2 * p + 1) * scale);
+  }
+  const v4u all = {r[0], r[1], r[2], r[3]};
+  return __builtin_bit_cast(typename T::v8, all);
+}
+
+// Whether code * 2^e is an element of fp16, or rounds to one, by a product in fp16: 2^e is a number of fp16, and no code times it is beyond fp16's largest.
+template <KvFormat F>
+__device__ __forceinline__ bool fits_half(int e) { return e >= -24 && e <= (F == kInt8 ? 9 : 7); }
+
+// decode8 for any power of two: each element rounded to T once, infinite beyond T's largest.  (Codes that were written from bf16, attended to in fp16.)
+template <typename T, KvFormat F>
+__device__ __forceinline__ typename T::v8 decode8_rounded(v2u w, float scale) {
+  unsigned r[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float x[4];
+    if constexpr (F == kE4m3) {
+      x[0] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 0);
+      x[1] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 1);
+      x[2] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 2);
+      x[3] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 3);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = int8_code(w[i], j);
+    }
+    r[2 * i] = T::pack(x[0] * scale, x[1] * scale);
+    r[2 * i + 1] = T::pack(x[2] * scale, x[3] * scale);
   }
   const v4u all = {r[0], r[1], r[2], r[3]};
   return __builtin_bit_cast(typename T::v8, all);

@@ -16,7 +16,8 @@
 // time for a second product, a weight is the rounded one and what that leaves, also in 16 bits (2^-22 of it fp16, 2^-16 bf16), so that a result is off by its own rounding
 // alone, whatever else the call holds.  In the wide form, bound by the matrix pipe, of which a second product would take half as much again, it is the rounded one
 // alone, half a step (2^-11 of it fp16, 2^-8 bf16), which with the result's own rounding makes sqrt(2) of the error of that alone in the mean.  A cache of 8
-// bits enters the products as its exact values.
+// bits enters the products as its exact values, which fp16 rows and bf16 rows have in their own type; with queries in fp16, those of bf16 rows that fp16 does not
+// have are rounded to it, tile by tile on a way of its own.
 #include <algorithm>
 #include <cmath>
 
@@ -366,10 +367,10 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
   for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
     for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[nq][s]));
-  // One tile.  MASKED: some row does not see all of it.
+  // One tile.  MASKED: some row does not see all of it.  ODD: some row of the cache has an exponent that fp16 elements do not.
   // keys_read and values_read come where the tile of K, and that of V, has been read.
-  auto step = [&](int key0, const unsigned char* kt, auto masked_c, auto&& keys_read, auto&& values_read) __attribute__((always_inline)) {
-    constexpr bool MASKED = decltype(masked_c)::value;
+  auto step = [&](int key0, const unsigned char* kt, auto masked_c, auto odd_c, auto&& keys_read, auto&& values_read) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(masked_c)::value, ODD = decltype(odd_c)::value;
     const unsigned char* const vt = kt + S::TILE;
     // lane (row m, kg) has keys 16 h + 4 kg + r: the factors of their scores (scale, and the power of two of K's row), and those of V's rows
     float kfac[2][4];
@@ -381,7 +382,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
         const unsigned ve = *reinterpret_cast<const unsigned*>(kt + 2 * S::TILE + 32 + 16 * h + 4 * kg);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          kfac[h][r] = ldexpf(a.scale_log2e, (signed char)(ke >> (8 * r)));
+          kfac[h][r] = ODD ? a.scale_log2e : ldexpf(a.scale_log2e, (signed char)(ke >> (8 * r)));
           vexp[h][r] = (signed char)(ve >> (8 * r));
           if constexpr (MASKED) {                                  // what lies behind a sequence's keys has no exponent
             const int key = key0 + 16 * h + 4 * kg + r;
@@ -402,8 +403,13 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
       for (int s = 0; s < KS; ++s) {
         const int row = 16 * h + m;
         v8 kf;
-        if constexpr (F == kSame) kf = *reinterpret_cast<const v8*>(kt + row * S::BYTES + (((4 * s + kg) ^ swizzle<S::BYTES>(row)) * 16));
-        else kf = decode8<T, F>(*reinterpret_cast<const v2u*>(kt + row * S::BYTES + (((2 * s + (kg >> 1)) ^ swizzle<S::BYTES>(row)) * 16) + 8 * (kg & 1)), 1.0f);
+        if constexpr (F == kSame) {
+          kf = *reinterpret_cast<const v8*>(kt + row * S::BYTES + (((4 * s + kg) ^ swizzle<S::BYTES>(row)) * 16));
+        } else {
+          const v2u w = *reinterpret_cast<const v2u*>(kt + row * S::BYTES + (((2 * s + (kg >> 1)) ^ swizzle<S::BYTES>(row)) * 16) + 8 * (kg & 1));
+          if constexpr (ODD) kf = decode8_rounded<T, F>(w, ldexpf(1.0f, (signed char)kt[2 * S::TILE + row]));
+          else kf = decode8<T, F>(w, 1.0f);
+        }
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) sc[nq][h] = T::mma16(kf, qf[nq][s], sc[nq][h]);
       }
@@ -465,7 +471,7 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
       rest[nq] = __builtin_bit_cast(v8, (v4u{u[0], u[1], u[2], u[3]}));
     }
     v2h vpair[4];
-    if constexpr (F != kSame && std::is_same<T, Half>::value) {
+    if constexpr (F != kSame && !ODD && std::is_same<T, Half>::value) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -497,7 +503,8 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
 #pragma unroll
           for (int i2 = 0; i2 < 4; ++i2) {
             const unsigned pair = pairs[i2];                      // (a bit cast of a vector's element itself takes the first element)
-            pairs[i2] = __builtin_bit_cast(unsigned, __builtin_bit_cast(v2h, pair) * vpair[i2]);
+            if constexpr (ODD) pairs[i2] = T::pack(ldexpf(T::low(pair), vexp[i2 / 2][2 * (i2 % 2)]), ldexpf(T::high(pair), vexp[i2 / 2][2 * (i2 % 2) + 1]));
+            else pairs[i2] = __builtin_bit_cast(unsigned, __builtin_bit_cast(v2h, pair) * vpair[i2]);
           }
           vf = __builtin_bit_cast(v8, pairs);
         }
@@ -556,8 +563,19 @@ __device__ __forceinline__ void narrow_attention(const AttnArgs& a, const Job& j
         if (i + STAGES + 1 < mine) next = blocks_of(i + STAGES + 1);
       }
     };
-    if (key0 < j.sure_lo || key0 + 32 > j.sure_hi || key0 < j.lo || key0 + 32 > j.hi) step(key0, ring + stage * S::STAGE, std::true_type{}, keys_read, values_read);
-    else step(key0, ring + stage * S::STAGE, std::false_type{}, keys_read, values_read);
+    const unsigned char* const kt = ring + stage * S::STAGE;
+    const bool masked = key0 < j.sure_lo || key0 + 32 > j.sure_hi || key0 < j.lo || key0 + 32 > j.hi;
+    bool odd = false;
+    if constexpr (F != kSame && std::is_same<T, Half>::value) {     // a lane looks at four of the tile's 64 exponents
+      const unsigned e = *reinterpret_cast<const unsigned*>(kt + 2 * S::TILE + 4 * (lane & 15));
+      odd = __builtin_amdgcn_ballot_w64(!(fits_half<F>((signed char)e) && fits_half<F>((signed char)(e >> 8)) && fits_half<F>((signed char)(e >> 16)) &&
+                                          fits_half<F>((signed char)(e >> 24)))) != 0;
+      if (__builtin_expect(odd, 0)) step(key0, kt, std::true_type{}, std::true_type{}, keys_read, values_read);
+    }
+    if (!odd) {
+      if (masked) step(key0, kt, std::true_type{}, std::false_type{}, keys_read, values_read);
+      else step(key0, kt, std::false_type{}, std::false_type{}, keys_read, values_read);
+    }
     stage = stage == STAGES - 1 ? 0 : stage + 1;
   }
 
@@ -766,7 +784,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
       const int p = min(64 * i + lane, D - 1), rw = p / (D / 16), piece = p - rw * (D / 16);
       const long long row_at = at + (decltype(inside_c)::value ? rw : min(max(key0 + rw - inside, least), most));
       codes[i] = *reinterpret_cast<const v4u*>(from + row_at * D + 16 * piece);
-      scale[i] = power_of_two(from_exps[row_at]);
+      scale[i] = ldexpf(1.0f, from_exps[row_at]);
     }
   };
   auto store = [&](unsigned char* to) __attribute__((always_inline)) {
@@ -774,12 +792,18 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
 #pragma unroll
       for (int i = 0; i < LD; ++i) {
         const int p = 64 * i + lane, rw = p / (D / 16), piece = p - rw * (D / 16), in_tile = 16 * cw + rw;
-        if (D % 64 == 0 || p < D) {
-          const int swz = half ? swizzle<S::BYTES>(in_tile) : v_swizzle<D>(in_tile);
+        const int swz = half ? swizzle<S::BYTES>(in_tile) : v_swizzle<D>(in_tile);
+        auto put = [&](auto decode) __attribute__((always_inline)) {
+          if (D % 64 == 0 || p < D) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-            *reinterpret_cast<v8*>(to + in_tile * S::BYTES + 16 * ((2 * piece + c) ^ swz)) = decode8<T, F>(v2u{codes[i][2 * c], codes[i][2 * c + 1]}, scale[i]);
-        }
+            for (int c = 0; c < 2; ++c)
+              *reinterpret_cast<v8*>(to + in_tile * S::BYTES + 16 * ((2 * piece + c) ^ swz)) = decode(v2u{codes[i][2 * c], codes[i][2 * c + 1]}, scale[i]);
+          }
+        };
+        // (the conversion of e4m3 rounds once whatever the scale)
+        constexpr bool LOOK = std::is_same<T, Half>::value && F == kInt8;
+        if (LOOK && __builtin_expect(__builtin_amdgcn_ballot_w64(!(scale[i] >= 0x1p-24f && scale[i] <= 0x1p9f)) != 0, 0)) put(decode8_rounded<T, F>);
+        else put(decode8<T, F>);
       }
     }
   };

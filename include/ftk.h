@@ -686,6 +686,10 @@ int ftk_kv_cache_read(const ftk_kv_pages* pages, const ftk_kv_batch* batch,
  * key gives the score that it gives, of which -inf has weight zero and any other
  * makes NaN.  Weights of up to 2^15 times values are summed in fp32: values of
  * bf16 beyond 2^100 may leave its range there, which makes NaN too.
+ * Codes of 8 bits count as their exact values where those are numbers of `type`, as
+ * they are if the rows they were written from were of it (and fp16's in bf16); with
+ * queries of fp16, codes of bf16 rows count as what fp16 rounds them to, infinite
+ * beyond 65504 (keys below 2^-14 may count as they are).
  * fp32 accumulation.  Sequences of any mixture of sizes go in one call: where max_queries
  * leaves none with more than 64 rows (new tokens times heads / pages->heads), all run
  * on a kernel made for reading the cache once; otherwise those of more than 16 rows run

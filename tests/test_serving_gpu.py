@@ -558,6 +558,40 @@ def test_infinite_keys_give_the_scores_that_they_give(core, dtype, new, length):
     assert bool(torch.isnan(o[:, 1]).all()) and bool(torch.isnan(lse[:, 1]).all())
 
 
+@pytest.mark.parametrize('cache', [I8, E4M3])
+@pytest.mark.parametrize('D,page,G,new,lens', [(64, 16, 4, [1, 3], [300, 90]), (96, 32, 4, [9, 4], [200, 150]), (128, 16, 8, [6] * 3, [900, 70, 6]), (64, 32, 2, [100, 1], [300, 200]),
+                                               (128, 16, 1, [80], [2500]), (32, 16, 1, [70, 2], [100, 300])])
+def test_queries_of_fp16_on_codes_of_bf16_rows(core, cache, D, page, G, new, lens):
+    """Rows of zeros, of values below and at the end of fp16's range and beyond it: elements count as fp16 numbers, on all kernels."""
+    heads, g = 2, torch.Generator().manual_seed(251)
+    batch = ref.make_batch(new, lens, page, 252)
+    factors = torch.tensor([1.0, 1.0, 0.0, 1e-5, 1e-6, 1e-7, 1e-8, 1e-12])
+    k, v = (torch.randn((sum(lens), heads, D), generator=g).clamp(-4, 4) * factors[torch.randint(0, 8, (sum(lens), heads, 1), generator=g)] for _ in range(2))
+    v[::7] = (v[::7] * 14000).clamp(-60000, 60000)
+    k[11:13], v[13], v[14] = 0.0, 0.0, 0.0
+    k[11, :, 0], k[12, :, 0] = 1e7, 3e30                            # q is -1 there: a score of -inf
+    v[13, :, 3], v[14, 1, 5] = 1e5, -1e20
+    pages = _cuda(ref.make_pages(batch, heads, D, cache, BF16, 253))
+    table, at, _ = ref.on_device(batch)
+    whole = torch.tensor([sum(lens[:b]) for b in range(len(lens) + 1)], dtype=torch.int32, device='cuda')
+    core.kv_cache_write(k.to(BF16).cuda(), v.to(BF16).cuda(), *pages[:2], table, at, whole, *pages[2:])
+    q = torch.randn((batch['tokens'], heads * G, D), generator=g).to(F16)
+    q[..., 0] = -1.0
+    as_half = lambda x: x.float().to(F16).double()                  # exact in fp32
+    keys, values = as_half(ref.held(pages[0], pages[2])), as_half(ref.held(pages[1], pages[3]))
+    assert int(torch.isinf(keys).sum()) == 2 * heads and int(torch.isinf(values).sum()) == heads + 1
+    most = ref.attention(q, torch.where(torch.isinf(keys), 0.0, keys), values, batch, heads, 0.125)['most']
+    want = ref.attention(q, torch.where(torch.isinf(keys), 60000.0, keys), values, batch, heads, 0.125)
+    want['most'] = most
+    # keys below 2^-14 may be as they are, less than 2^-25 off their fp16 number
+    bound = ref.attention_bounds_by_largest(want, F16, D) + (2 * 0.125 * 2.0 ** -25) * q.double().abs().sum(-1, keepdim=True) * want['mean']
+    got = core.paged_attention(q.cuda(), *pages[:2], *ref.on_device(batch), *pages[2:], scale=0.125, max_queries=max(new), max_keys=max(lens)).cpu().double()
+    nans = torch.isnan(want['o'])
+    assert bool(nans.any()) and not bool(nans.all()) and torch.equal(torch.isnan(got), nans)
+    worst = float(((got - want['o']).abs() / bound)[~nans].max())
+    assert worst <= 1.0, f'o is {worst:.3g} times its bound off'
+
+
 # ---- verification -----------------------------------------------------------------------
 
 def _drafts(B, K, V, dtype, wide, seed):
