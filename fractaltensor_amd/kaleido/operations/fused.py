@@ -336,9 +336,9 @@ def windowed_attention(query: FractalTensor, key: FractalTensor, value: FractalT
     return FractalTensor.from_dense(out.reshape(q.shape), depth)
 
 
-def _new_tokens(tss: FractalTensor, name: str, pages: torch.Tensor):
-    """[sequence][token] of [heads, D], ragged or not -> (the packed rows [tokens, heads, D] in the type that goes with the pages, tokens
-    of each sequence)."""
+def _new_tokens(tss: FractalTensor, name: str, pages: torch.Tensor, dtype: Optional[torch.dtype]):
+    """[sequence][token] of [heads, D], ragged or not -> (the packed rows [tokens, heads, D] in the type that goes with the pages (for codes of 8 bits: dtype, or
+    fp16), tokens of each sequence)."""
     if not isinstance(tss, FractalTensor):
         raise TypeError(f'{name} should be a FractalTensor.')
     if tss.depth != 2 or len(tss.element_shape) != 2:
@@ -348,7 +348,10 @@ def _new_tokens(tss: FractalTensor, name: str, pages: torch.Tensor):
     rows = tss.data.reshape(-1, *tss.element_shape)
     if not rows.is_cuda:
         raise RuntimeError(f'{name} lives on {rows.device}; the fused kernels run on the GPU only.')
-    return rows.to(torch.bfloat16 if pages.dtype == torch.bfloat16 else torch.float16), tss.width_by_depth(1)
+    own = pages.dtype if pages.dtype in (torch.float16, torch.bfloat16) else None
+    if dtype not in ((None, own) if own else (None, torch.float16, torch.bfloat16)):
+        raise TypeError(f'dtype should be {"that of the pages" if own else "float16 or bfloat16"}, got {dtype}.')
+    return rows.to(own or dtype or torch.float16), tss.width_by_depth(1)
 
 
 def _starts(counts, device) -> torch.Tensor:
@@ -372,13 +375,15 @@ def _by_sequence(rows: torch.Tensor, counts) -> FractalTensor:
     return ft
 
 
-def kv_cache_write(keyss: FractalTensor, valuess: FractalTensor, k_pages, v_pages, table, lens, k_exps=None, v_exps=None) -> None:
+def kv_cache_write(keyss: FractalTensor, valuess: FractalTensor, k_pages, v_pages, table, lens, k_exps=None, v_exps=None,
+                   dtype: Optional[torch.dtype] = None) -> None:
     """Writes the keys and values of new tokens, [sequence][token] of [kv heads, D] (any number of tokens in each sequence, none too), into their
     pages: the last positions of the lens[b] that sequence b has with them.  Pages [pages, kv heads, page size, D] are fp16, bf16, or 8-bit codes
     (float8_e4m3fn or int8) with an exponent for each row in k_exps, v_exps [pages, kv heads, page size] int8; table [B, columns] and lens [B] are int32.
-    fp32 tokens are rounded to fp16 (to bf16 for bf16 pages) first."""
-    keys, counts = _new_tokens(keyss, 'keyss', k_pages)
-    values, same = _new_tokens(valuess, 'valuess', k_pages)
+    Tokens are rounded first: to the type of 16-bit pages, and for codes to `dtype`, fp16 (the default) or bf16, which keeps fewer bits and values beyond
+    65504."""
+    keys, counts = _new_tokens(keyss, 'keyss', k_pages, dtype)
+    values, same = _new_tokens(valuess, 'valuess', k_pages, dtype)
     if counts != same:
         raise ValueError('keyss and valuess should have one structure.')
     _core().kv_cache_write(keys, values, k_pages, v_pages, table, lens, _starts(counts, keys.device), k_exps, v_exps)
@@ -395,12 +400,13 @@ def kv_cache_read(k_pages, v_pages, table, lens, counts: Sequence[int], dtype=to
 
 
 def paged_attention(qss: FractalTensor, k_pages, v_pages, table, lens, k_exps=None, v_exps=None, scale: Optional[float] = None, causal: bool = True,
-                    window: int = 0, max_keys: int = 0) -> FractalTensor:
+                    window: int = 0, max_keys: int = 0, dtype: Optional[torch.dtype] = None) -> FractalTensor:
     """Attention of new tokens, [sequence][token] of [heads, D], over a paged cache that holds their keys and values already (kv_cache_write): one
     token a sequence, drafted ones, chunks of prompts and whole prompts, in any mixture.  heads is a multiple of the cache's.  `scale` multiplies the
     scores and defaults to 1.0, as in flash_attention.  causal: a token sees the positions up to its own; window > 0: no more than that many of them.
-    max_keys: the greatest of lens where the program knows it.  The result has the structure and the type of qss; a token that sees nothing gets zeros."""
-    q, counts = _new_tokens(qss, 'qss', k_pages)
+    max_keys: the greatest of lens where the program knows it.  The result has the structure and the type of qss; a token that sees nothing gets zeros.
+    dtype: what the computation runs in on codes of 8 bits, that which they were written in: fp16 (the default) or bf16."""
+    q, counts = _new_tokens(qss, 'qss', k_pages, dtype)
     o = _core().paged_attention(q, k_pages, v_pages, table, lens, _starts(counts, q.device), k_exps, v_exps, 1.0 if scale is None else float(scale), causal, window,
                                 max(counts, default=0), max_keys)
     return _by_sequence(o.to(qss.data.dtype), counts)

@@ -800,6 +800,30 @@ def test_serving_on_fractal_tensors(core, new, dtype, cache):
         ops.fused.paged_attention(FractalTensor.from_dense(q, 1), *other[:2], table, lens, *other[2:])
 
 
+@pytest.mark.parametrize('cache', [E4M3, I8])
+def test_bf16_rows_in_codes_on_fractal_tensors(core, cache):
+    """Values beyond fp16's range: written and attended to in bf16, as the packed rows are, to the bit."""
+    from fractaltensor_amd.kaleido import operations as ops
+    heads, G, D, page, new = 2, 3, 64, 16, [3, 1, 17]
+    batch = ref.make_batch(new, new, page, 261)
+    table, lens, starts = ref.on_device(batch)
+    pages, other = ([t.cuda() for t in ref.make_pages(batch, heads, D, cache, BF16, 262)] for _ in range(2))
+    g = torch.Generator(device='cuda').manual_seed(263)
+    k, v, q = (torch.randn((sum(new), h, D), generator=g, device='cuda') for h in (heads, heads, heads * G))
+    v *= 1e6
+    core.kv_cache_write(k.to(BF16), v.to(BF16), *pages[:2], table, lens, starts, *pages[2:])
+    want = core.paged_attention(q.to(BF16), *pages[:2], table, lens, starts, *pages[2:], scale=0.2, max_queries=max(new)).float()
+    as_ft = lambda t: ops.fused._by_sequence(t, new)
+    ops.fused.kv_cache_write(as_ft(k), as_ft(v), *other[:2], table, lens, *other[2:], dtype=BF16)
+    assert all(_same(a, b) for a, b in zip(pages, other))
+    got = ops.fused.paged_attention(as_ft(q), *other[:2], table, lens, *other[2:], scale=0.2, dtype=BF16)
+    assert bool(torch.isfinite(want).all()) and float(want.abs().max()) > 1e5 and torch.equal(got.data.view_as(want), want)
+    with pytest.raises(TypeError, match='float16 or bfloat16'):
+        ops.fused.paged_attention(as_ft(q), *other[:2], table, lens, *other[2:], dtype=F32)
+    with pytest.raises(TypeError, match='that of the pages'):
+        ops.fused.paged_attention(as_ft(q), *[t.half() for t in pages[:2]], table, lens, dtype=BF16)
+
+
 def test_verification_on_fractal_tensors(core):
     from fractaltensor_amd.kaleido import FractalTensor, operations as ops
     B, K, V = 5, 4, 300
