@@ -412,21 +412,45 @@ def paged_attention(qss: FractalTensor, k_pages, v_pages, table, lens, k_exps=No
     return _by_sequence(o.to(qss.data.dtype), counts)
 
 
+def _padded(ft: FractalTensor, name: str, counts) -> torch.Tensor:
+    """[sequence][token], counts[b] tokens in sequence b -> dense [B, max(counts), *item]; what lies behind a sequence's tokens is not defined."""
+    if not isinstance(ft, FractalTensor):
+        raise TypeError(f'{name} should be a FractalTensor.')
+    if ft.depth != 2:
+        raise ValueError(f'{name} should have depth 2, got {ft.depth}.')
+    if ft._T is None or not ft.has_indices:
+        raise RuntimeError('FractalTensor is not initialized.')
+    if not ft.data.is_cuda:
+        raise RuntimeError(f'{name} lives on {ft.data.device}; the fused kernels run on the GPU only.')
+    if ft.width_by_depth(1) != counts:
+        raise ValueError(f'{name} should have {counts} tokens a sequence, got {ft.width_by_depth(1)}.')
+    rows, most = ft.data.reshape(-1, *ft.element_shape), max(counts, default=0)
+    if all(n == most for n in counts):
+        return rows.view(len(counts), most, *ft.element_shape)
+    out = rows.new_empty((len(counts), most, *ft.element_shape))
+    out[torch.tensor([[i < n for i in range(most)] for n in counts], device=rows.device)] = rows
+    return out
+
+
 def verify_drafts(targets: FractalTensor, drafts: FractalTensor, accept_uniforms: torch.Tensor, sample_uniforms: torch.Tensor,
                   draft_probabilities: Optional[FractalTensor] = None) -> FractalTensor:
     """Which drafted tokens a target model accepts, and the token that follows them: [sequence][token] of [1] integers, from one to K + 1 tokens a sequence.
 
     targets: [B][K + 1] of [1, V], the target's probabilities before each draft and behind the last; drafts: [B][K] of [1] int32 or int64; draft_probabilities:
-    [B][K] of [1, V] that the drafts were drawn from, or None for drafts that were not drawn at random; accept_uniforms [B, K] and sample_uniforms [B]:
-    uniform numbers of [0, 1), fp32.  The tokens left are distributed as the target's own."""
-    p = _dense_gpu(targets, 'targets', 2)
-    d = _dense_gpu(drafts, 'drafts', 2)
-    q = None if draft_probabilities is None else _dense_gpu(draft_probabilities, 'draft_probabilities', 2)
+    [B][K] of [1, V] that the drafts were drawn from, or None for drafts that were not drawn at random.  Sequences may have different numbers of drafts, K at
+    most, or none (dense arrays of all are made then, a copy).  accept_uniforms [B, K] and sample_uniforms [B]: uniform numbers of [0, 1), fp32.
+    The tokens left are distributed as the target's own."""
+    if not isinstance(drafts, FractalTensor):
+        raise TypeError('drafts should be a FractalTensor.')
+    if drafts.depth != 2 or drafts.element_size != 1:
+        raise ValueError(f'drafts should have depth 2 and hold single integers, got depth {drafts.depth} of {list(drafts.element_shape)}.')
+    counts = drafts.width_by_depth(1)
+    d = _padded(drafts, 'drafts', counts)
+    p = _padded(targets, 'targets', [n + 1 for n in counts])
+    q = None if draft_probabilities is None else _padded(draft_probabilities, 'draft_probabilities', counts)
     if p.dim() != 4 or p.shape[2] != 1 or (q is not None and (q.dim() != 4 or q.shape[2] != 1)):
         raise ValueError('targets and draft_probabilities should have [1, V] items.')
-    if drafts.element_size != 1:
-        raise ValueError('drafts should hold single integers.')
-    tokens, accepted = _core().verify_drafts(p.squeeze(2).contiguous(), None if q is None else q.squeeze(2).contiguous(), d.reshape(d.shape[0], d.shape[1]).contiguous(),
-                                             accept_uniforms, sample_uniforms)
+    lens = None if all(n == d.shape[1] for n in counts) else torch.tensor(counts, dtype=torch.int32, device=d.device)
+    tokens, accepted = _core().verify_drafts(p.squeeze(2), None if q is None else q.squeeze(2), d.reshape(d.shape[0], d.shape[1]), accept_uniforms, sample_uniforms, lens)
     kept = torch.arange(tokens.shape[1], device=tokens.device) <= accepted[:, None]
     return _by_sequence(tokens[kept].reshape(-1, 1), [n + 1 for n in accepted.tolist()])

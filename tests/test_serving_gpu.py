@@ -837,3 +837,22 @@ def test_verification_on_fractal_tensors(core):
     assert got.data.tolist() == [t for b, n in enumerate(counts) for t in want[0][b, :n].tolist()]
     with pytest.raises(ValueError, match=r'\[1, V\] items'):
         ops.fused.verify_drafts(FractalTensor.from_dense(target, 2), FractalTensor.from_dense(drafts.reshape(B, K, 1), 2), accept, sample)
+
+
+@pytest.mark.parametrize('counts', [[3, 0, 5, 1], [0, 0, 0], [2, 2, 0]])
+@pytest.mark.parametrize('drawn', [True, False])
+def test_ragged_drafts_on_fractal_tensors(core, counts, drawn):
+    """Sequences with different numbers of drafts, none among them."""
+    from fractaltensor_amd.kaleido import operations as ops
+    B, K, V = len(counts), max(counts), 300
+    target, draft, drafts, accept, sample = _drafts(B, K, V, F32, True, 141)
+    want = ref.verify(target, draft if drawn else None, drafts, accept, sample, counts)
+    rows = lambda t, more: torch.cat([t[b, :n + more] for b, n in enumerate(counts)]).cuda()
+    as_ft = lambda t, more: ops.fused._by_sequence(t, [n + more for n in counts])
+    p, q, d = as_ft(rows(target, 1).view(-1, 1, V), 1), as_ft(rows(draft, 0).view(-1, 1, V), 0), as_ft(rows(drafts, 0).view(-1, 1), 0)
+    got = ops.fused.verify_drafts(p, d, accept.cuda(), sample.cuda(), q if drawn else None)
+    left = [n + 1 for n in want[1].tolist()]
+    assert got.width_by_depth(1) == left and got.data.tolist() == [t for b, n in enumerate(left) for t in want[0][b, :n].tolist()]
+    if counts[0]:
+        with pytest.raises(ValueError, match='tokens a sequence'):
+            ops.fused.verify_drafts(q, d, accept.cuda(), sample.cuda())
