@@ -880,10 +880,11 @@ def kv_cache_read(k_pages, v_pages, table, lens, starts, tokens: int, dtype=None
     """The last starts[b + 1] - starts[b] positions of every sequence as dense keys and values [tokens, kv heads, D]; tokens is what the
     arrays hold rows of (rows that are no sequence's are left as they were).  dtype: fp16, bf16 or fp32, for pages of 16 bits their own type (the
     default) or fp32; for codes of 8 bits there is no default."""
+    own = getattr(k_pages, 'dtype', None)
     if dtype is None:
-        dtype = getattr(k_pages, 'dtype', None)
+        dtype = own
     ok, ov = (None, None) if out is None else out
-    if dtype in (torch.float16, torch.bfloat16, torch.float32) and (k_pages.dtype not in (torch.float16, torch.bfloat16) or dtype in (k_pages.dtype, torch.float32)):
+    if dtype in (torch.float16, torch.bfloat16, torch.float32) and (own not in (torch.float16, torch.bfloat16) or dtype in (own, torch.float32)):
         done = _serving.kv_cache_read(_LIKE[dtype], k_pages, v_pages, table, lens, starts, k_exps, v_exps, tokens, ok, ov)
         if done is not None:
             return done

@@ -139,6 +139,23 @@ def test_wrappers_say_what_is_wrong(core):
         core.verify_drafts(torch.zeros(1, 2, 8).double(), None, torch.zeros((1, 1), dtype=torch.int64), torch.zeros(1, 1), torch.zeros(1))
 
 
+def test_what_is_not_a_tensor_is_refused_by_name(core):
+    pages = torch.zeros((2, 2, 16, 64), dtype=torch.float16)
+    table, lens, starts = torch.zeros((1, 1), dtype=torch.int32), torch.ones(1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    rows = torch.zeros((1, 2, 64), dtype=torch.float16)
+    for dtype in (None, torch.float32):
+        with pytest.raises(TypeError, match='k_pages must be a torch.Tensor'):
+            core.kv_cache_read([pages], pages, table, lens, starts, 1, dtype)
+    with pytest.raises(TypeError, match='v_pages must be a torch.Tensor'):
+        core.kv_cache_read(pages, None, table, lens, starts, 1)
+    with pytest.raises(TypeError, match='k_pages must be a torch.Tensor'):
+        core.kv_cache_write(rows, rows, None, pages, table, lens, starts)
+    with pytest.raises(TypeError, match='k_pages must be a torch.Tensor'):
+        core.paged_attention(rows, pages.numpy(), pages, table, lens, starts)
+    with pytest.raises(TypeError, match='must be torch.Tensors'):
+        core.verify_drafts([0.5], None, [1], [0.5], [0.5])
+
+
 # ---- the reference itself ------------------------------------------------------------
 
 def test_reference_codes():
