@@ -169,7 +169,7 @@ struct RowPiece {
         x[2 * i + 1] = T::high(same[i]);
       }
     } else {
-      const float up = power_of_two(e);
+      const float up = ldexpf(1.0f, e);                          // (of any signed byte: 2^-128 too)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if constexpr (F == kInt8) {

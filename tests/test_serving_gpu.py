@@ -113,6 +113,21 @@ def test_read_rows_are_what_the_codes_stand_for(core, dtype, cache, D, page, hea
         assert torch.equal(x.cpu(), expected)
 
 
+@pytest.mark.parametrize('cache', [E4M3, I8])
+@pytest.mark.parametrize('dtype', [F16, BF16, F32])
+def test_read_rows_under_any_exponent(core, cache, dtype):
+    """Every signed byte for an exponent, once with each code: the product, rounded once, infinite beyond the type's largest."""
+    batch = ref.make_batch([256], [256], 256, 171, spare=0)
+    codes = torch.arange(256, dtype=torch.uint8)
+    if cache == E4M3:
+        codes[0x7f], codes[0xff] = 0, 0                            # NaN
+    pages = [codes.view(cache).view(2, 1, 128).expand(2, 256, 128).contiguous().view(1, 2, 256, 128) for _ in range(2)]
+    exps = [torch.arange(-128, 128).to(torch.int8).view(1, 1, 256).expand(1, 2, 256).contiguous() for _ in range(2)]
+    got = core.kv_cache_read(*_cuda(pages), *ref.on_device(batch), 256, dtype, *_cuda(exps))
+    want = ref.held(pages[0], exps[0])[0].transpose(0, 1).float().to(dtype)      # exact in fp32 where it is not beyond it
+    assert torch.equal(got[0].cpu(), want) and torch.equal(got[1].cpu(), want)
+
+
 def test_rows_of_a_joint_projection_are_written_in_place(core):
     """Views of one [tokens, query + key + value heads, D] product, and of one with the heads outermost."""
     heads, D, page = 2, 64, 16
