@@ -18,6 +18,8 @@
 // alone, half a step (2^-11 of it fp16, 2^-8 bf16), which with the result's own rounding makes sqrt(2) of the error of that alone in the mean.  A cache of 8
 // bits enters the products as its exact values, which fp16 rows and bf16 rows have in their own type; with queries in fp16, those of bf16 rows that fp16 does not
 // have are rounded to it, tile by tile on a way of its own.
+#include <float.h>
+
 #include <algorithm>
 #include <cmath>
 
@@ -1379,7 +1381,7 @@ int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long 
   if (rc || (rc = check_kv_batch(who, batch, &a.batch)) || (rc = check_attention(who, heads, pages))) return rc;
   if (type != FTK_F16 && type != FTK_BF16) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: queries must be fp16 or bf16", who);
   if ((pages->type == FTK_F16 || pages->type == FTK_BF16) && pages->type != type) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: pages of 16 bits must have the type of the queries", who);
-  if (!(scale > 0.0f) || scale > 3.0e38f) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: scale must be positive and finite", who);
+  if (!(scale > 0.0f) || !(scale * 1.4426950408889634f <= FLT_MAX)) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: scale must be positive, and its product with log2(e) finite", who);
   if (window < 0 || max_queries < 0 || max_keys < 0) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: window, max_queries and max_keys must not be negative", who);
   if (a.batch.tokens == 0) return FTK_OK;
   if (!q || !o || !aligned16(q) || !aligned16(o)) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: q and o must be non-NULL and 16-byte aligned", who);

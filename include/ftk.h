@@ -678,7 +678,7 @@ int ftk_kv_cache_read(const ftk_kv_pages* pages, const ftk_kv_batch* batch,
  * p sees the positions k < lens[b] with k <= p (causal != 0) and k > p - window
  * (window > 0).  Into o [tokens, heads, head_size], of q's type and 16-byte
  * aligned:
- *   o = sum_k w_k v_k / sum_k w_k,  w_k = exp(scale * q . k_k),  scale > 0,
+ *   o = sum_k w_k v_k / sum_k w_k,  w_k = exp(scale * q . k_k),  0 < scale < 2.3e38,
  * and into lse [tokens, heads] fp32, if not NULL, log sum_k w_k.  A token without
  * positions to see gets zeros and -inf.  Keys and values that a token does not
  * see never matter to it, NaN and infinities included.  A value that is not finite

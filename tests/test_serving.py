@@ -156,6 +156,16 @@ def test_what_is_not_a_tensor_is_refused_by_name(core):
         core.verify_drafts([0.5], None, [1], [0.5], [0.5])
 
 
+def test_scales_whose_product_with_log2_e_is_not_finite_are_refused(core):
+    lib, ci, cl, vp = core.lib, ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p
+    p, b = ctypes.byref(_pages(core)), ctypes.byref(_batch(core))
+    f = lambda scale, o: lib.ftk_paged_attn(vp(ONE), ci(0), cl(256), cl(64), p, b, vp(o), vp(None), ci(4), ctypes.c_float(scale), ci(1), ci(0), ci(0), ci(0), vp(None), ctypes.c_size_t(0),
+                                            vp(None))
+    for scale in (2.4e38, 2.9e38, 3.4e38):
+        assert f(scale, 24) == -1 and b'scale' in lib.ftk_last_error()
+    assert f(2.3e38, 24) == -1 and b'aligned' in lib.ftk_last_error()          # (refused for the address of o)
+
+
 # ---- the reference itself ------------------------------------------------------------
 
 def test_reference_codes():
