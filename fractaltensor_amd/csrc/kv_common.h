@@ -53,6 +53,9 @@ __device__ __forceinline__ int count_at_most(int n, long long x, F&& value) {
   return count;
 }
 
+// The position of packed row `start`, of those from 0 on, in a sequence whose new tokens end at row `end`, which may lie behind the packed rows.
+__device__ __forceinline__ int first_position(int len, int start, int end) { return len - max(end - start, 0); }
+
 // The new tokens of sequence b: packed rows [start, start + n), row start + t at position first + t (which may be negative or
 // past what the table has room for).
 struct KvChunk {
@@ -61,9 +64,10 @@ struct KvChunk {
 __device__ __forceinline__ KvChunk kv_chunk(const KvBatch& batch, int b) {
   KvChunk c;
   c.start = min(max(load_uniform(batch.starts, b), 0), batch.tokens);
-  c.n = min(max(load_uniform(batch.starts, b + 1), c.start), batch.tokens) - c.start;
+  const int end = load_uniform(batch.starts, b + 1);
+  c.n = min(max(end, c.start), batch.tokens) - c.start;
   c.len = max(load_uniform(batch.lens, b), 0);
-  c.first = c.len - c.n;
+  c.first = first_position(c.len, c.start, end);
   return c;
 }
 

@@ -1123,7 +1123,7 @@ __device__ __forceinline__ int row_parts(const AttnArgs& a, long long at, int fi
   if (b >= a.batch.sequences) return 1;
   const int start = min(max(a.batch.starts[b], 0), a.batch.tokens), end = min(max(a.batch.starts[b + 1], start), a.batch.tokens);
   if (token < start || token >= end) return 1;
-  const int all = max(a.batch.lens[b], 0), first = all - (end - start), len = min(all, kv_capacity(a.batch, a.pages.page_shift));
+  const int all = max(a.batch.lens[b], 0), first = first_position(all, start, a.batch.starts[b + 1]), len = min(all, kv_capacity(a.batch, a.pages.page_shift));
   const long long position = (long long)first + (token - start);
   *hi = a.causal ? clamp_position(position + 1, len) : len;
   *lo = a.window > 0 ? clamp_position(position - a.window + 1, len) : 0;

@@ -619,7 +619,8 @@ typedef struct ftk_kv_pages {
  * that they are its last positions.  Position p lies in row p % page_size of page
  * table[b, p / page_size] (table [sequences, table_width]).  `tokens` is how many
  * rows the packed arrays have; rows from starts[sequences] on are nobody's: they are
- * never written, and what they hold does not matter.  A sequence may have no new tokens, or no length;
+ * never written, and what they hold does not matter.  Of a sequence that `starts` lets end
+ * behind them, the rows that are there count, at their positions.  A sequence may have no new tokens, or no length;
  * without sequences or tokens a call does nothing.
  *
  * What the arrays hold is looked at on the device, where it cannot be refused:

@@ -378,6 +378,24 @@ def test_batches_that_make_no_sense_write_nothing_outside(core):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize('new,lens,rows', [([1, 6], [40, 90], 4), ([5, 100], [30, 300], 60), ([3], [2900], 2), ([90], [3000], 70)])
+def test_packed_rows_that_end_inside_a_sequence(core, new, lens, rows):
+    """Fewer packed rows than `starts` speaks of: those that are there are at their positions, as for writing and reading."""
+    D, page, heads, G = 64, 16, 2, 4
+    batch = ref.make_batch(new, lens, page, 87)
+    pages = ref.make_pages(batch, heads, D, None, F16, 88)
+    q = torch.randn((batch['tokens'], heads * G, D), generator=torch.Generator().manual_seed(89)).to(F16)
+    want = ref.attention(q, ref.held(pages[0], None), ref.held(pages[1], None), batch, heads, D ** -0.5)
+    bound, _ = ref.attention_bounds(want, F16, D)
+    dev = _cuda(pages)
+    got = core.paged_attention(q[:rows].cuda(), *dev[:2], *ref.on_device(batch), max_queries=max(new), max_keys=max(lens)).cpu().double()
+    assert bool(((got - want['o'][:rows]).abs() <= bound[:rows]).all())
+    k, _ = core.kv_cache_read(*dev[:2], *ref.on_device(batch), rows)
+    for b in range(len(new)):
+        for row, at, r in ref.places(batch, b):
+            assert row >= rows or torch.equal(k[row].cpu(), pages[0][at, :, r])
+
+
 @pytest.mark.parametrize('new,lens', [([1, 1], [100, 40]), ([100, 1], [130, 40])])
 def test_queries_as_views_and_results_in_their_place(core, new, lens):
     D, page, heads, G = 128, 32, 2, 4
