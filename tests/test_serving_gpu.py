@@ -249,6 +249,40 @@ def test_attention_over_a_paged_cache(core, dtype, cache, D, page, heads, G, new
     _attention_case(core, dtype, cache, D, page, heads, G, new, lens, 11, tail=2)
 
 
+def _slots_are_packed(new, G, most):
+    """Whether the wide kernel numbers its row blocks over the packed rows: with as many for each sequence as `most` tokens have, most would be empty."""
+    B, tokens = len(new), sum(new)
+    return most * G > 64 and B * -(-most * G // 256) > 2 * (tokens * G // 256 + B)
+
+
+@pytest.mark.parametrize('dtype,cache,D,page,heads,G', [(F16, None, 128, 16, 1, 4), (BF16, I8, 64, 32, 2, 4), (F16, E4M3, 96, 64, 1, 5)])
+@pytest.mark.parametrize('hints', [True, False])
+@pytest.mark.parametrize('new,lens', [
+    ([600, 1, 1, 0, 1, 1, 1], [650, 300, 40, 20, 1, 128, 77]),
+    ([1, 0, 1, 600, 1, 20, 0], [1, 0, 90, 600, 333, 64, 5]),
+    ([1, 0, 1] * 11 + [550] + [1, 1, 0] * 12, [(37 * b) % 90 + 1 for b in range(33)] + [700] + [(53 * b) % 90 + 1 for b in range(36)]),
+])
+def test_a_chunk_beside_sequences_that_decode_or_pause(core, dtype, cache, D, page, heads, G, hints, new, lens):
+    """Row blocks numbered over the packed rows, of up to 70 sequences."""
+    assert _slots_are_packed(new, G, max(new) if hints else sum(new))
+    _attention_case(core, dtype, cache, D, page, heads, G, new, lens, 271, hints=hints, tail=1)
+
+
+@pytest.mark.parametrize('dtype,cache,D', [(F16, None, 128), (BF16, E4M3, 128), (BF16, None, 64)])
+def test_small_sequences_alone_are_cut(core, dtype, cache, D):
+    """Room for the parts of sequences of up to 16 rows and for no others': sixteen rows to a wave that joins, most of which have nothing to join."""
+    heads, G, page = 2, 2, 16
+    long = 4000 * (1 if cache is None else 2) * (128 // D)
+    new, lens = [200, 1, 0, 300, 1, 8, 2], [210, long, 50, 300, long - 100, long - 700, 9]
+    keys, held = max(lens), 4 * D if cache is None else 2 * D + 2  # bytes of a position and head
+    n = min(keys * held // (20 * 17000), keys // 256 + 1)
+    part = -(-(-(-keys // n)) // 128) * 128
+    parts = -(-keys // part)
+    assert 1 < parts < 16                                          # (16 and few rows: a block to a row)
+    room = len(new) * heads * 16 * parts * (D + 2) * 4
+    _attention_case(core, dtype, cache, D, page, heads, G, new, lens, 281, tail=3, workspace=torch.empty(room, dtype=torch.uint8, device='cuda'))
+
+
 @pytest.mark.parametrize('causal,window', [(False, 0), (True, 1), (True, 16), (True, 50), (False, 33)])
 @pytest.mark.parametrize('cache,D,page,G', [(None, 64, 16, 3), (E4M3, 128, 64, 1), (I8, 96, 32, 8)])
 @pytest.mark.parametrize('new,lens', [([1, 1], [200, 31]), ([6, 2], [150, 40]), ([100, 3], [150, 90])])
@@ -376,6 +410,38 @@ def test_batches_that_make_no_sense_write_nothing_outside(core):
             core.paged_attention(q, *pages[:2], table, *ints, *pages[2:], max_queries=hint, out=whole[1:13])
             assert bool((whole[0] == 7).all()) and bool((whole[13] == 7).all())
     torch.cuda.synchronize()
+
+
+def test_batches_that_make_no_sense_leave_what_lies_around_alone(core):
+    """Pages, exponents, dense rows, results and log-sum-exps lie inside larger buffers of a pattern: what is written lies in them, and in pages that the table names."""
+    D, page, heads = 64, 16, 2
+    batch = ref.make_batch([4, 4, 4], [30, 40, 50], page, 75)
+    table = ref.on_device(batch)[0]
+    named = set(sum(batch['table'], []))
+    g = torch.Generator().manual_seed(76)
+    keys, values, q = (torch.randn((12, h, D), generator=g).to(F16).cuda() for h in (heads, heads, 4))
+    inside = lambda shape, dtype: torch.full((shape[0] + 2 * 8, *shape[1:]), 0x55, dtype=torch.uint8, device='cuda').view(dtype)
+    P = batch['pages']
+    for s, n in (([0, 8, 4, 12], [30, 40, 50]), ([0, 4, 8, 2 ** 31 - 1], [30, 40, 50]), ([-5, 4, 8, 12], [30, -40, 50]), ([0, 4, 8, 12], [30, 4000, 2 ** 31 - 1]), ([12, 0, 0, 0], [0, 0, 0]),
+                 ([3, 4, 9, 11], [-2 ** 31, 2 ** 31 - 1, 1])):
+        ints = [torch.tensor(v, dtype=torch.int32, device='cuda') for v in (n, s)]
+        whole = [inside((P, heads, page, D), E4M3) for _ in range(2)] + [inside((P, heads, page), I8) for _ in range(2)]
+        pages = [t[8:-8] for t in whole]
+        core.kv_cache_write(keys, values, *pages[:2], table, *ints, *pages[2:])
+        for t in whole:
+            raw = t.view(torch.uint8)
+            for i in range(len(raw)):
+                assert i - 8 in named or bool((raw[i] == 0x55).all()), (s, n, i)
+        before = [t.view(torch.uint8).clone() for t in whole]
+        rows = [inside((12, heads, D * 2), F16) for _ in range(2)]
+        core.kv_cache_read(*pages[:2], table, *ints, 12, F16, *pages[2:], out=tuple(t[8:-8] for t in rows))
+        for hint in (0, 4, 1):
+            o, lse = inside((12, 4, D * 2), F16), inside((12, 4 * 4), F32)
+            core.paged_attention(q, *pages[:2], table, *ints, *pages[2:], max_queries=hint, out=o[8:-8], return_lse=lse[8:-8])
+            for t in (*rows, o, lse):
+                raw = t.view(torch.uint8)
+                assert bool((raw[:8] == 0x55).all()) and bool((raw[-8:] == 0x55).all()), (s, n, hint)
+        assert all(torch.equal(a.view(torch.uint8), b) for a, b in zip(whole, before))
 
 
 @pytest.mark.parametrize('new,lens,rows', [([1, 6], [40, 90], 4), ([5, 100], [30, 300], 60), ([3], [2900], 2), ([90], [3000], 70)])
@@ -669,6 +735,28 @@ def test_verified_drafts_at_the_ends_of_their_ranges(core):
     accept[7] = 1.0
     want = _verified(core, target, draft, drafts, accept, sample)
     assert want[1].tolist()[0] == 0 and int(want[1][1]) <= 1 and int(want[1][2]) == 0 and int(want[1][3]) == 0 and int(want[0][6][0]) == -1
+
+
+@pytest.mark.parametrize('V', [(1 << 21) + 8, (1 << 21) + 1001])
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_verification_of_vocabularies_whose_segments_take_two_passes(core, V, dtype):
+    """Beyond 2^21 a segment has 4096 tokens, read 2048 at a time: drawn tokens in both halves of a segment, in the first, a late and the last one, from the target's row
+    and from what is left of it."""
+    g = torch.Generator().manual_seed(94)
+    weights = torch.rand((1, 2, V), generator=g)
+    wanted = [5, 2048 + 77, 300 * 4096 + 4000, (V // 4096 - 1) * 4096 + 1000, V - 1]
+    weights[0, :, wanted] = 500.0
+    target = (weights / weights.sum(-1, keepdim=True, dtype=torch.float64)).to(dtype)
+    draft = (target[:, :1].double() * 0.5).to(dtype)
+    for token in wanted:
+        for drafts, accept in (([[7]], 0.0), ([[7]], 1.0)):
+            n = 0 if accept else 1
+            draft[0, 0, 7] = 1.0 if accept else draft[0, 0, 8]      # rejected: 1 * 1 < target does not hold
+            w = target[0, n].double() - (draft[0, 0].double() if accept else 0.0)
+            ends = torch.where(w > 0, w, 0.0).cumsum(0)
+            u = float((ends[token] - w[token] / 2) / ends[-1])     # the middle of its weight, some 2^-13 of all
+            want = _verified(core, target, draft, torch.tensor(drafts), torch.tensor([[accept]]), torch.tensor([u]))
+            assert int(want[1][0]) == n and int(want[0][0, n]) == token
 
 
 def test_verified_drafts_at_odd_addresses(core):
