@@ -1085,7 +1085,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
 // The workgroups behind the first `wide` take sequences of at most small_rows = 16 rows, which would leave seven of the eight waves without
 // any: two (sequence, head, part) each, by four waves that cut the keys as in the narrow kernel.  They read on the compute units that the others
 // leave free, or have left, while those multiply.  (A chunk of 512 tokens beside five sequences that decode, 16 heads, 4 of keys, up to
-// 16384 of them, in int8: 165 us with all on the wide form, 100 so, and 11 for joining.)
+// 16384 of them, in int8: 165 us with all on the wide form, 108 so, and 12 for joining.)
 template <typename T, KvFormat F, int D>
 __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs a, int wide) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -1302,7 +1302,8 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
   if (window > 0) seen = std::min(seen, most + window + 64);   // from the first key that the first new token sees, down to a multiple of 64
   const int keys = (int)std::min<long long>(seen, INT_MAX - 1024);
   // 32 rows to a narrow workgroup read the keys half as often as 16; those are the faster ones where even parts of 256 keys are fewer than the compute
-  // units.  (Six tokens, 64 heads, 8 of keys of 128: 16 sequences of up to 4096 keys 64 us by 32 rows, 63 to 73 by 16; two of up to 1000 keys 15 and 12.)
+  // units.  (16 sequences of up to 4096 keys, 8 heads of them, 20 rows: 48 us by 32 rows and 54 by 16 at D 128, int8 46 and 48, 25 and 28 at D 64; 48 rows: 65 and 67, int8 69 and 71, but
+  // 38 and 34 at D 64; two sequences of up to 1000 keys, 48 rows: 15 and 12.)
   p.nq = most_rows <= 16 || (p.narrow && ((most_rows + 31) / 32) * b.sequences * pages.heads * ((keys + 255) / 256) < cus) ? 1 : 2;
   const int R = p.narrow ? 16 * p.nq : kWideRows;
   const long long per_seq = (most_rows + R - 1) / R, packed = (long long)b.tokens * group / R + b.sequences;
