@@ -32,6 +32,7 @@ EXPORTS = (
     'ftk_b2b_gemm_f16', 'ftk_b2b_gemm_f16_supported', 'ftk_b2b_gemm_rowmajor_f16', 'ftk_gemm_f16', 'ftk_batched_gemm_f16', 'ftk_flash_attn_f16', 'ftk_flash_attn_f16_workspace_bytes', 'ftk_flash_attn_ws_f16', 'ftk_flash_attn_f32_workspace_bytes', 'ftk_flash_attn_f32', 'ftk_online_softmax_f32', 'ftk_embedding_gather_f32',
     'ftk_grid_rnn_workspace_bytes', 'ftk_grid_rnn_f32', 'ftk_windowed_attn_f32',
     'ftk_kv_cache_write', 'ftk_kv_cache_read', 'ftk_paged_attn_workspace_bytes', 'ftk_paged_attn', 'ftk_verify_drafts_workspace_bytes', 'ftk_verify_drafts',
+    'ftk_paged_tree_attn_workspace_bytes', 'ftk_paged_tree_attn', 'ftk_verify_tree', 'ftk_kv_cache_weigh', 'ftk_kv_cache_select', 'ftk_kv_cache_keep',
 )
 
 
@@ -89,12 +90,14 @@ def _load() -> ctypes.CDLL:
     lib.ftk_flash_attn_f16_workspace_bytes.argtypes = [ctypes.c_int] * 5
     lib.ftk_paged_attn_workspace_bytes.restype = ctypes.c_size_t
     lib.ftk_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(KvPages), ctypes.POINTER(KvBatch)] + [ctypes.c_int] * 4
+    lib.ftk_paged_tree_attn_workspace_bytes.restype = ctypes.c_size_t
+    lib.ftk_paged_tree_attn_workspace_bytes.argtypes = lib.ftk_paged_attn_workspace_bytes.argtypes
     lib.ftk_verify_drafts_workspace_bytes.restype = ctypes.c_size_t
     lib.ftk_verify_drafts_workspace_bytes.argtypes = [ctypes.c_int] * 2
     for name in EXPORTS:
         if name not in ('ftk_last_error', 'ftk_stacked_lstm_workspace_bytes', 'ftk_stacked_lstm_f16_workspace_bytes', 'ftk_grid_rnn_workspace_bytes',
                         'ftk_flash_attn_f32_workspace_bytes', 'ftk_flash_attn_f16_workspace_bytes', 'ftk_paged_attn_workspace_bytes',
-                        'ftk_verify_drafts_workspace_bytes'):
+                        'ftk_verify_drafts_workspace_bytes', 'ftk_paged_tree_attn_workspace_bytes'):
             getattr(lib, name).restype = ctypes.c_int
     return lib
 
@@ -914,6 +917,25 @@ def paged_attention_workspace_bytes(q, k_pages, table, max_queries: int = 0, max
         return int(lib.ftk_paged_attn_workspace_bytes(ctypes.byref(pages), ctypes.byref(batch), q.shape[1], window, max_queries, max_keys))
 
 
+def _req_attention(q, args, out, lse, workspace, **numbers) -> None:
+    """Says what is wrong with queries, a cache and a batch, and where the results go, if something is."""
+    _req_cache(*args)
+    k_pages = args[0]
+    if not isinstance(q, torch.Tensor):
+        raise TypeError('q must be a torch.Tensor')
+    _req_pages_of(q.dtype, k_pages, 'q')
+    _req_rows(q, q.dtype, None, k_pages.shape[3], k_pages.device, 'q')
+    _not_negative(**numbers)
+    if out is not None:
+        _req_out(out, q.dtype, q.shape, 'out')
+        _req_on(out, q.dtype, q.shape, q.device, 'out')
+    if isinstance(lse, torch.Tensor):
+        _req_out(lse, torch.float32, q.shape[:2], 'return_lse')
+        _req_on(lse, torch.float32, q.shape[:2], q.device, 'return_lse')
+    if workspace is not None:
+        _req_on(_req_workspace(workspace), workspace.dtype, None, q.device, 'workspace')
+
+
 def paged_attention(q, k_pages, v_pages, table, lens, starts, k_exps=None, v_exps=None, scale: Optional[float] = None, causal: bool = True,
                     window: int = 0, max_queries: int = 0, max_keys: int = 0, out: Optional[torch.Tensor] = None, return_lse=False,
                     workspace: Optional[torch.Tensor] = None):
@@ -928,20 +950,7 @@ def paged_attention(q, k_pages, v_pages, table, lens, starts, k_exps=None, v_exp
     args = (k_pages, v_pages, table, lens, starts, k_exps, v_exps)
     done = _serving.paged_attention(q, *args, scale, causal, window, max_queries, max_keys, out, return_lse, workspace)
     if done is None:
-        _req_cache(*args)
-        if not isinstance(q, torch.Tensor):
-            raise TypeError('q must be a torch.Tensor')
-        _req_pages_of(q.dtype, k_pages, 'q')
-        _req_rows(q, q.dtype, None, k_pages.shape[3], k_pages.device, 'q')
-        _not_negative(window=window, max_queries=max_queries, max_keys=max_keys)
-        if out is not None:
-            _req_out(out, q.dtype, q.shape, 'out')
-            _req_on(out, q.dtype, q.shape, q.device, 'out')
-        if isinstance(return_lse, torch.Tensor):
-            _req_out(return_lse, torch.float32, q.shape[:2], 'return_lse')
-            _req_on(return_lse, torch.float32, q.shape[:2], q.device, 'return_lse')
-        if workspace is not None:
-            _req_on(_req_workspace(workspace), workspace.dtype, None, q.device, 'workspace')
+        _req_attention(q, args, out, return_lse, workspace, window=window, max_queries=max_queries, max_keys=max_keys)
         done = _serving.paged_attention(q, *args, None if scale is None else float(scale), bool(causal), window, max_queries, max_keys, out,
                                         return_lse if isinstance(return_lse, torch.Tensor) else bool(return_lse), workspace)
         if done is None:
@@ -983,3 +992,130 @@ def verify_drafts(target, draft, drafts, accept_uniforms, sample_uniforms, draft
     if workspace is not None:
         _req_on(_req_workspace(workspace), workspace.dtype, None, device, 'workspace')
     raise ValueError('verify_drafts: these arguments are not taken')
+
+
+# ---- trees of drafted tokens, and caches of limited length ----------------------------------
+#
+# A tree of drafts: the new tokens of a sequence, and for each of them parents [tokens] int32, the number of the token that it follows among those of
+# its sequence (counted from 0; a parent comes before its children), or a negative one for what follows the cache itself.
+# Weights [pages, kv heads, page size] fp32: what each position of the cache has been given, beside its keys.
+
+TREE_TOKENS = 256
+
+
+def paged_tree_attention_workspace_bytes(q, k_pages, table, max_queries: int = 0, max_keys: int = 0, window: int = 0) -> int:
+    """Bytes that paged_tree_attention wants for a batch of this shape on the device of q; 0 where the keys are not cut into parts."""
+    pages = KvPages(None, None, None, None, KV_TYPES[k_pages.dtype], *k_pages.shape)
+    batch = KvBatch(None, None, None, table.shape[0], table.shape[1], q.shape[0])
+    with torch.cuda.device(q.device):
+        return int(lib.ftk_paged_tree_attn_workspace_bytes(ctypes.byref(pages), ctypes.byref(batch), q.shape[1], window, max_queries, max_keys))
+
+
+def paged_tree_attention(q, k_pages, v_pages, table, lens, starts, parents, k_exps=None, v_exps=None, scale: Optional[float] = None, window: int = 0,
+                         max_queries: int = 0, max_keys: int = 0, out: Optional[torch.Tensor] = None, return_lse=False, workspace: Optional[torch.Tensor] = None):
+    """paged_attention for new tokens that form a tree: each sees the cache in front of its sequence's new tokens, its ancestors and itself, whose keys and
+    values the cache holds already, at the sequence's last positions in the order of their rows.  window > 0: of these the last `window` on the way that
+    ends with it.  At most 256 new tokens a sequence, which max_queries has to say where the call has more of all sequences together.  All else is as
+    in paged_attention, what it returns too."""
+    args = (k_pages, v_pages, table, lens, starts, k_exps, v_exps)
+    done = _serving.paged_tree_attention(q, *args, scale, parents, window, max_queries, max_keys, out, return_lse, workspace)
+    if done is None:
+        _req_attention(q, args, out, return_lse, workspace, window=window, max_queries=max_queries, max_keys=max_keys)
+        _req_on(parents, torch.int32, q.shape[:1], q.device, 'parents')
+        done = _serving.paged_tree_attention(q, *args, None if scale is None else float(scale), parents, window, max_queries, max_keys, out,
+                                             return_lse if isinstance(return_lse, torch.Tensor) else bool(return_lse), workspace)
+        if done is None:
+            raise ValueError('paged_tree_attention: these arguments are not taken')
+    return done[0] if done[1] is None else done
+
+
+def verify_tree(target, ids, parents, starts, uniforms) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The path through a tree of drafts that the target model's own draws follow, and the token behind it.
+
+    The packed rows starts[b] .. starts[b + 1] - 1 are the tokens of sequence b: first the root, the last token that is known already, then the drafts.
+    target [tokens, V] (fp32, fp16 or bf16): the target's probabilities of what follows each; ids [tokens] int32 or int64; parents [tokens] int32; uniforms
+    [B, M] fp32 of [0, 1), one for each step.  From the root on a token is drawn at each node; where the node has a child with it, the way goes on
+    there.  Returns next [B, M] of ids' type (the tokens that were drawn: the accepted drafts and one more, then -1), path [B, M] int32 (the nodes that
+    stay in the cache, by their number in the sequence, then -1: a list for kv_cache_keep) and accepted [B] int32.  The tokens are distributed as
+    the target's own, however the drafts were chosen."""
+    done = _serving.verify_tree(target, ids, parents, starts, uniforms)
+    if done is not None:
+        return done
+    if not isinstance(target, torch.Tensor) or not isinstance(ids, torch.Tensor):
+        raise TypeError('target and ids must be torch.Tensors')
+    if target.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f'target must be float32, float16 or bfloat16, got {target.dtype}')
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f'ids must be int32 or int64, got {ids.dtype}')
+    if target.dim() != 2:
+        raise ValueError(f'target must be [tokens, V], got {tuple(target.shape)}')
+    _req_on(target, target.dtype, None, target.device, 'target')
+    _req_on(ids, ids.dtype, target.shape[:1], target.device, 'ids')
+    _req_on(parents, torch.int32, target.shape[:1], target.device, 'parents')
+    _req_on(starts, torch.int32, None, target.device, 'starts')
+    if starts.dim() != 1 or starts.shape[0] < 1:
+        raise ValueError(f'starts must be [B + 1], got {tuple(starts.shape)}')
+    _req_on(uniforms, torch.float32, None, target.device, 'uniforms')
+    if uniforms.dim() != 2 or uniforms.shape[0] != starts.shape[0] - 1:
+        raise ValueError(f'uniforms must be [B, M] with B = {starts.shape[0] - 1}, got {tuple(uniforms.shape)}')
+    raise ValueError('verify_tree: these arguments are not taken')
+
+
+def _req_weights(weights, pages, device) -> None:
+    _req_on(weights, torch.float32, pages, device, 'weights')
+    if weights.dim() != 3:
+        raise ValueError(f'weights must be [pages, kv heads, page size], got {tuple(weights.shape)}')
+
+
+def kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps=None, scale: Optional[float] = None, decay: float = 1.0, causal: bool = True,
+                   window: int = 0, max_queries: int = 0, max_keys: int = 0) -> None:
+    """Adds to weights, of every position of the sequences that have new tokens, the attention weights that these give it: the sum of exp(scale q . k - lse) over
+    the new tokens that see it and the query heads that read its head.  q [tokens, heads, D] and lse [tokens, heads] as in, and out of, paged_attention
+    with the same scale, causal and window.  What older positions had is multiplied by decay (0 to 1) first, new ones begin at zero.  max_keys: the greatest
+    length where the program knows it.  (max_queries is taken so that the two calls can be given the same numbers.)"""
+    decay = decay if isinstance(decay, float) else float(decay)
+    if _serving.kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps, scale, decay, causal, window, max_keys):
+        return
+    _req_attention(q, (k_pages, k_pages, table, lens, starts, k_exps, k_exps), None, None, None, window=window, max_keys=max_keys)
+    _req_on(lse, torch.float32, q.shape[:2], q.device, 'lse')
+    _req_weights(weights, k_pages.shape[:3], q.device)
+    if not _serving.kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps, None if scale is None else float(scale), decay, bool(causal), window, max_keys):
+        raise ValueError('kv_cache_weigh: these arguments are not taken')
+
+
+def kv_cache_select(weights, table, lens, budget: int, sinks: int = 0, recent: int = 0, max_keys: int = 0) -> torch.Tensor:
+    """Which positions of every sequence and head stay in a cache of `budget` positions: the first `sinks`, the last `recent` and of the others those of the largest
+    weights, of equal ones the earlier.  Returns kept [B, kv heads, budget] int32, ascending, then -1: lists for kv_cache_keep.  A sequence of at most
+    `budget` positions keeps them all.  max_keys: the greatest length where the program knows it."""
+    done = _serving.kv_cache_select(weights, table, lens, budget, sinks, recent, max_keys)
+    if done is not None:
+        return done
+    _req(weights, torch.float32, 'weights')
+    _req_weights(weights, None, weights.device)
+    _req_on(lens, torch.int32, None, weights.device, 'lens')
+    if lens.dim() != 1:
+        raise ValueError(f'lens must be [B], got {tuple(lens.shape)}')
+    _req_on(table, torch.int32, None, weights.device, 'table')
+    if table.dim() != 2 or table.shape[0] != lens.shape[0]:
+        raise ValueError(f'table must be [B, W] with B = {lens.shape[0]}, got {tuple(table.shape)}')
+    _not_negative(budget=budget, sinks=sinks, recent=recent, max_keys=max_keys)
+    raise ValueError('kv_cache_select: these arguments are not taken')
+
+
+def kv_cache_keep(k_pages, v_pages, table, lens, kept, starts=None, k_exps=None, v_exps=None, weights=None) -> torch.Tensor:
+    """Moves the rows that stay together, in place: row kept[b, j] (or kept[b, head, j]) of sequence b goes to place j, for keys, values, exponents and, where they are
+    given, weights.  Rows are counted from the sequence's begin, or with starts from its first new token.  kept [B, M] or [B, kv heads, M] int32
+    ascends and has -1 behind its end; the lists of a sequence's heads are of one length.  Returns the new lengths [B] int32."""
+    done = _serving.kv_cache_keep(k_pages, v_pages, table, lens, kept, starts, k_exps, v_exps, weights)
+    if done is not None:
+        return done
+    if starts is None and isinstance(lens, torch.Tensor) and lens.dim() == 1:
+        _req_cache(k_pages, v_pages, table, lens, lens.new_zeros(lens.shape[0] + 1, dtype=torch.int32), k_exps, v_exps)
+    else:
+        _req_cache(k_pages, v_pages, table, lens, starts, k_exps, v_exps)
+    _req_on(kept, torch.int32, None, k_pages.device, 'kept')
+    if kept.dim() not in (2, 3) or kept.shape[0] != lens.shape[0] or (kept.dim() == 3 and kept.shape[1] != k_pages.shape[1]):
+        raise ValueError(f'kept must be [B, M] or [B, kv heads, M] with B = {lens.shape[0]}, got {tuple(kept.shape)}')
+    if weights is not None:
+        _req_weights(weights, k_pages.shape[:3], k_pages.device)
+    raise ValueError('kv_cache_keep: these arguments are not taken')

@@ -34,21 +34,23 @@ bool number(PyObject* o, int* out) {
   return true;
 }
 
-// The cache and the batch out of k_pages, v_pages, table, lens, starts, k_exps, v_exps.
+// The cache and the batch out of k_pages, v_pages, table, lens, starts (or None where a call does without), k_exps, v_exps.
 struct Cache {
   ftk_kv_pages pages;
   ftk_kv_batch batch;
 };
-bool cache_of(PyObject* const* a, int64_t tokens, Cache* c) {
+bool cache_of(PyObject* const* a, int64_t tokens, Cache* c, bool starts_needed = true) {
   if (!is_tensor(a[0]) || !is_tensor(a[1])) return false;
   const at::Tensor &k = tensor_of(a[0]), &v = tensor_of(a[1]);
   const int type = type_code(k.scalar_type());
   if (type < 0 || type == FTK_F32 || !plain(a[0], k.scalar_type()) || !plain_on(a[1], k.scalar_type(), k) || k.dim() != 4 || k.sizes() != v.sizes()) return false;
   for (int i = 0; i < 4; ++i)
     if (!small(k.size(i))) return false;
-  if (!plain_on(a[2], at::kInt, k) || !plain_on(a[3], at::kInt, k) || !plain_on(a[4], at::kInt, k)) return false;
-  const at::Tensor &table = tensor_of(a[2]), &lens = tensor_of(a[3]), &starts = tensor_of(a[4]);
-  if (table.dim() != 2 || lens.dim() != 1 || starts.dim() != 1 || table.size(0) != lens.size(0) || starts.size(0) != lens.size(0) + 1) return false;
+  const bool started = starts_needed || a[4] != Py_None;
+  if (!plain_on(a[2], at::kInt, k) || !plain_on(a[3], at::kInt, k) || (started && !plain_on(a[4], at::kInt, k))) return false;
+  const at::Tensor &table = tensor_of(a[2]), &lens = tensor_of(a[3]);
+  if (table.dim() != 2 || lens.dim() != 1 || table.size(0) != lens.size(0)) return false;
+  if (started && (tensor_of(a[4]).dim() != 1 || tensor_of(a[4]).size(0) != lens.size(0) + 1)) return false;
   if (!small(table.size(0)) || !small(table.size(1)) || !small(tokens)) return false;
   c->pages = {k.data_ptr(), v.data_ptr(), nullptr, nullptr, type, dim(k, 0), dim(k, 1), dim(k, 2), dim(k, 3)};
   if (type == FTK_E4M3 || type == FTK_INT8) {
@@ -61,7 +63,7 @@ bool cache_of(PyObject* const* a, int64_t tokens, Cache* c) {
   } else if (a[5] != Py_None || a[6] != Py_None) {
     return false;
   }
-  c->batch = {(const int*)table.data_ptr(), (const int*)lens.data_ptr(), (const int*)starts.data_ptr(), dim(table, 0), dim(table, 1), (int)tokens};
+  c->batch = {(const int*)table.data_ptr(), (const int*)lens.data_ptr(), started ? (const int*)tensor_of(a[4]).data_ptr() : nullptr, dim(table, 0), dim(table, 1), (int)tokens};
   return true;
 }
 
@@ -137,9 +139,20 @@ PyObject* kv_cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// None: the default of a head size; false: no number, or an error is set.
+bool scale_of(PyObject* o, int head_size, double* scale) {
+  *scale = 1.0 / std::sqrt((double)head_size);
+  if (o == Py_None) return true;
+  if (!PyFloat_Check(o) && !PyLong_Check(o)) return false;
+  *scale = PyFloat_AsDouble(o);
+  return !PyErr_Occurred();
+}
+
 // paged_attention(q, k_pages, v_pages, table, lens, starts, k_exps, v_exps, scale or None, causal, window, max_queries, max_keys, out or None,
 //                 lse (True: allocated, False: none, or a tensor), workspace or None) -> (o, lse or None)
-PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// paged_tree_attention: the same with parents in the place of causal
+template <bool TREE>
+PyObject* attention(PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 16 || !is_tensor(a[0])) Py_RETURN_NONE;
     const at::Tensor& q = tensor_of(a[0]);
@@ -150,14 +163,20 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if ((type != FTK_F16 && type != FTK_BF16) || !cache_of(a + 1, q.size(0), &c) || !on(a[1], q)) Py_RETURN_NONE;
     if ((c.pages.type == FTK_F16 || c.pages.type == FTK_BF16) && c.pages.type != type) Py_RETURN_NONE;
     if (!strided(a[0], q.scalar_type(), q, 0, c.pages.head_size, &st)) Py_RETURN_NONE;
-    double scale = 1.0 / std::sqrt((double)c.pages.head_size);
-    if (a[8] != Py_None) {
-      if (!PyFloat_Check(a[8]) && !PyLong_Check(a[8])) Py_RETURN_NONE;
-      scale = PyFloat_AsDouble(a[8]);
+    double scale;
+    if (!scale_of(a[8], c.pages.head_size, &scale)) {
       if (PyErr_Occurred()) return nullptr;
+      Py_RETURN_NONE;
+    }
+    const int* parents = nullptr;
+    if constexpr (TREE) {
+      if (!plain_on(a[9], at::kInt, q) || tensor_of(a[9]).dim() != 1 || tensor_of(a[9]).size(0) != q.size(0)) Py_RETURN_NONE;
+      parents = (const int*)tensor_of(a[9]).data_ptr();
+    } else if (a[9] != Py_True && a[9] != Py_False) {
+      Py_RETURN_NONE;
     }
     int window, max_queries, max_keys;
-    if ((a[9] != Py_True && a[9] != Py_False) || !number(a[10], &window) || !number(a[11], &max_queries) || !number(a[12], &max_keys)) Py_RETURN_NONE;
+    if (!number(a[10], &window) || !number(a[11], &max_queries) || !number(a[12], &max_keys)) Py_RETURN_NONE;
     at::Tensor o, lse, ws;
     if (a[13] == Py_None) {
       o = empty(q.sizes(), q.scalar_type(), q);
@@ -177,15 +196,17 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (a[15] != Py_None) {
       if (!on(a[15], q) || !tensor_of(a[15]).is_contiguous()) Py_RETURN_NONE;
       ws = tensor_of(a[15]);
-    } else if (const size_t need = ftk_paged_attn_workspace_bytes(&c.pages, &c.batch, heads, window, max_queries, max_keys)) {
+    } else if (const size_t need = (TREE ? ftk_paged_tree_attn_workspace_bytes : ftk_paged_attn_workspace_bytes)(&c.pages, &c.batch, heads, window, max_queries, max_keys)) {
       ws = empty({(int64_t)need}, at::kByte, q);
     }
-    if (!count("paged_attention")) return nullptr;
+    if (!count(TREE ? "paged_tree_attention" : "paged_attention")) return nullptr;
     void *const op = o.data_ptr(), *const wp = ws.defined() && ws.nbytes() ? ws.data_ptr() : nullptr, *const s = stream();
     float* const lp = lse.defined() ? (float*)lse.data_ptr() : nullptr;
     const size_t bytes = wp ? ws.nbytes() : 0;
     const bool causal = a[9] == Py_True;
     const int rc = in_library([&] {
+      if constexpr (TREE)
+        return ftk_paged_tree_attn(st.data, type, st.token, st.head, &c.pages, &c.batch, parents, op, lp, heads, (float)scale, window, max_queries, max_keys, wp, bytes, s);
       return ftk_paged_attn(st.data, type, st.token, st.head, &c.pages, &c.batch, op, lp, heads, (float)scale, causal, window, max_queries, max_keys, wp, bytes, s);
     });
     if (rc) return raise(rc);
@@ -199,6 +220,140 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       PyTuple_SET_ITEM(both, 1, Py_None);
     }
     return both;
+  });
+}
+
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) { return attention<false>(a, n); }
+PyObject* paged_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) { return attention<true>(a, n); }
+
+// kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps, scale or None, decay, causal, window, max_keys) -> True
+PyObject* kv_cache_weigh(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 13 || !is_tensor(a[0])) Py_RETURN_NONE;
+    const at::Tensor& q = tensor_of(a[0]);
+    if (!q.is_cuda() || q.dim() != 3 || !small(q.size(1))) Py_RETURN_NONE;
+    const int type = type_code(q.scalar_type());
+    PyObject* const batch[] = {a[2], a[2], a[4], a[5], a[6], a[7], a[7]};
+    Cache c;
+    Strided st;
+    if ((type != FTK_F16 && type != FTK_BF16) || !cache_of(batch, q.size(0), &c) || !on(a[2], q)) Py_RETURN_NONE;
+    if ((c.pages.type == FTK_F16 || c.pages.type == FTK_BF16) && c.pages.type != type) Py_RETURN_NONE;
+    if (!strided(a[0], q.scalar_type(), q, 0, c.pages.head_size, &st)) Py_RETURN_NONE;
+    if (!plain_on(a[1], at::kFloat, q) || !plain_on(a[3], at::kFloat, q)) Py_RETURN_NONE;
+    const at::Tensor &lse = tensor_of(a[1]), &weights = tensor_of(a[3]), &keys = tensor_of(a[2]);
+    if (lse.dim() != 2 || lse.size(0) != q.size(0) || lse.size(1) != q.size(1)) Py_RETURN_NONE;
+    if (weights.dim() != 3 || weights.size(0) != keys.size(0) || weights.size(1) != keys.size(1) || weights.size(2) != keys.size(2)) Py_RETURN_NONE;
+    double scale;
+    if (!scale_of(a[8], c.pages.head_size, &scale)) {
+      if (PyErr_Occurred()) return nullptr;
+      Py_RETURN_NONE;
+    }
+    int window, max_keys;
+    if (!PyFloat_Check(a[9]) || (a[10] != Py_True && a[10] != Py_False) || !number(a[11], &window) || !number(a[12], &max_keys)) Py_RETURN_NONE;
+    const float decay = (float)PyFloat_AS_DOUBLE(a[9]);
+    const bool causal = a[10] == Py_True;
+    if (!count("kv_cache_weigh")) return nullptr;
+    const c10::DeviceGuard guard(q.device());
+    const float* const lp = (const float*)lse.data_ptr();
+    float* const wp = (float*)weights.data_ptr();
+    void* const s = stream();
+    const int heads = dim(q, 1);
+    const int rc = in_library(
+        [&] { return ftk_kv_cache_weigh(st.data, type, st.token, st.head, lp, &c.pages, wp, &c.batch, heads, (float)scale, decay, causal, window, max_keys, s); });
+    if (rc) return raise(rc);
+    Py_RETURN_TRUE;
+  });
+}
+
+// kv_cache_select(weights, table, lens, budget, sinks, recent, max_keys) -> kept
+PyObject* kv_cache_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 7 || !plain(a[0], at::kFloat)) Py_RETURN_NONE;
+    const at::Tensor& weights = tensor_of(a[0]);
+    if (!plain_on(a[1], at::kInt, weights) || !plain_on(a[2], at::kInt, weights)) Py_RETURN_NONE;
+    const at::Tensor &table = tensor_of(a[1]), &lens = tensor_of(a[2]);
+    if (weights.dim() != 3 || table.dim() != 2 || lens.dim() != 1 || table.size(0) != lens.size(0) || !small(table.size(0)) || !small(table.size(1))) Py_RETURN_NONE;
+    for (int i = 0; i < 3; ++i)
+      if (!small(weights.size(i))) Py_RETURN_NONE;
+    int budget, sinks, recent, max_keys;
+    if (!number(a[3], &budget) || !number(a[4], &sinks) || !number(a[5], &recent) || !number(a[6], &max_keys)) Py_RETURN_NONE;
+    const c10::DeviceGuard guard(weights.device());
+    at::Tensor kept = empty({table.size(0), weights.size(1), budget}, at::kInt, weights);
+    if (!count("kv_cache_select")) return nullptr;
+    const float* const wp = (const float*)weights.data_ptr();
+    const int *const tp = (const int*)table.data_ptr(), *const lp = (const int*)lens.data_ptr();
+    int* const kp = (int*)kept.data_ptr();
+    void* const s = stream();
+    const int rc = in_library([&] {
+      return ftk_kv_cache_select(wp, dim(weights, 0), dim(weights, 1), dim(weights, 2), tp, lp, dim(table, 0), dim(table, 1), budget, sinks, recent, max_keys, kp, s);
+    });
+    if (rc) return raise(rc);
+    return THPVariable_Wrap(std::move(kept));
+  });
+}
+
+// kv_cache_keep(k_pages, v_pages, table, lens, kept, starts or None, k_exps, v_exps, weights or None) -> lens
+PyObject* kv_cache_keep(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 9 || !is_tensor(a[0]) || !is_tensor(a[3]) || !plain_on(a[4], at::kInt, tensor_of(a[0]))) Py_RETURN_NONE;
+    const at::Tensor &pages = tensor_of(a[0]), &lens = tensor_of(a[3]), &kept = tensor_of(a[4]);
+    PyObject* const batch[] = {a[0], a[1], a[2], a[3], a[5], a[6], a[7]};
+    Cache c;
+    if (!cache_of(batch, 0, &c, false)) Py_RETURN_NONE;
+    const int64_t B = lens.size(0);
+    if ((kept.dim() != 2 && kept.dim() != 3) || kept.size(0) != B || (kept.dim() == 3 && kept.size(1) != pages.size(1)) || !small(kept.size(-1))) Py_RETURN_NONE;
+    float* wp = nullptr;
+    if (a[8] != Py_None) {
+      if (!plain_on(a[8], at::kFloat, pages)) Py_RETURN_NONE;
+      const at::Tensor& w = tensor_of(a[8]);
+      if (w.dim() != 3 || w.size(0) != pages.size(0) || w.size(1) != pages.size(1) || w.size(2) != pages.size(2)) Py_RETURN_NONE;
+      wp = (float*)w.data_ptr();
+    }
+    const c10::DeviceGuard guard(pages.device());
+    at::Tensor out = empty({B}, at::kInt, pages);
+    if (!count("kv_cache_keep")) return nullptr;
+    const int* const kp = (const int*)kept.data_ptr();
+    int* const op = (int*)out.data_ptr();
+    void* const s = stream();
+    const int rc = in_library([&] {
+      return ftk_kv_cache_keep(&c.pages, c.batch.table, c.batch.lens, c.batch.starts, c.batch.sequences, c.batch.table_width, kp, (int)kept.size(-1), kept.dim() == 3, wp, op, s);
+    });
+    if (rc) return raise(rc);
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// verify_tree(target [tokens,V], ids [tokens], parents [tokens], starts [B+1], uniforms [B,M]) -> (next, path, accepted)
+PyObject* verify_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 5 || !is_tensor(a[0]) || !is_tensor(a[1])) Py_RETURN_NONE;
+    const at::Tensor &target = tensor_of(a[0]), &ids = tensor_of(a[1]);
+    const int type = type_code(target.scalar_type());
+    const auto id_type = ids.scalar_type();
+    if ((type != FTK_F16 && type != FTK_BF16 && type != FTK_F32) || !plain(a[0], target.scalar_type()) || target.dim() != 2) Py_RETURN_NONE;
+    if ((id_type != at::kInt && id_type != at::kLong) || !plain_on(a[1], id_type, target) || ids.dim() != 1) Py_RETURN_NONE;
+    if (!plain_on(a[2], at::kInt, target) || !plain_on(a[3], at::kInt, target) || !plain_on(a[4], at::kFloat, target)) Py_RETURN_NONE;
+    const at::Tensor &parents = tensor_of(a[2]), &starts = tensor_of(a[3]), &uniforms = tensor_of(a[4]);
+    const int64_t T = target.size(0), V = target.size(1);
+    if (ids.size(0) != T || parents.dim() != 1 || parents.size(0) != T || starts.dim() != 1 || starts.size(0) < 1 || uniforms.dim() != 2) Py_RETURN_NONE;
+    const int64_t B = starts.size(0) - 1, M = uniforms.size(1);
+    if (uniforms.size(0) != B || !small(B) || !small(M) || !small(T) || !small(V)) Py_RETURN_NONE;
+    const c10::DeviceGuard guard(target.device());
+    at::Tensor next = empty({B, M}, id_type, target), path = empty({B, M}, at::kInt, target), accepted = empty({B}, at::kInt, target);
+    if (!count("verify_tree")) return nullptr;
+    const void *const tp = target.data_ptr(), *const ip = ids.data_ptr();
+    const int *const pp = (const int*)parents.data_ptr(), *const sp = (const int*)starts.data_ptr();
+    const float* const up = (const float*)uniforms.data_ptr();
+    void *const np = next.data_ptr(), *const s = stream();
+    int *const wp = (int*)path.data_ptr(), *const ap = (int*)accepted.data_ptr();
+    const int rc = in_library([&] { return ftk_verify_tree(tp, type, ip, id_type == at::kLong, pp, sp, up, np, wp, ap, (int)B, (int)T, (int)M, (int)V, s); });
+    if (rc) return raise(rc);
+    PyObject* all = PyTuple_New(3);
+    if (!all) return nullptr;
+    PyTuple_SET_ITEM(all, 0, THPVariable_Wrap(std::move(next)));
+    PyTuple_SET_ITEM(all, 1, THPVariable_Wrap(std::move(path)));
+    PyTuple_SET_ITEM(all, 2, THPVariable_Wrap(std::move(accepted)));
+    return all;
   });
 }
 
@@ -261,6 +416,13 @@ PyMethodDef methods[] = {
      "kv_cache_read(like, k_pages, v_pages, table, lens, starts, k_exps, v_exps, tokens, keys, values)"},
     {"paged_attention", (PyCFunction)(void*)paged_attention, METH_FASTCALL,
      "paged_attention(q, k_pages, v_pages, table, lens, starts, k_exps, v_exps, scale, causal, window, max_queries, max_keys, out, lse, workspace)"},
+    {"paged_tree_attention", (PyCFunction)(void*)paged_tree_attention, METH_FASTCALL,
+     "paged_tree_attention(q, k_pages, v_pages, table, lens, starts, k_exps, v_exps, scale, parents, window, max_queries, max_keys, out, lse, workspace)"},
+    {"kv_cache_weigh", (PyCFunction)(void*)kv_cache_weigh, METH_FASTCALL,
+     "kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps, scale, decay, causal, window, max_keys)"},
+    {"kv_cache_select", (PyCFunction)(void*)kv_cache_select, METH_FASTCALL, "kv_cache_select(weights, table, lens, budget, sinks, recent, max_keys)"},
+    {"kv_cache_keep", (PyCFunction)(void*)kv_cache_keep, METH_FASTCALL, "kv_cache_keep(k_pages, v_pages, table, lens, kept, starts, k_exps, v_exps, weights)"},
+    {"verify_tree", (PyCFunction)(void*)verify_tree, METH_FASTCALL, "verify_tree(target, ids, parents, starts, uniforms)"},
     {"verify_drafts", (PyCFunction)(void*)verify_drafts, METH_FASTCALL, "verify_drafts(target, draft, drafts, accept, sample, lens, workspace)"},
     {nullptr, nullptr, 0, nullptr}};
 

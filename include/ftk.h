@@ -748,6 +748,109 @@ int ftk_verify_drafts(const void* target, const void* draft, int type,
                       void* workspace, size_t workspace_bytes,
                       ftk_stream_t stream);
 
+/*
+ * ftk_paged_attn for new tokens that form a tree of drafts: parents [tokens] int32 says
+ * for each packed row which of its sequence's new tokens, counted from 0, it
+ * follows; a negative number: none, it follows the cache itself.  A parent comes before
+ * its children; a number that does not counts as none.  The new tokens are the last positions
+ * of the sequence in the order of their rows (which is where ftk_kv_cache_write puts
+ * them), and each sees the positions in front of the new tokens, its ancestors and
+ * itself.  window > 0: of these the last `window` on the way that ends with it; a
+ * token d steps below a root counts as d positions behind the first new one's.
+ * All else is as in ftk_paged_attn.  A sequence has at most 256 new tokens: max_queries
+ * promises it, or `tokens` is no larger.
+ */
+size_t ftk_paged_tree_attn_workspace_bytes(const ftk_kv_pages* pages,
+                                           const ftk_kv_batch* batch,
+                                           int heads, int window,
+                                           int max_queries, int max_keys);
+int ftk_paged_tree_attn(const void* q, int type, long long q_token_stride,
+                        long long q_head_stride, const ftk_kv_pages* pages,
+                        const ftk_kv_batch* batch, const int* parents, void* o,
+                        float* lse, int heads, float scale, int window,
+                        int max_queries, int max_keys, void* workspace,
+                        size_t workspace_bytes, ftk_stream_t stream);
+
+/*
+ * Verifies trees of drafted tokens against a target model.  The packed rows starts[b]
+ * .. starts[b + 1] - 1 are the tokens of sequence b: the first is the root, the
+ * last token that is known already, the others are drafts, parents [tokens] as in
+ * ftk_paged_tree_attn.  target [tokens, vocabulary] (fp32, fp16 or bf16): the target's
+ * probabilities of what follows each token; ids [tokens] int32 or int64 (that of a
+ * root is not looked at); uniforms [sequences, most] fp32 of [0, 1).  Beginning with
+ * the root, step i draws what follows the node from the target: the least t with
+ * sum_{k <= t} w_k > uniforms[b, i] * sum_k w_k, w the node's row, sums in 64 bits in a
+ * fixed order, NaN and negative weights as zero (no positive weight: t = -1).  If
+ * the node has a child with that id (the first of them), the way goes on there; else,
+ * or after `most` steps, it ends.  What leaves this way is distributed as
+ * the target's own, however the drafts were chosen, if they do not depend on the uniform numbers.
+ * next [sequences, most], of ids' type: the tokens that were drawn, of which all but the
+ * last are accepted drafts, then -1; path [sequences, most] int32: the nodes, counted from
+ * 0 in their sequence, that they follow, which stay in the cache
+ * (ftk_kv_cache_keep), then -1; accepted [sequences] int32: how many drafts were
+ * accepted, one less than the nodes of the path, or 0.  A sequence without tokens gets -1
+ * everywhere.  most is 1 to 64.
+ */
+int ftk_verify_tree(const void* target, int type, const void* ids,
+                    int ids_are_64bit, const int* parents, const int* starts,
+                    const float* uniforms, void* next, int* path, int* accepted,
+                    int sequences, int tokens, int most, int vocabulary,
+                    ftk_stream_t stream);
+
+/*
+ * Adds up what new tokens give to each position of the cache.  lse [tokens, heads]
+ * fp32 as ftk_paged_attn leaves it for the same q, scale, causal and window.  weights
+ * [pages->pages, pages->heads, pages->page_size] fp32, 4-byte aligned, beside the keys:
+ * for every position k < lens[b] of a sequence with new tokens and each head of keys
+ *   weights = before + sum exp(scale * q . k_k - lse)
+ * over the new tokens that see k and the query heads that read this head; before is
+ * decay * weights (0 <= decay <= 1) where k is older than the new tokens, and 0 for the
+ * new ones' own positions and with a decay of 0, where what the array held is not read.
+ * A row whose lse is -inf gives nothing; an lse of NaN, or a key that is not finite, makes
+ * NaN or zero of the positions that it is seen at, and of no others.  Sequences without new tokens,
+ * and what is no position of a sequence, are left alone.  pages->v and v_exps are not
+ * looked at.  Codes of 8 bits count as their exact values.  fp32 sums in an order that depends on
+ * the sizes of the call alone.  max_keys promises that no sequence is longer (0: no
+ * promise).  A page belongs to one place of the table.
+ */
+int ftk_kv_cache_weigh(const void* q, int type, long long q_token_stride,
+                       long long q_head_stride, const float* lse,
+                       const ftk_kv_pages* pages, float* weights,
+                       const ftk_kv_batch* batch, int heads, float scale,
+                       float decay, int causal, int window, int max_keys,
+                       ftk_stream_t stream);
+
+/*
+ * Which positions of each sequence and head stay in a cache of `budget` positions:
+ * the first `sinks`, the last `recent` and, of the others, those of the largest
+ * weights [pages, heads, page_size] (16-byte aligned), of equal ones the earlier; both zeros are equal, a
+ * NaN, and a position whose page does not exist, is below everything.  A sequence
+ * of no more than `budget` positions stays as it is.  kept [sequences, heads, budget] int32: the positions
+ * that stay, ascending, then -1.  max_keys: as above, it only decides which kernel runs.
+ */
+int ftk_kv_cache_select(const float* weights, int pages, int heads,
+                        int page_size, const int* table, const int* lens,
+                        int sequences, int table_width, int budget, int sinks,
+                        int recent, int max_keys, int* kept,
+                        ftk_stream_t stream);
+
+/*
+ * Moves the rows that stay together, in place: keys, values, exponents and, if not
+ * NULL, weights [pages, heads, page_size] fp32 of position first + kept[j] go to position first + j.
+ * first is 0, or with starts [sequences + 1] not NULL the position of the sequence's first
+ * new token (so that a path of ftk_verify_tree is a list).  kept: [sequences, most] int32 for all heads alike, or
+ * with per_head [sequences, heads, most]; a list ascends strictly and ends at its first
+ * negative entry, behind which all are negative.  new_lens [sequences] int32: first and how many stay (by the
+ * first head's list; the lists of a sequence's heads are of one length), which is
+ * another array than lens.  Rows that are not written to stay as they are.  Positions from lens[b] on, or without a page, are neither
+ * read nor written; a list that does not ascend leaves its rows open, and nothing else.  A page belongs to one
+ * place of the table.
+ */
+int ftk_kv_cache_keep(const ftk_kv_pages* pages, const int* table,
+                      const int* lens, const int* starts, int sequences,
+                      int table_width, const int* kept, int most, int per_head,
+                      float* weights, int* new_lens, ftk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
