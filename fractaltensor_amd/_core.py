@@ -32,7 +32,7 @@ EXPORTS = (
     'ftk_b2b_gemm_f16', 'ftk_b2b_gemm_f16_supported', 'ftk_b2b_gemm_rowmajor_f16', 'ftk_gemm_f16', 'ftk_batched_gemm_f16', 'ftk_flash_attn_f16', 'ftk_flash_attn_f16_workspace_bytes', 'ftk_flash_attn_ws_f16', 'ftk_flash_attn_f32_workspace_bytes', 'ftk_flash_attn_f32', 'ftk_online_softmax_f32', 'ftk_embedding_gather_f32',
     'ftk_grid_rnn_workspace_bytes', 'ftk_grid_rnn_f32', 'ftk_windowed_attn_f32',
     'ftk_kv_cache_write', 'ftk_kv_cache_read', 'ftk_paged_attn_workspace_bytes', 'ftk_paged_attn', 'ftk_verify_drafts_workspace_bytes', 'ftk_verify_drafts',
-    'ftk_paged_tree_attn_workspace_bytes', 'ftk_paged_tree_attn', 'ftk_verify_tree', 'ftk_kv_cache_weigh', 'ftk_kv_cache_select', 'ftk_kv_cache_keep',
+    'ftk_paged_tree_attn_workspace_bytes', 'ftk_paged_tree_attn', 'ftk_verify_tree', 'ftk_kv_cache_weigh_workspace_bytes', 'ftk_kv_cache_weigh', 'ftk_kv_cache_select', 'ftk_kv_cache_keep',
 )
 
 
@@ -92,12 +92,15 @@ def _load() -> ctypes.CDLL:
     lib.ftk_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(KvPages), ctypes.POINTER(KvBatch)] + [ctypes.c_int] * 4
     lib.ftk_paged_tree_attn_workspace_bytes.restype = ctypes.c_size_t
     lib.ftk_paged_tree_attn_workspace_bytes.argtypes = lib.ftk_paged_attn_workspace_bytes.argtypes
+    lib.ftk_kv_cache_weigh_workspace_bytes.restype = ctypes.c_size_t
+    lib.ftk_kv_cache_weigh_workspace_bytes.argtypes = [ctypes.POINTER(KvPages), ctypes.POINTER(KvBatch)] + [ctypes.c_int] * 3
     lib.ftk_verify_drafts_workspace_bytes.restype = ctypes.c_size_t
     lib.ftk_verify_drafts_workspace_bytes.argtypes = [ctypes.c_int] * 2
     for name in EXPORTS:
         if name not in ('ftk_last_error', 'ftk_stacked_lstm_workspace_bytes', 'ftk_stacked_lstm_f16_workspace_bytes', 'ftk_grid_rnn_workspace_bytes',
                         'ftk_flash_attn_f32_workspace_bytes', 'ftk_flash_attn_f16_workspace_bytes', 'ftk_paged_attn_workspace_bytes',
-                        'ftk_verify_drafts_workspace_bytes', 'ftk_paged_tree_attn_workspace_bytes'):
+                        'ftk_verify_drafts_workspace_bytes', 'ftk_paged_tree_attn_workspace_bytes',
+                        'ftk_kv_cache_weigh_workspace_bytes'):
             getattr(lib, name).restype = ctypes.c_int
     return lib
 
@@ -1067,19 +1070,28 @@ def _req_weights(weights, pages, device) -> None:
         raise ValueError(f'weights must be [pages, kv heads, page size], got {tuple(weights.shape)}')
 
 
+def kv_cache_weigh_workspace_bytes(q, k_pages, table, max_queries: int = 0, max_keys: int = 0) -> int:
+    """Bytes that kv_cache_weigh wants for a batch of this shape on the device of q; 0 where the rows are not cut into parts."""
+    pages = KvPages(None, None, None, None, KV_TYPES[k_pages.dtype], *k_pages.shape)
+    batch = KvBatch(None, None, None, table.shape[0], table.shape[1], q.shape[0])
+    with torch.cuda.device(q.device):
+        return int(lib.ftk_kv_cache_weigh_workspace_bytes(ctypes.byref(pages), ctypes.byref(batch), q.shape[1], max_queries, max_keys))
+
+
 def kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps=None, scale: Optional[float] = None, decay: float = 1.0, causal: bool = True,
-                   window: int = 0, max_queries: int = 0, max_keys: int = 0) -> None:
+                   window: int = 0, max_queries: int = 0, max_keys: int = 0, workspace: Optional[torch.Tensor] = None) -> None:
     """Adds to weights, of every position of the sequences that have new tokens, the attention weights that these give it: the sum of exp(scale q . k - lse) over
     the new tokens that see it and the query heads that read its head.  q [tokens, heads, D] and lse [tokens, heads] as in, and out of, paged_attention
-    with the same scale, causal and window.  What older positions had is multiplied by decay (0 to 1) first, new ones begin at zero.  max_keys: the greatest
-    length where the program knows it.  (max_queries is taken so that the two calls can be given the same numbers.)"""
+    with the same scale, causal and window.  What older positions had is multiplied by decay (0 to 1) first, new ones begin at zero.  max_queries, max_keys: as in
+    paged_attention.  The workspace (kv_cache_weigh_workspace_bytes) is allocated here unless one is given."""
     decay = decay if isinstance(decay, float) else float(decay)
-    if _serving.kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps, scale, decay, causal, window, max_keys):
+    if _serving.kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps, scale, decay, causal, window, max_queries, max_keys, workspace):
         return
-    _req_attention(q, (k_pages, k_pages, table, lens, starts, k_exps, k_exps), None, None, None, window=window, max_keys=max_keys)
+    _req_attention(q, (k_pages, k_pages, table, lens, starts, k_exps, k_exps), None, None, workspace, window=window, max_queries=max_queries, max_keys=max_keys)
     _req_on(lse, torch.float32, q.shape[:2], q.device, 'lse')
     _req_weights(weights, k_pages.shape[:3], q.device)
-    if not _serving.kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps, None if scale is None else float(scale), decay, bool(causal), window, max_keys):
+    if not _serving.kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps, None if scale is None else float(scale), decay, bool(causal), window, max_queries, max_keys,
+                                   workspace):
         raise ValueError('kv_cache_weigh: these arguments are not taken')
 
 

@@ -226,10 +226,10 @@ PyObject* attention(PyObject* const* a, Py_ssize_t n) {
 PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) { return attention<false>(a, n); }
 PyObject* paged_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) { return attention<true>(a, n); }
 
-// kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps, scale or None, decay, causal, window, max_keys) -> True
+// kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps, scale or None, decay, causal, window, max_queries, max_keys, workspace or None) -> True
 PyObject* kv_cache_weigh(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    if (n != 13 || !is_tensor(a[0])) Py_RETURN_NONE;
+    if (n != 15 || !is_tensor(a[0])) Py_RETURN_NONE;
     const at::Tensor& q = tensor_of(a[0]);
     if (!q.is_cuda() || q.dim() != 3 || !small(q.size(1))) Py_RETURN_NONE;
     const int type = type_code(q.scalar_type());
@@ -248,18 +248,28 @@ PyObject* kv_cache_weigh(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (PyErr_Occurred()) return nullptr;
       Py_RETURN_NONE;
     }
-    int window, max_keys;
-    if (!PyFloat_Check(a[9]) || (a[10] != Py_True && a[10] != Py_False) || !number(a[11], &window) || !number(a[12], &max_keys)) Py_RETURN_NONE;
+    int window, max_queries, max_keys;
+    if (!PyFloat_Check(a[9]) || (a[10] != Py_True && a[10] != Py_False) || !number(a[11], &window) || !number(a[12], &max_queries) || !number(a[13], &max_keys)) Py_RETURN_NONE;
     const float decay = (float)PyFloat_AS_DOUBLE(a[9]);
     const bool causal = a[10] == Py_True;
-    if (!count("kv_cache_weigh")) return nullptr;
+    const int heads = dim(q, 1);
     const c10::DeviceGuard guard(q.device());
+    at::Tensor ws;
+    if (a[14] != Py_None) {
+      if (!on(a[14], q) || !tensor_of(a[14]).is_contiguous()) Py_RETURN_NONE;
+      ws = tensor_of(a[14]);
+    } else if (const size_t need = ftk_kv_cache_weigh_workspace_bytes(&c.pages, &c.batch, heads, max_queries, max_keys)) {
+      ws = empty({(int64_t)need}, at::kByte, q);
+    }
+    if (!count("kv_cache_weigh")) return nullptr;
+    void* const room = ws.defined() && ws.nbytes() ? ws.data_ptr() : nullptr;
+    const size_t bytes = room ? ws.nbytes() : 0;
     const float* const lp = (const float*)lse.data_ptr();
     float* const wp = (float*)weights.data_ptr();
     void* const s = stream();
-    const int heads = dim(q, 1);
-    const int rc = in_library(
-        [&] { return ftk_kv_cache_weigh(st.data, type, st.token, st.head, lp, &c.pages, wp, &c.batch, heads, (float)scale, decay, causal, window, max_keys, s); });
+    const int rc = in_library([&] {
+      return ftk_kv_cache_weigh(st.data, type, st.token, st.head, lp, &c.pages, wp, &c.batch, heads, (float)scale, decay, causal, window, max_queries, max_keys, room, bytes, s);
+    });
     if (rc) return raise(rc);
     Py_RETURN_TRUE;
   });
@@ -419,7 +429,7 @@ PyMethodDef methods[] = {
     {"paged_tree_attention", (PyCFunction)(void*)paged_tree_attention, METH_FASTCALL,
      "paged_tree_attention(q, k_pages, v_pages, table, lens, starts, k_exps, v_exps, scale, parents, window, max_queries, max_keys, out, lse, workspace)"},
     {"kv_cache_weigh", (PyCFunction)(void*)kv_cache_weigh, METH_FASTCALL,
-     "kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps, scale, decay, causal, window, max_keys)"},
+     "kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps, scale, decay, causal, window, max_queries, max_keys, workspace)"},
     {"kv_cache_select", (PyCFunction)(void*)kv_cache_select, METH_FASTCALL, "kv_cache_select(weights, table, lens, budget, sinks, recent, max_keys)"},
     {"kv_cache_keep", (PyCFunction)(void*)kv_cache_keep, METH_FASTCALL, "kv_cache_keep(k_pages, v_pages, table, lens, kept, starts, k_exps, v_exps, weights)"},
     {"verify_tree", (PyCFunction)(void*)verify_tree, METH_FASTCALL, "verify_tree(target, ids, parents, starts, uniforms)"},

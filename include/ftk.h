@@ -810,14 +810,21 @@ int ftk_verify_tree(const void* target, int type, const void* ids,
  * NaN or zero of the positions that it is seen at, and of no others.  Sequences without new tokens,
  * and what is no position of a sequence, are left alone.  pages->v and v_exps are not
  * looked at.  Codes of 8 bits count as their exact values.  fp32 sums in an order that depends on
- * the sizes of the call alone.  max_keys promises that no sequence is longer (0: no
- * promise).  A page belongs to one place of the table.
+ * the sizes of the call alone, workspace_bytes among them.  max_queries and max_keys promise that no
+ * sequence has more new tokens, or is longer (0: no promise); tokens beyond max_queries may
+ * be left out.  The workspace (16-byte aligned) holds the sums of parts of many rows; with NULL or less than
+ * ftk_kv_cache_weigh_workspace_bytes they are not cut, which costs time.  Calls that may run at the same time need
+ * workspaces of their own.  A page belongs to one place of the table.
  */
+size_t ftk_kv_cache_weigh_workspace_bytes(const ftk_kv_pages* pages,
+                                          const ftk_kv_batch* batch, int heads,
+                                          int max_queries, int max_keys);
 int ftk_kv_cache_weigh(const void* q, int type, long long q_token_stride,
                        long long q_head_stride, const float* lse,
                        const ftk_kv_pages* pages, float* weights,
                        const ftk_kv_batch* batch, int heads, float scale,
-                       float decay, int causal, int window, int max_keys,
+                       float decay, int causal, int window, int max_queries,
+                       int max_keys, void* workspace, size_t workspace_bytes,
                        ftk_stream_t stream);
 
 /*

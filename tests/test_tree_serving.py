@@ -35,9 +35,9 @@ def _tree(core, q=ONE, type=0, qt=256, heads=4, scale=1.0, window=0, mq=0, mk=0,
                                         ci(heads), cf(scale), ci(window), ci(mq), ci(mk), vp(ws), ctypes.c_size_t(n), NUL)
 
 
-def _weigh(core, q=ONE, type=0, qt=256, lse=ONE, weights=ONE, heads=4, scale=1.0, decay=1.0, window=0, mk=0, pages={}, batch={}):
+def _weigh(core, q=ONE, type=0, qt=256, lse=ONE, weights=ONE, heads=4, scale=1.0, decay=1.0, window=0, mq=0, mk=0, ws=None, n=0, pages={}, batch={}):
     return core.lib.ftk_kv_cache_weigh(vp(q), ci(type), cl(qt), cl(64), vp(lse), ctypes.byref(_pages(core, **pages)), vp(weights), ctypes.byref(_batch(core, **batch)), ci(heads),
-                                       cf(scale), cf(decay), ci(1), ci(window), ci(mk), NUL)
+                                       cf(scale), cf(decay), ci(1), ci(window), ci(mq), ci(mk), vp(ws), ctypes.c_size_t(n), NUL)
 
 
 def _keep(core, table=ONE, lens=ONE, starts=None, B=1, W=1, kept=ONE, most=4, per_head=0, weights=None, out=32, pages={}):
@@ -81,10 +81,11 @@ def test_bad_operands_of_attention_over_a_tree_are_refused(core):
 
 def test_bad_operands_of_weighing_are_refused(core):
     f = lambda **over: _weigh(core, **over)
-    assert f(heads=3) == -1 and f(heads=0) == -1 and f(type=1) == -1 and f(type=4) == -1 and f(window=-1) == -1 and f(mk=-1) == -1
+    assert f(heads=3) == -1 and f(heads=0) == -1 and f(type=1) == -1 and f(type=4) == -1 and f(window=-1) == -1 and f(mq=-1) == -1 and f(mk=-1) == -1
     assert f(scale=-1.0) == -1 and f(scale=math.inf) == -1 and f(scale=2.9e38) == -1
     assert f(decay=-0.1) == -1 and f(decay=1.1) == -1 and f(decay=math.nan) == -1 and b'decay' in core.lib.ftk_last_error()
-    assert f(q=None) == -1 and f(lse=None) == -1 and f(weights=None) == -1 and f(q=24) == -1 and f(lse=18) == -1 and f(weights=18) == -1 and f(qt=100) == -1
+    assert f(q=None) == -1 and f(lse=None) == -1 and f(weights=None) == -1 and f(q=24) == -1 and f(lse=18) == -1 and f(weights=18) == -1 and f(qt=100) == -1 and f(ws=24, n=100) == -1
+    assert core.lib.ftk_kv_cache_weigh_workspace_bytes(None, None, 1, 0, 0) == 0
     assert f(batch=dict(tokens=0), q=None, lse=None, weights=None) == 0
     assert f(pages=dict(v=None), batch=dict(tokens=0)) == 0                    # values are not looked at
 
