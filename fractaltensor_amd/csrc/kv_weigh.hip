@@ -554,7 +554,7 @@ struct RowCut {
 static RowCut cut_rows(long long pairs, long long most, long long most_rows, int cus, size_t room) {
   const long long tiles = std::max(1LL, (most + kBlock - 1) / kBlock);
   long long rows = 2048;
-  while (rows > 128 && pairs * tiles * ((most_rows + rows - 1) / rows) < 4 * cus) rows /= 2;
+  while (rows > 512 && pairs * tiles * ((most_rows + rows - 1) / rows) < 4 * cus) rows /= 2;
   const long long parts = (most_rows + rows - 1) / rows;
   if (parts <= 1 || pairs * tiles * parts > INT_MAX / 2 || (size_t)(pairs * tiles * parts * kBlock) > room / sizeof(float)) return {1, INT_MAX};
   return {(int)parts, (int)rows};
