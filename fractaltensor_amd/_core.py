@@ -32,7 +32,7 @@ EXPORTS = (
     'ftk_b2b_gemm_f16', 'ftk_b2b_gemm_f16_supported', 'ftk_b2b_gemm_rowmajor_f16', 'ftk_gemm_f16', 'ftk_batched_gemm_f16', 'ftk_flash_attn_f16', 'ftk_flash_attn_f16_workspace_bytes', 'ftk_flash_attn_ws_f16', 'ftk_flash_attn_f32_workspace_bytes', 'ftk_flash_attn_f32', 'ftk_online_softmax_f32', 'ftk_embedding_gather_f32',
     'ftk_grid_rnn_workspace_bytes', 'ftk_grid_rnn_f32', 'ftk_windowed_attn_f32',
     'ftk_kv_cache_write', 'ftk_kv_cache_read', 'ftk_paged_attn_workspace_bytes', 'ftk_paged_attn', 'ftk_verify_drafts_workspace_bytes', 'ftk_verify_drafts',
-    'ftk_paged_tree_attn_workspace_bytes', 'ftk_paged_tree_attn', 'ftk_verify_tree', 'ftk_kv_cache_weigh_workspace_bytes', 'ftk_kv_cache_weigh', 'ftk_kv_cache_select', 'ftk_kv_cache_keep',
+    'ftk_paged_tree_attn_workspace_bytes', 'ftk_paged_tree_attn', 'ftk_verify_tree_workspace_bytes', 'ftk_verify_tree', 'ftk_kv_cache_weigh_workspace_bytes', 'ftk_kv_cache_weigh', 'ftk_kv_cache_select', 'ftk_kv_cache_keep',
 )
 
 
@@ -92,6 +92,8 @@ def _load() -> ctypes.CDLL:
     lib.ftk_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(KvPages), ctypes.POINTER(KvBatch)] + [ctypes.c_int] * 4
     lib.ftk_paged_tree_attn_workspace_bytes.restype = ctypes.c_size_t
     lib.ftk_paged_tree_attn_workspace_bytes.argtypes = lib.ftk_paged_attn_workspace_bytes.argtypes
+    lib.ftk_verify_tree_workspace_bytes.restype = ctypes.c_size_t
+    lib.ftk_verify_tree_workspace_bytes.argtypes = [ctypes.c_int]
     lib.ftk_kv_cache_weigh_workspace_bytes.restype = ctypes.c_size_t
     lib.ftk_kv_cache_weigh_workspace_bytes.argtypes = [ctypes.POINTER(KvPages), ctypes.POINTER(KvBatch)] + [ctypes.c_int] * 3
     lib.ftk_verify_drafts_workspace_bytes.restype = ctypes.c_size_t
@@ -100,7 +102,7 @@ def _load() -> ctypes.CDLL:
         if name not in ('ftk_last_error', 'ftk_stacked_lstm_workspace_bytes', 'ftk_stacked_lstm_f16_workspace_bytes', 'ftk_grid_rnn_workspace_bytes',
                         'ftk_flash_attn_f32_workspace_bytes', 'ftk_flash_attn_f16_workspace_bytes', 'ftk_paged_attn_workspace_bytes',
                         'ftk_verify_drafts_workspace_bytes', 'ftk_paged_tree_attn_workspace_bytes',
-                        'ftk_kv_cache_weigh_workspace_bytes'):
+                        'ftk_kv_cache_weigh_workspace_bytes', 'ftk_verify_tree_workspace_bytes'):
             getattr(lib, name).restype = ctypes.c_int
     return lib
 
@@ -1032,7 +1034,7 @@ def paged_tree_attention(q, k_pages, v_pages, table, lens, starts, parents, k_ex
     return done[0] if done[1] is None else done
 
 
-def verify_tree(target, ids, parents, starts, uniforms) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def verify_tree(target, ids, parents, starts, uniforms, workspace: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The path through a tree of drafts that the target model's own draws follow, and the token behind it.
 
     The packed rows starts[b] .. starts[b + 1] - 1 are the tokens of sequence b: first the root, the last token that is known already, then the drafts.
@@ -1040,8 +1042,8 @@ def verify_tree(target, ids, parents, starts, uniforms) -> Tuple[torch.Tensor, t
     [B, M] fp32 of [0, 1), one for each step.  From the root on a token is drawn at each node; where the node has a child with it, the way goes on
     there.  Returns next [B, M] of ids' type (the tokens that were drawn: the accepted drafts and one more, then -1), path [B, M] int32 (the nodes that
     stay in the cache, by their number in the sequence, then -1: a list for kv_cache_keep) and accepted [B] int32.  The tokens are distributed as
-    the target's own, however the drafts were chosen."""
-    done = _serving.verify_tree(target, ids, parents, starts, uniforms)
+    the target's own, however the drafts were chosen.  The workspace (4 bytes a token) is allocated here unless one is given."""
+    done = _serving.verify_tree(target, ids, parents, starts, uniforms, workspace)
     if done is not None:
         return done
     if not isinstance(target, torch.Tensor) or not isinstance(ids, torch.Tensor):
@@ -1061,6 +1063,8 @@ def verify_tree(target, ids, parents, starts, uniforms) -> Tuple[torch.Tensor, t
     _req_on(uniforms, torch.float32, None, target.device, 'uniforms')
     if uniforms.dim() != 2 or uniforms.shape[0] != starts.shape[0] - 1:
         raise ValueError(f'uniforms must be [B, M] with B = {starts.shape[0] - 1}, got {tuple(uniforms.shape)}')
+    if workspace is not None:
+        _req_on(_req_workspace(workspace), workspace.dtype, None, target.device, 'workspace')
     raise ValueError('verify_tree: these arguments are not taken')
 
 

@@ -333,10 +333,10 @@ PyObject* kv_cache_keep(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// verify_tree(target [tokens,V], ids [tokens], parents [tokens], starts [B+1], uniforms [B,M]) -> (next, path, accepted)
+// verify_tree(target [tokens,V], ids [tokens], parents [tokens], starts [B+1], uniforms [B,M], workspace or None) -> (next, path, accepted)
 PyObject* verify_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    if (n != 5 || !is_tensor(a[0]) || !is_tensor(a[1])) Py_RETURN_NONE;
+    if (n != 6 || !is_tensor(a[0]) || !is_tensor(a[1])) Py_RETURN_NONE;
     const at::Tensor &target = tensor_of(a[0]), &ids = tensor_of(a[1]);
     const int type = type_code(target.scalar_type());
     const auto id_type = ids.scalar_type();
@@ -349,14 +349,22 @@ PyObject* verify_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t B = starts.size(0) - 1, M = uniforms.size(1);
     if (uniforms.size(0) != B || !small(B) || !small(M) || !small(T) || !small(V)) Py_RETURN_NONE;
     const c10::DeviceGuard guard(target.device());
+    at::Tensor ws;
+    if (a[5] != Py_None) {
+      if (!on(a[5], target) || !tensor_of(a[5]).is_contiguous()) Py_RETURN_NONE;
+      ws = tensor_of(a[5]);
+    } else {
+      ws = empty({(int64_t)ftk_verify_tree_workspace_bytes((int)T)}, at::kByte, target);
+    }
     at::Tensor next = empty({B, M}, id_type, target), path = empty({B, M}, at::kInt, target), accepted = empty({B}, at::kInt, target);
     if (!count("verify_tree")) return nullptr;
     const void *const tp = target.data_ptr(), *const ip = ids.data_ptr();
     const int *const pp = (const int*)parents.data_ptr(), *const sp = (const int*)starts.data_ptr();
     const float* const up = (const float*)uniforms.data_ptr();
-    void *const np = next.data_ptr(), *const s = stream();
+    void *const np = next.data_ptr(), *const s = stream(), *const room = ws.nbytes() ? ws.data_ptr() : nullptr;
+    const size_t bytes = room ? ws.nbytes() : 0;
     int *const wp = (int*)path.data_ptr(), *const ap = (int*)accepted.data_ptr();
-    const int rc = in_library([&] { return ftk_verify_tree(tp, type, ip, id_type == at::kLong, pp, sp, up, np, wp, ap, (int)B, (int)T, (int)M, (int)V, s); });
+    const int rc = in_library([&] { return ftk_verify_tree(tp, type, ip, id_type == at::kLong, pp, sp, up, np, wp, ap, (int)B, (int)T, (int)M, (int)V, room, bytes, s); });
     if (rc) return raise(rc);
     PyObject* all = PyTuple_New(3);
     if (!all) return nullptr;
@@ -432,7 +440,7 @@ PyMethodDef methods[] = {
      "kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps, scale, decay, causal, window, max_queries, max_keys, workspace)"},
     {"kv_cache_select", (PyCFunction)(void*)kv_cache_select, METH_FASTCALL, "kv_cache_select(weights, table, lens, budget, sinks, recent, max_keys)"},
     {"kv_cache_keep", (PyCFunction)(void*)kv_cache_keep, METH_FASTCALL, "kv_cache_keep(k_pages, v_pages, table, lens, kept, starts, k_exps, v_exps, weights)"},
-    {"verify_tree", (PyCFunction)(void*)verify_tree, METH_FASTCALL, "verify_tree(target, ids, parents, starts, uniforms)"},
+    {"verify_tree", (PyCFunction)(void*)verify_tree, METH_FASTCALL, "verify_tree(target, ids, parents, starts, uniforms, workspace)"},
     {"verify_drafts", (PyCFunction)(void*)verify_drafts, METH_FASTCALL, "verify_drafts(target, draft, drafts, accept, sample, lens, workspace)"},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -789,12 +789,16 @@ int ftk_paged_tree_attn(const void* q, int type, long long q_token_stride,
  * 0 in their sequence, that they follow, which stay in the cache
  * (ftk_kv_cache_keep), then -1; accepted [sequences] int32: how many drafts were
  * accepted, one less than the nodes of the path, or 0.  A sequence without tokens gets -1
- * everywhere.  most is 1 to 64.
+ * everywhere.  most is 1 to 64.  The workspace (16-byte aligned, ftk_verify_tree_workspace_bytes) lets
+ * small calls draw at all nodes at once; with NULL or less they are drawn at one behind the other, with the same
+ * results.  Calls that may run at the same time need workspaces of their own.
  */
+size_t ftk_verify_tree_workspace_bytes(int tokens);
 int ftk_verify_tree(const void* target, int type, const void* ids,
                     int ids_are_64bit, const int* parents, const int* starts,
                     const float* uniforms, void* next, int* path, int* accepted,
                     int sequences, int tokens, int most, int vocabulary,
+                    void* workspace, size_t workspace_bytes,
                     ftk_stream_t stream);
 
 /*

@@ -112,14 +112,15 @@ def test_bad_operands_of_keeping_are_refused(core):
 
 
 def test_bad_operands_of_the_verification_are_refused(core):
-    f = lambda target=ONE, type=4, ids=ONE, wide=0, parents=ONE, starts=ONE, u=ONE, out=ONE, path=ONE, acc=ONE, B=2, T=5, M=4, V=100: core.lib.ftk_verify_tree(
-        vp(target), ci(type), vp(ids), ci(wide), vp(parents), vp(starts), vp(u), vp(out), vp(path), vp(acc), ci(B), ci(T), ci(M), ci(V), NUL)
+    f = lambda target=ONE, type=4, ids=ONE, wide=0, parents=ONE, starts=ONE, u=ONE, out=ONE, path=ONE, acc=ONE, B=2, T=5, M=4, V=100, ws=None: core.lib.ftk_verify_tree(
+        vp(target), ci(type), vp(ids), ci(wide), vp(parents), vp(starts), vp(u), vp(out), vp(path), vp(acc), ci(B), ci(T), ci(M), ci(V), vp(ws), ctypes.c_size_t(1 << 20), NUL)
     assert f(B=-1) == -1 and f(T=-1) == -1 and f(V=0) == -1 and f(M=0) == -1
     assert f(M=65) == -2 and f(V=(1 << 30) + 1) == -2
     assert f(type=2) == -1 and f(type=3) == -1
     for name in ('target', 'ids', 'parents', 'starts', 'u', 'out', 'path', 'acc'):
         assert f(**{name: None}) == -1 and f(**{name: 18 if name != 'target' else 17}) == -1
-    assert f(ids=20, wide=1) == -1
+    assert f(ids=20, wide=1) == -1 and f(ws=24) == -1
+    assert core.lib.ftk_verify_tree_workspace_bytes(5) == 20 and core.lib.ftk_verify_tree_workspace_bytes(-1) == 0
     assert f(B=0) == 0
 
 

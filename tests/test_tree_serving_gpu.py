@@ -251,16 +251,18 @@ def _verify_case(core, dtype, new, V, M, seed, ids_type=torch.int64, kind='any',
     t = buffer[shift:].view(T, V)
     t.copy_(target)
     ids = ids.to(ids_type)
-    got = core.verify_tree(t, ids.cuda(), _ints(parents), _ints(starts), uniforms.cuda())
     want = ref.verify(target, ids, torch.tensor(parents), starts, uniforms)
-    for x, y, name in zip(got, want, ('next', 'path', 'accepted')):
-        assert x.dtype == y.dtype and torch.equal(x.cpu(), y), (name, x.cpu(), y)
+    for workspace in (None, torch.empty(0, dtype=torch.uint8, device='cuda')):       # drawn all at once where that is less, and one behind the other
+        got = core.verify_tree(t, ids.cuda(), _ints(parents), _ints(starts), uniforms.cuda(), workspace)
+        for x, y, name in zip(got, want, ('next', 'path', 'accepted')):
+            assert x.dtype == y.dtype and torch.equal(x.cpu(), y), (name, x.cpu(), y)
     return want
 
 
 @pytest.mark.parametrize('dtype', [F32, F16, BF16])
 @pytest.mark.parametrize('new,V,M,kind', [([1], 17, 1, 'any'), ([5, 0, 26, 1, 60], 1000, 7, 'any'), ([12, 30], 32000, 5, 'star'), ([9, 8, 7], 4099, 12, 'chain'), ([40, 3], 50257, 6, 'wild'),
-                                          ([20] * 5, 1, 4, 'any'), ([64], 131072, 3, 'any')])
+                                          ([20] * 5, 1, 4, 'any'), ([64], 131072, 3, 'any'),
+                                          ([600, 300], 500, 10, 'any'), ([700], 300, 20, 'star'), ([3, 2], 200003, 4, 'any')])
 def test_verified_trees(core, dtype, new, V, M, kind):
     want = _verify_case(core, dtype, new, V, M, 400 + V, kind=kind)
     if V > 1 and M > 2 and max(new) > 8:
