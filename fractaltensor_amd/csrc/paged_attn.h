@@ -730,17 +730,24 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_narrow_kernel(AttnArgs a
 // waves of a SIMD one feeds the matrix unit while the other works out weights.  A barrier ends every phase.  Waves 0 to 3 bring V(t + 1),
 // which is read from their M(t + 1) on, into one of three places, waves 4 to 7 K(t + 2) into that of K(t).  16-bit elements are copied straight into
 // LDS; codes of 8 bits go through registers, a tile earlier, and are written as 16-bit elements.
-constexpr int kWideWaves = 8, kWideRows = 32 * kWideWaves;
+//
+// PAIRED, for trees, most of which have 128 rows or fewer: waves 4 to 7 have the rows of waves 0 to 3, and every other tile, each half of them tiles of K and V
+// of its own; the two sums are joined at the end.
+constexpr int kWideWaves = 8, kWideRows = 32 * kWideWaves, kPairedRows = kWideRows / 2;
 constexpr float kMostSum = 32768.0f;          // a lane's sum of 32 weights above this moves the reference, to where it is at most 32 * 2^kLift
 
-template <int D>
+template <int D, bool PAIRED>
 struct WideShape {
   static constexpr int BYTES = 2 * D, TILE = 64 * BYTES;
+  static constexpr int ROWS = PAIRED ? kPairedRows : kWideRows;
   static constexpr int ORS = BYTES + 16;                       // a padded row of the O tiles that the waves turn round at the end
-  static constexpr int RING = 5 * TILE;                        // two tiles of K, three of V
-  static constexpr int LDS = RING + 64 > kWideWaves * 32 * ORS ? RING + 64 : kWideWaves * 32 * ORS;
+  static constexpr int RING = (PAIRED ? 8 : 5) * TILE;         // two tiles of K, three of V; PAIRED: two of each, twice
+  static constexpr int NOTES = PAIRED ? 2 * 2 * 16 : 64;       // of each place of V and wave
+  static constexpr int ENDS = kWideWaves * 32 * ORS;           // PAIRED: four waves' rows, and what the other four have of them
+  static constexpr int TILES_LDS = RING + NOTES > ENDS ? RING + NOTES : ENDS;
   static constexpr int WORDS = kTreeMost / 64 + 1;             // TREE, behind those: of each row, which new tokens it sees
-  static constexpr int TREE_LDS = LDS + kWideRows * WORDS * 8;
+  static constexpr int LDS = TILES_LDS + (PAIRED ? ROWS * WORDS * 8 : 0);
+  static_assert(!PAIRED || ROWS * ORS + ROWS * D * 4 + ROWS * 16 <= RING, "what waves 4 to 7 have summed lies in the ring, behind the rows");
 };
 
 // V: the transposing read of a 32-lane pass covers 4 keys x 64 bytes, which these bring into four different groups of 64 bytes
@@ -753,7 +760,8 @@ __device__ __forceinline__ int v_swizzle(int row) {
 
 template <typename T, KvFormat F, int D, bool TREE>
 __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, int kv_head, unsigned char* smem) {
-  using S = WideShape<D>;
+  constexpr bool PAIRED = TREE;
+  using S = WideShape<D, PAIRED>;
   using v8 = typename T::v8;
   using scalar = typename T::scalar;
   constexpr int DS = D / 16, DT = D / 32, CH = S::BYTES / 16;
@@ -767,13 +775,15 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = wave >> 2, cw = wave & 3;                   // which of the two run behind; whose 16 keys of a tile this wave brings
   const int jr = lane & 31, hh = lane >> 5;
-  unsigned char* const Kb = smem;
-  unsigned char* const Vb = smem + 2 * S::TILE;
+  unsigned char* const tiles = smem + (PAIRED ? half * (4 * S::TILE) : 0);
+  unsigned char* const Kb = tiles;
+  unsigned char* const Vb = tiles + 2 * S::TILE;
   const int base = j.lo & ~63;
   const int ntiles = j.hi > j.lo ? (j.hi - base + 63) / 64 : 0;
 
   // rows of this wave
-  const int wrow0 = j.row0 + 32 * wave;
+  const int in_rows = 32 * (PAIRED ? cw : wave);
+  const int wrow0 = j.row0 + in_rows;
   const bool idle = wrow0 >= j.rows;
   const int row = min(wrow0 + jr, j.rows - 1);
   const Row r = row_of<TREE>(a, j, kv_head, row);
@@ -788,11 +798,14 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   }
   int my_lo = max(r.lo, j.lo);
   const int my_hi = min(r.hi, j.hi);
-  // TREE: a row's bits for the 64 keys of a tile, in words that begin where tiles do
-  unsigned long long* const ways = reinterpret_cast<unsigned long long*>(smem + S::LDS) + (32 * wave + jr) * S::WORDS;
+  // TREE: which of the 64 keys of a tile a row sees; those of new tokens stand in words that begin where tiles do
+  unsigned long long* const ways = reinterpret_cast<unsigned long long*>(smem + S::TILES_LDS) + (in_rows + jr) * S::WORDS;
   auto way_of = [&](int t) __attribute__((always_inline)) {
-    const int word = (base + 64 * t - (j.first & ~63)) / 64;    // (both are multiples of 64)
-    return word < 0 ? ~0ULL : word < S::WORDS ? ways[word] : 0ULL;
+    const int key0 = base + 64 * t, word = (key0 - (j.first & ~63)) / 64;    // (both are multiples of 64)
+    const int lo = my_lo - key0, hi = my_hi - key0;
+    unsigned long long bits = word < 0 ? ~0ULL : word < S::WORDS ? ways[word] : 0ULL;
+    bits &= lo <= 0 ? ~0ULL : lo < 64 ? ~0ULL << lo : 0ULL;
+    return bits & (hi >= 64 ? ~0ULL : hi > 0 ? (1ULL << hi) - 1 : 0ULL);
   };
   auto sees = [&](int t) __attribute__((always_inline)) { return base + 64 * t < wave_hi && base + 64 * t + 64 > wave_lo; };
   auto masked = [&](int t) __attribute__((always_inline)) { return base + 64 * t < sure_lo || base + 64 * t + 64 > sure_hi; };
@@ -805,14 +818,21 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   }
   asm volatile("" ::: "memory");
 
-  // ---- tiles into LDS: a wave brings the 16 keys from 16 cw on, which lie in one page; waves 0 to 3 those of V, the others those of K
+  // ---- tiles into LDS: a wave brings the 16 keys from 16 cw on, which lie in one page; waves 0 to 3 those of V, the others those of K (PAIRED: each those of both)
   constexpr int CP = D / 32;                                   // 1 KB copies of 16 rows of 16-bit elements
   const int shift = a.pages.page_shift;
   const long long page_rows = (long long)a.pages.heads << shift;
   const long long head_row = (long long)kv_head << shift;
   const int* const table = a.batch.table + (long long)j.b * a.batch.width;
-  const unsigned char* const from = (half ? a.pages.k : a.pages.v) + head_row * (F == kSame ? S::BYTES : D);
-  const signed char* const from_exps = F == kSame ? nullptr : (half ? a.pages.k_exps : a.pages.v_exps) + head_row;
+  constexpr int LD = (D + 63) / 64;                            // 8 bits, 16 codes a lane: 16-byte pieces of a block of 16 rows, D of them, by 64 lanes
+  struct Bring {
+    bool keys;
+    const unsigned char* from;
+    const signed char* exps;
+    unsigned src[D == 96 ? CP : 1];
+    v4u codes[LD];
+    float scale[LD];
+  };
   // Cache row (from this head's first) of the 16 keys of this wave in tile t; of the nearest 16 in [lo, hi) where those lie outside (INSIDE: they
   // do not).
   auto block_at = [&](int t, auto inside_c) __attribute__((always_inline)) {
@@ -822,37 +842,40 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
     return page * page_rows + (key & ((1 << shift) - 1));
   };
   // Where a lane's 16 bytes of a copy lie: with 64 and 128 elements the swizzle makes copy i's places those of the first with some bits turned over.
-  unsigned src[D == 96 ? CP : 1];
+  auto begin = [&](Bring& b, bool of_keys) __attribute__((always_inline)) {
+    b.keys = of_keys;
+    b.from = (of_keys ? a.pages.k : a.pages.v) + head_row * (F == kSame ? S::BYTES : D);
+    b.exps = F == kSame ? nullptr : (of_keys ? a.pages.k_exps : a.pages.v_exps) + head_row;
 #pragma unroll
-  for (int i = 0; i < (D == 96 ? CP : 1); ++i) {
-    const int p = 64 * i + lane, rw = p / CH, slot = p - rw * CH, in_tile = 16 * cw + rw;
-    src[i] = rw * S::BYTES + 16 * (slot ^ (half ? swizzle<S::BYTES>(in_tile) : v_swizzle<D>(in_tile)));
-  }
-  const unsigned turned = half && D != 96 ? 64 : 0;
-  auto source = [&](int i) __attribute__((always_inline)) { return D == 96 ? src[D == 96 ? i : 0] : (src[0] ^ (i * turned)) + 1024 * i; };
+    for (int i = 0; i < (D == 96 ? CP : 1); ++i) {
+      const int p = 64 * i + lane, rw = p / CH, slot = p - rw * CH, in_tile = 16 * cw + rw;
+      b.src[i] = rw * S::BYTES + 16 * (slot ^ (of_keys ? swizzle<S::BYTES>(in_tile) : v_swizzle<D>(in_tile)));
+    }
+  };
+  auto source = [&](const Bring& b, int i) __attribute__((always_inline)) {
+    const unsigned turned = b.keys && D != 96 ? 64 : 0;
+    return D == 96 ? b.src[D == 96 ? i : 0] : (b.src[0] ^ (i * turned)) + 1024 * i;
+  };
   // 16 rows of tile t, `at` what block_at gave, into the tile at `to`
-  auto copy = [&](unsigned char* to, int t, long long at, auto inside_c) __attribute__((always_inline)) {
+  auto copy = [&](const Bring& b, unsigned char* to, int t, long long at, auto inside_c) __attribute__((always_inline)) {
     const int key0 = base + 64 * t + 16 * cw;
-    const unsigned char* const block = uniform(from + at * S::BYTES);
+    const unsigned char* const block = uniform(b.from + at * S::BYTES);
     unsigned char* const dst = to + cw * (16 * S::BYTES);
     if (decltype(inside_c)::value || (key0 >= j.lo && key0 + 16 <= j.hi)) {
 #pragma unroll
-      for (int i = 0; i < CP; ++i) lds_dma16(block, source(i), dst + 1024 * i);
+      for (int i = 0; i < CP; ++i) lds_dma16(block, source(b, i), dst + 1024 * i);
     } else {                                                   // rows outside [lo, hi) repeat the nearest key inside
       const int inside = min(max(key0, j.lo & ~15), (j.hi - 1) & ~15);   // where `at` begins
       const int least = max(j.lo - inside, 0), most = min(j.hi - 1 - inside, 15);
 #pragma unroll
       for (int i = 0; i < CP; ++i) {
         const int rw = (64 * i + lane) / CH;
-        lds_dma16(block, source(i) + (min(max(key0 + rw - inside, least), most) - rw) * S::BYTES, dst + 1024 * i);
+        lds_dma16(block, source(b, i) + (min(max(key0 + rw - inside, least), most) - rw) * S::BYTES, dst + 1024 * i);
       }
     }
   };
-  // 8 bits: 16 codes a lane
-  constexpr int LD = (D + 63) / 64;                            // 16-byte pieces of a block of 16 rows, D of them, by 64 lanes
-  v4u codes[LD];
-  float scale[LD];
-  auto load = [&](int t, long long at, auto inside_c) __attribute__((always_inline)) {
+  // 8 bits
+  auto load = [&](Bring& b, int t, long long at, auto inside_c) __attribute__((always_inline)) {
     const int key0 = base + 64 * t + 16 * cw;
     const int inside = min(max(key0, j.lo & ~15), (j.hi - 1) & ~15);
     const int least = max(j.lo - inside, 0), most = min(j.hi - 1 - inside, 15);
@@ -860,30 +883,33 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
     for (int i = 0; i < LD; ++i) {
       const int p = min(64 * i + lane, D - 1), rw = p / (D / 16), piece = p - rw * (D / 16);
       const long long row_at = at + (decltype(inside_c)::value ? rw : min(max(key0 + rw - inside, least), most));
-      codes[i] = *reinterpret_cast<const v4u*>(from + row_at * D + 16 * piece);
-      scale[i] = ldexpf(1.0f, from_exps[row_at]);
+      b.codes[i] = *reinterpret_cast<const v4u*>(b.from + row_at * D + 16 * piece);
+      b.scale[i] = ldexpf(1.0f, b.exps[row_at]);
     }
   };
-  auto store = [&](unsigned char* to) __attribute__((always_inline)) {
+  auto store = [&](const Bring& b, unsigned char* to) __attribute__((always_inline)) {
     if constexpr (F != kSame) {
 #pragma unroll
       for (int i = 0; i < LD; ++i) {
         const int p = 64 * i + lane, rw = p / (D / 16), piece = p - rw * (D / 16), in_tile = 16 * cw + rw;
-        const int swz = half ? swizzle<S::BYTES>(in_tile) : v_swizzle<D>(in_tile);
+        const int swz = b.keys ? swizzle<S::BYTES>(in_tile) : v_swizzle<D>(in_tile);
         auto put = [&](auto decode) __attribute__((always_inline)) {
           if (D % 64 == 0 || p < D) {
 #pragma unroll
             for (int c = 0; c < 2; ++c)
-              *reinterpret_cast<v8*>(to + in_tile * S::BYTES + 16 * ((2 * piece + c) ^ swz)) = decode(v2u{codes[i][2 * c], codes[i][2 * c + 1]}, scale[i]);
+              *reinterpret_cast<v8*>(to + in_tile * S::BYTES + 16 * ((2 * piece + c) ^ swz)) = decode(v2u{b.codes[i][2 * c], b.codes[i][2 * c + 1]}, b.scale[i]);
           }
         };
         // (the conversion of e4m3 rounds once whatever the scale)
         constexpr bool LOOK = std::is_same<T, Half>::value && F == kInt8;
-        if (LOOK && __builtin_expect(__builtin_amdgcn_ballot_w64(!(scale[i] >= 0x1p-24f && scale[i] <= 0x1p9f)) != 0, 0)) put(decode8_rounded<T, F>);
+        if (LOOK && __builtin_expect(__builtin_amdgcn_ballot_w64(!(b.scale[i] >= 0x1p-24f && b.scale[i] <= 0x1p9f)) != 0, 0)) put(decode8_rounded<T, F>);
         else put(decode8<T, F>);
       }
     }
   };
+  Bring mine, keys;                                            // PAIRED: V and K; else the one that this wave brings
+  begin(mine, PAIRED ? false : half != 0);
+  if constexpr (PAIRED) begin(keys, true);
 
   // ---- fragments: K row 32 h + jr, bytes [32 s + 16 hh, +16); V the block of 4 keys x 16 columns that 16 lanes hand in
   // (The swizzles touch bits of the chunk's index that are zero in a row's address, so that a step's offset is the first one's with some bits turned
@@ -948,7 +974,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int in = 32 * h + 8 * (e >> 2) + (e & 3), key = key0 + in;
-          if (key < my_lo || key >= my_hi || (TREE && !(drawn >> in & 1))) sc[h][e] = -INFINITY;
+          if (TREE ? !(drawn >> in & 1) : key < my_lo || key >= my_hi) sc[h][e] = -INFINITY;
         }
     }
     float psum = weights();
@@ -1002,8 +1028,8 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
     });
     __builtin_amdgcn_s_setprio(0);
   };
-  // Waves 0 to 3 look whether their 16 keys of a tile of V hold anything that is not finite, and leave word for all.
-  unsigned* const words = reinterpret_cast<unsigned*>(smem + S::RING);   // [three places of V][wave]
+  // Waves 0 to 3 (PAIRED: all) look whether their 16 keys of a tile of V hold anything that is not finite, and leave word for all.
+  unsigned* const words = reinterpret_cast<unsigned*>(smem + S::RING) + (PAIRED ? 8 * half : 0);   // [three places of V][wave]; PAIRED: [two][wave], twice
   auto look = [&](const unsigned char* vt, int place) __attribute__((always_inline)) {
     unsigned bad = 0;
 #pragma unroll
@@ -1028,7 +1054,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int in = 8 * (e >> 2) + (e & 3), key = key0 + in;
-        if (key >= my_lo && key < my_hi && (!TREE || (drawn >> in & 1))) seen |= 1u << e;
+        if (TREE ? (drawn >> in & 1) != 0 : key >= my_lo && key < my_hi) seen |= 1u << e;
       }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
@@ -1054,27 +1080,45 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   if (ntiles > 0) {
     // V(0) by waves 0 to 3, K(0) by the others, and K(1) behind it
     constexpr int AHEAD = F == kSame ? 0 : 1;                  // codes go through registers a tile earlier
-    if constexpr (F == kSame) {
-      copy(half ? Kb : Vb, 0, block_at(0, no{}), no{});
-      if (half && ntiles > 1) copy(Kb + S::TILE, 1, block_at(1, no{}), no{});
+    if constexpr (PAIRED) {                                    // (both halves; tiles behind the last hold the last keys once more)
+      const long long at0 = block_at(half, no{}), at1 = block_at(half + 2, no{});
+      if constexpr (F == kSame) {
+        copy(keys, Kb, half, at0, no{});
+        copy(mine, Vb, half, at0, no{});
+        copy(keys, Kb + S::TILE, half + 2, at1, no{});
+      } else {
+        Bring second = keys;
+        load(keys, half, at0, no{});
+        load(mine, half, at0, no{});
+        load(second, half + 2, at1, no{});
+        store(keys, Kb);
+        store(mine, Vb);
+        store(second, Kb + S::TILE);
+        load(mine, half + 2, at1, no{});
+        load(keys, half + 4, block_at(half + 4, no{}), no{});
+      }
+    } else if constexpr (F == kSame) {
+      copy(mine, half ? Kb : Vb, 0, block_at(0, no{}), no{});
+      if (half && ntiles > 1) copy(mine, Kb + S::TILE, 1, block_at(1, no{}), no{});
     } else {
-      load(0, block_at(0, no{}), no{});
-      store(half ? Kb : Vb);
-      if (ntiles > 1) load(1, block_at(1, no{}), no{});
+      load(mine, 0, block_at(0, no{}), no{});
+      store(mine, half ? Kb : Vb);
+      if (ntiles > 1) load(mine, 1, block_at(1, no{}), no{});
       if (half) {
-        if (ntiles > 1) store(Kb + S::TILE);
-        if (ntiles > 2) load(2, block_at(2, no{}), no{});
+        if (ntiles > 1) store(mine, Kb + S::TILE);
+        if (ntiles > 2) load(mine, 2, block_at(2, no{}), no{});
       }
     }
-    const int ahead = (half ? 2 : 1) + AHEAD;                  // S(t) asks for tile t + ahead
-    long long next = ahead < ntiles ? block_at(ahead, no{}) : 0;
+    const int ahead = PAIRED ? 2 * (2 + AHEAD) : (half ? 2 : 1) + AHEAD;          // S(t) asks for tile t + ahead; PAIRED: that one of K, the one before it of V
+    const int asked = (PAIRED ? half : 0) + ahead;
+    long long next = PAIRED || asked < ntiles ? block_at(asked, no{}) : 0;
     if constexpr (TREE) {
       unsigned long long bits[S::WORDS];
       int depth;
       const int before = j.first & 63;                         // keys in front of the new tokens in the first word
       walk_up<S::WORDS>(a, j, row / a.group, before, bits, &depth);
       bits[0] |= (1ULL << before) - 1;
-      if (hh == 0) {
+      if (hh == 0 && half == 0) {
 #pragma unroll
         for (int w = 0; w < S::WORDS; ++w) ways[w] = bits[w];
       }
@@ -1083,53 +1127,129 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
     __builtin_amdgcn_s_waitcnt(0x0F70);                        // vmcnt(0)
     __syncthreads();
     phase_m(Vb, Kb, no{}, yes{});
-    int vcur = 2 * S::TILE, vnext = 3 * S::TILE, vfree = 4 * S::TILE;             // V(t), V(t + 1), the place of V(t + 2)
-    int kcur = 0, knext = S::TILE;                                                // K(t), K(t + 1)
-    // Tiles [clean, dirty): every row sees all of them, and the tiles that they ask for lie inside [lo, hi)
-    const int whole = (j.hi - base) / 64;
-    const int clean = (max(j.sure_lo, j.lo) - base + 63) / 64, dirty = min((min(j.sure_hi, j.hi) - base) / 64, whole - 2 - AHEAD - 1);
-    auto turn = [&](int t, auto clean_c) __attribute__((always_inline)) {
-      constexpr bool CLEAN = decltype(clean_c)::value;
-      // K(t) was last read in the phase before this one, V(t - 2) two before
-      const int bring = t + ahead;
-      if constexpr (F == kSame) {
-        if (CLEAN || bring < ntiles) copy(smem + (half ? kcur : vnext), bring, next, clean_c);
-      } else {
-        if (CLEAN || bring - 1 < ntiles) store(smem + (half ? kcur : vnext));
-        if (CLEAN || bring < ntiles) load(bring, next, clean_c);
-      }
-      if (CLEAN || bring + 1 < ntiles) next = block_at(bring + 1, clean_c);
-      __builtin_amdgcn_sched_barrier(0);                       // the copies go out before the weights are begun
-      if (CLEAN || sees(t)) phase_s(t, clean_c);
-      if (!CLEAN && !half) look(smem + vcur, vcur / S::TILE - 2);
-      if constexpr (!CLEAN || F != kSame) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // what was written to LDS
-      phase_barrier();
-      const unsigned char *const vt = smem + vcur, *const kt = smem + knext;
-      if constexpr (CLEAN) {
-        phase_m(vt, kt, yes{}, yes{});
-      } else {
-        if (sees(t)) {
-          if (masked(t) && __builtin_expect(!all_finite(vcur / S::TILE - 2), 0)) careful_pv(vt, t);
-          else phase_m(vt, kt, yes{}, no{});
+    if constexpr (PAIRED) {
+      // What a turn asks for and puts away behind the last tile is that tile once more, and its scores go nowhere: code that runs once takes longer to fetch than to run.
+      phase_barrier();                                         // waves 0 to 3 are about to write where K(0) was read
+      int vcur = 2 * S::TILE, vnext = 3 * S::TILE, kcur = 0, knext = S::TILE;     // V(t), V(t + 2), K(t), K(t + 2)
+      long long behind = block_at(asked - 2, no{});
+      // Tiles [clean, dirty): every row sees all of them
+      const int clean = (max(j.sure_lo, j.lo) - base + 63) / 64, dirty = (min(j.sure_hi, j.hi) - base) / 64;
+      auto turn = [&](int t, auto clean_c) __attribute__((always_inline)) {
+        constexpr bool CLEAN = decltype(clean_c)::value;
+        const int bring = t + ahead;
+        if constexpr (F == kSame) {
+          copy(keys, tiles + kcur, bring, next, no{});
+          copy(mine, tiles + vnext, bring - 2, behind, no{});
+        } else {
+          store(keys, tiles + kcur);
+          store(mine, tiles + vnext);
+          load(keys, bring, next, no{});
+          load(mine, bring - 2, behind, no{});
         }
-        if (t + 1 < ntiles) phase_m(vt, kt, no{}, yes{});
+        behind = next;
+        next = block_at(bring + 2, no{});
+        __builtin_amdgcn_sched_barrier(0);                     // the copies go out before the weights are begun
+        const bool works = !idle && (CLEAN || t < ntiles);
+        if (works) phase_s(t, clean_c);
+        if (!CLEAN) look(tiles + vcur, vcur / S::TILE - 2);
+        if constexpr (!CLEAN || F != kSame) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // what was written to LDS
+        phase_barrier();
+        if (works) {
+          const unsigned char *const vt = tiles + vcur, *const kt = tiles + knext;
+          if constexpr (CLEAN) {
+            phase_m(vt, kt, yes{}, yes{});
+          } else {
+            if (masked(t) && __builtin_expect(!all_finite(vcur / S::TILE - 2), 0)) careful_pv(vt, t);
+            else phase_m(vt, kt, yes{}, no{});
+            phase_m(vt, kt, no{}, yes{});
+          }
+        }
+        if constexpr (F == kSame) __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the copies that this wave asked for in S(t)
+        phase_barrier();
+        const int k = kcur, v = vcur;
+        kcur = knext;
+        knext = k;
+        vcur = vnext;
+        vnext = v;
+      };
+      if (half) phase_barrier();
+      for (int t = half; t < ntiles + half; t += 2) {          // both halves take as many turns, the last of which may have no tile for waves 4 to 7
+        if (t >= clean)
+          for (; t < dirty; t += 2) turn(t, yes{});
+        if (t < ntiles + half) turn(t, no{});
       }
-      if constexpr (F == kSame) __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the copies that this wave asked for in S(t)
-      phase_barrier();
-      const int v = vcur, k = kcur;
-      vcur = vnext;
-      vnext = vfree;
-      vfree = v;
-      kcur = knext;
-      knext = k;
-    };
-    if (half) phase_barrier();
-    for (int t = 0; t < ntiles; ++t) {
-      if (t == clean)
-        for (; t < dirty; ++t) turn(t, yes{});
-      turn(t, no{});
+      if (!half) phase_barrier();
+    } else {
+      int vcur = 2 * S::TILE, vnext = 3 * S::TILE, vfree = 4 * S::TILE;           // V(t), V(t + 1), the place of V(t + 2)
+      int kcur = 0, knext = S::TILE;                                              // K(t), K(t + 1)
+      // Tiles [clean, dirty): every row sees all of them, and the tiles that they ask for lie inside [lo, hi)
+      const int whole = (j.hi - base) / 64;
+      const int clean = (max(j.sure_lo, j.lo) - base + 63) / 64, dirty = min((min(j.sure_hi, j.hi) - base) / 64, whole - 2 - AHEAD - 1);
+      auto turn = [&](int t, auto clean_c) __attribute__((always_inline)) {
+        constexpr bool CLEAN = decltype(clean_c)::value;
+        // K(t) was last read in the phase before this one, V(t - 2) two before
+        const int bring = t + ahead;
+        if constexpr (F == kSame) {
+          if (CLEAN || bring < ntiles) copy(mine, smem + (half ? kcur : vnext), bring, next, clean_c);
+        } else {
+          if (CLEAN || bring - 1 < ntiles) store(mine, smem + (half ? kcur : vnext));
+          if (CLEAN || bring < ntiles) load(mine, bring, next, clean_c);
+        }
+        if (CLEAN || bring + 1 < ntiles) next = block_at(bring + 1, clean_c);
+        __builtin_amdgcn_sched_barrier(0);                     // the copies go out before the weights are begun
+        if (CLEAN || sees(t)) phase_s(t, clean_c);
+        if (!CLEAN && !half) look(smem + vcur, vcur / S::TILE - 2);
+        if constexpr (!CLEAN || F != kSame) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // what was written to LDS
+        phase_barrier();
+        const unsigned char *const vt = smem + vcur, *const kt = smem + knext;
+        if constexpr (CLEAN) {
+          phase_m(vt, kt, yes{}, yes{});
+        } else {
+          if (sees(t)) {
+            if (masked(t) && __builtin_expect(!all_finite(vcur / S::TILE - 2), 0)) careful_pv(vt, t);
+            else phase_m(vt, kt, yes{}, no{});
+          }
+          if (t + 1 < ntiles) phase_m(vt, kt, no{}, yes{});
+        }
+        if constexpr (F == kSame) __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the copies that this wave asked for in S(t)
+        phase_barrier();
+        const int v = vcur, k = kcur;
+        vcur = vnext;
+        vnext = vfree;
+        vfree = v;
+        kcur = knext;
+        knext = k;
+      };
+      if (half) phase_barrier();
+      for (int t = 0; t < ntiles; ++t) {
+        if (t == clean)
+          for (; t < dirty; ++t) turn(t, yes{});
+        turn(t, no{});
+      }
+      if (!half) phase_barrier();
     }
-    if (!half) phase_barrier();
+  }
+  if constexpr (PAIRED) {                                      // waves 4 to 7 leave what they have, and waves 0 to 3 take it
+    v4f* const so = reinterpret_cast<v4f*>(smem + S::ROWS * S::ORS) + cw * (DT * 4 * 64) + lane;
+    float* const sml = reinterpret_cast<float*>(smem + S::ROWS * (S::ORS + D * 4)) + (cw * 64 + lane) * 2;
+    __syncthreads();
+    if (half) {
+#pragma unroll
+      for (int i = 0; i < DT * 4; ++i) so[64 * i] = v4f{o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1], o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]};
+      sml[0] = ref;
+      sml[1] = l;
+    }
+    __syncthreads();
+    if (half) return;
+    const float its = sml[0], top = fmaxf(ref, its), wa = __builtin_amdgcn_exp2f(ref - top), wb = __builtin_amdgcn_exp2f(its - top);
+    ref = top;
+    l = l * wa + sml[1] * wb;
+#pragma unroll
+    for (int i = 0; i < DT * 4; ++i) {
+      const v4f x = so[64 * i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i / 4][4 * (i % 4) + e] = o[i / 4][4 * (i % 4) + e] * wa + x[e] * wb;
+    }
   }
   l += __shfl_xor(l, 32);
   if (j.parts > 1) {
@@ -1179,6 +1299,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
 // 16384 of them, in int8: 165 us with all on the wide form, 108 so, and 12 for joining.)
 template <typename T, KvFormat F, int D, bool TREE>
 __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs a, int wide) {
+  constexpr int R = WideShape<D, TREE>::ROWS;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   Job j;
   if ((int)blockIdx.x >= wide) {
@@ -1197,7 +1318,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs
   const int id = blockIdx.x, kv_head = id % a.pages.heads, rest = id / a.pages.heads;
   const int slot = rest / a.cut.nparts, part = rest - slot * a.cut.nparts;
   int b, tile;
-  if (!find_rows<kWideRows>(a, slot, &b, &tile) || !find_job<kWideRows, TREE>(a, b, tile, part, false, j)) return;
+  if (!find_rows<R>(a, slot, &b, &tile) || !find_job<R, TREE>(a, b, tile, part, false, j)) return;
   wide_attention<T, F, D, TREE>(a, j, kv_head, smem);
 }
 
@@ -1206,20 +1327,18 @@ __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs
 constexpr int kPartsMost = 256;
 
 // The parts of the sequence that row `at` of the packed rows times heads belongs to (1: nothing to join), the first of them, and the keys [*lo, *hi) that the row
-// sees (in a tree at most; *lo below zero: its own key has no room).  first_token: that of the wave's first lane.
-template <bool TREE>
+// sees.  first_token: that of the wave's first lane.
 __device__ __forceinline__ int row_parts(const AttnArgs& a, long long at, int first_token, int* lo, int* hi, long long* first_of) {
   const int token = (int)(at / a.heads), head = (int)(at - (long long)token * a.heads);
   int b = count_at_most(a.batch.sequences, first_token, [&](int k) { return a.batch.starts[k + 1]; });
   while (b < a.batch.sequences && a.batch.starts[b + 1] <= token) ++b;
   if (b >= a.batch.sequences) return 1;
   const int start = min(max(a.batch.starts[b], 0), a.batch.tokens), end = min(max(a.batch.starts[b + 1], start), a.batch.tokens);
-  if (token < start || token >= end || (TREE && token - start >= kTreeMost)) return 1;
+  if (token < start || token >= end) return 1;
   const int all = max(a.batch.lens[b], 0), first = first_position(all, start, a.batch.starts[b + 1]), len = min(all, kv_capacity(a.batch, a.pages.page_shift));
   const long long position = (long long)first + (token - start);
-  *hi = TREE || a.causal ? clamp_position(position + 1, len) : len;
-  *lo = a.window > 0 ? clamp_position((TREE ? (long long)first : position) - a.window + 1, len) : 0;
-  if (TREE && position >= len) *lo = -1;
+  *hi = a.causal ? clamp_position(position + 1, len) : len;
+  *lo = a.window > 0 ? clamp_position(position - a.window + 1, len) : 0;
   const int kv_head = head / a.group;
   const bool small = (end - start) * a.group <= a.small_rows;
   *first_of = first_part(a, small, b, kv_head, (token - start) * a.group + head - kv_head * a.group, at);
@@ -1229,7 +1348,7 @@ __device__ __forceinline__ int row_parts(const AttnArgs& a, long long at, int fi
 // m = max m_p, l = sum l_p 2^(m_p - m), O = sum O_p 2^(m_p - m) / l over the parts of a row.  A wave (WAVES = 4: the four of a block) to a row: the
 // weights 2^(m_p - m) first, a lane a part, then the sums of O, D / 4 lanes a part, by loads that do not wait for one another.  A wave is given `rows` rows: one, or
 // many where only small sequences are cut and most waves find nothing to do.
-template <typename T, int D, int WAVES, bool TREE>
+template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) {
   constexpr int L = D / 4, SL = 64 / L, K = kPartsMost / 64;    // lanes of a part, parts of a wave at once
   constexpr int TURN = SL * WAVES, PRE = WAVES == 4 ? kPartsMost / TURN : std::min(8, 64 / TURN);    // parts at once; turns whose loads go out first
@@ -1241,14 +1360,14 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
   if (row0 >= all_rows) return;
   int lo = 0, hi = 0;
   long long first = 0;
-  const int parts = row_parts<TREE>(a, min(row0 + min(lane, rows - 1), all_rows - 1), __builtin_amdgcn_readfirstlane((int)(row0 / a.heads)), &lo, &hi, &first);
+  const int parts = row_parts(a, min(row0 + min(lane, rows - 1), all_rows - 1), __builtin_amdgcn_readfirstlane((int)(row0 / a.heads)), &lo, &hi, &first);
   unsigned long long todo = __builtin_amdgcn_ballot_w64(lane < rows && row0 + lane < all_rows && parts > 1);
   while (todo) {
     const int r = (int)__builtin_ctzll(todo);
     todo &= todo - 1;
     const long long at = row0 + r;
     const int n = __builtin_amdgcn_readlane(parts, r);
-    const bool some = __builtin_amdgcn_readlane(hi, r) > __builtin_amdgcn_readlane(lo, r), loose = TREE && __builtin_amdgcn_readlane(lo, r) < 0;
+    const bool none = __builtin_amdgcn_readlane(hi, r) <= __builtin_amdgcn_readlane(lo, r);
     const long long part0 = (long long)(((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(first >> 32), r) << 32) |
                                         (unsigned)__builtin_amdgcn_readlane((int)first, r));
     const float* const ml = a.part_ml + 2 * part0;
@@ -1316,13 +1435,102 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
       }
     }
     if ((WAVES == 1 || wave == 0) && lane < L) {
-      const bool none = !some || (loose && sum == 0.0f);
       const float inv = none ? 0.0f : 1.0f / sum;
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] = finite_or_nan(acc[e]);
       *reinterpret_cast<v2u*>((typename T::scalar*)a.o + at * D + 4 * c) = v2u{T::pack(acc[0] * inv, acc[1] * inv), T::pack(acc[2] * inv, acc[3] * inv)};
       if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : log_sum(top, sum);
     }
+  }
+}
+
+// The same for trees, a token's rows by one wave after the other, `rows` heads of them each.  Lanes have columns, so that a part's weight is the same for all and
+// nothing passes between lanes but the largest reference and the sum of the weights; the first sixteen parts are asked for before those are known.
+// (25 tokens, 32 heads, 32 parts: @JOIN@)
+template <typename T, int D>
+__global__ __launch_bounds__(256) void tree_join_kernel(AttnArgs a, int rows) {
+  constexpr int VEC = D > 64 ? 2 : 1, TURN = 16, K = kPartsMost / 64;
+  typedef float vec __attribute__((ext_vector_type(VEC)));
+  const int lane = threadIdx.x & 63;
+  const int chunks = (a.heads + rows - 1) / rows, unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const int token = unit / chunks, head0 = (unit - token * chunks) * rows;
+  if (token >= a.batch.tokens) return;
+  // the sequence, and what it says of the token
+  int start = 0, end = 0, place = 0, all = 0, b = -1;
+  for (int from = 0; from < a.batch.sequences && b < 0; from += 64) {
+    const int i = min(from + lane, a.batch.sequences - 1), s0 = a.batch.starts[i], s1 = a.batch.starts[i + 1], n = a.batch.lens[i];
+    const unsigned long long here = __builtin_amdgcn_ballot_w64(from + lane < a.batch.sequences && max(s0, 0) <= token && token < s1);
+    if (here) {
+      const int l = (int)__builtin_ctzll(here);
+      b = from + l;
+      start = max(__builtin_amdgcn_readlane(s0, l), 0);
+      place = __builtin_amdgcn_readlane(s1, l);
+      end = min(place, a.batch.tokens);
+      all = max(__builtin_amdgcn_readlane(n, l), 0);
+    }
+  }
+  if (b < 0 || token - start >= kTreeMost) return;
+  const int first = first_position(all, start, place), len = min(all, kv_capacity(a.batch, a.pages.page_shift));
+  const long long position = (long long)first + (token - start);
+  const int hi = clamp_position(position + 1, len), lo = a.window > 0 ? clamp_position((long long)first - a.window + 1, len) : 0;
+  const bool some = hi > lo, loose = position >= len, small = (end - start) * a.group <= a.small_rows;
+  const int n = seq_parts(a, small ? a.small : a.cut, first, len);
+  if (n <= 1) return;
+  const int col = min(lane * VEC, D - VEC);
+  for (int head = head0; head < min(head0 + rows, a.heads); ++head) {
+    const int kv_head = head / a.group;
+    const long long at = (long long)token * a.heads + head, part0 = first_part(a, small, b, kv_head, (token - start) * a.group + head - kv_head * a.group, at);
+    const float* const ml = a.part_ml + 2 * part0;
+    const float* const po = a.part_o + part0 * D + col;
+    vec x[TURN];
+#pragma unroll
+    for (int i = 0; i < TURN; ++i) x[i] = *reinterpret_cast<const vec*>(po + (size_t)min(i, n - 1) * D);
+    float m[K], w[K], top = kNoRef, sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int p = 64 * k + lane;
+      m[k] = p < n ? ml[2 * p] : kNoRef;
+      w[k] = p < n ? ml[2 * p + 1] : 0.0f;
+      top = fmaxf(top, m[k]);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float e = __builtin_amdgcn_exp2f(m[k] - top);
+      sum += e * w[k];
+      w[k] = e;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    vec acc = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll 1
+      for (int p0 = 0; p0 < min(n - 64 * k, 64); p0 += TURN) {
+        if (k + p0 > 0) {
+#pragma unroll
+          for (int i = 0; i < TURN; ++i) x[i] = *reinterpret_cast<const vec*>(po + (size_t)min(64 * k + p0 + i, n - 1) * D);
+        }
+#pragma unroll
+        for (int i = 0; i < TURN; ++i) {
+          const float weight = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w[k]), p0 + i));
+          if (64 * k + p0 + i < n) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[e] += weight * x[i][e];
+          }
+        }
+      }
+    }
+    const bool none = !some || (loose && sum == 0.0f);
+    const float inv = none ? 0.0f : 1.0f / sum;
+    if (lane * VEC < D) {
+      typename T::scalar* const o = (typename T::scalar*)a.o + at * D + col;
+      const unsigned pair = T::pack(finite_or_nan(acc[0]) * inv, finite_or_nan(acc[VEC - 1]) * inv);
+      if constexpr (VEC == 2) *reinterpret_cast<unsigned*>(o) = pair;
+      else *reinterpret_cast<unsigned short*>(o) = (unsigned short)pair;
+    }
+    if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : log_sum(top, sum);
   }
 }
 
@@ -1352,9 +1560,9 @@ static double narrow_cost(double workgroups, int part_keys, int held, int cus, b
 }
 
 // The same of the wide kernel: rounds of one workgroup to a compute unit, which takes 2 us for a tile of 64 keys of 128; then what is left of `small` us of
-// other workgroups when these have filled the last round.
-static double wide_cost(double workgroups, double part_keys, int D, int cus, double small) {
-  const double each = 6.0 + part_keys / 64 * (2.0 * D / 128), rounds = std::ceil(workgroups / cus);
+// other workgroups when these have filled the last round.  (Those of trees have half the rows.)
+static double wide_cost(double workgroups, double part_keys, int D, int cus, double small, bool tree) {
+  const double each = 6.0 + part_keys / 64 * ((tree ? 1.0 : 2.0) * D / 128), rounds = std::ceil(workgroups / cus);
   return rounds * each + std::max(0.0, small - (rounds * cus - workgroups) * each) / cus;
 }
 
@@ -1385,12 +1593,12 @@ static Cut best_cut(int keys, int least_keys, long long rows, int D, size_t room
   return best;
 }
 
-static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, int heads, int window, int max_queries, int max_keys, int cus, size_t room) {
+static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, int heads, int window, int max_queries, int max_keys, int cus, size_t room, bool tree) {
   const int D = pages.head_size, group = heads / pages.heads;
   Plan p;
   const long long most = max_queries > 0 ? std::min(max_queries, b.tokens) : b.tokens;   // new tokens of a sequence
   const long long most_rows = most * group, rows = (long long)b.tokens * heads;
-  p.narrow = most_rows <= 64;
+  p.narrow = most_rows <= (tree && getenv("NARROW") ? atoi(getenv("NARROW")) : 64);
   const long long capacity = (long long)b.width << page_shift;
   long long seen = max_keys > 0 ? std::min<long long>(max_keys, capacity) : capacity;
   if (window > 0) seen = std::min(seen, most + window + 64);   // from the first key that the first new token sees, down to a multiple of 64
@@ -1399,7 +1607,7 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
   // units.  (16 sequences of up to 4096 keys, 8 heads of them, 20 rows: 48 us by 32 rows and 54 by 16 at D 128, int8 46 and 48, 25 and 28 at D 64; 48 rows: 65 and 67, int8 69 and 71, but
   // 38 and 34 at D 64; two sequences of up to 1000 keys, 48 rows: 15 and 12.)
   p.nq = most_rows <= 16 || (p.narrow && ((most_rows + 31) / 32) * b.sequences * pages.heads * ((keys + 255) / 256) < cus) ? 1 : 2;
-  const int R = p.narrow ? 16 * p.nq : kWideRows;
+  const int R = p.narrow ? 16 * p.nq : tree ? kPairedRows : kWideRows;
   const long long per_seq = (most_rows + R - 1) / R, packed = (long long)b.tokens * group / R + b.sequences;
   // numbered by row blocks, unless most of such slots would be empty (as those of narrow workgroups, four to a sequence at most, cannot be)
   p.slots_per_seq = p.narrow || b.sequences * per_seq <= 2 * packed ? (int)per_seq : 0;
@@ -1424,7 +1632,7 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
     // whole row blocks; a chunk that sees itself under a causal mask works on half of its own keys
     const double units = (double)std::max<long long>(1, b.tokens * (long long)group / R) * pages.heads, own = std::min<double>(most, keys) / 2;
     p.cut = best_cut(keys, 512, rows, D, room,
-                     [&](const Cut& c) { return wide_cost(units * c.nparts, c.part_keys * (1 - own / keys), D, cus, small) + join_cost(rows, D, c.nparts); });
+                     [&](const Cut& c) { return wide_cost(units * c.nparts, c.part_keys * (1 - own / keys), D, cus, small, tree) + join_cost(rows, D, c.nparts); });
   }
   p.large = parts_of(rows, p.cut.nparts);
   p.all = p.large + parts_of(small_rows, p.small.nparts);
@@ -1448,7 +1656,7 @@ static int launch_with_lds(const char* name, K kernel, DeviceOnce& once, long lo
   return check_launch(name);
 }
 
-static size_t attend_workspace_bytes(const ftk_kv_pages* pages, const ftk_kv_batch* batch, int heads, int window, int max_queries, int max_keys) {
+static size_t attend_workspace_bytes(const ftk_kv_pages* pages, const ftk_kv_batch* batch, int heads, int window, int max_queries, int max_keys, bool tree) {
   const DeviceProps* d = nullptr;
   if (!pages || !batch || pages->heads <= 0 || heads <= 0 || heads % pages->heads || batch->tokens <= 0 || batch->sequences <= 0 || batch->table_width <= 0 ||
       pages->page_size <= 0 || window < 0 || device_props(&d))
@@ -1457,7 +1665,7 @@ static size_t attend_workspace_bytes(const ftk_kv_pages* pages, const ftk_kv_bat
   b.tokens = batch->tokens;
   b.sequences = batch->sequences;
   b.width = batch->table_width;
-  const Plan p = plan(*pages, b, __builtin_ctz((unsigned)pages->page_size), heads, window, max_queries, max_keys, d->cus, SIZE_MAX);
+  const Plan p = plan(*pages, b, __builtin_ctz((unsigned)pages->page_size), heads, window, max_queries, max_keys, d->cus, SIZE_MAX, tree);
   return workspace_of(p.all, pages->head_size);
 }
 
@@ -1485,7 +1693,7 @@ static int attend(const char* who, const void* q, int type, long long q_token_st
   const DeviceProps* d = nullptr;
   if ((rc = device_props(&d))) return rc;
   if (workspace && !aligned16(workspace)) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", who);
-  const Plan p = plan(*pages, a.batch, a.pages.page_shift, heads, window, max_queries, max_keys, d->cus, workspace ? workspace_bytes : 0);
+  const Plan p = plan(*pages, a.batch, a.pages.page_shift, heads, window, max_queries, max_keys, d->cus, workspace ? workspace_bytes : 0, TREE);
   a.q = q;
   a.o = o;
   a.lse = lse;
@@ -1526,20 +1734,28 @@ static int attend(const char* who, const void* q, int type, long long q_token_st
       bad = p.nq == 2 ? with_kept(std::integral_constant<int, 2>{}) : with_kept(std::integral_constant<int, 1>{});
     } else {
       static DeviceOnce once;
-      constexpr int lds = std::max(TREE ? WideShape<D>::TREE_LDS : WideShape<D>::LDS, 2 * NarrowShape<F, D>::LDS);
+      constexpr int lds = std::max(WideShape<D, TREE>::LDS, 2 * NarrowShape<F, D>::LDS);
       bad = launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D, TREE>, once, blocks + pairs, kWideWaves, lds, s, a, (int)blocks);
     }
     if (bad || p.all == 0) return bad;
-    // few rows of many parts: a block to each; only small sequences cut: 16 rows to a wave, most of which have nothing to join
-    if (rows <= 4096 && std::max(p.cut.nparts, p.small.nparts) >= 16) {
-      hipLaunchKernelGGL((paged_merge_kernel<T, D, 4, TREE>), dim3((unsigned)rows), dim3(256), 0, s, a, 1);
+    if constexpr (TREE) {
+      const int per_wave = rows <= 8192 ? 1 : 4;
+      const long long jblocks = ((long long)a.batch.tokens * ((heads + per_wave - 1) / per_wave) + 3) / 4;
+      if (jblocks > INT_MAX / 4) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: grid too large", who);
+      hipLaunchKernelGGL((tree_join_kernel<T, D>), dim3((unsigned)jblocks), dim3(256), 0, s, a, per_wave);
+      return check_launch("tree_join_kernel");
     } else {
-      const int per_wave = p.cut.nparts > 1 ? 1 : 16;
-      const long long mblocks = (rows + 4 * per_wave - 1) / (4 * per_wave);
-      if (mblocks > INT_MAX) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: grid too large", who);
-      hipLaunchKernelGGL((paged_merge_kernel<T, D, 1, TREE>), dim3((unsigned)mblocks), dim3(256), 0, s, a, per_wave);
+      // few rows of many parts: a block to each; only small sequences cut: 16 rows to a wave, most of which have nothing to join
+      if (rows <= 4096 && std::max(p.cut.nparts, p.small.nparts) >= 16) {
+        hipLaunchKernelGGL((paged_merge_kernel<T, D, 4>), dim3((unsigned)rows), dim3(256), 0, s, a, 1);
+      } else {
+        const int per_wave = p.cut.nparts > 1 ? 1 : 16;
+        const long long mblocks = (rows + 4 * per_wave - 1) / (4 * per_wave);
+        if (mblocks > INT_MAX) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: grid too large", who);
+        hipLaunchKernelGGL((paged_merge_kernel<T, D, 1>), dim3((unsigned)mblocks), dim3(256), 0, s, a, per_wave);
+      }
+      return check_launch("paged_merge_kernel");
     }
-    return check_launch("paged_merge_kernel");
   });
 }
 

@@ -4,7 +4,7 @@
 extern "C" {
 
 size_t ftk_paged_attn_workspace_bytes(const ftk_kv_pages* pages, const ftk_kv_batch* batch, int heads, int window, int max_queries, int max_keys) {
-  return ftk::attend_workspace_bytes(pages, batch, heads, window, max_queries, max_keys);
+  return ftk::attend_workspace_bytes(pages, batch, heads, window, max_queries, max_keys, false);
 }
 
 int ftk_paged_attn(const void* q, int type, long long q_token_stride, long long q_head_stride, const ftk_kv_pages* pages, const ftk_kv_batch* batch,

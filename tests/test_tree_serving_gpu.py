@@ -139,17 +139,20 @@ def test_trees_behind_long_sequences_in_parts(core, dtype, cache, D, page, heads
 
 @pytest.mark.parametrize('dtype,cache', [(F16, None), (BF16, E4M3)])
 def test_a_chain_is_what_a_tree_without_branches_is(core, dtype, cache):
-    """The same bits as attention of new tokens one behind the other: the same sums in the same order."""
+    """What attention of new tokens one behind the other gives.  Trees have their keys summed in another order, and where many rows share a head's keys each weight is
+    rounded to 16 bits, at most half a step, eps / 2 of it, in both: the sums differ by at most eps of the same sum over |values|, and their own rounding by eps of
+    them, which is less.  (1 % is for sums in fp32.)"""
     for new, lens, G in (([5, 1, 16, 0], [900, 40, 16, 9], 4), ([200, 3, 256], [1500, 60, 300], 2)):
         batch = base.make_batch(new, lens, 32, 330)
         pages = _cuda(base.make_pages(batch, 2, 128, cache, dtype, 331))
         q = torch.randn((batch['tokens'], 2 * G, 128), generator=torch.Generator().manual_seed(332)).to(dtype).cuda()
+        sizes = (pages[0], pages[1].float().abs().to(pages[1].dtype))
         for window in (0, 3, 50):
             args = dict(window=window, max_queries=max(new), max_keys=max(lens))
             a = core.paged_attention(q, *pages[:2], *base.on_device(batch), *pages[2:], **args)
             b = core.paged_tree_attention(q, *pages[:2], *base.on_device(batch), _ints(_trees(new, 0, 'chain')), *pages[2:], **args)
-            # (with a window the parts' borders may differ, and with them the last bit)
-            assert torch.equal(a, b) if window == 0 else bool(((a - b).abs().float() <= 2 * torch.finfo(dtype).eps * (1 + a.abs().float())).all())
+            most = core.paged_attention(q, *sizes, *base.on_device(batch), *pages[2:], **args).float()
+            assert ((a.float() - b.float()).abs() <= 2.02 * torch.finfo(dtype).eps * most).all()
 
 
 @pytest.mark.parametrize('dtype,cache,G,new,lens', [(F16, None, 2, [20, 6], [70, 6]), (BF16, E4M3, 4, [60, 2], [200, 31]), (F16, I8, 1, [256], [290])])
