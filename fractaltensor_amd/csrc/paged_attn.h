@@ -69,6 +69,8 @@ struct AttnArgs {
   long long small_first;                      // parts of small sequences stand behind these many
   float *part_o, *part_ml;                    // [tokens * heads][cut.nparts] parts, then [sequences][kv heads][kSmallRows][small.nparts]: D floats; two
   const int* parents;                         // trees: of each packed row, by its number among the sequence's new tokens; negative: none
+  int shares, grain_shift, row_blocks;        // trees, wide: workgroups of a kv head that the work is shared out to (0: a workgroup to a block of rows), of
+                                              // grains of 2^grain_shift keys; blocks of kPairedRows rows that a sequence may have
 };
 
 // ---- which rows and which keys a workgroup has ----------------------------------------
@@ -81,6 +83,7 @@ struct Job {
   int sure_lo, sure_hi;        // keys that each of its rows sees
   int part, parts;             // parts of this sequence
   bool small;
+  long long left;              // trees, wide, parts > 1: where the first row's is left, in parts
 };
 
 // The keys that some row of the sequence sees begin here (a multiple of 64).
@@ -742,7 +745,8 @@ struct WideShape {
   static constexpr int ROWS = PAIRED ? kPairedRows : kWideRows;
   static constexpr int ORS = BYTES + 16;                       // a padded row of the O tiles that the waves turn round at the end
   static constexpr int RING = (PAIRED ? 8 : 5) * TILE;         // two tiles of K, three of V; PAIRED: two of each, twice
-  static constexpr int NOTES = PAIRED ? 2 * 2 * 16 : 64;       // of each place of V and wave
+  static constexpr int FLAGS = 64 * D / 8;                     // PAIRED: of a place of V, a bit for each value that was not finite, [key][chunk of 8]
+  static constexpr int NOTES = 64 + (PAIRED ? 4 * FLAGS : 0);  // of each place of V and wave; flags
   static constexpr int ENDS = kWideWaves * 32 * ORS;           // PAIRED: four waves' rows, and what the other four have of them
   static constexpr int TILES_LDS = RING + NOTES > ENDS ? RING + NOTES : ENDS;
   static constexpr int WORDS = kTreeMost / 64 + 1;             // TREE, behind those: of each row, which new tokens it sees
@@ -831,7 +835,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
     const signed char* exps;
     unsigned src[D == 96 ? CP : 1];
     v4u codes[LD];
-    float scale[LD];
+    int exps_of[LD];                                           // as they are held: what is made of them waits for them
   };
   // Cache row (from this head's first) of the 16 keys of this wave in tile t; of the nearest 16 in [lo, hi) where those lie outside (INSIDE: they
   // do not).
@@ -884,7 +888,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
       const int p = min(64 * i + lane, D - 1), rw = p / (D / 16), piece = p - rw * (D / 16);
       const long long row_at = at + (decltype(inside_c)::value ? rw : min(max(key0 + rw - inside, least), most));
       b.codes[i] = *reinterpret_cast<const v4u*>(b.from + row_at * D + 16 * piece);
-      b.scale[i] = ldexpf(1.0f, b.exps[row_at]);
+      b.exps_of[i] = b.exps[row_at];
     }
   };
   auto store = [&](const Bring& b, unsigned char* to) __attribute__((always_inline)) {
@@ -893,16 +897,17 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
       for (int i = 0; i < LD; ++i) {
         const int p = 64 * i + lane, rw = p / (D / 16), piece = p - rw * (D / 16), in_tile = 16 * cw + rw;
         const int swz = b.keys ? swizzle<S::BYTES>(in_tile) : v_swizzle<D>(in_tile);
+        const float scale = ldexpf(1.0f, b.exps_of[i]);
         auto put = [&](auto decode) __attribute__((always_inline)) {
           if (D % 64 == 0 || p < D) {
 #pragma unroll
             for (int c = 0; c < 2; ++c)
-              *reinterpret_cast<v8*>(to + in_tile * S::BYTES + 16 * ((2 * piece + c) ^ swz)) = decode(v2u{b.codes[i][2 * c], b.codes[i][2 * c + 1]}, b.scale[i]);
+              *reinterpret_cast<v8*>(to + in_tile * S::BYTES + 16 * ((2 * piece + c) ^ swz)) = decode(v2u{b.codes[i][2 * c], b.codes[i][2 * c + 1]}, scale);
           }
         };
         // (the conversion of e4m3 rounds once whatever the scale)
         constexpr bool LOOK = std::is_same<T, Half>::value && F == kInt8;
-        if (LOOK && __builtin_expect(__builtin_amdgcn_ballot_w64(!(b.scale[i] >= 0x1p-24f && b.scale[i] <= 0x1p9f)) != 0, 0)) put(decode8_rounded<T, F>);
+        if (LOOK && __builtin_expect(__builtin_amdgcn_ballot_w64(!(scale >= 0x1p-24f && scale <= 0x1p9f)) != 0, 0)) put(decode8_rounded<T, F>);
         else put(decode8<T, F>);
       }
     }
@@ -1030,12 +1035,42 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   };
   // Waves 0 to 3 (PAIRED: all) look whether their 16 keys of a tile of V hold anything that is not finite, and leave word for all.
   unsigned* const words = reinterpret_cast<unsigned*>(smem + S::RING) + (PAIRED ? 8 * half : 0);   // [three places of V][wave]; PAIRED: [two][wave], twice
-  auto look = [&](const unsigned char* vt, int place) __attribute__((always_inline)) {
+  unsigned char* const flags = smem + S::RING + 64 + (PAIRED ? 2 * S::FLAGS * half : 0);
+  auto look = [&](unsigned char* vt, int place) __attribute__((always_inline)) {
     unsigned bad = 0;
 #pragma unroll
     for (int i = 0; i < CP; ++i) bad |= not_finite<T>(*reinterpret_cast<const v8*>(vt + cw * (16 * S::BYTES) + 1024 * i + 16 * lane));
     const bool any = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
     if (lane == 0) words[4 * place + cw] = any;
+    if constexpr (PAIRED) {
+      if (__builtin_expect(any, 0)) {                            // those leave the tile, for 0 x inf, and a bit is left for each
+#pragma unroll 1
+        for (int i = 0; i < CP; ++i) {
+          const int p = 64 * i + lane, key = 16 * cw + p / CH, chunk = (p % CH) ^ v_swizzle<D>(key);
+          v8* const at = reinterpret_cast<v8*>(vt + cw * (16 * S::BYTES) + 16 * p);
+          const v8 x = *at;
+          const unsigned bits = not_finite<T>(x);
+          *at = zeros_at<T>(x, bits);
+          flags[place * S::FLAGS + key * (D / 8) + chunk] = (unsigned char)bits;
+        }
+      }
+    }
+  };
+  // PAIRED: NaN for the rows that see a key whose value was not finite
+  auto mark = [&](int t, int place) __attribute__((always_inline)) {
+    const unsigned long long drawn = way_of(t);
+#pragma unroll 1
+    for (int key = 0; key < 64; ++key) {
+      if (words[4 * place + (key >> 4)] == 0) continue;
+      const bool sees_it = drawn >> key & 1;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const unsigned four = *reinterpret_cast<const unsigned*>(flags + place * S::FLAGS + key * (D / 8) + 4 * dt) >> (4 * hh);   // (chunks 4 dt .. +3)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (sees_it && (four >> (8 * (e >> 2) + (e & 3)) & 1)) o[dt][e] = __builtin_nanf("");
+      }
+    }
   };
   auto all_finite = [&](int place) __attribute__((always_inline)) {
     const v4u w = *reinterpret_cast<const v4u*>(words + 4 * place);
@@ -1049,12 +1084,10 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
       const v8 p = step == 0 ? pf[0][0] : step == 1 ? pf[0][1] : step == 2 ? pf[1][0] : pf[1][1];
       const int key0 = base + 64 * t + 16 * step + 4 * hh;
       unsigned seen = 0;
-      unsigned long long drawn = ~0ULL;
-      if constexpr (TREE) drawn = way_of(t) >> (16 * step + 4 * hh);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int in = 8 * (e >> 2) + (e & 3), key = key0 + in;
-        if (TREE ? (drawn >> in & 1) != 0 : key >= my_lo && key < my_hi) seen |= 1u << e;
+        if (key >= my_lo && key < my_hi) seen |= 1u << e;
       }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
@@ -1128,14 +1161,13 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
     __syncthreads();
     phase_m(Vb, Kb, no{}, yes{});
     if constexpr (PAIRED) {
-      // What a turn asks for and puts away behind the last tile is that tile once more, and its scores go nowhere: code that runs once takes longer to fetch than to run.
+      // One turn for all tiles, as code that runs once takes longer to fetch than to run: what a turn asks for and puts away behind the last tile is that tile once more,
+      // and its scores go nowhere.
       phase_barrier();                                         // waves 0 to 3 are about to write where K(0) was read
       int vcur = 2 * S::TILE, vnext = 3 * S::TILE, kcur = 0, knext = S::TILE;     // V(t), V(t + 2), K(t), K(t + 2)
       long long behind = block_at(asked - 2, no{});
-      // Tiles [clean, dirty): every row sees all of them
-      const int clean = (max(j.sure_lo, j.lo) - base + 63) / 64, dirty = (min(j.sure_hi, j.hi) - base) / 64;
-      auto turn = [&](int t, auto clean_c) __attribute__((always_inline)) {
-        constexpr bool CLEAN = decltype(clean_c)::value;
+      if (half) phase_barrier();
+      for (int t = half; t < ntiles + half; t += 2) {          // both halves take as many turns, the last of which may have no tile for waves 4 to 7
         const int bring = t + ahead;
         if constexpr (F == kSame) {
           copy(keys, tiles + kcur, bring, next, no{});
@@ -1149,21 +1181,14 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
         behind = next;
         next = block_at(bring + 2, no{});
         __builtin_amdgcn_sched_barrier(0);                     // the copies go out before the weights are begun
-        const bool works = !idle && (CLEAN || t < ntiles);
-        if (works) phase_s(t, clean_c);
-        if (!CLEAN) look(tiles + vcur, vcur / S::TILE - 2);
-        if constexpr (!CLEAN || F != kSame) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // what was written to LDS
+        const bool works = !idle && t < ntiles;
+        const bool some = base + 64 * t < max(j.sure_lo, j.lo) || base + 64 * t + 64 > min(j.sure_hi, j.hi);   // some wave's rows do not see all of it
+        if (works) phase_s(t, no{});
+        if (some) look(tiles + vcur, vcur / S::TILE - 2);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // what was written to LDS
         phase_barrier();
-        if (works) {
-          const unsigned char *const vt = tiles + vcur, *const kt = tiles + knext;
-          if constexpr (CLEAN) {
-            phase_m(vt, kt, yes{}, yes{});
-          } else {
-            if (masked(t) && __builtin_expect(!all_finite(vcur / S::TILE - 2), 0)) careful_pv(vt, t);
-            else phase_m(vt, kt, yes{}, no{});
-            phase_m(vt, kt, no{}, yes{});
-          }
-        }
+        if (works) phase_m(tiles + vcur, tiles + knext, yes{}, yes{});
+        if (some && works && __builtin_expect(!all_finite(vcur / S::TILE - 2), 0)) mark(t, vcur / S::TILE - 2);
         if constexpr (F == kSame) __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the copies that this wave asked for in S(t)
         phase_barrier();
         const int k = kcur, v = vcur;
@@ -1171,12 +1196,6 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
         knext = k;
         vcur = vnext;
         vnext = v;
-      };
-      if (half) phase_barrier();
-      for (int t = half; t < ntiles + half; t += 2) {          // both halves take as many turns, the last of which may have no tile for waves 4 to 7
-        if (t >= clean)
-          for (; t < dirty; t += 2) turn(t, yes{});
-        if (t < ntiles + half) turn(t, no{});
       }
       if (!half) phase_barrier();
     } else {
@@ -1254,14 +1273,15 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   l += __shfl_xor(l, 32);
   if (j.parts > 1) {
     if (wrow0 + jr < j.rows) {
-      float* const po = a.part_o + (r.at * a.cut.nparts + j.part) * D;
+      const long long left = PAIRED ? j.left + in_rows + jr : r.at * a.cut.nparts + j.part;
+      float* const po = a.part_o + left * D;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
           *reinterpret_cast<v4f*>(po + 32 * dt + 8 * g + 4 * hh) = v4f{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
       if (hh == 0) {
-        float* const ml = a.part_ml + 2 * (r.at * a.cut.nparts + j.part);
+        float* const ml = a.part_ml + 2 * left;
         ml[0] = ref;
         ml[1] = l;
       }
@@ -1293,6 +1313,124 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   }
 }
 
+// Trees: how the work of a kv head is shared out to `shares` workgroups, which the arrays on the device say alone.  The keys of the sequences that are not small, in
+// grains and one sequence behind the other, are a line for each block of rows (the k-th line of those sequences that have more than k of them), and each
+// workgroup has as many grains of one line, of one sequence or of several, whose block of rows it works on one after the other; a block of rows that more than one
+// workgroup has is left in parts.  (16 sequences of 2064 to 8192 positions, 60 tokens each, 8 heads: @SHARE@)
+constexpr int kLeastGrains = 4;
+
+__device__ __forceinline__ int wave_sum(int x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+  return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+struct Shares {
+  int each;                    // grains
+  int grains, groups, before;  // lane k: of line k, the workgroups that have them, and those of the lines before
+};
+
+// Sequence i, a lane's own: its grains, and its blocks of rows.
+__device__ __forceinline__ int share_work(const AttnArgs& a, int i, int* blocks) {
+  *blocks = 0;
+  if (i >= a.batch.sequences) return 0;
+  const int start = min(max(a.batch.starts[i], 0), a.batch.tokens), end = a.batch.starts[i + 1], all = max(a.batch.lens[i], 0);
+  const int rows = min(min(max(end, start), a.batch.tokens) - start, kTreeMost) * a.group;
+  if (rows <= a.small_rows) return 0;
+  *blocks = min((rows + kPairedRows - 1) / kPairedRows, a.row_blocks);
+  const int keys = max(min(all, kv_capacity(a.batch, a.pages.page_shift)) - seq_first_key(a, first_position(all, start, end)), 1);
+  return (int)(((long long)keys + (1LL << a.grain_shift) - 1) >> a.grain_shift);
+}
+
+// All lanes of a wave call these.
+__device__ __forceinline__ Shares share_out(const AttnArgs& a) {
+  const int lane = threadIdx.x & 63;
+  Shares s{0, 0, 0, 0};
+  for (int from = 0; from < a.batch.sequences; from += 64) {
+    int blocks;
+    const int grains = share_work(a, from + lane, &blocks);
+    for (int k = 0; k < a.row_blocks; ++k) {
+      const int sum = wave_sum(blocks > k ? grains : 0);
+      if (lane == k) s.grains += sum;
+    }
+  }
+  s.each = max((int)(((long long)wave_sum(s.grains) + a.shares - 1) / a.shares), kLeastGrains);
+  for (;;) {                                                   // (it ends: there are as many shares as lines at least)
+    s.groups = (int)(((long long)s.grains + s.each - 1) / s.each);
+    const int before = wave_scan(s.groups);
+    s.before = before - s.groups;
+    if (__builtin_amdgcn_readlane(before, 63) <= a.shares) break;
+    s.each += s.each / 32 + 1;
+  }
+  return s;
+}
+// Which workgroup of which line the w-th is: lines have no more of them than those before, and the same one of all lines, which read the same keys, go together.
+__device__ __forceinline__ bool share_of(const AttnArgs& a, const Shares& s, int w, int* line, int* at) {
+  int done = 0;
+  for (int k = a.row_blocks; k > 0; --k) {
+    const int groups = __builtin_amdgcn_readlane(s.groups, k - 1), here = (groups - done) * k;
+    if (w < here) {
+      *at = done + w / k;
+      *line = w % k;
+      return true;
+    }
+    w -= here;
+    done = groups;
+  }
+  return false;
+}
+// The sequence that has grain x of a line, or (seek >= 0) sequence `seek` itself; where it begins there, and how many it has.
+__device__ __forceinline__ int share_find(const AttnArgs& a, int line, int x, int seek, int* begin, int* grains) {
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  for (int from = 0; from < a.batch.sequences; from += 64) {
+    int blocks;
+    int mine = share_work(a, from + lane, &blocks);
+    if (blocks <= line) mine = 0;
+    const int upto = base + wave_scan(mine);
+    const unsigned long long here = __builtin_amdgcn_ballot_w64(seek >= 0 ? from + lane == seek : mine > 0 && x < upto);
+    if (here) {
+      const int l = (int)__builtin_ctzll(here);
+      *grains = __builtin_amdgcn_readlane(mine, l);
+      *begin = __builtin_amdgcn_readlane(upto, l) - *grains;
+      return from + l;
+    }
+    base = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return -1;
+}
+
+// Grains [from, to) of `grains` of sequence b for a line's block of rows.
+__device__ __forceinline__ void share_job(const AttnArgs& a, int b, int line, int from, int to, int grains, Job& j) {
+  j.b = b;
+  const KvChunk c = kv_chunk(a.batch, b);
+  j.start = c.start;
+  j.n = min(c.n, kTreeMost);
+  j.first = c.first;
+  j.rows = j.n * a.group;
+  j.row0 = line * kPairedRows;
+  j.len = min(c.len, kv_capacity(a.batch, a.pages.page_shift));
+  const long long p_hi = (long long)c.first + (min(j.row0 + kPairedRows, j.rows) - 1) / a.group, key0 = seq_first_key(a, c.first);
+  j.hi = clamp_position(p_hi + 1, j.len);
+  j.sure_hi = clamp_position(c.first, j.len);
+  j.lo = a.window > 0 ? clamp_position((long long)c.first - a.window + 1, j.len) : 0;
+  j.sure_lo = a.window > 0 ? clamp_position(p_hi - a.window + 1, j.len) : 0;
+  if (from > 0) j.lo = max(j.lo, clamp_position(key0 + ((long long)from << a.grain_shift), j.len));
+  if (to < grains) j.hi = min(j.hi, clamp_position(key0 + ((long long)to << a.grain_shift), j.len));
+  j.part = 0;
+  j.parts = from > 0 || to < grains ? 2 : 1;
+  j.small = false;
+}
+
 // The workgroups behind the first `wide` take sequences of at most small_rows = 16 rows, which would leave seven of the eight waves without
 // any: two (sequence, head, part) each, by four waves that cut the keys as in the narrow kernel.  They read on the compute units that the others
 // leave free, or have left, while those multiply.  (A chunk of 512 tokens beside five sequences that decode, 16 heads, 4 of keys, up to
@@ -1302,24 +1440,55 @@ __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs
   constexpr int R = WideShape<D, TREE>::ROWS;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   Job j;
-  if ((int)blockIdx.x >= wide) {
-    const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
-    const int item = 2 * (blockIdx.x - wide) + half, kv_head = item % a.pages.heads, rest = item / a.pages.heads;
-    const int b = rest / a.small.nparts, part = rest - b * a.small.nparts;
-    if (b < a.batch.sequences && find_job<16, TREE>(a, b, 0, part, true, j)) {
-      narrow_attention<T, F, D, 1, false, TREE>(a, j, kv_head, smem + half * NarrowShape<F, D>::LDS, threadIdx.x & 255);
-    } else {                                                     // the other half's two barriers
-      __syncthreads();
-      __syncthreads();
+  if constexpr (!TREE) {
+    if ((int)blockIdx.x >= wide) {
+      const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+      const int item = 2 * (blockIdx.x - wide) + half, kv_head = item % a.pages.heads, rest = item / a.pages.heads;
+      const int b = rest / a.small.nparts, part = rest - b * a.small.nparts;
+      if (b < a.batch.sequences && find_job<16, false>(a, b, 0, part, true, j)) {
+        narrow_attention<T, F, D, 1, false, false>(a, j, kv_head, smem + half * NarrowShape<F, D>::LDS, threadIdx.x & 255);
+      } else {                                                     // the other half's two barriers
+        __syncthreads();
+        __syncthreads();
+      }
+      return;
     }
-    return;
   }
   // the head goes fastest, so that the row blocks of a head meet on the XCDs that have its keys
   const int id = blockIdx.x, kv_head = id % a.pages.heads, rest = id / a.pages.heads;
-  const int slot = rest / a.cut.nparts, part = rest - slot * a.cut.nparts;
-  int b, tile;
-  if (!find_rows<R>(a, slot, &b, &tile) || !find_job<R, TREE>(a, b, tile, part, false, j)) return;
-  wide_attention<T, F, D, TREE>(a, j, kv_head, smem);
+  if constexpr (TREE) {
+    const bool shared = a.shares > 0;
+    Shares s{1, 0, 0, 0};
+    int line = 0, at = 0, x0 = 0, x = 0, end = 1;
+    if (shared) {
+      s = share_out(a);
+      if (!share_of(a, s, rest, &line, &at)) return;
+      x = x0 = at * s.each;
+      end = min(x0 + s.each, __builtin_amdgcn_readlane(s.grains, line));
+    }
+    const long long slot = ((long long)(__builtin_amdgcn_readlane(s.before, line) + at) * a.pages.heads + kv_head) * 2;
+    while (x < end) {
+      int b, tile, begin, grains;
+      if (shared) {
+        b = share_find(a, line, x, -1, &begin, &grains);
+        if (b < 0) return;
+        const int to = min(end - begin, grains);
+        share_job(a, __builtin_amdgcn_readfirstlane(b), line, x - begin, to, grains, j);
+        j.left = (slot + (x > x0)) * R;
+        x = begin + to;
+      } else {
+        if (!find_rows<R>(a, rest, &b, &tile) || !find_job<R, TREE>(a, b, tile, 0, false, j)) return;
+        x = end;
+      }
+      wide_attention<T, F, D, TREE>(a, j, kv_head, smem);
+      if (x < end) __syncthreads();
+    }
+  } else {
+    const int slot = rest / a.cut.nparts, part = rest - slot * a.cut.nparts;
+    int b, tile;
+    if (!find_rows<R>(a, slot, &b, &tile) || !find_job<R, TREE>(a, b, tile, part, false, j)) return;
+    wide_attention<T, F, D, TREE>(a, j, kv_head, smem);
+  }
 }
 
 // ---- parts ------------------------------------------------------------------------------
@@ -1444,19 +1613,20 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
   }
 }
 
-// The same for trees, a token's rows by one wave after the other, `rows` heads of them each.  Lanes have columns, so that a part's weight is the same for all and
-// nothing passes between lanes but the largest reference and the sum of the weights; the first sixteen parts are asked for before those are known.
-// (25 tokens, 32 heads, 32 parts: @JOIN@)
-template <typename T, int D>
-__global__ __launch_bounds__(256) void tree_join_kernel(AttnArgs a, int rows) {
-  constexpr int VEC = D > 64 ? 2 : 1, TURN = 16, K = kPartsMost / 64;
+// The same for trees: a wave has ROWS heads of a token.  Lanes have columns, so that a part's weight is the same for all of them.  Rows in at most four parts, which most
+// are where there are many, are joined at once, everything of theirs being asked for before any of it is needed; others one after the other, their
+// weights a lane each.  (25 tokens, 32 heads, 32 parts: 6 us, 19 by the kernel above.)
+template <typename T, int D, int ROWS>
+__global__ __launch_bounds__(256) void tree_join_kernel(AttnArgs a) {
+  constexpr int VEC = D > 64 ? 2 : 1, TURN = 16, K = kPartsMost / 64, FEW = 4;
   typedef float vec __attribute__((ext_vector_type(VEC)));
+  typedef float v2f __attribute__((ext_vector_type(2)));
   const int lane = threadIdx.x & 63;
-  const int chunks = (a.heads + rows - 1) / rows, unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-  const int token = unit / chunks, head0 = (unit - token * chunks) * rows;
+  const int chunks = (a.heads + ROWS - 1) / ROWS, unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const int token = unit / chunks, head0 = (unit - token * chunks) * ROWS;
   if (token >= a.batch.tokens) return;
   // the sequence, and what it says of the token
-  int start = 0, end = 0, place = 0, all = 0, b = -1;
+  int start = 0, place = 0, all = 0, b = -1;
   for (int from = 0; from < a.batch.sequences && b < 0; from += 64) {
     const int i = min(from + lane, a.batch.sequences - 1), s0 = a.batch.starts[i], s1 = a.batch.starts[i + 1], n = a.batch.lens[i];
     const unsigned long long here = __builtin_amdgcn_ballot_w64(from + lane < a.batch.sequences && max(s0, 0) <= token && token < s1);
@@ -1465,7 +1635,6 @@ __global__ __launch_bounds__(256) void tree_join_kernel(AttnArgs a, int rows) {
       b = from + l;
       start = max(__builtin_amdgcn_readlane(s0, l), 0);
       place = __builtin_amdgcn_readlane(s1, l);
-      end = min(place, a.batch.tokens);
       all = max(__builtin_amdgcn_readlane(n, l), 0);
     }
   }
@@ -1473,24 +1642,104 @@ __global__ __launch_bounds__(256) void tree_join_kernel(AttnArgs a, int rows) {
   const int first = first_position(all, start, place), len = min(all, kv_capacity(a.batch, a.pages.page_shift));
   const long long position = (long long)first + (token - start);
   const int hi = clamp_position(position + 1, len), lo = a.window > 0 ? clamp_position((long long)first - a.window + 1, len) : 0;
-  const bool some = hi > lo, loose = position >= len, small = (end - start) * a.group <= a.small_rows;
-  const int n = seq_parts(a, small ? a.small : a.cut, first, len);
-  if (n <= 1) return;
+  const bool some = hi > lo, loose = position >= len;
+  Shares s{0, 0, 0, 0};
+  if (a.shares > 0) s = share_out(a);
+  // where the first part of each row is, the second, and how far those behind are from one another
+  int n[ROWS], line = -1, begin = 0, grains = 0;
+  long long part0[ROWS], part1[ROWS];
+  const long long step = a.shares > 0 ? 2LL * a.pages.heads * kPairedRows : 1;
+  bool few = true;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int head = min(head0 + r, a.heads - 1), kv_head = head / a.group, row = (token - start) * a.group + head - kv_head * a.group;
+    if (a.shares == 0) {
+      n[r] = seq_parts(a, a.cut, first, len);
+      part0[r] = ((long long)token * a.heads + head) * a.cut.nparts;
+      part1[r] = part0[r] + 1;
+    } else {
+      if (line != row / kPairedRows) {
+        line = row / kPairedRows;
+        if (line >= a.row_blocks) return;
+        share_find(a, line, 0, b, &begin, &grains);
+      }
+      const int group0 = begin / s.each;
+      n[r] = (begin + max(grains, 1) - 1) / s.each - group0 + 1;
+      const long long slot = ((long long)(__builtin_amdgcn_readlane(s.before, line) + group0) * a.pages.heads + kv_head) * 2;
+      part0[r] = (slot + (begin > group0 * s.each)) * kPairedRows + row % kPairedRows;
+      part1[r] = slot * kPairedRows + row % kPairedRows + step;
+    }
+    few = few && n[r] <= FEW;
+  }
   const int col = min(lane * VEC, D - VEC);
-  for (int head = head0; head < min(head0 + rows, a.heads); ++head) {
-    const int kv_head = head / a.group;
-    const long long at = (long long)token * a.heads + head, part0 = first_part(a, small, b, kv_head, (token - start) * a.group + head - kv_head * a.group, at);
-    const float* const ml = a.part_ml + 2 * part0;
-    const float* const po = a.part_o + part0 * D + col;
+  const float* const po = a.part_o + col;
+  const auto finish = [&](int head, vec acc, float top, float sum) __attribute__((always_inline)) {
+    const long long at = (long long)token * a.heads + head;
+    const bool none = !some || (loose && sum == 0.0f);
+    const float inv = none ? 0.0f : 1.0f / sum;
+    if (lane * VEC < D) {
+      typename T::scalar* const o = (typename T::scalar*)a.o + at * D + col;
+      const unsigned pair = T::pack(finite_or_nan(acc[0]) * inv, finite_or_nan(acc[VEC - 1]) * inv);
+      if constexpr (VEC == 2) *reinterpret_cast<unsigned*>(o) = pair;
+      else *reinterpret_cast<unsigned short*>(o) = (unsigned short)pair;
+    }
+    if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : log_sum(top, sum);
+  };
+  if (few) {
+    vec x[ROWS][FEW];
+    v2f ml[ROWS][FEW];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int p = 0; p < FEW; ++p) {
+        if (n[r] <= 1 || p >= n[r]) continue;
+        const long long at = p == 0 ? part0[r] : part1[r] + (p - 1) * step;
+        ml[r][p] = *reinterpret_cast<const v2f*>(a.part_ml + 2 * at);
+        x[r][p] = *reinterpret_cast<const vec*>(po + at * D);
+      }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if (n[r] <= 1 || head0 + r >= a.heads) continue;
+      float top = kNoRef, sum = 0.0f;
+      vec acc = 0.0f;
+#pragma unroll
+      for (int p = 0; p < FEW; ++p)
+        if (p < n[r]) top = fmaxf(top, ml[r][p][0]);
+#pragma unroll
+      for (int p = 0; p < FEW; ++p) {
+        if (p >= n[r]) continue;
+        const float w = __builtin_amdgcn_exp2f(ml[r][p][0] - top);
+        sum += w * ml[r][p][1];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] += w * x[r][p][e];
+      }
+      finish(head0 + r, acc, top, sum);
+    }
+    return;
+  }
+#pragma unroll 1
+  for (int r = 0; r < ROWS; ++r) {
+    int count = n[0];
+    long long at0 = part0[0], at1 = part1[0];
+#pragma unroll
+    for (int i = 1; i < ROWS; ++i)
+      if (r == i) {
+        count = n[i];
+        at0 = part0[i];
+        at1 = part1[i];
+      }
+    if (count <= 1 || head0 + r >= a.heads) continue;
+    const auto part_at = [&](int p) { return p == 0 ? at0 : at1 + (p - 1) * step; };
     vec x[TURN];
 #pragma unroll
-    for (int i = 0; i < TURN; ++i) x[i] = *reinterpret_cast<const vec*>(po + (size_t)min(i, n - 1) * D);
+    for (int i = 0; i < TURN; ++i) x[i] = *reinterpret_cast<const vec*>(po + part_at(min(i, count - 1)) * D);
     float m[K], w[K], top = kNoRef, sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int p = 64 * k + lane;
-      m[k] = p < n ? ml[2 * p] : kNoRef;
-      w[k] = p < n ? ml[2 * p + 1] : 0.0f;
+      const v2f ml = *reinterpret_cast<const v2f*>(a.part_ml + 2 * part_at(min(p, count - 1)));
+      m[k] = p < count ? ml[0] : kNoRef;
+      w[k] = p < count ? ml[1] : 0.0f;
       top = fmaxf(top, m[k]);
     }
 #pragma unroll
@@ -1507,30 +1756,22 @@ __global__ __launch_bounds__(256) void tree_join_kernel(AttnArgs a, int rows) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll 1
-      for (int p0 = 0; p0 < min(n - 64 * k, 64); p0 += TURN) {
+      for (int p0 = 0; p0 < min(count - 64 * k, 64); p0 += TURN) {
         if (k + p0 > 0) {
 #pragma unroll
-          for (int i = 0; i < TURN; ++i) x[i] = *reinterpret_cast<const vec*>(po + (size_t)min(64 * k + p0 + i, n - 1) * D);
+          for (int i = 0; i < TURN; ++i) x[i] = *reinterpret_cast<const vec*>(po + part_at(min(64 * k + p0 + i, count - 1)) * D);
         }
 #pragma unroll
         for (int i = 0; i < TURN; ++i) {
           const float weight = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w[k]), p0 + i));
-          if (64 * k + p0 + i < n) {
+          if (64 * k + p0 + i < count) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) acc[e] += weight * x[i][e];
           }
         }
       }
     }
-    const bool none = !some || (loose && sum == 0.0f);
-    const float inv = none ? 0.0f : 1.0f / sum;
-    if (lane * VEC < D) {
-      typename T::scalar* const o = (typename T::scalar*)a.o + at * D + col;
-      const unsigned pair = T::pack(finite_or_nan(acc[0]) * inv, finite_or_nan(acc[VEC - 1]) * inv);
-      if constexpr (VEC == 2) *reinterpret_cast<unsigned*>(o) = pair;
-      else *reinterpret_cast<unsigned short*>(o) = (unsigned short)pair;
-    }
-    if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : log_sum(top, sum);
+    finish(head0 + r, acc, top, sum);
   }
 }
 
@@ -1544,6 +1785,7 @@ struct Plan {
   Cut cut, small;
   int small_rows;
   size_t large, all;       // parts that there is room for: of sequences that are not small, and with those that are
+  int shares, grain_shift; // trees, wide
 };
 
 static size_t parts_of(long long rows, int nparts) { return nparts > 1 ? (size_t)rows * nparts : 0; }
@@ -1560,9 +1802,9 @@ static double narrow_cost(double workgroups, int part_keys, int held, int cus, b
 }
 
 // The same of the wide kernel: rounds of one workgroup to a compute unit, which takes 2 us for a tile of 64 keys of 128; then what is left of `small` us of
-// other workgroups when these have filled the last round.  (Those of trees have half the rows.)
-static double wide_cost(double workgroups, double part_keys, int D, int cus, double small, bool tree) {
-  const double each = 6.0 + part_keys / 64 * ((tree ? 1.0 : 2.0) * D / 128), rounds = std::ceil(workgroups / cus);
+// other workgroups when these have filled the last round.
+static double wide_cost(double workgroups, double part_keys, int D, int cus, double small) {
+  const double each = 6.0 + part_keys / 64 * (2.0 * D / 128), rounds = std::ceil(workgroups / cus);
   return rounds * each + std::max(0.0, small - (rounds * cus - workgroups) * each) / cus;
 }
 
@@ -1612,13 +1854,45 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
   // numbered by row blocks, unless most of such slots would be empty (as those of narrow workgroups, four to a sequence at most, cannot be)
   p.slots_per_seq = p.narrow || b.sequences * per_seq <= 2 * packed ? (int)per_seq : 0;
   p.slots = (int)std::min<long long>(p.slots_per_seq ? b.sequences * per_seq : packed, INT_MAX);
-  p.small_rows = p.narrow || b.sequences == 1 ? 0 : kSmallRows;
+  p.small_rows = p.narrow || tree || b.sequences == 1 ? 0 : kSmallRows;
   const int held = pages.type == FTK_F16 || pages.type == FTK_BF16 ? 4 * D : 2 * D + 2;   // bytes of a position and head
   const long long small_rows = (long long)b.sequences * pages.heads * kSmallRows;
   p.small = Cut{1, keys};
+  p.shares = 0;
+  p.grain_shift = 7;
   if (p.narrow) {
     const double units = (double)p.slots * pages.heads;
     p.cut = best_cut(keys, 256, rows, D, room, [&](const Cut& c) { return narrow_cost(units * c.nparts, c.part_keys, held, cus, b.sequences == 1) + join_cost(rows, D, c.nparts); });
+  } else if (tree) {
+    // Work shared out to as many workgroups as there are compute units, or to twice as many and more where the heads divide those badly; unless
+    // a workgroup for each block of rows is expected to be done sooner: us as in wide_cost(), several sequences being two thirds as long as the longest in the mean.
+    const double turn = 2.2 * D / 128, turns = std::ceil(keys / 128.0), units = (double)b.sequences * per_seq * pages.heads;
+    const double whole = std::ceil(units / cus) * (8.0 + turns * turn);
+    p.cut = cut_into(keys, 1);
+    while (b.sequences * (double)per_seq * (((double)keys + (1 << p.grain_shift)) / (1 << p.grain_shift)) > 2e9) ++p.grain_shift;
+    long long shares = 0;
+    double used = 0.0;
+    for (int rounds = 1; rounds <= 4 && used < 0.9; ++rounds) {
+      const long long n = std::max<long long>(rounds * (long long)cus / pages.heads, 1);
+      const double u = (double)n * pages.heads / (std::ceil((double)n * pages.heads / cus) * cus);
+      if (u > used) {
+        used = u;
+        shares = n;
+      }
+    }
+    shares = std::max(shares, per_seq);
+    const double rounds = std::ceil((double)shares * pages.heads / cus);
+    const double shared = 18.0 + rounds * 6.0 + std::max(units * turns * (b.sequences > 1 ? 2.0 / 3 : 1.0) / (shares * pages.heads), (double)kLeastGrains) * turn * rounds;
+    const size_t parts = (size_t)shares * pages.heads * 2 * kPairedRows;
+    if (shared < whole && per_seq <= 64 && workspace_of(parts, D) <= room) {
+      p.shares = (int)shares;
+      p.slots = p.shares;
+      p.large = parts;
+      p.all = parts;
+      return p;
+    }
+    p.large = p.all = 0;
+    return p;
   } else {
     // the small sequences: as many as there can be beside ones of `most` tokens, in parts of some 20 us
     double small = 0.0;
@@ -1632,7 +1906,7 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
     // whole row blocks; a chunk that sees itself under a causal mask works on half of its own keys
     const double units = (double)std::max<long long>(1, b.tokens * (long long)group / R) * pages.heads, own = std::min<double>(most, keys) / 2;
     p.cut = best_cut(keys, 512, rows, D, room,
-                     [&](const Cut& c) { return wide_cost(units * c.nparts, c.part_keys * (1 - own / keys), D, cus, small, tree) + join_cost(rows, D, c.nparts); });
+                     [&](const Cut& c) { return wide_cost(units * c.nparts, c.part_keys * (1 - own / keys), D, cus, small) + join_cost(rows, D, c.nparts); });
   }
   p.large = parts_of(rows, p.cut.nparts);
   p.all = p.large + parts_of(small_rows, p.small.nparts);
@@ -1710,6 +1984,9 @@ static int attend(const char* who, const void* q, int type, long long q_token_st
   a.small = p.small;
   a.small_rows = p.small_rows;
   a.small_first = (long long)p.large;
+  a.shares = p.shares;
+  a.grain_shift = p.grain_shift;
+  a.row_blocks = p.narrow ? 0 : (int)std::min<long long>(((long long)(max_queries > 0 ? std::min(max_queries, a.batch.tokens) : a.batch.tokens) * a.group + kPairedRows - 1) / kPairedRows, INT_MAX);
   const long long rows = (long long)a.batch.tokens * heads;
   a.part_o = (float*)workspace;
   a.part_ml = a.part_o + p.all * pages->head_size;
@@ -1734,15 +2011,20 @@ static int attend(const char* who, const void* q, int type, long long q_token_st
       bad = p.nq == 2 ? with_kept(std::integral_constant<int, 2>{}) : with_kept(std::integral_constant<int, 1>{});
     } else {
       static DeviceOnce once;
-      constexpr int lds = std::max(WideShape<D, TREE>::LDS, 2 * NarrowShape<F, D>::LDS);
+      constexpr int lds = std::max(WideShape<D, TREE>::LDS, TREE ? 0 : 2 * NarrowShape<F, D>::LDS);
       bad = launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D, TREE>, once, blocks + pairs, kWideWaves, lds, s, a, (int)blocks);
     }
     if (bad || p.all == 0) return bad;
     if constexpr (TREE) {
-      const int per_wave = rows <= 8192 ? 1 : 4;
-      const long long jblocks = ((long long)a.batch.tokens * ((heads + per_wave - 1) / per_wave) + 3) / 4;
-      if (jblocks > INT_MAX / 4) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: grid too large", who);
-      hipLaunchKernelGGL((tree_join_kernel<T, D>), dim3((unsigned)jblocks), dim3(256), 0, s, a, per_wave);
+      // a wave to a row while the compute units have room for all of them
+      auto join = [&](auto each) -> int {
+        constexpr int ROWS = decltype(each)::value;
+        const long long jblocks = ((long long)a.batch.tokens * ((heads + ROWS - 1) / ROWS) + 3) / 4;
+        if (jblocks > INT_MAX / 4) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: grid too large", who);
+        hipLaunchKernelGGL((tree_join_kernel<T, D, ROWS>), dim3((unsigned)jblocks), dim3(256), 0, s, a);
+        return FTK_OK;
+      };
+      if ((bad = rows <= 16 * d->cus ? join(std::integral_constant<int, 1>{}) : join(std::integral_constant<int, 4>{}))) return bad;
       return check_launch("tree_join_kernel");
     } else {
       // few rows of many parts: a block to each; only small sequences cut: 16 rows to a wave, most of which have nothing to join
