@@ -1113,22 +1113,23 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   if (ntiles > 0) {
     // V(0) by waves 0 to 3, K(0) by the others, and K(1) behind it
     constexpr int AHEAD = F == kSame ? 0 : 1;                  // codes go through registers a tile earlier
-    if constexpr (PAIRED) {                                    // (both halves; tiles behind the last hold the last keys once more)
+    if constexpr (PAIRED) {                                    // What lies behind the last tile is the nearest 16 keys once more; rows in front of and
+      // behind [lo, hi) that share 16 keys with it come as they are, and no row sees them
       const long long at0 = block_at(half, no{}), at1 = block_at(half + 2, no{});
       if constexpr (F == kSame) {
-        copy(keys, Kb, half, at0, no{});
-        copy(mine, Vb, half, at0, no{});
-        copy(keys, Kb + S::TILE, half + 2, at1, no{});
+        copy(keys, Kb, half, at0, yes{});
+        copy(mine, Vb, half, at0, yes{});
+        copy(keys, Kb + S::TILE, half + 2, at1, yes{});
       } else {
         Bring second = keys;
-        load(keys, half, at0, no{});
-        load(mine, half, at0, no{});
-        load(second, half + 2, at1, no{});
+        load(keys, half, at0, yes{});
+        load(mine, half, at0, yes{});
+        load(second, half + 2, at1, yes{});
         store(keys, Kb);
         store(mine, Vb);
         store(second, Kb + S::TILE);
-        load(mine, half + 2, at1, no{});
-        load(keys, half + 4, block_at(half + 4, no{}), no{});
+        load(mine, half + 2, at1, yes{});
+        load(keys, half + 4, block_at(half + 4, no{}), yes{});
       }
     } else if constexpr (F == kSame) {
       copy(mine, half ? Kb : Vb, 0, block_at(0, no{}), no{});
@@ -1170,13 +1171,13 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
       for (int t = half; t < ntiles + half; t += 2) {          // both halves take as many turns, the last of which may have no tile for waves 4 to 7
         const int bring = t + ahead;
         if constexpr (F == kSame) {
-          copy(keys, tiles + kcur, bring, next, no{});
-          copy(mine, tiles + vnext, bring - 2, behind, no{});
+          copy(keys, tiles + kcur, bring, next, yes{});
+          copy(mine, tiles + vnext, bring - 2, behind, yes{});
         } else {
           store(keys, tiles + kcur);
           store(mine, tiles + vnext);
-          load(keys, bring, next, no{});
-          load(mine, bring - 2, behind, no{});
+          load(keys, bring, next, yes{});
+          load(mine, bring - 2, behind, yes{});
         }
         behind = next;
         next = block_at(bring + 2, no{});
@@ -1840,7 +1841,7 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
   Plan p;
   const long long most = max_queries > 0 ? std::min(max_queries, b.tokens) : b.tokens;   // new tokens of a sequence
   const long long most_rows = most * group, rows = (long long)b.tokens * heads;
-  p.narrow = most_rows <= (tree && getenv("NARROW") ? atoi(getenv("NARROW")) : 64);
+  p.narrow = most_rows <= (tree ? 16 : 64);
   const long long capacity = (long long)b.width << page_shift;
   long long seen = max_keys > 0 ? std::min<long long>(max_keys, capacity) : capacity;
   if (window > 0) seen = std::min(seen, most + window + 64);   // from the first key that the first new token sees, down to a multiple of 64

@@ -87,7 +87,7 @@ def _tree_case(core, dtype, cache, D, page, heads, G, new, lens, seed, kind='any
         k, v = k.half().double(), v.half().double()
     at = batch['starts']
     want = ref.attention(q[:at[-1]], k, v, batch | dict(tokens=at[-1]), heads, scale, lambda b, n, first, length: ref.tree_sees(parents[at[b]:at[b + 1]], n, first, length, window))
-    narrow = (most or batch['tokens']) * G <= 64 if narrow is None else narrow
+    narrow = (most or batch['tokens']) * G <= 16 if narrow is None else narrow
     bound = base.attention_bounds_by_largest(want, dtype, D, split=narrow)
     lse_bound = base.attention_bounds(want, dtype, D)[1]
     o, got_lse = o.cpu().double(), got_lse.cpu().double()
@@ -134,7 +134,7 @@ def test_windows_over_trees(core, window, kind, dtype, cache, D, page, heads, G,
 def test_trees_behind_long_sequences_in_parts(core, dtype, cache, D, page, heads, G, new, lens, window):
     _tree_case(core, dtype, cache, D, page, heads, G, new, lens, 320, window=window)
     _tree_case(core, dtype, cache, D, page, heads, G, new, lens, 320, window=window, hints=False, workspace=torch.empty(0, dtype=torch.uint8, device='cuda'),
-               narrow=sum(new) * G <= 64)
+               narrow=sum(new) * G <= 16)
 
 
 @pytest.mark.parametrize('dtype,cache', [(F16, None), (BF16, E4M3)])
