@@ -21,7 +21,9 @@
 //
 // TREE: the new tokens of a sequence are a tree of drafts.  Each sees the cache in front of them, its ancestors and itself, so that only the tiles that hold new tokens'
 // own keys differ: there a row has a bit for each of those keys, found by walking up from it through the parents, a lane a row, which are passed from lane to
-// lane.  (Position and depth differ in a tree; a window counts the steps on the way.)
+// lane.  (Position and depth differ in a tree; a window counts the steps on the way.)  The narrow form has up to 16 rows of them, and the wide form
+// more, their weights rounded once: up to 128 rows by both halves of a workgroup, on different keys, and the work of sequences of different lengths shared
+// out evenly.  (16 sequences of 2064 to 8192 positions in int8, 8 heads of keys, 40 rows: 76 us, 118 by the narrow form; 64 rows: 78 and 119.)
 #pragma once
 
 #include <float.h>
@@ -69,8 +71,8 @@ struct AttnArgs {
   long long small_first;                      // parts of small sequences stand behind these many
   float *part_o, *part_ml;                    // [tokens * heads][cut.nparts] parts, then [sequences][kv heads][kSmallRows][small.nparts]: D floats; two
   const int* parents;                         // trees: of each packed row, by its number among the sequence's new tokens; negative: none
-  int shares, grain_shift, row_blocks;        // trees, wide: workgroups of a kv head that the work is shared out to (0: a workgroup to a block of rows), of
-                                              // grains of 2^grain_shift keys; blocks of kPairedRows rows that a sequence may have
+  int shares, grain_shift, block_rows, row_blocks;   // trees, wide: workgroups of a kv head that the work is shared out to (0: a workgroup to a block of rows), of
+                                              // grains of 2^grain_shift keys; rows of a block of them, and blocks that a sequence may have
 };
 
 // ---- which rows and which keys a workgroup has ----------------------------------------
@@ -210,6 +212,7 @@ __device__ __forceinline__ void walk_up(const AttnArgs& a, const Job& j, int tok
     int next = __shfl(up[0], at & 63);
 #pragma unroll
     for (int c = 1; c < CHUNKS; ++c) {
+      if (64 * c >= j.n) break;
       const int x = __shfl(up[c], at & 63);
       if (at >> 6 == c) next = x;
     }
@@ -739,7 +742,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_narrow_kernel(AttnArgs a
 constexpr int kWideWaves = 8, kWideRows = 32 * kWideWaves, kPairedRows = kWideRows / 2;
 constexpr float kMostSum = 32768.0f;          // a lane's sum of 32 weights above this moves the reference, to where it is at most 32 * 2^kLift
 
-template <int D, bool PAIRED>
+template <int D, bool TREE, bool PAIRED>
 struct WideShape {
   static constexpr int BYTES = 2 * D, TILE = 64 * BYTES;
   static constexpr int ROWS = PAIRED ? kPairedRows : kWideRows;
@@ -750,8 +753,8 @@ struct WideShape {
   static constexpr int ENDS = kWideWaves * 32 * ORS;           // PAIRED: four waves' rows, and what the other four have of them
   static constexpr int TILES_LDS = RING + NOTES > ENDS ? RING + NOTES : ENDS;
   static constexpr int WORDS = kTreeMost / 64 + 1;             // TREE, behind those: of each row, which new tokens it sees
-  static constexpr int LDS = TILES_LDS + (PAIRED ? ROWS * WORDS * 8 : 0);
-  static_assert(!PAIRED || ROWS * ORS + ROWS * D * 4 + ROWS * 16 <= RING, "what waves 4 to 7 have summed lies in the ring, behind the rows");
+  static constexpr int LDS = TILES_LDS + (TREE ? ROWS * WORDS * 8 : 0);
+  static_assert(!PAIRED || ROWS * ORS + ROWS * D * 4 + ROWS * 32 <= RING, "what halves hand to one another lies in the ring, behind the rows");
 };
 
 // V: the transposing read of a 32-lane pass covers 4 keys x 64 bytes, which these bring into four different groups of 64 bytes
@@ -762,10 +765,9 @@ __device__ __forceinline__ int v_swizzle(int row) {
   else return 0;                                               // rows of 192 and 64 bytes lie that way
 }
 
-template <typename T, KvFormat F, int D, bool TREE>
+template <typename T, KvFormat F, int D, bool TREE, bool PAIRED>
 __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, int kv_head, unsigned char* smem) {
-  constexpr bool PAIRED = TREE;
-  using S = WideShape<D, PAIRED>;
+  using S = WideShape<D, TREE, PAIRED>;
   using v8 = typename T::v8;
   using scalar = typename T::scalar;
   constexpr int DS = D / 16, DT = D / 32, CH = S::BYTES / 16;
@@ -1084,10 +1086,12 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
       const v8 p = step == 0 ? pf[0][0] : step == 1 ? pf[0][1] : step == 2 ? pf[1][0] : pf[1][1];
       const int key0 = base + 64 * t + 16 * step + 4 * hh;
       unsigned seen = 0;
+      unsigned long long drawn = 0;
+      if constexpr (TREE) drawn = way_of(t) >> (16 * step + 4 * hh);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int in = 8 * (e >> 2) + (e & 3), key = key0 + in;
-        if (key >= my_lo && key < my_hi) seen |= 1u << e;
+        if (TREE ? (drawn >> in & 1) != 0 : key >= my_lo && key < my_hi) seen |= 1u << e;
       }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
@@ -1146,13 +1150,13 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
     const int ahead = PAIRED ? 2 * (2 + AHEAD) : (half ? 2 : 1) + AHEAD;          // S(t) asks for tile t + ahead; PAIRED: that one of K, the one before it of V
     const int asked = (PAIRED ? half : 0) + ahead;
     long long next = PAIRED || asked < ntiles ? block_at(asked, no{}) : 0;
-    if constexpr (TREE) {
+    if (TREE && (j.hi > (j.first & ~63) || a.window > 0)) {    // (no tile of another part has a word)
       unsigned long long bits[S::WORDS];
       int depth;
       const int before = j.first & 63;                         // keys in front of the new tokens in the first word
       walk_up<S::WORDS>(a, j, row / a.group, before, bits, &depth);
       bits[0] |= (1ULL << before) - 1;
-      if (hh == 0 && half == 0) {
+      if (hh == 0 && (!PAIRED || half == 0)) {
 #pragma unroll
         for (int w = 0; w < S::WORDS; ++w) ways[w] = bits[w];
       }
@@ -1249,39 +1253,51 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
       if (!half) phase_barrier();
     }
   }
-  if constexpr (PAIRED) {                                      // waves 4 to 7 leave what they have, and waves 0 to 3 take it
+  // PAIRED: each half has the first or the last of the columns in the end, and hands the others over
+  const auto columns = [&](auto&& f) __attribute__((always_inline)) {
+    static_for<DT>([&](auto dt) __attribute__((always_inline)) {
+      if (!PAIRED || (decltype(dt)::value < (DT + 1) / 2) == (half == 0)) f(dt);
+    });
+  };
+  if constexpr (PAIRED) {
     v4f* const so = reinterpret_cast<v4f*>(smem + S::ROWS * S::ORS) + cw * (DT * 4 * 64) + lane;
     float* const sml = reinterpret_cast<float*>(smem + S::ROWS * (S::ORS + D * 4)) + (cw * 64 + lane) * 2;
     __syncthreads();
-    if (half) {
+    static_for<DT>([&](auto dt_c) __attribute__((always_inline)) {
+      constexpr int dt = decltype(dt_c)::value;
+      if ((dt < (DT + 1) / 2) == (half != 0)) {
 #pragma unroll
-      for (int i = 0; i < DT * 4; ++i) so[64 * i] = v4f{o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1], o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]};
-      sml[0] = ref;
-      sml[1] = l;
-    }
+        for (int g = 0; g < 4; ++g) so[64 * (4 * dt + g)] = v4f{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+      }
+    });
+    sml[8 * 64 * half] = ref;
+    sml[8 * 64 * half + 1] = l;
     __syncthreads();
-    if (half) return;
-    const float its = sml[0], top = fmaxf(ref, its), wa = __builtin_amdgcn_exp2f(ref - top), wb = __builtin_amdgcn_exp2f(its - top);
+    const float its = sml[8 * 64 * (1 - half)], top = fmaxf(ref, its), wa = __builtin_amdgcn_exp2f(ref - top), wb = __builtin_amdgcn_exp2f(its - top);
     ref = top;
-    l = l * wa + sml[1] * wb;
+    l = l * wa + sml[8 * 64 * (1 - half) + 1] * wb;
+    columns([&](auto dt_c) __attribute__((always_inline)) {
+      constexpr int dt = decltype(dt_c)::value;
 #pragma unroll
-    for (int i = 0; i < DT * 4; ++i) {
-      const v4f x = so[64 * i];
+      for (int g = 0; g < 4; ++g) {
+        const v4f x = so[64 * (4 * dt + g)];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i / 4][4 * (i % 4) + e] = o[i / 4][4 * (i % 4) + e] * wa + x[e] * wb;
-    }
+        for (int e = 0; e < 4; ++e) o[dt][4 * g + e] = o[dt][4 * g + e] * wa + x[e] * wb;
+      }
+    });
   }
   l += __shfl_xor(l, 32);
   if (j.parts > 1) {
     if (wrow0 + jr < j.rows) {
-      const long long left = PAIRED ? j.left + in_rows + jr : r.at * a.cut.nparts + j.part;
+      const long long left = TREE ? j.left + in_rows + jr : r.at * a.cut.nparts + j.part;
       float* const po = a.part_o + left * D;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+      columns([&](auto dt_c) __attribute__((always_inline)) {
+        constexpr int dt = decltype(dt_c)::value;
 #pragma unroll
         for (int g = 0; g < 4; ++g)
           *reinterpret_cast<v4f*>(po + 32 * dt + 8 * g + 4 * hh) = v4f{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
-      if (hh == 0) {
+      });
+      if (hh == 0 && (!PAIRED || half == 0)) {
         float* const ml = a.part_ml + 2 * left;
         ml[0] = ref;
         ml[1] = l;
@@ -1289,24 +1305,24 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
     }
     return;
   }
-  if (idle) return;
-  // the wave turns its 32 x D tile round through LDS (nobody reads tiles any more) and stores whole rows
+  if (!PAIRED && idle) return;
+  // the wave (PAIRED: two of them) turns its 32 x D tile round through LDS (nobody reads tiles any more) and stores whole rows
   const bool none = r.hi <= r.lo || (TREE && r.loose && l == 0.0f);
   const float inv = none ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+  unsigned char* const ot = smem + in_rows * S::ORS;
+  columns([&](auto dt_c) __attribute__((always_inline)) {
+    constexpr int dt = decltype(dt_c)::value;
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[dt][e] = finite_or_nan(o[dt][e]);
-  unsigned char* const ot = smem + wave * (32 * S::ORS);
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int g = 0; g < 4; ++g)
       *reinterpret_cast<v2u*>(ot + jr * S::ORS + 2 * (32 * dt + 8 * g + 4 * hh)) =
           v2u{T::pack(o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv), T::pack(o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv)};
-  if (a.lse && hh == 0 && wrow0 + jr < j.rows) a.lse[r.at] = none ? -INFINITY : log_sum(ref, l);
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  for (int idx = lane; idx < 32 * CH; idx += 64) {
+  });
+  if (a.lse && hh == 0 && wrow0 + jr < j.rows && (!PAIRED || half == 0)) a.lse[r.at] = none ? -INFINITY : log_sum(ref, l);
+  if constexpr (PAIRED) __syncthreads();
+  else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  for (int idx = lane + (PAIRED ? 64 * half : 0); idx < 32 * CH; idx += PAIRED ? 128 : 64) {
     const int rw = idx / CH, c = idx - rw * CH;
     if (wrow0 + rw >= j.rows) break;
     const Row to = row_of<TREE>(a, j, kv_head, wrow0 + rw);
@@ -1317,23 +1333,24 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
 // Trees: how the work of a kv head is shared out to `shares` workgroups, which the arrays on the device say alone.  The keys of the sequences that are not small, in
 // grains and one sequence behind the other, are a line for each block of rows (the k-th line of those sequences that have more than k of them), and each
 // workgroup has as many grains of one line, of one sequence or of several, whose block of rows it works on one after the other; a block of rows that more than one
-// workgroup has is left in parts.  (16 sequences of 2064 to 8192 positions, 60 tokens each, 8 heads: @SHARE@)
+// workgroup has is left in parts.  (16 sequences of 2064 to 8192 positions, 60 tokens each, 8 heads: 146 us, 157 with a workgroup
+// for each block of rows and part of a sequence)
 constexpr int kLeastGrains = 4;
 
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-  return __builtin_amdgcn_readfirstlane(x);
+// The sum of the lanes up to a lane's own, from register to register: a shuffle through LDS takes twenty times as long.
+template <int DPP, int ROWS>
+__device__ __forceinline__ int plus_moved(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, DPP, ROWS, 0xf, false);
 }
 __device__ __forceinline__ int wave_scan(int x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
-  return x;
+  x = plus_moved<0x111, 0xf>(x);                               // lanes 1, 2, 4 and 8 to the left in its row of 16
+  x = plus_moved<0x112, 0xf>(x);
+  x = plus_moved<0x114, 0xf>(x);
+  x = plus_moved<0x118, 0xf>(x);
+  x = plus_moved<0x142, 0xa>(x);                               // the last of the row before, into rows 1 and 3
+  return plus_moved<0x143, 0xc>(x);                            // the last of the first half, into the second
 }
+__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
 struct Shares {
   int each;                    // grains
@@ -1347,7 +1364,7 @@ __device__ __forceinline__ int share_work(const AttnArgs& a, int i, int* blocks)
   const int start = min(max(a.batch.starts[i], 0), a.batch.tokens), end = a.batch.starts[i + 1], all = max(a.batch.lens[i], 0);
   const int rows = min(min(max(end, start), a.batch.tokens) - start, kTreeMost) * a.group;
   if (rows <= a.small_rows) return 0;
-  *blocks = min((rows + kPairedRows - 1) / kPairedRows, a.row_blocks);
+  *blocks = min((rows + a.block_rows - 1) / a.block_rows, a.row_blocks);
   const int keys = max(min(all, kv_capacity(a.batch, a.pages.page_shift)) - seq_first_key(a, first_position(all, start, end)), 1);
   return (int)(((long long)keys + (1LL << a.grain_shift) - 1) >> a.grain_shift);
 }
@@ -1364,9 +1381,9 @@ __device__ __forceinline__ Shares share_out(const AttnArgs& a) {
       if (lane == k) s.grains += sum;
     }
   }
-  s.each = max((int)(((long long)wave_sum(s.grains) + a.shares - 1) / a.shares), kLeastGrains);
+  s.each = max((int)(((unsigned)wave_sum(s.grains) + a.shares - 1) / (unsigned)a.shares), kLeastGrains);
   for (;;) {                                                   // (it ends: there are as many shares as lines at least)
-    s.groups = (int)(((long long)s.grains + s.each - 1) / s.each);
+    s.groups = (int)(((unsigned)s.grains + s.each - 1) / (unsigned)s.each);
     const int before = wave_scan(s.groups);
     s.before = before - s.groups;
     if (__builtin_amdgcn_readlane(before, 63) <= a.shares) break;
@@ -1380,8 +1397,8 @@ __device__ __forceinline__ bool share_of(const AttnArgs& a, const Shares& s, int
   for (int k = a.row_blocks; k > 0; --k) {
     const int groups = __builtin_amdgcn_readlane(s.groups, k - 1), here = (groups - done) * k;
     if (w < here) {
-      *at = done + w / k;
-      *line = w % k;
+      *at = done + (int)((unsigned)w / (unsigned)k);
+      *line = (int)((unsigned)w % (unsigned)k);
       return true;
     }
     w -= here;
@@ -1418,9 +1435,9 @@ __device__ __forceinline__ void share_job(const AttnArgs& a, int b, int line, in
   j.n = min(c.n, kTreeMost);
   j.first = c.first;
   j.rows = j.n * a.group;
-  j.row0 = line * kPairedRows;
+  j.row0 = line * a.block_rows;
   j.len = min(c.len, kv_capacity(a.batch, a.pages.page_shift));
-  const long long p_hi = (long long)c.first + (min(j.row0 + kPairedRows, j.rows) - 1) / a.group, key0 = seq_first_key(a, c.first);
+  const long long p_hi = (long long)c.first + (min(j.row0 + a.block_rows, j.rows) - 1) / a.group, key0 = seq_first_key(a, c.first);
   j.hi = clamp_position(p_hi + 1, j.len);
   j.sure_hi = clamp_position(c.first, j.len);
   j.lo = a.window > 0 ? clamp_position((long long)c.first - a.window + 1, j.len) : 0;
@@ -1436,9 +1453,9 @@ __device__ __forceinline__ void share_job(const AttnArgs& a, int b, int line, in
 // any: two (sequence, head, part) each, by four waves that cut the keys as in the narrow kernel.  They read on the compute units that the others
 // leave free, or have left, while those multiply.  (A chunk of 512 tokens beside five sequences that decode, 16 heads, 4 of keys, up to
 // 16384 of them, in int8: 165 us with all on the wide form, 108 so, and 12 for joining.)
-template <typename T, KvFormat F, int D, bool TREE>
+template <typename T, KvFormat F, int D, bool TREE, bool PAIRED>
 __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs a, int wide) {
-  constexpr int R = WideShape<D, TREE>::ROWS;
+  constexpr int R = WideShape<D, TREE, PAIRED>::ROWS;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   Job j;
   if constexpr (!TREE) {
@@ -1481,14 +1498,14 @@ __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs
         if (!find_rows<R>(a, rest, &b, &tile) || !find_job<R, TREE>(a, b, tile, 0, false, j)) return;
         x = end;
       }
-      wide_attention<T, F, D, TREE>(a, j, kv_head, smem);
+      wide_attention<T, F, D, TREE, PAIRED>(a, j, kv_head, smem);
       if (x < end) __syncthreads();
     }
   } else {
     const int slot = rest / a.cut.nparts, part = rest - slot * a.cut.nparts;
     int b, tile;
     if (!find_rows<R>(a, slot, &b, &tile) || !find_job<R, TREE>(a, b, tile, part, false, j)) return;
-    wide_attention<T, F, D, TREE>(a, j, kv_head, smem);
+    wide_attention<T, F, D, TREE, PAIRED>(a, j, kv_head, smem);
   }
 }
 
@@ -1649,7 +1666,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(AttnArgs a) {
   // where the first part of each row is, the second, and how far those behind are from one another
   int n[ROWS], line = -1, begin = 0, grains = 0;
   long long part0[ROWS], part1[ROWS];
-  const long long step = a.shares > 0 ? 2LL * a.pages.heads * kPairedRows : 1;
+  const long long step = a.shares > 0 ? 2LL * a.pages.heads * a.block_rows : 1;
   bool few = true;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
@@ -1659,16 +1676,16 @@ __global__ __launch_bounds__(256) void tree_join_kernel(AttnArgs a) {
       part0[r] = ((long long)token * a.heads + head) * a.cut.nparts;
       part1[r] = part0[r] + 1;
     } else {
-      if (line != row / kPairedRows) {
-        line = row / kPairedRows;
+      if (line != row / a.block_rows) {
+        line = row / a.block_rows;
         if (line >= a.row_blocks) return;
         share_find(a, line, 0, b, &begin, &grains);
       }
       const int group0 = begin / s.each;
       n[r] = (begin + max(grains, 1) - 1) / s.each - group0 + 1;
       const long long slot = ((long long)(__builtin_amdgcn_readlane(s.before, line) + group0) * a.pages.heads + kv_head) * 2;
-      part0[r] = (slot + (begin > group0 * s.each)) * kPairedRows + row % kPairedRows;
-      part1[r] = slot * kPairedRows + row % kPairedRows + step;
+      part0[r] = (slot + (begin > group0 * s.each)) * a.block_rows + row % a.block_rows;
+      part1[r] = slot * a.block_rows + row % a.block_rows + step;
     }
     few = few && n[r] <= FEW;
   }
@@ -1786,7 +1803,7 @@ struct Plan {
   Cut cut, small;
   int small_rows;
   size_t large, all;       // parts that there is room for: of sequences that are not small, and with those that are
-  int shares, grain_shift; // trees, wide
+  int shares, grain_shift, block_rows; // trees, wide
 };
 
 static size_t parts_of(long long rows, int nparts) { return nparts > 1 ? (size_t)rows * nparts : 0; }
@@ -1850,7 +1867,8 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
   // units.  (16 sequences of up to 4096 keys, 8 heads of them, 20 rows: 48 us by 32 rows and 54 by 16 at D 128, int8 46 and 48, 25 and 28 at D 64; 48 rows: 65 and 67, int8 69 and 71, but
   // 38 and 34 at D 64; two sequences of up to 1000 keys, 48 rows: 15 and 12.)
   p.nq = most_rows <= 16 || (p.narrow && ((most_rows + 31) / 32) * b.sequences * pages.heads * ((keys + 255) / 256) < cus) ? 1 : 2;
-  const int R = p.narrow ? 16 * p.nq : tree ? kPairedRows : kWideRows;
+  p.block_rows = most_rows <= kPairedRows ? kPairedRows : kWideRows;
+  const int R = p.narrow ? 16 * p.nq : tree ? p.block_rows : kWideRows;
   const long long per_seq = (most_rows + R - 1) / R, packed = (long long)b.tokens * group / R + b.sequences;
   // numbered by row blocks, unless most of such slots would be empty (as those of narrow workgroups, four to a sequence at most, cannot be)
   p.slots_per_seq = p.narrow || b.sequences * per_seq <= 2 * packed ? (int)per_seq : 0;
@@ -1867,7 +1885,7 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
   } else if (tree) {
     // Work shared out to as many workgroups as there are compute units, or to twice as many and more where the heads divide those badly; unless
     // a workgroup for each block of rows is expected to be done sooner: us as in wide_cost(), several sequences being two thirds as long as the longest in the mean.
-    const double turn = 2.2 * D / 128, turns = std::ceil(keys / 128.0), units = (double)b.sequences * per_seq * pages.heads;
+    const double turn = (p.block_rows == kPairedRows ? 2.4 : 4.0) * D / 128, turns = std::ceil(keys / 128.0), units = (double)b.sequences * per_seq * pages.heads;
     const double whole = std::ceil(units / cus) * (8.0 + turns * turn);
     p.cut = cut_into(keys, 1);
     while (b.sequences * (double)per_seq * (((double)keys + (1 << p.grain_shift)) / (1 << p.grain_shift)) > 2e9) ++p.grain_shift;
@@ -1884,7 +1902,7 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
     shares = std::max(shares, per_seq);
     const double rounds = std::ceil((double)shares * pages.heads / cus);
     const double shared = 18.0 + rounds * 6.0 + std::max(units * turns * (b.sequences > 1 ? 2.0 / 3 : 1.0) / (shares * pages.heads), (double)kLeastGrains) * turn * rounds;
-    const size_t parts = (size_t)shares * pages.heads * 2 * kPairedRows;
+    const size_t parts = (size_t)shares * pages.heads * 2 * p.block_rows;
     if (shared < whole && per_seq <= 64 && workspace_of(parts, D) <= room) {
       p.shares = (int)shares;
       p.slots = p.shares;
@@ -1987,7 +2005,8 @@ static int attend(const char* who, const void* q, int type, long long q_token_st
   a.small_first = (long long)p.large;
   a.shares = p.shares;
   a.grain_shift = p.grain_shift;
-  a.row_blocks = p.narrow ? 0 : (int)std::min<long long>(((long long)(max_queries > 0 ? std::min(max_queries, a.batch.tokens) : a.batch.tokens) * a.group + kPairedRows - 1) / kPairedRows, INT_MAX);
+  a.block_rows = p.block_rows;
+  a.row_blocks = p.narrow ? 0 : (int)(((max_queries > 0 ? std::min(max_queries, a.batch.tokens) : a.batch.tokens) * (long long)a.group + p.block_rows - 1) / p.block_rows);
   const long long rows = (long long)a.batch.tokens * heads;
   a.part_o = (float*)workspace;
   a.part_ml = a.part_o + p.all * pages->head_size;
@@ -2008,12 +2027,21 @@ static int attend(const char* who, const void* q, int type, long long q_token_st
         return launch_with_lds("paged_narrow_kernel", paged_narrow_kernel<T, F, D, decltype(nq)::value, decltype(kept)::value, TREE>, once, blocks, kWaves, NarrowShape<F, D>::LDS, s,
                                a, p.slots_per_seq);
       };
-      auto with_kept = [&](auto nq) { return p.slots_per_seq == 1 ? launch(nq, no{}) : launch(nq, yes{}); };
-      bad = p.nq == 2 ? with_kept(std::integral_constant<int, 2>{}) : with_kept(std::integral_constant<int, 1>{});
+      if constexpr (TREE) {                                      // (one block of 16 rows to a sequence and head)
+        bad = launch(std::integral_constant<int, 1>{}, no{});
+      } else {
+        auto with_kept = [&](auto nq) { return p.slots_per_seq == 1 ? launch(nq, no{}) : launch(nq, yes{}); };
+        bad = p.nq == 2 ? with_kept(std::integral_constant<int, 2>{}) : with_kept(std::integral_constant<int, 1>{});
+      }
     } else {
-      static DeviceOnce once;
-      constexpr int lds = std::max(WideShape<D, TREE>::LDS, TREE ? 0 : 2 * NarrowShape<F, D>::LDS);
-      bad = launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D, TREE>, once, blocks + pairs, kWideWaves, lds, s, a, (int)blocks);
+      auto launch = [&](auto paired) -> int {
+        static DeviceOnce once;
+        constexpr bool PAIRED = decltype(paired)::value;
+        constexpr int lds = std::max(WideShape<D, TREE, PAIRED>::LDS, TREE ? 0 : 2 * NarrowShape<F, D>::LDS);
+        return launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D, TREE, PAIRED>, once, blocks + pairs, kWideWaves, lds, s, a, (int)blocks);
+      };
+      if constexpr (TREE) bad = a.block_rows == kPairedRows ? launch(std::true_type{}) : launch(std::false_type{});
+      else bad = launch(std::false_type{});
     }
     if (bad || p.all == 0) return bad;
     if constexpr (TREE) {
