@@ -1888,7 +1888,8 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
     const double turn = (p.block_rows == kPairedRows ? 2.4 : 4.0) * D / 128, turns = std::ceil(keys / 128.0), units = (double)b.sequences * per_seq * pages.heads;
     const double whole = std::ceil(units / cus) * (8.0 + turns * turn);
     p.cut = cut_into(keys, 1);
-    while (b.sequences * (double)per_seq * (((double)keys + (1 << p.grain_shift)) / (1 << p.grain_shift)) > 2e9) ++p.grain_shift;
+    // (whatever lengths the device finds: their sums have 32 bits)
+    while (b.sequences * (double)per_seq * ((double)std::min<long long>(capacity, INT_MAX) / (1 << p.grain_shift) + 1.0) > 1e9) ++p.grain_shift;
     long long shares = 0;
     double used = 0.0;
     for (int rounds = 1; rounds <= 4 && used < 0.9; ++rounds) {

@@ -10,6 +10,8 @@ kernel calls on FractalTensors that live on the GPU.
   windowed_attention  shifted_slide + the map of sparse_attn of examples/sparse_attention/sparse_attention.py:25-71
   kv_cache_write, kv_cache_read, paged_attention, verify_drafts   serving: the new tokens of a batch of sequences and a paged cache
                  of keys and values; one sequence is one item of a FractalTensor, of any length
+  paged_tree_attention, verify_tree, kv_cache_keep   the same with trees of drafts: what a target model makes of one in a step, and the cache behind it
+  kv_cache_select, kv_cache_keep   caches of limited length: which positions stay, by the weights that paged_attention gathers, and moving those
 
 A regular (non-ragged) FractalTensor already is a dense row-major tensor in
 its flat buffer, so inputs are handed to the kernels as views and outputs are
@@ -29,7 +31,7 @@ from ..types import FractalTensorStorage, TensorStorage, torch_type_to_internal_
 
 __all__ = ['pack_lstm_weights', 'pad_time_major', 'unpad_time_major', 'stacked_lstm', 'dilated_lstm', 'lstm_cell', 'flash_attention', 'b2b_gemm', 'mm',
            'online_softmax', 'embedding_lookup', 'grid_rnn', 'windowed_attention', 'kv_cache_write', 'kv_cache_read', 'paged_attention',
-           'verify_drafts']
+           'verify_drafts', 'paged_tree_attention', 'verify_tree', 'kv_cache_select', 'kv_cache_keep']
 
 
 def _core():
@@ -400,16 +402,88 @@ def kv_cache_read(k_pages, v_pages, table, lens, counts: Sequence[int], dtype=to
 
 
 def paged_attention(qss: FractalTensor, k_pages, v_pages, table, lens, k_exps=None, v_exps=None, scale: Optional[float] = None, causal: bool = True,
-                    window: int = 0, max_keys: int = 0, dtype: Optional[torch.dtype] = None) -> FractalTensor:
+                    window: int = 0, max_keys: int = 0, dtype: Optional[torch.dtype] = None, weights: Optional[torch.Tensor] = None,
+                    decay: float = 1.0) -> FractalTensor:
     """Attention of new tokens, [sequence][token] of [heads, D], over a paged cache that holds their keys and values already (kv_cache_write): one
     token a sequence, drafted ones, chunks of prompts and whole prompts, in any mixture.  heads is a multiple of the cache's.  `scale` multiplies the
     scores and defaults to 1.0, as in flash_attention.  causal: a token sees the positions up to its own; window > 0: no more than that many of them.
     max_keys: the greatest of lens where the program knows it.  The result has the structure and the type of qss; a token that sees nothing gets zeros.
-    dtype: what the computation runs in on codes of 8 bits, that which they were written in: fp16 (the default) or bf16."""
+    dtype: what the computation runs in on codes of 8 bits, that which they were written in: fp16 (the default) or bf16.
+    weights [pages, kv heads, page size] fp32: what each position gets of the new tokens' attention is added there, behind a product of what older ones had with decay
+    (for kv_cache_select); new positions begin at zero."""
     q, counts = _new_tokens(qss, 'qss', k_pages, dtype)
-    o = _core().paged_attention(q, k_pages, v_pages, table, lens, _starts(counts, q.device), k_exps, v_exps, 1.0 if scale is None else float(scale), causal, window,
-                                max(counts, default=0), max_keys)
+    core, starts, scale, most = _core(), _starts(counts, q.device), 1.0 if scale is None else float(scale), max(counts, default=0)
+    o = core.paged_attention(q, k_pages, v_pages, table, lens, starts, k_exps, v_exps, scale, causal, window, most, max_keys, return_lse=weights is not None)
+    if weights is not None:
+        o, lse = o
+        core.kv_cache_weigh(q, lse, k_pages, weights, table, lens, starts, k_exps, scale, decay, causal, window, most, max_keys)
     return _by_sequence(o.to(qss.data.dtype), counts)
+
+
+def _integers(ft: FractalTensor, name: str, counts, dtypes=(torch.int32, torch.int64)) -> torch.Tensor:
+    """[sequence][token] of [1] integers, counts[b] tokens in sequence b -> packed [tokens]."""
+    if not isinstance(ft, FractalTensor):
+        raise TypeError(f'{name} should be a FractalTensor.')
+    if ft.depth != 2 or ft.element_size != 1:
+        raise ValueError(f'{name} should have depth 2 and hold single integers, got depth {ft.depth} of {list(ft.element_shape)}.')
+    if ft._T is None or not ft.has_indices:
+        raise RuntimeError('FractalTensor is not initialized.')
+    if not ft.data.is_cuda:
+        raise RuntimeError(f'{name} lives on {ft.data.device}; the fused kernels run on the GPU only.')
+    if ft.data.dtype not in dtypes:
+        raise TypeError(f'{name} should be int32 or int64, got {ft.data.dtype}.')
+    if counts is not None and ft.width_by_depth(1) != counts:
+        raise ValueError(f'{name} should have {counts} tokens a sequence, got {ft.width_by_depth(1)}.')
+    return ft.data.reshape(-1)
+
+
+def paged_tree_attention(qss: FractalTensor, parentss: FractalTensor, k_pages, v_pages, table, lens, k_exps=None, v_exps=None, scale: Optional[float] = None,
+                         window: int = 0, max_keys: int = 0, dtype: Optional[torch.dtype] = None) -> FractalTensor:
+    """paged_attention of new tokens that form a tree in each sequence, at most 256 of them: each sees what is in front of its sequence's new tokens, its ancestors and
+    itself.  parentss: [sequence][token] of [1] int32 or int64, the number of a token's parent among its sequence's new tokens, one in front of it; negative: none.
+    window > 0: the last that many on the way that ends with the token.  All else as in paged_attention."""
+    q, counts = _new_tokens(qss, 'qss', k_pages, dtype)
+    parents = _integers(parentss, 'parentss', counts).to(torch.int32)
+    o = _core().paged_tree_attention(q, k_pages, v_pages, table, lens, _starts(counts, q.device), parents, k_exps, v_exps, 1.0 if scale is None else float(scale), window,
+                                     max(counts, default=0), max_keys)
+    return _by_sequence(o.to(qss.data.dtype), counts)
+
+
+def verify_tree(targets: FractalTensor, tokens: FractalTensor, parentss: FractalTensor, uniforms: torch.Tensor):
+    """The path through each sequence's tree of drafts that the target model's own draws follow: (nextss, path).
+
+    tokens: [B][n] of [1] int32 or int64, in each sequence the last token that is known, which is the root, and behind it the drafts; parentss: as in
+    paged_tree_attention; targets: [B][n] of [1, V], the target's probabilities of what follows each token.  uniforms [B, M]: uniform numbers of [0, 1), fp32, one
+    for each draw.  nextss, [B][token] of [1]: what was drawn, the accepted drafts and one token more (nothing for a sequence without tokens).  path [B, M] int32: the
+    places of the tokens that stay in the cache, behind them -1, for kv_cache_keep."""
+    ids = _integers(tokens, 'tokens', None)
+    counts = tokens.width_by_depth(1)
+    parents = _integers(parentss, 'parentss', counts).to(torch.int32)
+    if not isinstance(targets, FractalTensor):
+        raise TypeError('targets should be a FractalTensor.')
+    if targets.depth != 2 or len(targets.element_shape) != 2 or targets.element_shape[0] != 1:
+        raise ValueError(f'targets should have depth 2 and [1, V] items, got depth {targets.depth} of {list(targets.element_shape)}.')
+    if targets.width_by_depth(1) != counts:
+        raise ValueError(f'targets should have {counts} tokens a sequence, got {targets.width_by_depth(1)}.')
+    drawn, path, _ = _core().verify_tree(targets.data.reshape(-1, targets.element_shape[1]), ids, parents, _starts(counts, ids.device), uniforms)
+    there = drawn >= 0
+    return _by_sequence(drawn[there].reshape(-1, 1), there.sum(1).tolist()), path
+
+
+def kv_cache_select(weights: torch.Tensor, table, lens, budget: int, sinks: int = 0, recent: int = 0, max_keys: int = 0) -> torch.Tensor:
+    """The positions of every sequence and head that a cache of `budget` positions keeps, [B, kv heads, budget] int32, ascending, then -1 (for kv_cache_keep): the first
+    `sinks`, the last `recent`, and of the others those of the largest weights (paged_attention), of equal ones the earlier.  max_keys: the greatest of lens where the
+    program knows it."""
+    return _core().kv_cache_select(weights, table, lens, budget, sinks, recent, max_keys)
+
+
+def kv_cache_keep(k_pages, v_pages, table, lens, kept: torch.Tensor, counts: Optional[Sequence[int]] = None, k_exps=None, v_exps=None,
+                  weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Moves the positions that stay together, in place, and returns the new lens [B] int32: kept [B, M], or [B, kv heads, M] with as many in each head of a sequence, int32,
+    ascends and has -1 behind its end.  It counts from a sequence's begin (kv_cache_select), or with counts, the number of new tokens of each sequence, from the first of
+    these (verify_tree).  weights: theirs move with them."""
+    starts = None if counts is None else _starts([int(n) for n in counts], k_pages.device)
+    return _core().kv_cache_keep(k_pages, v_pages, table, lens, kept, starts, k_exps, v_exps, weights)
 
 
 def _padded(ft: FractalTensor, name: str, counts) -> torch.Tensor:

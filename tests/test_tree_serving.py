@@ -189,3 +189,20 @@ def test_reference_verification():
     assert [t.tolist() for t in got] == [[[2, 1, -1]], [[0, 2, -1]], [1]]
     got = ref.verify(p, ids, parents, [0, 3], torch.tensor([[0.0]]))
     assert [t.tolist() for t in got] == [[[1]], [[0]], [0]]
+
+
+def test_fractal_tensors_are_refused_by_name():
+    from fractaltensor_amd.kaleido import FractalTensor, operations as ops
+    pages, table, lens = torch.zeros((2, 2, 16, 32), dtype=torch.float16), torch.zeros((2, 1), dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    q = FractalTensor.from_dense(torch.zeros((2, 3, 4, 32), dtype=torch.float16), 2)
+    ids = FractalTensor.from_dense(torch.zeros((2, 3, 1), dtype=torch.int64), 2)
+    for call, error, text in (
+            (lambda: ops.fused.paged_tree_attention(q, ids, pages, pages, table, lens), RuntimeError, 'qss lives on cpu'),
+            (lambda: ops.fused.paged_tree_attention(table, ids, pages, pages, table, lens), TypeError, 'qss should be a FractalTensor'),
+            (lambda: ops.fused.verify_tree(q, ids, ids, torch.zeros(2, 2)), RuntimeError, 'tokens lives on cpu'),
+            (lambda: ops.fused.verify_tree(q, table, ids, torch.zeros(2, 2)), TypeError, 'tokens should be a FractalTensor'),
+            (lambda: ops.fused.verify_tree(q, q, ids, torch.zeros(2, 2)), ValueError, 'single integers'),
+            (lambda: ops.fused.kv_cache_select(table, table, lens, 3), (TypeError, RuntimeError, ValueError), 'weights'),
+            (lambda: ops.fused.kv_cache_keep(pages, pages, table, lens, table), (TypeError, RuntimeError, ValueError), 'k_pages')):
+        with pytest.raises(error, match=text):
+            call()

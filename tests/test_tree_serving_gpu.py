@@ -137,6 +137,53 @@ def test_trees_behind_long_sequences_in_parts(core, dtype, cache, D, page, heads
                narrow=sum(new) * G <= 16)
 
 
+@pytest.mark.parametrize('dtype,cache,D,page,heads,G,new,lens,window', [
+    (BF16, E4M3, 64, 64, 3, 8, [(7 * i) % 6 + 1 for i in range(70)], [40 + (1237 * i) % 2600 for i in range(69)] + [3000], 0),
+    (F16, None, 32, 32, 2, 8, [60, 0, 33, 5, 1, 40], [5000, 10, 3000, 700, 2500, 64], 0),
+    (F16, I8, 128, 16, 1, 4, [30, 32, 9, 1, 0, 17], [4000, 1000, 2500, 30, 7, 3333], 700),
+    (BF16, None, 96, 128, 5, 2, [17, 64, 3], [2100, 6000, 129], 0),
+    (BF16, I8, 64, 32, 1, 16, [100, 3, 50], [3000, 3500, 2900], 0)])
+def test_trees_of_sequences_of_different_lengths_shared_out(core, dtype, cache, D, page, heads, G, new, lens, window):
+    """Blocks of rows and sequences that workgroups share, begin and end in: more than 64 of them, several blocks of rows in some and none in others."""
+    _tree_case(core, dtype, cache, D, page, heads, G, new, lens, 325, window=window, tail=1)
+    _tree_case(core, dtype, cache, D, page, heads, G, new, lens, 325, window=window, workspace=torch.empty(0, dtype=torch.uint8, device='cuda'))
+
+
+def test_one_graph_for_lengths_that_change(core):
+    """The arrays on the device alone say how the work is shared out: each replay against the eager result, with other lengths and numbers of new tokens."""
+    heads, G, D, page, most = 2, 4, 64, 32, 40
+    g = torch.Generator().manual_seed(340)
+    batch = base.make_batch([most] * 4, [6000] * 4, page, 341)
+    pages = _cuda(base.make_pages(batch, heads, D, E4M3, BF16, 342))
+    table = _ints(batch['table'])
+    lens, starts, parents = _ints([6000] * 4), _ints([0, most, 2 * most, 3 * most, 4 * most]), _ints(_trees([most] * 4, 343))
+    q = torch.randn((4 * most, heads * G, D), generator=g).to(BF16).cuda()
+    out, lse = torch.zeros_like(q), torch.zeros(q.shape[:2], device='cuda')
+    size = core.paged_tree_attention_workspace_bytes(q, pages[0], table, most, 6000)
+    assert size > 0
+    space = torch.empty(size, dtype=torch.uint8, device='cuda')
+    call = lambda o, z, w: core.paged_tree_attention(q, *pages[:2], table, lens, starts, parents, *pages[2:], max_queries=most, max_keys=6000, out=o, return_lse=z, workspace=w)
+    call(out, lse, space)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out, lse, space)
+    for new, length in (([40, 40, 40, 40], [6000, 6000, 6000, 6000]), ([1, 40, 0, 7], [50, 6000, 3, 4000]), ([40, 5, 5, 5], [40, 5, 5, 5]), ([30, 30, 30, 30], [777, 6000, 5999, 31])):
+        at = [0]
+        for n in new:
+            at.append(at[-1] + n)
+        lens.copy_(_ints(length))
+        starts.copy_(_ints(at))
+        parents[:at[-1]] = _ints(_trees(new, 344))
+        out.fill_(7.0)
+        lse.fill_(7.0)
+        graph.replay()
+        o, z = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device='cuda')
+        call(o, z, None)
+        torch.cuda.synchronize()
+        assert torch.equal(_bits(out), _bits(o)) and torch.equal(lse, z) and bool((out[at[-1]:] == 7).all())
+
+
 @pytest.mark.parametrize('dtype,cache', [(F16, None), (BF16, E4M3)])
 def test_a_chain_is_what_a_tree_without_branches_is(core, dtype, cache):
     """What attention of new tokens one behind the other gives.  Trees have their keys summed in another order, and where many rows share a head's keys each weight is
@@ -457,6 +504,11 @@ def test_selected_positions_of_long_sequences(core, kind, lens, budget):
     _select_case(core, lens, 256, 1, budget, 4, 100, KINDS[kind], 610)
 
 
+@pytest.mark.parametrize('kind', ['normal', 'few values', 'all bits'])
+def test_selected_positions_of_the_longest_sequences(core, kind):
+    _select_case(core, [524288 + 77, 131073], 1024, 1, 20000, 4, 100, KINDS[kind], 615)
+
+
 def test_selection_on_tables_that_point_nowhere(core):
     _select_case(core, [300, 100], 16, 2, 90, 2, 3, KINDS['normal'], 620, table=lambda t: [[10 ** 9 if i % 3 == 1 else -5 if i % 3 == 2 else x for i, x in enumerate(row)] for row in t])
     got = core.kv_cache_select(torch.rand((2, 1, 16), device='cuda'), _ints([[0, 1]]), _ints([10 ** 9]), 20)     # a length past the table
@@ -505,6 +557,11 @@ def test_many_sequences_and_heads_move_at_once(core):
     lens = [200 + 11 * i for i in range(24)]
     _keep_case(core, BF16, E4M3, 128, 32, 16, lens, _lists(lens, 16, 256, 710, 0.6), 711)
     _keep_case(core, F16, None, 32, 16, 16, lens, _lists(lens, 16, 500, 712, 0.9), 713, weights=False)
+
+
+def test_lists_of_thousands_of_rows(core):
+    lens = [9000, 2049, 7001]
+    _keep_case(core, F16, I8, 64, 64, 2, lens, _lists(lens, 2, 6500, 714, 0.8), 715)
 
 
 def test_paths_of_trees_move_behind_the_cache(core):
@@ -763,3 +820,58 @@ def test_refusals_on_the_device(core):
                         (core.FtkError, (p, ids, parents, starts, torch.rand((2, 65), device='cuda'))), (core.FtkError, (p, ids, parents, starts, u[:, :0])), (RuntimeError, (p, ids, parents, starts, u.cpu()))):
         with pytest.raises(error):
             core.verify_tree(*args)
+
+
+# ---- FractalTensors --------------------------------------------------------------------------------
+
+def test_a_step_with_a_tree_on_fractal_tensors(core):
+    from fractaltensor_amd.kaleido import FractalTensor, operations as ops
+    heads, G, D, page, V = 2, 2, 64, 16, 300
+    new, lens = [9, 0, 4], [50, 20, 4]
+    g = torch.Generator().manual_seed(900)
+    batch = base.make_batch(new, lens, page, 901)
+    table, dlens, starts = base.on_device(batch)
+    pages = _cuda(base.make_pages(batch, heads, D, E4M3, F16, 902))
+    other = [t.clone() for t in pages]
+    parents = _ints(_trees(new, 903))
+    ft = lambda t: ops.fused._by_sequence(t, new)
+    q = torch.randn((13, heads * G, D), generator=g).half().cuda()
+    o = ops.fused.paged_tree_attention(ft(q), ft(parents.reshape(-1, 1)), *pages[:2], table, dlens, *pages[2:], scale=0.2, window=30, max_keys=50)
+    assert o.width_by_depth(1) == new
+    assert torch.equal(o.data.reshape(13, heads * G, D), core.paged_tree_attention(q, *pages[:2], table, dlens, starts, parents, *pages[2:], 0.2, 30, 9, 50))
+    p = torch.softmax(torch.randn((13, V), generator=g), -1).cuda()
+    ids, u = torch.randint(0, 4, (13,), generator=g).cuda(), torch.rand((3, 4), generator=g).cuda()
+    p[:, 4:] = 0
+    drawn, path = ops.fused.verify_tree(ft(p.reshape(13, 1, V)), ft(ids.reshape(-1, 1)), ft(parents.reshape(-1, 1)), u)
+    want, where, accepted = core.verify_tree(p, ids, parents, starts, u)
+    assert torch.equal(path, where) and drawn.width_by_depth(1) == [int((r >= 0).sum()) for r in want]
+    assert torch.equal(drawn.data.reshape(-1), want[want >= 0])
+    left = ops.fused.kv_cache_keep(*pages[:2], table, dlens, path, new, *pages[2:])
+    assert torch.equal(left, core.kv_cache_keep(*other[:2], table, dlens, where, starts, *other[2:]))
+    assert all(torch.equal(_bits(a), _bits(b)) for a, b in zip(pages, other))
+    with pytest.raises(ValueError, match='tokens a sequence'):
+        ops.fused.paged_tree_attention(ft(q), ops.fused._by_sequence(parents.reshape(-1, 1), [13]), *pages[:2], table, dlens, *pages[2:])
+    with pytest.raises(TypeError, match='int32 or int64'):
+        ops.fused.verify_tree(ft(p.reshape(13, 1, V)), ft(ids.float().reshape(-1, 1)), ft(parents.reshape(-1, 1)), u)
+    with pytest.raises(ValueError, match='single integers'):
+        ops.fused.verify_tree(ft(p.reshape(13, 1, V)), FractalTensor.from_dense(ids, 1), ft(parents.reshape(-1, 1)), u)
+    with pytest.raises(ValueError, match=r'\[1, V\]'):
+        ops.fused.verify_tree(ft(p), ft(ids.reshape(-1, 1)), ft(parents.reshape(-1, 1)), u)
+
+
+def test_a_cache_of_limited_length_on_fractal_tensors(core):
+    from fractaltensor_amd.kaleido import operations as ops
+    heads, G, D, page, new, lens = 2, 2, 64, 16, [3, 30], [60, 30]
+    batch = base.make_batch(new, lens, page, 910)
+    table, dlens, starts = base.on_device(batch)
+    pages = _cuda(base.make_pages(batch, heads, D, None, F16, 911))[:2]
+    q = torch.randn((33, heads * G, D), generator=torch.Generator().manual_seed(912)).half().cuda()
+    weights = torch.rand((batch['pages'], heads, page), generator=torch.Generator().manual_seed(913)).cuda()
+    mine = weights.clone()
+    o = ops.fused.paged_attention(ops.fused._by_sequence(q, new), *pages, table, dlens, scale=0.2, max_keys=60, weights=weights, decay=0.5)
+    want, lse = core.paged_attention(q, *pages, table, dlens, starts, scale=0.2, max_queries=30, max_keys=60, return_lse=True)
+    core.kv_cache_weigh(q, lse, pages[0], mine, table, dlens, starts, None, 0.2, 0.5, max_queries=30, max_keys=60)
+    assert torch.equal(o.data.reshape(33, heads * G, D), want) and torch.equal(weights, mine)
+    kept = ops.fused.kv_cache_select(weights, table, dlens, 25, 2, 5, 60)
+    assert torch.equal(kept, core.kv_cache_select(weights, table, dlens, 25, 2, 5))
+    assert ops.fused.kv_cache_keep(*pages, table, dlens, kept, weights=weights).tolist() == [25, 25]
