@@ -748,8 +748,8 @@ struct WideShape {
   static constexpr int ROWS = PAIRED ? kPairedRows : kWideRows;
   static constexpr int ORS = BYTES + 16;                       // a padded row of the O tiles that the waves turn round at the end
   static constexpr int RING = (PAIRED ? 8 : 5) * TILE;         // two tiles of K, three of V; PAIRED: two of each, twice
-  static constexpr int FLAGS = 64 * D / 8;                     // PAIRED: of a place of V, a bit for each value that was not finite, [key][chunk of 8]
-  static constexpr int NOTES = 64 + (PAIRED ? 4 * FLAGS : 0);  // of each place of V and wave; flags
+  static constexpr int FLAGS = 64 * D / 8;                     // TREE: of a place of V, a bit for each value that was not finite, [key][chunk of 8]
+  static constexpr int NOTES = 64 + (TREE ? 4 * FLAGS : 0);  // of each place of V and wave; flags
   static constexpr int ENDS = kWideWaves * 32 * ORS;           // PAIRED: four waves' rows, and what the other four have of them
   static constexpr int TILES_LDS = RING + NOTES > ENDS ? RING + NOTES : ENDS;
   static constexpr int WORDS = kTreeMost / 64 + 1;             // TREE, behind those: of each row, which new tokens it sees
@@ -1044,7 +1044,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
     for (int i = 0; i < CP; ++i) bad |= not_finite<T>(*reinterpret_cast<const v8*>(vt + cw * (16 * S::BYTES) + 1024 * i + 16 * lane));
     const bool any = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
     if (lane == 0) words[4 * place + cw] = any;
-    if constexpr (PAIRED) {
+    if constexpr (TREE) {
       if (__builtin_expect(any, 0)) {                            // those leave the tile, for 0 x inf, and a bit is left for each
 #pragma unroll 1
         for (int i = 0; i < CP; ++i) {
@@ -1058,7 +1058,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
       }
     }
   };
-  // PAIRED: NaN for the rows that see a key whose value was not finite
+  // TREE: NaN for the rows that see a key whose value was not finite
   auto mark = [&](int t, int place) __attribute__((always_inline)) {
     const unsigned long long drawn = way_of(t);
 #pragma unroll 1
@@ -1086,12 +1086,10 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
       const v8 p = step == 0 ? pf[0][0] : step == 1 ? pf[0][1] : step == 2 ? pf[1][0] : pf[1][1];
       const int key0 = base + 64 * t + 16 * step + 4 * hh;
       unsigned seen = 0;
-      unsigned long long drawn = 0;
-      if constexpr (TREE) drawn = way_of(t) >> (16 * step + 4 * hh);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int in = 8 * (e >> 2) + (e & 3), key = key0 + in;
-        if (TREE ? (drawn >> in & 1) != 0 : key >= my_lo && key < my_hi) seen |= 1u << e;
+        if (key >= my_lo && key < my_hi) seen |= 1u << e;
       }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
@@ -1117,8 +1115,9 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
   if (ntiles > 0) {
     // V(0) by waves 0 to 3, K(0) by the others, and K(1) behind it
     constexpr int AHEAD = F == kSame ? 0 : 1;                  // codes go through registers a tile earlier
-    if constexpr (PAIRED) {                                    // What lies behind the last tile is the nearest 16 keys once more; rows in front of and
-      // behind [lo, hi) that share 16 keys with it come as they are, and no row sees them
+    // TREE: what lies behind the last tile is the nearest 16 keys once more; rows in front of and behind [lo, hi) that share 16 keys with it come as they are, and
+    // no row sees them
+    if constexpr (PAIRED) {
       const long long at0 = block_at(half, no{}), at1 = block_at(half + 2, no{});
       if constexpr (F == kSame) {
         copy(keys, Kb, half, at0, yes{});
@@ -1135,6 +1134,19 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
         load(mine, half + 2, at1, yes{});
         load(keys, half + 4, block_at(half + 4, no{}), yes{});
       }
+    } else if constexpr (TREE) {
+      const long long at0 = block_at(0, no{}), at1 = block_at(1, no{});
+      if constexpr (F == kSame) {
+        copy(mine, half ? Kb : Vb, 0, at0, yes{});
+        if (half) copy(mine, Kb + S::TILE, 0, at1, yes{});
+      } else {
+        Bring second = mine;
+        load(mine, 0, at0, yes{});
+        if (half) load(second, 0, at1, yes{});
+        store(mine, half ? Kb : Vb);
+        if (half) store(second, Kb + S::TILE);
+        load(mine, 0, half ? block_at(2, no{}) : at1, yes{});
+      }
     } else if constexpr (F == kSame) {
       copy(mine, half ? Kb : Vb, 0, block_at(0, no{}), no{});
       if (half && ntiles > 1) copy(mine, Kb + S::TILE, 1, block_at(1, no{}), no{});
@@ -1149,7 +1161,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
     }
     const int ahead = PAIRED ? 2 * (2 + AHEAD) : (half ? 2 : 1) + AHEAD;          // S(t) asks for tile t + ahead; PAIRED: that one of K, the one before it of V
     const int asked = (PAIRED ? half : 0) + ahead;
-    long long next = PAIRED || asked < ntiles ? block_at(asked, no{}) : 0;
+    long long next = TREE || asked < ntiles ? block_at(asked, no{}) : 0;
     if (TREE && (j.hi > (j.first & ~63) || a.window > 0)) {    // (no tile of another part has a word)
       unsigned long long bits[S::WORDS];
       int depth;
@@ -1165,42 +1177,51 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
     __builtin_amdgcn_s_waitcnt(0x0F70);                        // vmcnt(0)
     __syncthreads();
     phase_m(Vb, Kb, no{}, yes{});
-    if constexpr (PAIRED) {
+    if constexpr (TREE) {
       // One turn for all tiles, as code that runs once takes longer to fetch than to run: what a turn asks for and puts away behind the last tile is that tile once more,
       // and its scores go nowhere.
-      phase_barrier();                                         // waves 0 to 3 are about to write where K(0) was read
-      int vcur = 2 * S::TILE, vnext = 3 * S::TILE, kcur = 0, knext = S::TILE;     // V(t), V(t + 2), K(t), K(t + 2)
-      long long behind = block_at(asked - 2, no{});
+      constexpr int STEP = PAIRED ? 2 : 1;                     // from a wave's tile to its next
+      if constexpr (PAIRED) phase_barrier();                   // waves 0 to 3 are about to write where K(0) was read
+      int kcur = 0, knext = S::TILE;                           // K(t), that of the next
+      int vcur = 2 * S::TILE, vnext = 3 * S::TILE, vfree = (PAIRED ? 2 : 4) * S::TILE;   // V(t), the next, and the place of the one behind: PAIRED, that of V(t)
+      long long behind = PAIRED ? block_at(asked - 2, no{}) : 0;
       if (half) phase_barrier();
-      for (int t = half; t < ntiles + half; t += 2) {          // both halves take as many turns, the last of which may have no tile for waves 4 to 7
-        const int bring = t + ahead;
-        if constexpr (F == kSame) {
-          copy(keys, tiles + kcur, bring, next, yes{});
-          copy(mine, tiles + vnext, bring - 2, behind, yes{});
-        } else {
+      const int first_tile = PAIRED ? half : 0;                // PAIRED: both halves take as many turns, the last of which may have no tile for waves 4 to 7
+      for (int t = first_tile; t < ntiles + first_tile; t += STEP) {
+        if constexpr (PAIRED && F == kSame) {
+          copy(keys, tiles + kcur, 0, next, yes{});
+          copy(mine, tiles + vnext, 0, behind, yes{});
+        } else if constexpr (PAIRED) {
           store(keys, tiles + kcur);
           store(mine, tiles + vnext);
-          load(keys, bring, next, yes{});
-          load(mine, bring - 2, behind, yes{});
+          load(keys, 0, next, yes{});
+          load(mine, 0, behind, yes{});
+        } else if constexpr (F == kSame) {
+          copy(mine, tiles + (half ? kcur : vnext), 0, next, yes{});
+        } else {
+          store(mine, tiles + (half ? kcur : vnext));
+          load(mine, 0, next, yes{});
         }
         behind = next;
-        next = block_at(bring + 2, no{});
+        next = block_at(t + ahead + STEP, no{});
         __builtin_amdgcn_sched_barrier(0);                     // the copies go out before the weights are begun
         const bool works = !idle && t < ntiles;
         const bool some = base + 64 * t < max(j.sure_lo, j.lo) || base + 64 * t + 64 > min(j.sure_hi, j.hi);   // some wave's rows do not see all of it
+        const int place = vcur / S::TILE - 2;
         if (works) phase_s(t, no{});
-        if (some) look(tiles + vcur, vcur / S::TILE - 2);
+        if (some && (PAIRED || !half)) look(tiles + vcur, place);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // what was written to LDS
         phase_barrier();
         if (works) phase_m(tiles + vcur, tiles + knext, yes{}, yes{});
-        if (some && works && __builtin_expect(!all_finite(vcur / S::TILE - 2), 0)) mark(t, vcur / S::TILE - 2);
+        if (some && works && __builtin_expect(!all_finite(place), 0)) mark(t, place);
         if constexpr (F == kSame) __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the copies that this wave asked for in S(t)
         phase_barrier();
         const int k = kcur, v = vcur;
         kcur = knext;
         knext = k;
         vcur = vnext;
-        vnext = v;
+        vnext = vfree;
+        vfree = PAIRED ? vcur : v;
       }
       if (!half) phase_barrier();
     } else {
