@@ -71,8 +71,8 @@ struct AttnArgs {
   long long small_first;                      // parts of small sequences stand behind these many
   float *part_o, *part_ml;                    // [tokens * heads][cut.nparts] parts, then [sequences][kv heads][kSmallRows][small.nparts]: D floats; two
   const int* parents;                         // trees: of each packed row, by its number among the sequence's new tokens; negative: none
-  int shares, grain_shift, block_rows, row_blocks;   // trees, wide: workgroups of a kv head that the work is shared out to (0: a workgroup to a block of rows), of
-                                              // grains of 2^grain_shift keys; rows of a block of them, and blocks that a sequence may have
+  int shares, grain_shift, block_shift, row_blocks;  // trees, wide: workgroups of a kv head that the work is shared out to (0: a workgroup to a block of rows), of
+                                              // grains of 2^grain_shift keys; blocks of 2^block_shift rows, as many as a sequence may have
 };
 
 // ---- which rows and which keys a workgroup has ----------------------------------------
@@ -1385,7 +1385,7 @@ __device__ __forceinline__ int share_work(const AttnArgs& a, int i, int* blocks)
   const int start = min(max(a.batch.starts[i], 0), a.batch.tokens), end = a.batch.starts[i + 1], all = max(a.batch.lens[i], 0);
   const int rows = min(min(max(end, start), a.batch.tokens) - start, kTreeMost) * a.group;
   if (rows <= a.small_rows) return 0;
-  *blocks = min((rows + a.block_rows - 1) / a.block_rows, a.row_blocks);
+  *blocks = min((rows + (1 << a.block_shift) - 1) >> a.block_shift, a.row_blocks);
   const int keys = max(min(all, kv_capacity(a.batch, a.pages.page_shift)) - seq_first_key(a, first_position(all, start, end)), 1);
   return (int)(((long long)keys + (1LL << a.grain_shift) - 1) >> a.grain_shift);
 }
@@ -1456,9 +1456,9 @@ __device__ __forceinline__ void share_job(const AttnArgs& a, int b, int line, in
   j.n = min(c.n, kTreeMost);
   j.first = c.first;
   j.rows = j.n * a.group;
-  j.row0 = line * a.block_rows;
+  j.row0 = line << a.block_shift;
   j.len = min(c.len, kv_capacity(a.batch, a.pages.page_shift));
-  const long long p_hi = (long long)c.first + (min(j.row0 + a.block_rows, j.rows) - 1) / a.group, key0 = seq_first_key(a, c.first);
+  const long long p_hi = (long long)c.first + (min(j.row0 + (1 << a.block_shift), j.rows) - 1) / a.group, key0 = seq_first_key(a, c.first);
   j.hi = clamp_position(p_hi + 1, j.len);
   j.sure_hi = clamp_position(c.first, j.len);
   j.lo = a.window > 0 ? clamp_position((long long)c.first - a.window + 1, j.len) : 0;
@@ -1654,7 +1654,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
 
 // The same for trees: a wave has ROWS heads of a token.  Lanes have columns, so that a part's weight is the same for all of them.  Rows in at most four parts, which most
 // are where there are many, are joined at once, everything of theirs being asked for before any of it is needed; others one after the other, their
-// weights a lane each.  (25 tokens, 32 heads, 32 parts: 6 us, 19 by the kernel above.)
+// weights a lane each.  (25 tokens, 32 heads, 32 parts: 7 us, 19 by the kernel above.)
 template <typename T, int D, int ROWS>
 __global__ __launch_bounds__(256) void tree_join_kernel(AttnArgs a) {
   constexpr int VEC = D > 64 ? 2 : 1, TURN = 16, K = kPartsMost / 64, FEW = 4;
@@ -1685,30 +1685,38 @@ __global__ __launch_bounds__(256) void tree_join_kernel(AttnArgs a) {
   Shares s{0, 0, 0, 0};
   if (a.shares > 0) s = share_out(a);
   // where the first part of each row is, the second, and how far those behind are from one another
-  int n[ROWS], line = -1, begin = 0, grains = 0;
-  long long part0[ROWS], part1[ROWS];
-  const long long step = a.shares > 0 ? 2LL * a.pages.heads * a.block_rows : 1;
+  int n[ROWS], line = -1, parts = 1, after = 0, kv_head = (int)((unsigned)head0 / (unsigned)a.group), in_group = head0 - kv_head * a.group;
+  long long part0[ROWS], part1[ROWS], slot = 0;
+  const long long step = a.shares > 0 ? 2LL * a.pages.heads << a.block_shift : 1;
+  const int own_parts = a.shares > 0 ? 1 : seq_parts(a, a.cut, first, len);
   bool few = true;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
-    const int head = min(head0 + r, a.heads - 1), kv_head = head / a.group, row = (token - start) * a.group + head - kv_head * a.group;
     if (a.shares == 0) {
-      n[r] = seq_parts(a, a.cut, first, len);
-      part0[r] = ((long long)token * a.heads + head) * a.cut.nparts;
+      n[r] = own_parts;
+      part0[r] = ((long long)token * a.heads + min(head0 + r, a.heads - 1)) * a.cut.nparts;
       part1[r] = part0[r] + 1;
     } else {
-      if (line != row / a.block_rows) {
-        line = row / a.block_rows;
+      const int row = (token - start) * a.group + in_group, in_block = row & ((1 << a.block_shift) - 1);
+      if (line != row >> a.block_shift) {
+        line = row >> a.block_shift;
         if (line >= a.row_blocks) return;
+        int begin, grains;
         share_find(a, line, 0, b, &begin, &grains);
+        const int group0 = (int)((unsigned)begin / (unsigned)s.each);
+        parts = (int)((unsigned)(begin + max(grains, 1) - 1) / (unsigned)s.each) - group0 + 1;
+        after = begin > group0 * s.each;
+        slot = (long long)(__builtin_amdgcn_readlane(s.before, line) + group0) * a.pages.heads * 2;
       }
-      const int group0 = begin / s.each;
-      n[r] = (begin + max(grains, 1) - 1) / s.each - group0 + 1;
-      const long long slot = ((long long)(__builtin_amdgcn_readlane(s.before, line) + group0) * a.pages.heads + kv_head) * 2;
-      part0[r] = (slot + (begin > group0 * s.each)) * a.block_rows + row % a.block_rows;
-      part1[r] = slot * a.block_rows + row % a.block_rows + step;
+      n[r] = parts;
+      part1[r] = ((slot + 2 * kv_head) << a.block_shift) + in_block + step;
+      part0[r] = part1[r] - step + ((long long)after << a.block_shift);
     }
     few = few && n[r] <= FEW;
+    if (head0 + r + 1 < a.heads && ++in_group == a.group) {
+      in_group = 0;
+      ++kv_head;
+    }
   }
   const int col = min(lane * VEC, D - VEC);
   const float* const po = a.part_o + col;
@@ -2027,7 +2035,7 @@ static int attend(const char* who, const void* q, int type, long long q_token_st
   a.small_first = (long long)p.large;
   a.shares = p.shares;
   a.grain_shift = p.grain_shift;
-  a.block_rows = p.block_rows;
+  a.block_shift = __builtin_ctz((unsigned)p.block_rows);
   a.row_blocks = p.narrow ? 0 : (int)(((max_queries > 0 ? std::min(max_queries, a.batch.tokens) : a.batch.tokens) * (long long)a.group + p.block_rows - 1) / p.block_rows);
   const long long rows = (long long)a.batch.tokens * heads;
   a.part_o = (float*)workspace;
@@ -2062,7 +2070,7 @@ static int attend(const char* who, const void* q, int type, long long q_token_st
         constexpr int lds = std::max(WideShape<D, TREE, PAIRED>::LDS, TREE ? 0 : 2 * NarrowShape<F, D>::LDS);
         return launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D, TREE, PAIRED>, once, blocks + pairs, kWideWaves, lds, s, a, (int)blocks);
       };
-      if constexpr (TREE) bad = a.block_rows == kPairedRows ? launch(std::true_type{}) : launch(std::false_type{});
+      if constexpr (TREE) bad = p.block_rows == kPairedRows ? launch(std::true_type{}) : launch(std::false_type{});
       else bad = launch(std::false_type{});
     }
     if (bad || p.all == 0) return bad;
