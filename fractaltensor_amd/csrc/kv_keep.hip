@@ -7,8 +7,8 @@
 // Then every wave writes the positions of its own stretch in their order, behind those of the waves before it.
 //
 // keep.  Row kept[j] of a list that ascends goes to place j <= kept[j].  In place, that is safe without a second buffer as long as no place
-// is written before it has been read: rows of later j come from behind all places of earlier ones, so a workgroup takes the list in order, 256 pieces of 16
-// bytes or more at a time, with all of a step's reads done before its first write.  Rows are cut into slices of 16 to 256 bytes, each a workgroup's of its own with
+// is written before it has been read: rows of later j come from behind all places of earlier ones, so a workgroup takes the list in order, some
+// pieces of 16 bytes a thread at a time, with all of a step's reads done before its first write.  Rows are cut into slices of 16 to 256 bytes, each a workgroup's of its own with
 // nothing to wait for, where sequences and heads alone leave compute units idle.  Bound by reading and writing each moved byte once.
 #include <algorithm>
 
