@@ -225,6 +225,28 @@ def test_what_a_token_does_not_see_of_a_tree_never_matters(core, dtype, cache, G
     _tree_case(core, dtype, cache, D, page, heads, G, new, lens, 340, pages=pages)
 
 
+@pytest.mark.parametrize('dtype,cache,G,new,lens', [(BF16, E4M3, 4, [20, 2], [200, 31]), (F16, I8, 2, [50], [90]), (BF16, None, 1, [200], [300])])
+def test_what_a_token_does_not_see_of_other_trees_never_matters(core, dtype, cache, G, new, lens):
+    test_what_a_token_does_not_see_of_a_tree_never_matters(core, dtype, cache, G, new, lens)
+
+
+def test_sequences_that_make_no_sense_beside_one_that_does(core):
+    """Lengths past the table's room and below zero, pages that are not there: the work is shared out all the same, and the first sequence has its own results (to the sums'
+    order and the weights' rounding, as above)."""
+    heads, G, D, page, new = 2, 2, 64, 32, [40, 30, 50]
+    batch = base.make_batch(new, [3000] * 3, page, 350)
+    pages = _cuda(base.make_pages(batch, heads, D, E4M3, BF16, 351))
+    table, lens, starts = base.on_device(batch)
+    parents = _ints(_trees(new, 352))
+    q = torch.randn((120, heads * G, D), generator=torch.Generator().manual_seed(353)).to(BF16).cuda()
+    call = lambda v, t, n, s: core.paged_tree_attention(q, pages[0], v, t, n, s, parents, *pages[2:], max_queries=50, max_keys=3000)
+    want, most = call(pages[1], table, lens, starts), call(pages[1].float().abs().to(E4M3), table, lens, starts).float()
+    table[1:] = _ints([[(7919 * i) % 2 ** 31 - 2 ** 30 for i in range(table.shape[1])]] * 2)
+    for bad_lens, bad_starts in (([3000, 2 ** 31 - 1, -7], [0, 40, 70, 120]), ([3000, 10, 0], [0, 40, 70, 2 ** 31 - 1]), ([3000, -2 ** 31, 5], [0, 40, -3, 1000]), ([3000, 9, 9], [0, 40, 40, 40])):
+        got = call(pages[1], table, _ints(bad_lens), _ints(bad_starts))
+        assert ((got[:40].float() - want[:40].float()).abs() <= 2.02 * torch.finfo(BF16).eps * most[:40]).all()
+
+
 def test_trees_on_batches_that_make_no_sense(core):
     """More new tokens than positions, lengths past the table, pages that do not exist: nothing outside is touched, and who is right is served."""
     dtype, D, page, heads, G = F16, 64, 16, 2, 2
