@@ -885,12 +885,13 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
     const int key0 = base + 64 * t + 16 * cw;
     const int inside = min(max(key0, j.lo & ~15), (j.hi - 1) & ~15);
     const int least = max(j.lo - inside, 0), most = min(j.hi - 1 - inside, 15);
+    const unsigned char *const block = uniform(b.from + at * D), *const block_exps = uniform((const unsigned char*)b.exps + at);
 #pragma unroll
     for (int i = 0; i < LD; ++i) {
       const int p = min(64 * i + lane, D - 1), rw = p / (D / 16), piece = p - rw * (D / 16);
-      const long long row_at = at + (decltype(inside_c)::value ? rw : min(max(key0 + rw - inside, least), most));
-      b.codes[i] = *reinterpret_cast<const v4u*>(b.from + row_at * D + 16 * piece);
-      b.exps_of[i] = b.exps[row_at];
+      const unsigned row = decltype(inside_c)::value ? rw : min(max(key0 + rw - inside, least), most);
+      b.codes[i] = *reinterpret_cast<const v4u*>(block + (decltype(inside_c)::value ? 16u * p : row * D + 16u * piece));
+      b.exps_of[i] = (signed char)block_exps[row];
     }
   };
   auto store = [&](const Bring& b, unsigned char* to) __attribute__((always_inline)) {
