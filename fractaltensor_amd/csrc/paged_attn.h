@@ -22,8 +22,10 @@
 // TREE: the new tokens of a sequence are a tree of drafts.  Each sees the cache in front of them, its ancestors and itself, so that only the tiles that hold new tokens'
 // own keys differ: there a row has a bit for each of those keys, found by walking up from it through the parents, a lane a row, which are passed from lane to
 // lane.  (Position and depth differ in a tree; a window counts the steps on the way.)  The narrow form has up to 16 rows of them, and the wide form
-// more, their weights rounded once: up to 128 rows by both halves of a workgroup, on different keys, and the work of sequences of different lengths shared
-// out evenly.  (16 sequences of 2064 to 8192 positions in int8, 8 heads of keys, 40 rows: 76 us, 118 by the narrow form; 64 rows: 78 and 119.)
+// more: up to 128 rows by both halves of a workgroup, on different keys, and the work of sequences of different lengths shared
+// out evenly.  Sequences of up to 64 rows have their weights as two operands on either, by their own rows alone, so that a tree's results are no less exact than those of the same tokens
+// one behind the other, nor for a larger tree beside it; the wide form has a second body for them.  (16 sequences of 2064 to 8192 positions in e4m3, 8 heads of keys, 64 rows: 89 us, 73 with
+// weights rounded once, 92 by the narrow form; 16 bits 87, 85 and 107.)
 #pragma once
 
 #include <float.h>
@@ -38,6 +40,7 @@ namespace ftk {
 constexpr int kWaves = 4;
 constexpr float kNoRef = -3.402823466e38f;   // the reference before any score: finite, so that -inf minus it is -inf
 constexpr int kSmallRows = 16;                // sequences of at most so many rows, beside larger ones, are small
+constexpr int kNarrowRows = 64;               // calls of no more rows to a sequence are narrow (trees: have weights as narrow ones do)
 constexpr int kTreeMost = 256;                // new tokens of a tree
 
 // Weights are 2^(score - reference), and the reference is moved to the largest score less kLift, so that the largest weight is 2^kLift then.  fp16 has 15
@@ -765,7 +768,8 @@ __device__ __forceinline__ int v_swizzle(int row) {
   else return 0;                                               // rows of 192 and 64 bytes lie that way
 }
 
-template <typename T, KvFormat F, int D, bool TREE, bool PAIRED>
+// TWO: weights as two operands.
+template <typename T, KvFormat F, int D, bool TREE, bool PAIRED, bool TWO>
 __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, int kv_head, unsigned char* smem) {
   using S = WideShape<D, TREE, PAIRED>;
   using v8 = typename T::v8;
@@ -947,9 +951,10 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
 #pragma unroll
     for (int e = 0; e < 16; ++e) sc[h][e] = 0.0f;
   float ref = kNoRef, l = 0.0f;
-  v8 pf[2][2];
+  v8 pf[2][2], rest[2][2];                                     // weights as operands, and (TWO) what their rounding leaves
 
-  // the weights of the tile's scores as operands of P V; returns this lane's share of their sum
+  // The weights of the tile's scores as operands of P V; returns this lane's share of their sum.  (TWO: still in 32 bits, in p.)
+  float p[TWO ? 32 : 1];
   auto weights = [&]() __attribute__((always_inline)) {
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -963,11 +968,32 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
           const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[h][8 * s + 2 * i + 1], a.scale_log2e, -ref));
           sum[i] += p0;
           sum[i] += p1;
-          w[i] = T::pack(p0, p1);
+          if constexpr (TWO) {
+            p[16 * h + 8 * s + 2 * i] = p0;
+            p[16 * h + 8 * s + 2 * i + 1] = p1;
+          } else {
+            w[i] = T::pack(p0, p1);
+          }
         }
-        pf[h][s] = __builtin_bit_cast(v8, w);
+        if constexpr (!TWO) pf[h][s] = __builtin_bit_cast(v8, w);
       }
     return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  };
+  auto two_operands = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v4u w, left;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p0 = p[8 * k + 2 * i], p1 = p[8 * k + 2 * i + 1];
+        unsigned pair = T::pack(p0, p1);
+        asm("" : "+v"(pair));                                  // (taken out of the pair: the compiler would round each once more)
+        w[i] = pair;
+        left[i] = T::pack(__builtin_fmaf(T::low(pair), -1.0f, p0), __builtin_fmaf(T::high(pair), -1.0f, p1));
+      }
+      pf[k / 2][k % 2] = __builtin_bit_cast(v8, w);
+      rest[k / 2][k % 2] = __builtin_bit_cast(v8, left);
+    }
   };
   // The reference is not compared with every tile's maximum: weights are worked out against it as it is, and only when a lane's sum says that
   // one of them may not fit 16 bits (or came out infinite, as all do before there is a reference) are the maxima taken, the reference moved, O and the sums
@@ -1000,6 +1026,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
         for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
       psum = weights();
     }
+    if constexpr (TWO) two_operands();
     l += psum;
   };
 
@@ -1024,6 +1051,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
       if constexpr (i < N0) {
         constexpr int h = i / (2 * DT), s = (i % (2 * DT)) / DT, dt = i % DT;
         o[dt] = T::mma32(fr[i], pf[h][s], o[dt]);
+        if constexpr (TWO) o[dt] = T::mma32(fr[i], rest[h][s], o[dt]);
       } else {
         constexpr int s = (i - N0) / 2, h = (i - N0) % 2;
         v16f zero;
@@ -1520,14 +1548,15 @@ __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs
         if (!find_rows<R>(a, rest, &b, &tile) || !find_job<R, TREE>(a, b, tile, 0, false, j)) return;
         x = end;
       }
-      wide_attention<T, F, D, TREE, PAIRED>(a, j, kv_head, smem);
+      if (j.rows <= kNarrowRows) wide_attention<T, F, D, TREE, PAIRED, true>(a, j, kv_head, smem);
+      else wide_attention<T, F, D, TREE, PAIRED, false>(a, j, kv_head, smem);
       if (x < end) __syncthreads();
     }
   } else {
     const int slot = rest / a.cut.nparts, part = rest - slot * a.cut.nparts;
     int b, tile;
     if (!find_rows<R>(a, slot, &b, &tile) || !find_job<R, TREE>(a, b, tile, part, false, j)) return;
-    wide_attention<T, F, D, TREE, PAIRED>(a, j, kv_head, smem);
+    wide_attention<T, F, D, TREE, PAIRED, false>(a, j, kv_head, smem);
   }
 }
 
@@ -1888,7 +1917,7 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
   Plan p;
   const long long most = max_queries > 0 ? std::min(max_queries, b.tokens) : b.tokens;   // new tokens of a sequence
   const long long most_rows = most * group, rows = (long long)b.tokens * heads;
-  p.narrow = most_rows <= (tree ? 16 : 64);
+  p.narrow = most_rows <= (tree ? kSmallRows : kNarrowRows);
   const long long capacity = (long long)b.width << page_shift;
   long long seen = max_keys > 0 ? std::min<long long>(max_keys, capacity) : capacity;
   if (window > 0) seen = std::min(seen, most + window + 64);   // from the first key that the first new token sees, down to a multiple of 64

@@ -757,8 +757,10 @@ int ftk_verify_drafts(const void* target, const void* draft, int type,
  * them), and each sees the positions in front of the new tokens, its ancestors and
  * itself.  window > 0: of these the last `window` on the way that ends with it; a
  * token d steps below a root counts as d positions behind the first new one's.
- * All else is as in ftk_paged_attn.  A sequence has at most 256 new tokens: max_queries
- * promises it, or `tokens` is no larger.
+ * All else is as in ftk_paged_attn, but that a sequence's own rows (new tokens times heads
+ * / pages->heads) say alone how its weights enter the products with values: up to 64 as two
+ * numbers of 16 bits, whatever else the call holds.  A sequence has at most 256 new tokens:
+ * max_queries promises it, or `tokens` is no larger.
  */
 size_t ftk_paged_tree_attn_workspace_bytes(const ftk_kv_pages* pages,
                                            const ftk_kv_batch* batch,

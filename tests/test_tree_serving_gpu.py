@@ -301,6 +301,36 @@ def test_trees_with_queries_as_views(core):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize('dtype,cache,D,page,heads,G,new,lens,window', [
+    (BF16, E4M3, 128, 64, 2, 4, [16, 9, 3, 0, 5], [900, 2500, 40, 9, 17], 0), (F16, I8, 128, 32, 1, 4, [16], [9000], 0), (BF16, None, 128, 16, 2, 4, [10, 5], [300, 900], 0),
+    (F16, None, 64, 32, 1, 2, [32, 1, 20], [400, 50, 33], 7), (BF16, I8, 96, 16, 1, 7, [9, 3], [333, 5000], 0), (F16, E4M3, 32, 128, 2, 1, [64, 40, 17], [64, 3000, 18], 0)])
+def test_trees_of_up_to_64_rows_are_off_by_their_own_rounding(core, dtype, cache, D, page, heads, G, new, lens, window):
+    """Their weights enter the second product as the rounded one and what that leaves, on either kernel: the bounds are those of few rows."""
+    for kind in ('any', 'chain', 'wild'):
+        _tree_case(core, dtype, cache, D, page, heads, G, new, lens, 380, kind, window=window, narrow=True)
+
+
+@pytest.mark.parametrize('dtype,cache,tree', [(BF16, None, 3), (F16, E4M3, 3), (BF16, I8, 3), (BF16, E4M3, 16), (F16, I8, 16), (F16, None, 7)])
+def test_a_small_tree_does_not_depend_on_the_trees_beside_it(core, dtype, cache, tree):
+    """Trees of 12 to 64 rows alone, and beside one of 40 rows, of 128 and of 256: each is off from the definition by its own rounding alone."""
+    heads, G, D, page, length = 2, 4, 64, 32, 700
+    for other in (0, 10, 32, 64):
+        new, lens = ([tree, other], [length, 1500]) if other else ([tree], [length])
+        batch = base.make_batch([tree, 64], [length, 1500], page, 390)
+        pages = base.make_pages(batch, heads, D, cache, dtype, 392)
+        q = torch.randn((tree + 64, heads * G, D), generator=torch.Generator().manual_seed(391)).to(dtype)
+        batch.update(table=batch['table'][:len(new)], lens=lens, starts=[0, tree, tree + other][:len(new) + 1], tokens=sum(new))
+        q, parents, dev = q[:sum(new)], _trees(new, 393), _cuda(pages)
+        o = core.paged_tree_attention(q.cuda(), *dev[:2], *base.on_device(batch), _ints(parents), *dev[2:], max_queries=max(new), max_keys=max(lens)).cpu().double()
+        k, v = base.held(pages[0], pages[2]), base.held(pages[1], pages[3])
+        if dtype == F16:
+            k, v = k.half().double(), v.half().double()
+        at = batch['starts']
+        want = ref.attention(q, k, v, batch, heads, D ** -0.5, lambda b, n, first, length: ref.tree_sees(parents[at[b]:at[b + 1]], n, first, length))
+        off = (o - want['o']).abs() / base.attention_bounds_by_largest(want, dtype, D, split=True)
+        assert bool((off[:tree] <= 1).all()), (other, float(off[:tree].max()))
+
+
 # ---- verification ------------------------------------------------------------------------------
 
 def _verify_case(core, dtype, new, V, M, seed, ids_type=torch.int64, kind='any', shift=0):
