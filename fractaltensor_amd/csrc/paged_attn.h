@@ -34,6 +34,7 @@
 #include <cmath>
 
 #include "kv_common.h"
+#include "tree_shares.h"
 
 namespace ftk {
 
@@ -1942,29 +1943,18 @@ static Plan plan(const ftk_kv_pages& pages, const KvBatch& b, int page_shift, in
     const double units = (double)p.slots * pages.heads;
     p.cut = best_cut(keys, 256, rows, D, room, [&](const Cut& c) { return narrow_cost(units * c.nparts, c.part_keys, held, cus, b.sequences == 1) + join_cost(rows, D, c.nparts); });
   } else if (tree) {
-    // Work shared out to as many workgroups as there are compute units, or to twice as many and more where the heads divide those badly; unless
-    // a workgroup for each block of rows is expected to be done sooner: us as in wide_cost(), several sequences being two thirds as long as the longest in the mean.
+    // Work shared out, unless a workgroup for each block of rows is expected to be done sooner: us as in wide_cost(), several sequences being two thirds as long as
+    // the longest in the mean.
     const double turn = (p.block_rows == kPairedRows ? 2.4 : 4.0) * D / 128, turns = std::ceil(keys / 128.0), units = (double)b.sequences * per_seq * pages.heads;
     const double whole = std::ceil(units / cus) * (8.0 + turns * turn);
     p.cut = cut_into(keys, 1);
-    // (whatever lengths the device finds: their sums have 32 bits)
-    while (b.sequences * (double)per_seq * ((double)std::min<long long>(capacity, INT_MAX) / (1 << p.grain_shift) + 1.0) > 1e9) ++p.grain_shift;
-    long long shares = 0;
-    double used = 0.0;
-    for (int rounds = 1; rounds <= 4 && used < 0.9; ++rounds) {
-      const long long n = std::max<long long>(rounds * (long long)cus / pages.heads, 1);
-      const double u = (double)n * pages.heads / (std::ceil((double)n * pages.heads / cus) * cus);
-      if (u > used) {
-        used = u;
-        shares = n;
-      }
-    }
-    shares = std::max(shares, per_seq);
-    const double rounds = std::ceil((double)shares * pages.heads / cus);
-    const double shared = 18.0 + rounds * 6.0 + std::max(units * turns * (b.sequences > 1 ? 2.0 / 3 : 1.0) / (shares * pages.heads), (double)kLeastGrains) * turn * rounds;
-    const size_t parts = (size_t)shares * pages.heads * 2 * p.block_rows;
-    if (shared < whole && per_seq <= 64 && workspace_of(parts, D) <= room) {
-      p.shares = (int)shares;
+    const TreeShares s = share_trees(b.sequences, per_seq, pages.heads, capacity, cus);
+    p.grain_shift = s.grain_shift;
+    const double rounds = std::ceil((double)s.shares * pages.heads / cus);
+    const double shared = 18.0 + rounds * 6.0 + std::max(units * turns * (b.sequences > 1 ? 2.0 / 3 : 1.0) / ((double)s.shares * pages.heads), (double)kLeastGrains) * turn * rounds;
+    const size_t parts = (size_t)s.shares * pages.heads * 2 * p.block_rows;
+    if (s.shares > 0 && shared < whole && workspace_of(parts, D) <= room) {
+      p.shares = s.shares;
       p.slots = p.shares;
       p.large = parts;
       p.all = parts;
@@ -2009,10 +1999,13 @@ static int launch_with_lds(const char* name, K kernel, DeviceOnce& once, long lo
   return check_launch(name);
 }
 
+// A sequence's new tokens at most.
+static int most_tokens(int max_queries, int tokens) { return max_queries > 0 ? std::min(max_queries, tokens) : tokens; }
+
 static size_t attend_workspace_bytes(const ftk_kv_pages* pages, const ftk_kv_batch* batch, int heads, int window, int max_queries, int max_keys, bool tree) {
   const DeviceProps* d = nullptr;
   if (!pages || !batch || pages->heads <= 0 || heads <= 0 || heads % pages->heads || batch->tokens <= 0 || batch->sequences <= 0 || batch->table_width <= 0 ||
-      pages->page_size <= 0 || window < 0 || device_props(&d))
+      pages->page_size <= 0 || window < 0 || (tree && most_tokens(max_queries, batch->tokens) > kTreeMost) || device_props(&d))
     return 0;
   KvBatch b{};
   b.tokens = batch->tokens;
@@ -2036,7 +2029,7 @@ static int attend(const char* who, const void* q, int type, long long q_token_st
   if (a.batch.tokens == 0) return FTK_OK;
   if constexpr (TREE) {
     if (!parents || ((uintptr_t)parents & 3)) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: parents must be non-NULL and 4-byte aligned", who);
-    const int most = max_queries > 0 ? std::min(max_queries, a.batch.tokens) : a.batch.tokens;
+    const int most = most_tokens(max_queries, a.batch.tokens);
     if (most > kTreeMost) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: trees of at most %d tokens, max_queries says how many there may be, got %d", who, kTreeMost, most);
   }
   if (!q || !o || !aligned16(q) || !aligned16(o)) return fail(FTK_ERR_INVALID_ARGUMENT, "%s: q and o must be non-NULL and 16-byte aligned", who);
@@ -2066,7 +2059,7 @@ static int attend(const char* who, const void* q, int type, long long q_token_st
   a.shares = p.shares;
   a.grain_shift = p.grain_shift;
   a.block_shift = __builtin_ctz((unsigned)p.block_rows);
-  a.row_blocks = p.narrow ? 0 : (int)(((max_queries > 0 ? std::min(max_queries, a.batch.tokens) : a.batch.tokens) * (long long)a.group + p.block_rows - 1) / p.block_rows);
+  a.row_blocks = p.narrow ? 0 : (int)((most_tokens(max_queries, a.batch.tokens) * (long long)a.group + p.block_rows - 1) / p.block_rows);
   const long long rows = (long long)a.batch.tokens * heads;
   a.part_o = (float*)workspace;
   a.part_ml = a.part_o + p.all * pages->head_size;

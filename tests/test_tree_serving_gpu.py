@@ -331,6 +331,19 @@ def test_a_small_tree_does_not_depend_on_the_trees_beside_it(core, dtype, cache,
         assert bool((off[:tree] <= 1).all()), (other, float(off[:tree].max()))
 
 
+def test_more_tokens_than_trees_have_are_refused_at_once(core):
+    """A large batch whose program does not say how many tokens a sequence has at most: nothing to allocate, and an error."""
+    q, pages = torch.zeros((1 << 16, 64, 32), dtype=F16, device='cuda'), torch.zeros((4, 1, 16, 32), dtype=F16, device='cuda')
+    table, lens, starts, parents = (torch.zeros(s, dtype=torch.int32, device='cuda') for s in ((4096, 1024), 4096, 4097, 1 << 16))
+    assert core.paged_tree_attention_workspace_bytes(q, pages, table) == 0 and core.paged_tree_attention_workspace_bytes(q, pages, table, 257) == 0
+    with pytest.raises(core.FtkError, match='256'):
+        core.paged_tree_attention(q, pages, pages, table, lens, starts, parents)
+    # none of the sequences has any: nothing is written
+    out = torch.full_like(q, 7.0)
+    core.paged_tree_attention(q, pages, pages, table, lens, starts, parents, max_queries=256, out=out)
+    assert bool((out == 7).all())
+
+
 # ---- verification ------------------------------------------------------------------------------
 
 def _verify_case(core, dtype, new, V, M, seed, ids_type=torch.int64, kind='any', shift=0):
