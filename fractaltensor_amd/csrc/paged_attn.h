@@ -1563,8 +1563,6 @@ __global__ __launch_bounds__(kWideWaves * 64, 1) void paged_wide_kernel(AttnArgs
 
 // ---- parts ------------------------------------------------------------------------------
 
-constexpr int kPartsMost = 256;
-
 // The parts of the sequence that row `at` of the packed rows times heads belongs to (1: nothing to join), the first of them, and the keys [*lo, *hi) that the row
 // sees.  first_token: that of the wave's first lane.
 __device__ __forceinline__ int row_parts(const AttnArgs& a, long long at, int first_token, int* lo, int* hi, long long* first_of) {

@@ -8,6 +8,8 @@
 
 namespace ftk {
 
+constexpr int kPartsMost = 256;  // parts of a row: what joins them has registers for the weights of so many
+
 struct TreeShares {
   int shares;                    // 0: the work cannot be shared out
   int grain_shift;               // grains of 2^grain_shift keys
@@ -32,7 +34,8 @@ inline TreeShares share_trees(long long sequences, long long row_blocks, int hea
       shares = n;
     }
   }
-  s.shares = (int)std::max(shares, row_blocks);
+  // (one sequence may be left in as many parts as there are shares)
+  s.shares = (int)std::min<long long>(std::max(shares, row_blocks), kPartsMost);
   return s;
 }
 

@@ -12,7 +12,7 @@ int main() {
     for (long long k : blocks)
       for (long long c : capacities)
         for (int h : heads)
-          for (int cus : {1, 64, 256}) {
+          for (int cus : {1, 64, 256, 304, 1000}) {
             const ftk::TreeShares s = ftk::share_trees(n, k, h, c, cus);
             if (s.shares == 0) {
               ++refused;
@@ -22,7 +22,7 @@ int main() {
             // all lines' grains are added up in 32 bits, a line of a lane each
             const long long keys = std::min<long long>(c, INT_MAX);
             const bool fits = s.grain_shift >= 7 && s.grain_shift <= 30 && (double)n * k * (double)((keys + (1LL << s.grain_shift) - 1) >> s.grain_shift) <= INT_MAX;
-            if (!fits || k > 64 || s.shares < k) {
+            if (!fits || k > 64 || s.shares < k || s.shares > ftk::kPartsMost) {
               std::printf("%lld sequences, %lld blocks, %d heads, %lld positions, %d units: %d shares of 2^%d keys\n", n, k, h, c, cus, s.shares, s.grain_shift);
               ++bad;
             }
