@@ -437,13 +437,22 @@ def _integers(ft: FractalTensor, name: str, counts, dtypes=(torch.int32, torch.i
     return ft.data.reshape(-1)
 
 
+def _parents(ft: FractalTensor, counts) -> torch.Tensor:
+    """Parents of the packed tokens in int32.  A number that has no place there stays one that comes before no token: it counts as none, as in int64."""
+    return _narrowed(_integers(ft, 'parentss', counts))
+
+
+def _narrowed(x: torch.Tensor) -> torch.Tensor:
+    return x if x.dtype == torch.int32 else x.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+
+
 def paged_tree_attention(qss: FractalTensor, parentss: FractalTensor, k_pages, v_pages, table, lens, k_exps=None, v_exps=None, scale: Optional[float] = None,
                          window: int = 0, max_keys: int = 0, dtype: Optional[torch.dtype] = None) -> FractalTensor:
     """paged_attention of new tokens that form a tree in each sequence, at most 256 of them: each sees what is in front of its sequence's new tokens, its ancestors and
     itself.  parentss: [sequence][token] of [1] int32 or int64, the number of a token's parent among its sequence's new tokens, one in front of it; negative: none.
     window > 0: the last that many on the way that ends with the token.  All else as in paged_attention."""
     q, counts = _new_tokens(qss, 'qss', k_pages, dtype)
-    parents = _integers(parentss, 'parentss', counts).to(torch.int32)
+    parents = _parents(parentss, counts)
     o = _core().paged_tree_attention(q, k_pages, v_pages, table, lens, _starts(counts, q.device), parents, k_exps, v_exps, 1.0 if scale is None else float(scale), window,
                                      max(counts, default=0), max_keys)
     return _by_sequence(o.to(qss.data.dtype), counts)
@@ -458,7 +467,7 @@ def verify_tree(targets: FractalTensor, tokens: FractalTensor, parentss: Fractal
     places of the tokens that stay in the cache, behind them -1, for kv_cache_keep."""
     ids = _integers(tokens, 'tokens', None)
     counts = tokens.width_by_depth(1)
-    parents = _integers(parentss, 'parentss', counts).to(torch.int32)
+    parents = _parents(parentss, counts)
     if not isinstance(targets, FractalTensor):
         raise TypeError('targets should be a FractalTensor.')
     if targets.depth != 2 or len(targets.element_shape) != 2 or targets.element_shape[0] != 1:

@@ -206,3 +206,11 @@ def test_fractal_tensors_are_refused_by_name():
             (lambda: ops.fused.kv_cache_keep(pages, pages, table, lens, table), (TypeError, RuntimeError, ValueError), 'k_pages')):
         with pytest.raises(error, match=text):
             call()
+
+
+def test_parents_outside_of_int32_stay_none():
+    from fractaltensor_amd.kaleido.operations import fused
+    wide = torch.tensor([2 ** 32, 2 ** 32 + 3, -2 ** 32, -2 ** 63, 2 ** 63 - 1, 2 ** 31, -1, 0, 5, 255])
+    assert fused._narrowed(wide).tolist() == [2 ** 31 - 1, 2 ** 31 - 1, -1, -1, 2 ** 31 - 1, 2 ** 31 - 1, -1, 0, 5, 255]
+    narrow = torch.tensor([-7, 3], dtype=torch.int32)
+    assert fused._narrowed(narrow) is narrow

@@ -924,6 +924,25 @@ def test_a_step_with_a_tree_on_fractal_tensors(core):
         ops.fused.verify_tree(ft(p), ft(ids.reshape(-1, 1)), ft(parents.reshape(-1, 1)), u)
 
 
+def test_parents_past_32_bits_on_fractal_tensors(core):
+    """Numbers that wrap to those of earlier tokens point nowhere all the same: their tokens follow the cache itself."""
+    from fractaltensor_amd.kaleido import operations as ops
+    heads, G, D, page, V, new, lens = 1, 2, 32, 16, 6, [6, 5], [30, 9]
+    g = torch.Generator().manual_seed(905)
+    batch = base.make_batch(new, lens, page, 906)
+    table, dlens, starts = base.on_device(batch)
+    pages = _cuda(base.make_pages(batch, heads, D, None, F16, 907))[:2]
+    ft = lambda t: ops.fused._by_sequence(t, new)
+    q = torch.randn((11, heads * G, D), generator=g).half().cuda()
+    wide = torch.tensor([-1, 0, 2 ** 32, 2 ** 32 + 1, 1, 2 ** 33 + 4, -1, 2 ** 32, -2 ** 32, -2 ** 32 + 1, 0])
+    none = _ints([-1, 0, -1, -1, 1, -1, -1, -1, -1, -1, 0])
+    o = ops.fused.paged_tree_attention(ft(q), ft(wide.reshape(-1, 1).cuda()), *pages, table, dlens, max_keys=30)
+    assert torch.equal(o.data.reshape(11, heads * G, D), core.paged_tree_attention(q, *pages, table, dlens, starts, none, scale=1.0, max_queries=6, max_keys=30))
+    p, ids, u = torch.full((11, V), 1 / V).cuda(), torch.arange(11).cuda() % V, torch.rand((2, 4), generator=g).cuda()
+    _, path = ops.fused.verify_tree(ft(p.reshape(11, 1, V)), ft(ids.reshape(-1, 1)), ft(wide.reshape(-1, 1).cuda()), u)
+    assert torch.equal(path, core.verify_tree(p, ids, none, starts, u)[1])
+
+
 def test_a_cache_of_limited_length_on_fractal_tensors(core):
     from fractaltensor_amd.kaleido import operations as ops
     heads, G, D, page, new, lens = 2, 2, 64, 16, [3, 30], [60, 30]
