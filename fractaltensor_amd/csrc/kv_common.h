@@ -75,6 +75,9 @@ __device__ __forceinline__ int kv_page(const KvBatch& batch, int b, int index, i
   return min(max(load_uniform(batch.table, (long long)b * batch.width + index), 0), pages - 1);
 }
 
+// A sum as it leaves: one that is infinite, because a value or a key is, as NaN, which it is already where a weight of zero met that value, or a mask cut its tile.
+__device__ __forceinline__ float finite_or_nan(float x) { return __builtin_fmaf(x, 0.0f, x); }
+
 // ---- element types ------------------------------------------------------------
 
 struct Half {

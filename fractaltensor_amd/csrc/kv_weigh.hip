@@ -288,7 +288,7 @@ __global__ __launch_bounds__(256, TILES == 1 ? (F == kSame && D > 64 ? 4 : 5) : 
         if (kg == nb) mine = x;
       }
     }
-    if (here) *here = old + mine;
+    if (here) *here = old + finite_or_nan(mine);
   }
 }
 
@@ -522,7 +522,8 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(WeighArgs a) {
     }
     // the two lanes of a key meet; lane 32 nb + m takes key m of block nb
     const float x = acc[0] + __shfl_xor(acc[0], 32), y = acc[1] + __shfl_xor(acc[1], 32);
-    if (at) *at = before + (kg ? y : x);
+    const float mine = kg ? y : x;
+    if (at) *at = before + (parts > 1 ? mine : finite_or_nan(mine));
   }
 }
 
@@ -542,7 +543,7 @@ __global__ __launch_bounds__(kBlock) void kv_weigh_join_kernel(WeighArgs a) {
     const BlockRows r = rows_of_part(a, all, p, parts);
     if (r.lo < r.hi) sum += from[(long long)p * a.tiles * kBlock];
   }
-  if (at) *at = gathered(a, c, at, key) + sum;
+  if (at) *at = gathered(a, c, at, key) + finite_or_nan(sum);
 }
 
 // Rows in parts of 2048, or of fewer while there are less than four workgroups to a compute unit; the results are joined by a second launch.  (A workgroup needs 3 to 4 us

@@ -285,9 +285,6 @@ __device__ __forceinline__ typename T::v8 zeros_at(typename T::v8 x, unsigned bi
 // log of the sum of exponentials from the reference (in powers of two) and the sum
 __device__ __forceinline__ float log_sum(float ref, float l) { return (ref + __builtin_log2f(l)) * 0.6931471805599453f; }
 
-// A sum over values as it leaves: one that is infinite, because a value is, as NaN, which it is already where a weight of zero met that value, or a mask cut its tile.
-__device__ __forceinline__ float finite_or_nan(float x) { return __builtin_fmaf(x, 0.0f, x); }
-
 // ---- narrow ---------------------------------------------------------------------------
 
 template <KvFormat F, int D>

@@ -813,7 +813,8 @@ int ftk_verify_tree(const void* target, int type, const void* ids,
  * decay * weights (0 <= decay <= 1) where k is older than the new tokens, and 0 for the
  * new ones' own positions and with a decay of 0, where what the array held is not read.
  * A row whose lse is -inf gives nothing; an lse of NaN, or a key that is not finite, makes
- * NaN or zero of the positions that it is seen at, and of no others.  Sequences without new tokens,
+ * NaN or zero of the positions that it is seen at, and of no others; a sum beyond fp32's
+ * range is NaN too, so that nothing but what the array held is infinite.  Sequences without new tokens,
  * and what is no position of a sequence, are left alone.  pages->v and v_exps are not
  * looked at.  Codes of 8 bits count as their exact values.  fp32 sums in an order that depends on
  * the sizes of the call alone, workspace_bytes among them.  max_queries and max_keys promise that no

@@ -532,6 +532,39 @@ def test_keys_that_are_not_finite_reach_their_own_weight_alone(core, dtype):
     assert bool(((w - want).abs() <= off + (off == 0) * 0.0)[near].all())
 
 
+@pytest.mark.parametrize('dtype', [F16, BF16])
+@pytest.mark.parametrize('new,lens', [([1, 1], [70, 33]), ([20, 1], [70, 33]), ([150, 1], [300, 33]), ([3000, 1], [3000, 33])])
+def test_an_infinite_key_makes_nan_or_zero_of_its_weight(core, dtype, new, lens):
+    """A score of +inf gives NaN, which selection ranks below everything, and one of -inf nothing: few rows, many, and many in parts."""
+    page, D, G, scale = 16, 64, 2, 0.125
+    batch = base.make_batch(new, lens, page, 556)
+    pages = base.make_pages(batch, 1, D, None, dtype, 557)
+    q = torch.randn((sum(new), G, D), generator=torch.Generator().manual_seed(558)).to(dtype)
+    q[:, :, 5], q[:, 0, 6], q[:, 1, 6] = 0.75, 0.5, -0.5
+    lse = torch.full((sum(new), G), 3.0)
+    before = torch.rand((batch['pages'], 1, page), generator=torch.Generator().manual_seed(559))
+    sees = lambda b, n, first, length: ref.causal_sees(n, first, length)
+    want, off = ref.weigh(q, lse, base.held(pages[0], None), before, batch, 1, scale, sees, 0.5)
+    # element 5: all rows score +inf; element 5 negative: all -inf; element 6: of the two heads one each
+    odd = [(0, 3, 5, math.inf), (0, lens[0] - 1, 5, math.inf), (1, 32, 5, -math.inf), (0, 17, 5, -math.inf), (0, 40, 6, math.inf), (1, 9, 6, -math.inf)]
+    for b, p, e, x in odd:
+        at = (batch['table'][b][p // page], 0, p % page)
+        pages[0][(*at, e)] = x
+        old = p < lens[b] - new[b]
+        want[at] = math.nan if x > 0 or e == 6 else 0.5 * float(before[at]) if old else 0.0
+    w = before.cuda()
+    core.kv_cache_weigh(q.cuda(), lse.cuda(), pages[0].cuda(), w, *base.on_device(batch), scale=scale, decay=0.5, max_queries=max(new), max_keys=max(lens))
+    kept = core.kv_cache_select(w, _ints(batch['table']), _ints(lens), 30).cpu()
+    w = w.cpu().double()
+    assert torch.equal(torch.isnan(w), torch.isnan(want))
+    fine = ~torch.isnan(want)
+    assert bool(((w - want).abs() <= off)[fine].all())
+    for b in (0, 1):
+        finite = [p for p in range(lens[b]) if (b, p) not in [o[:2] for o in odd if o[3] > 0 or o[2] == 6]]
+        if len(finite) >= 30:
+            assert set(kept[b, 0].tolist()) <= set(finite)
+
+
 # ---- selecting ---------------------------------------------------------------------------------
 
 def _select_case(core, lens, page, heads, budget, sinks, recent, weights, seed, hints=True, table=None):
