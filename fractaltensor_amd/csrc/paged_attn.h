@@ -839,7 +839,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
     const signed char* exps;
     unsigned src[D == 96 ? CP : 1];
     v4u codes[LD];
-    int exps_of[LD];                                           // as they are held: what is made of them waits for them
+    std::conditional_t<TREE, int, float> power[LD];            // of two; TREE: the exponent as it is held, since what is made of it waits for it
   };
   // Cache row (from this head's first) of the 16 keys of this wave in tile t; of the nearest 16 in [lo, hi) where those lie outside (INSIDE: they
   // do not).
@@ -882,18 +882,25 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
       }
     }
   };
-  // 8 bits
+  // 8 bits.  (TREE: from addresses of the whole wave, which frees registers there; chunks and prompts have none to spare for them: four prompts of 4096 in int8, 16 heads of
+  // 128, fp16, 197 us, and 211 that way.)
   auto load = [&](Bring& b, int t, long long at, auto inside_c) __attribute__((always_inline)) {
     const int key0 = base + 64 * t + 16 * cw;
     const int inside = min(max(key0, j.lo & ~15), (j.hi - 1) & ~15);
     const int least = max(j.lo - inside, 0), most = min(j.hi - 1 - inside, 15);
-    const unsigned char *const block = uniform(b.from + at * D), *const block_exps = uniform((const unsigned char*)b.exps + at);
 #pragma unroll
     for (int i = 0; i < LD; ++i) {
       const int p = min(64 * i + lane, D - 1), rw = p / (D / 16), piece = p - rw * (D / 16);
-      const unsigned row = decltype(inside_c)::value ? rw : min(max(key0 + rw - inside, least), most);
-      b.codes[i] = *reinterpret_cast<const v4u*>(block + (decltype(inside_c)::value ? 16u * p : row * D + 16u * piece));
-      b.exps_of[i] = (signed char)block_exps[row];
+      const int row = decltype(inside_c)::value ? rw : min(max(key0 + rw - inside, least), most);
+      if constexpr (TREE) {
+        const unsigned char *const block = uniform(b.from + at * D), *const block_exps = uniform((const unsigned char*)b.exps + at);
+        b.codes[i] = *reinterpret_cast<const v4u*>(block + (decltype(inside_c)::value ? 16u * p : (unsigned)row * D + 16u * piece));
+        b.power[i] = (signed char)block_exps[(unsigned)row];
+      } else {
+        const long long row_at = at + row;
+        b.codes[i] = *reinterpret_cast<const v4u*>(b.from + row_at * D + 16 * piece);
+        b.power[i] = ldexpf(1.0f, b.exps[row_at]);
+      }
     }
   };
   auto store = [&](const Bring& b, unsigned char* to) __attribute__((always_inline)) {
@@ -902,7 +909,7 @@ __device__ __forceinline__ void wide_attention(const AttnArgs& a, const Job& j, 
       for (int i = 0; i < LD; ++i) {
         const int p = 64 * i + lane, rw = p / (D / 16), piece = p - rw * (D / 16), in_tile = 16 * cw + rw;
         const int swz = b.keys ? swizzle<S::BYTES>(in_tile) : v_swizzle<D>(in_tile);
-        const float scale = ldexpf(1.0f, b.exps_of[i]);
+        const float scale = TREE ? ldexpf(1.0f, (int)b.power[i]) : (float)b.power[i];
         auto put = [&](auto decode) __attribute__((always_inline)) {
           if (D % 64 == 0 || p < D) {
 #pragma unroll
