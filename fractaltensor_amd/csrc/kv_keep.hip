@@ -2,14 +2,15 @@
 //
 // select.  The budget's heaviest positions, without sorting: a workgroup to a (sequence, head) finds the weight at the border by counting.  Weights are
 // taken as whole numbers that have their order; the range that holds the border, at first from the least to the greatest, is cut into 1024 or 2048 equal
-// parts, the positions of each are counted in LDS, and the part that holds the border is the next range: three rounds at most, mostly two, since a range of some binades
-// has hundreds of parts in each.  (Cutting by the bits from the top instead puts nearly all positions into a few parts, whose counting takes turns.)
+// parts, the positions of each are counted in LDS, and the part that holds the border is the next range: mostly two rounds, since a range of some binades
+// has hundreds of parts in each, and at most four (32 bits by 10; 32 by 11 take three; the upper and the lower 16 bits by 11 two each).  (Cutting by the bits from the top instead puts nearly all positions into a few parts, whose counting takes turns.)
 // Then every wave writes the positions of its own stretch in their order, behind those of the waves before it.
 //
 // keep.  Row kept[j] of a list that ascends goes to place j <= kept[j].  In place, that is safe without a second buffer as long as no place
 // is written before it has been read: rows of later j come from behind all places of earlier ones, so a workgroup takes the list in order, some
-// pieces of 16 bytes a thread at a time, with all of a step's reads done before its first write.  Rows are cut into slices of 16 to 256 bytes, each a workgroup's of its own with
-// nothing to wait for, where sequences and heads alone leave compute units idle.  Bound by reading and writing each moved byte once.
+// pieces of 16 bytes a thread at a time, with all of a step's reads done before its first write.  Rows are cut into slices of 32 to 256 bytes, each a workgroup's of its own with
+// nothing to wait for, where sequences and heads alone leave compute units idle.  The first slice's workgroup moves a row's exponent too, that of K its weight.  Bound by reading
+// and writing each moved byte once, beside whole lines for the exponents and weights of rows that lie apart.
 #include <algorithm>
 
 #include "kv_common.h"
@@ -399,7 +400,8 @@ struct KeepArgs {
 constexpr int kKeepThreads = 512, kKeepItems = 8;
 constexpr int kKeepList = 2048;                      // entries of a list whose rows are looked up at once
 
-// Every lane loads, those whose row does not move the cache's first: only loads that are always there can be waited for by their number.
+// Every lane loads, those whose row does not move the cache's first: only loads that are always there can be waited for by their number.  (In the place of exponents and weights
+// that another workgroup moves, and may be writing, it is the list's first entry.)
 template <int LANES, bool EXPS, bool WEIGHTS>
 __global__ __launch_bounds__(kKeepThreads, 4) void kv_keep_kernel(KeepArgs a) {
   constexpr int ROWS = kKeepThreads / LANES, STEP = ROWS * kKeepItems;
@@ -420,6 +422,9 @@ __global__ __launch_bounds__(kKeepThreads, 4) void kv_keep_kernel(KeepArgs a) {
   unsigned char* const data = (values ? a.pages.v : a.pages.k) + slice * 16 * LANES + 16 * piece;
   signed char* const exps = values ? a.pages.v_exps : a.pages.k_exps;
   const bool with_exps = EXPS && slice == 0 && piece == 0, with_weights = WEIGHTS && slice == 0 && piece == 0 && !values;
+  const signed char* const exps_from = slice == 0 ? exps : reinterpret_cast<const signed char*>(kept);
+  const float* const weights_from = slice == 0 && !values ? a.weights : reinterpret_cast<const float*>(kept);
+  const long long exps_mask = slice == 0 ? -1 : 0, weights_mask = slice == 0 && !values ? -1 : 0;
   const bool counts = slice == 0 && !values && head == 0;        // one workgroup of a sequence says how many stay
   // the cache row of a position, -1: it has none
   const auto row_of = [&](long long position) __attribute__((always_inline)) -> long long {
@@ -460,8 +465,8 @@ __global__ __launch_bounds__(kKeepThreads, 4) void kv_keep_kernel(KeepArgs a) {
 #pragma unroll
       for (int u = 0; u < kKeepItems; ++u) {
         x[u] = *reinterpret_cast<const v4u*>(data + from[u] * a.row_bytes);
-        if constexpr (EXPS) e[u] = exps[from[u]];
-        if constexpr (WEIGHTS) w[u] = a.weights[from[u]];
+        if constexpr (EXPS) e[u] = exps_from[from[u] & exps_mask];
+        if constexpr (WEIGHTS) w[u] = weights_from[from[u] & weights_mask];
       }
     };
     const auto write = [&](int s, v4u (&x)[kKeepItems], int (&e)[kKeepItems], float (&w)[kKeepItems]) __attribute__((always_inline)) {
