@@ -922,6 +922,44 @@ def test_refusals_on_the_device(core):
 
 # ---- FractalTensors --------------------------------------------------------------------------------
 
+@pytest.mark.parametrize('dtype,cache,window', [(F16, I8, 0), (BF16, None, 0), (BF16, E4M3, 20)])
+def test_weights_of_an_accepted_path(core, dtype, cache, window):
+    """Behind kv_cache_keep a path is a chain: its queries, with what attention over the tree left for them, give the weights of their positions and of all in front."""
+    heads, G, D, page, V = 2, 4, 64, 16, 50
+    new, lens = [12, 0, 40, 1], [60, 20, 300, 9]
+    g = torch.Generator().manual_seed(930)
+    batch = base.make_batch(new, lens, page, 931)
+    table, dlens, starts = base.on_device(batch)
+    pages = _cuda(base.make_pages(batch, heads, D, cache, dtype, 932))
+    parents = _ints(_trees(new, 933))
+    q = torch.randn((53, heads * G, D), generator=g).to(dtype).cuda()
+    _, lse = core.paged_tree_attention(q, *pages[:2], table, dlens, starts, parents, *pages[2:], window=window, max_queries=40, max_keys=300, return_lse=True)
+    p, ids = torch.zeros((53, V)), torch.arange(53) % V
+    for b, n in enumerate(new):                                    # the way goes on at a node's last child
+        for i in range(n):
+            children = [c for c in range(n) if int(parents[batch['starts'][b] + c]) == i]
+            p[batch['starts'][b] + i, int(ids[batch['starts'][b] + children[-1]]) if children else V - 1] = 1.0
+    _, path, accepted = core.verify_tree(p.cuda(), ids.cuda(), parents, starts, torch.rand((4, 8), generator=g).cuda())
+    assert int(accepted[0]) > 0 and int(accepted[2]) > 1
+    weights = torch.rand((batch['pages'], heads, page), generator=g).cuda()
+    left = core.kv_cache_keep(*pages[:2], table, dlens, path, starts, *pages[2:], weights)
+    rows = (path + starts[:-1, None])[path >= 0].long()
+    count = (path >= 0).sum(1).tolist()
+    at = [sum(count[:b]) for b in range(5)]
+    before = weights.cpu()
+    qp, lp = q[rows].contiguous(), lse[rows].contiguous()
+    core.kv_cache_weigh(qp, lp, pages[0], weights, table, left, _ints(at), pages[2], decay=0.5, window=window, max_queries=max(count), max_keys=300)
+    k = base.held(pages[0].cpu(), None if pages[2] is None else pages[2].cpu())
+    kept = batch | dict(starts=at, lens=left.tolist(), tokens=at[-1])
+    sees = lambda b, n, first, length: ref.causal_sees(n, first, length, True, window)
+    want, off = ref.weigh(qp, lp, k, before, kept, heads, D ** -0.5, sees, 0.5)
+    assert bool(((weights.cpu().double() - want).abs() <= off).all())
+    given = ref.weigh(qp, lp, k, torch.zeros_like(before), kept, heads, D ** -0.5, sees)[0].sum()
+    exact = ref.attention(qp.cpu(), k.half().double() if dtype == F16 else k, k, kept, heads, D ** -0.5, sees)
+    assert bool(((lp.cpu().double() - exact['lse']).abs() <= base.attention_bounds(exact, dtype, D)[1]).all())
+    assert abs(float(given) - at[-1] * heads * G) < 1e-3 * at[-1] * heads * G      # each row gives one in all
+
+
 def test_a_step_with_a_tree_on_fractal_tensors(core):
     from fractaltensor_amd.kaleido import FractalTensor, operations as ops
     heads, G, D, page, V = 2, 2, 64, 16, 300
