@@ -9,9 +9,10 @@
 //              4.4 TB/s with all that is read and written; in bf16 5.2, and 6.0 for one sequence of 131072.  (A lane's 16 bytes lie beside those of three others of its row: copies of
 //              whole lines, whose rows the product could not use, were 6 % faster.)
 //   many rows  (chunks, prompts): the keys' fragments stay in registers, and the products of 32 rows go beside the exponentials of the 32 in front of them (32x32x16:
-//              with 16x16x32 the two pipes got in each other's way).  At 0.8 PFLOP/s, two thirds of what a large library product reaches, it is the card's power that
-//              bounds it: without the exponentials 1.0, and neither less LDS traffic nor fewer instructions changed the time.  Four prompts of 4096, 16 heads of 128,
-//              fp16: 176 us under a causal mask, 340 without one.
+//              with 16x16x32 the two pipes got in each other's way).  Four prompts of 4096, 16 heads of 128, fp16: 168 us under a causal mask, 0.82 PFLOP/s, three quarters
+//              of what a large library product reaches beside it, and 340 without one.  There it is the card's power that bounds it: without the exponentials 1.0, and neither
+//              less LDS traffic nor fewer instructions changed the time.  Prompts of unlike lengths end unevenly: 4096, 1749 and 3648 tokens, 864 workgroups of up to 2048 rows on
+//              the 512 that there is room for, take 126 us, 0.54 PFLOP/s; in parts of 1024 rows 140, of 512 161, since each begins with 3 to 4 us.  (At D 128 six registers spill.)
 //
 // Scores and sums are fp32; codes of 8 bits enter the product as they are, exact in both 16-bit types, and the power of two of a key's row multiplies its scores.
 #include <float.h>
@@ -547,8 +548,8 @@ __global__ __launch_bounds__(kBlock) void kv_weigh_join_kernel(WeighArgs a) {
 }
 
 // Rows in parts of 2048, or of fewer while there are less than four workgroups to a compute unit; the results are joined by a second launch.  (A workgroup needs 3 to 4 us
-// before its first product: a prompt of 4096 tokens, 16 heads of 128: 71 us in parts of 2048, 68 in 1024 or 512; four such prompts 176, 194 and 205; one of 2048 tokens, 8 heads
-// on one of keys: 82, 48 and 34.)
+// before its first product: a prompt of 4096 tokens, 16 heads of 128: 71 us in parts of 2048, 68 in 1024 or 512; four such prompts 168, 185 and 213; one of 2048 tokens, 8 heads
+// on one of keys: 82, 48 and 34.  Workgroups are counted from the sizes that the call could have, among them those of sequences that pause and of blocks behind shorter ones' ends.)
 struct RowCut {
   int parts, rows;
 };

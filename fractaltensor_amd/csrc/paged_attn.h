@@ -24,8 +24,8 @@
 // lane.  (Position and depth differ in a tree; a window counts the steps on the way.)  The narrow form has up to 16 rows of them, and the wide form
 // more: up to 128 rows by both halves of a workgroup, on different keys, and the work of sequences of different lengths shared
 // out evenly.  Sequences of up to 64 rows have their weights as two operands on either, by their own rows alone, so that a tree's results are no less exact than those of the same tokens
-// one behind the other, nor for a larger tree beside it; the wide form has a second body for them.  (16 sequences of 2064 to 8192 positions in e4m3, 8 heads of keys, 64 rows: 89 us, 73 with
-// weights rounded once, 92 by the narrow form; 16 bits 87, 85 and 107.)
+// one behind the other, nor for a larger tree beside it; the wide form has a second body for them.  (16 sequences of 2064 to 8192 positions in e4m3, 8 heads of keys, 64 rows: 89 us, 74 with
+// weights rounded once, 92 by the narrow form; 16 bits 87, 86 and 107.)
 #pragma once
 
 #include <float.h>

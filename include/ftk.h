@@ -759,8 +759,11 @@ int ftk_verify_drafts(const void* target, const void* draft, int type,
  * token d steps below a root counts as d positions behind the first new one's.
  * All else is as in ftk_paged_attn, but that a sequence's own rows (new tokens times heads
  * / pages->heads) say alone how its weights enter the products with values: up to 64 as two
- * numbers of 16 bits, whatever else the call holds.  A sequence has at most 256 new tokens:
- * max_queries promises it, or `tokens` is no larger.
+ * numbers of 16 bits, whatever else the call holds; more are rounded to 16 bits once, against
+ * references that move with how the work of all sequences is shared out, so that there
+ * results may differ by that rounding with what else the call holds.  A sequence has at most
+ * 256 new tokens: max_queries promises it, or `tokens` is no larger (where neither does, the
+ * call is refused and its workspace is 0).
  */
 size_t ftk_paged_tree_attn_workspace_bytes(const ftk_kv_pages* pages,
                                            const ftk_kv_batch* batch,
