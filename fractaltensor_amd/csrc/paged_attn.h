@@ -1990,8 +1990,8 @@ static int check_attention(const char* who, int heads, const ftk_kv_pages* pages
 }
 
 template <typename K, typename... Args>
-static int launch_with_lds(const char* name, K kernel, DeviceOnce& once, long long blocks, int waves, int lds, hipStream_t s, Args... args) {
-  if (blocks > INT_MAX) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "ftk_paged_attn: grid too large");
+static int launch_with_lds(const char* who, const char* name, K kernel, DeviceOnce& once, long long blocks, int waves, int lds, hipStream_t s, Args... args) {
+  if (blocks > INT_MAX) return fail(FTK_ERR_UNSUPPORTED_SHAPE, "%s: grid too large", who);
   unsigned bit;
   if (once.pending(&bit)) {
     FTK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
@@ -2079,7 +2079,7 @@ static int attend(const char* who, const void* q, int type, long long q_token_st
       using no = std::false_type;
       auto launch = [&](auto nq, auto kept) -> int {
         static DeviceOnce once;
-        return launch_with_lds("paged_narrow_kernel", paged_narrow_kernel<T, F, D, decltype(nq)::value, decltype(kept)::value, TREE>, once, blocks, kWaves, NarrowShape<F, D>::LDS, s,
+        return launch_with_lds(who, "paged_narrow_kernel", paged_narrow_kernel<T, F, D, decltype(nq)::value, decltype(kept)::value, TREE>, once, blocks, kWaves, NarrowShape<F, D>::LDS, s,
                                a, p.slots_per_seq);
       };
       if constexpr (TREE) {                                      // (one block of 16 rows to a sequence and head)
@@ -2093,7 +2093,7 @@ static int attend(const char* who, const void* q, int type, long long q_token_st
         static DeviceOnce once;
         constexpr bool PAIRED = decltype(paired)::value;
         constexpr int lds = std::max(WideShape<D, TREE, PAIRED>::LDS, TREE ? 0 : 2 * NarrowShape<F, D>::LDS);
-        return launch_with_lds("paged_wide_kernel", paged_wide_kernel<T, F, D, TREE, PAIRED>, once, blocks + pairs, kWideWaves, lds, s, a, (int)blocks);
+        return launch_with_lds(who, "paged_wide_kernel", paged_wide_kernel<T, F, D, TREE, PAIRED>, once, blocks + pairs, kWideWaves, lds, s, a, (int)blocks);
       };
       if constexpr (TREE) bad = p.block_rows == kPairedRows ? launch(std::true_type{}) : launch(std::false_type{});
       else bad = launch(std::false_type{});

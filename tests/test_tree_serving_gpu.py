@@ -344,6 +344,16 @@ def test_more_tokens_than_trees_have_are_refused_at_once(core):
     assert bool((out == 7).all())
 
 
+def test_grids_that_are_too_large_are_refused_by_name(core):
+    B, heads = 1 << 20, 4096
+    q, pages = torch.zeros((1, heads, 32), dtype=F16, device='cuda'), torch.zeros((1, heads, 16, 32), dtype=F16, device='cuda')
+    table, lens, starts, parents = (torch.zeros(s, dtype=torch.int32, device='cuda') for s in ((B, 1), B, B + 1, 1))
+    with pytest.raises(core.FtkError, match='ftk_paged_tree_attn: grid too large'):
+        core.paged_tree_attention(q, pages, pages, table, lens, starts, parents, max_queries=1)
+    with pytest.raises(core.FtkError, match='ftk_paged_attn: grid too large'):
+        core.paged_attention(q, pages, pages, table, lens, starts, max_queries=1)
+
+
 # ---- verification ------------------------------------------------------------------------------
 
 def _verify_case(core, dtype, new, V, M, seed, ids_type=torch.int64, kind='any', shift=0):
